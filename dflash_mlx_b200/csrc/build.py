@@ -10,9 +10,12 @@ from pathlib import Path
 CSRC = Path(__file__).resolve().parent
 PKG = CSRC.parent
 LIB = PKG / "libdflash_b200.so"
-SOURCES = ["runtime.cu", "qmm.cu", "qmm_tc.cu", "gdn.cu", "gdn_layer.cu", "sdpa.cu", "sdpa_tc.cu", "glue.cu", "peer.cu"]
+SOURCES = ["runtime.cu", "qmm.cu", "qmm_tc.cu", "gdn.cu", "gdn_layer.cu", "sdpa.cu", "sdpa_tc.cu", "glue.cu", "peer.cu", "kv4.cu",
+           "logprobs.cu"]
 FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17", "--use_fast_math",
          "-Xcompiler", "-fPIC", "-Xcompiler", "-fvisibility=hidden", "-Xptxas", "-v"]
+# Sources whose results are defined to the last bit, subnormals included: IEEE division and no flush to zero.
+IEEE_SOURCES = {"kv4.cu"}
 
 
 def _nvcc() -> str:
@@ -40,7 +43,8 @@ def build(force: bool = False, verbose: bool = False) -> Path:
             continue
         obj = objdir / (src.stem + ".o")
         if force or _stale(obj, src):
-            cmd = [nvcc, *FLAGS, "-c", str(src), "-o", str(obj)]
+            flags = [f for f in FLAGS if f != "--use_fast_math" or name not in IEEE_SOURCES]
+            cmd = [nvcc, *flags, "-c", str(src), "-o", str(obj)]
             res = subprocess.run(cmd, capture_output=True, text=True)
             (objdir / (src.stem + ".ptxas.txt")).write_text(res.stderr)
             if res.returncode != 0:

@@ -1,0 +1,864 @@
+// The 4-bit KV cache: quantising new rows as they are written, reading rows back, and softmax attention over the codes.
+//
+// Layout (that of mlx-lm's quantised cache and of this library's packed weights): per position D/8 words of eight codes, one
+// scale and one bias per 64 channels; a channel stands for code * scale + bias.
+//
+// Attention over the codes, per KV head with rows = (Hq/Hk) * T query rows r and keys n, group g = 64 channels:
+//   S[r,n] = scale * sum_g ( sk[n,g] * sum_{d in g} q[r,d] (ck[n,d] - 8)  +  (bk[n,g] + 8 sk[n,g]) * sum_{d in g} q[r,d] )
+//   O[r,d] = sum_n p[r,n] sv[n,g] (cv[n,d] - 8)  +  sum_n p[r,n] (bv[n,g] + 8 sv[n,g])          (g the group of d)
+// The codes enter both products as exact small integers; scales and biases are applied in fp32 around them, so the only
+// rounding besides fp32 sums is that of p * sv to fp16 (11 bits; the cache's values themselves are never rounded).
+#include <mutex>
+
+#include "kv4.cuh"
+
+namespace dflash {
+namespace kv4 {
+namespace {
+
+constexpr float kLog2e = 1.4426950408889634f;
+
+// ---- write -------------------------------------------------------------------------------------------------------------
+// A lane owns the eight channels of one word, eight lanes a group: minimum and maximum in three shuffles, no shared memory.
+// Bound by HBM (prompts) or by the launch (single tokens): kRows rows per warp are loaded before the first is used, so that a
+// warp has 16 * kRows bytes a lane in flight.
+struct WriteArgs {
+  const void* x[2];
+  long long sb[2], sh[2], st[2];
+  dflash_kv4_cache c[2];
+  const int* offsets;
+  const int* counts;
+  int Hk, T, capacity;
+  long long rows;   // B * Hk * T
+};
+
+template <typename T, int D, int kRows>
+__global__ void __launch_bounds__(128) kv4_write_kernel(const WriteArgs a, int* __restrict__ err) {
+  using TR = MmaTraits<T>;
+  constexpr int kLanes = D / 8, kPer = 32 / kLanes;   // lanes of a row, rows of a warp at once
+  pdl_wait();
+  pdl_trigger();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, side = blockIdx.y;
+  const int j = lane % kLanes;
+  const long long row0 = ((long long)blockIdx.x * 4 + warp) * (kPer * kRows) + lane / kLanes;
+  const T* x = (const T*)a.x[side];
+  const dflash_kv4_cache c = a.c[side];
+  uint4 raw[kRows];
+  int pos[kRows], bb[kRows], hh[kRows];
+#pragma unroll
+  for (int i = 0; i < kRows; ++i) {
+    const long long row = row0 + (long long)i * kPer;
+    pos[i] = -1;
+    raw[i] = make_uint4(0, 0, 0, 0);
+    bb[i] = hh[i] = 0;
+    if (row < a.rows) {
+      const int t = (int)(row % a.T), bh = (int)(row / a.T);
+      bb[i] = bh / a.Hk;
+      hh[i] = bh % a.Hk;
+      const int n = a.counts ? a.counts[bb[i]] : a.T;
+      if (t < n) {
+        const long long p = (long long)a.offsets[bb[i]] + t;
+        if (p >= 0 && p < a.capacity) {
+          pos[i] = (int)p;
+          raw[i] = *(const uint4*)(x + bb[i] * a.sb[side] + hh[i] * a.sh[side] + t * a.st[side] + 8 * j);
+        } else if (j == 0) {
+          atomicCAS(err, 0, 61 | ((t & 0x7FFFFF) << 8));
+        }
+      }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < kRows; ++i) {
+    float v[8];
+    const uint32_t u[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+    float lo = INFINITY, hi = -INFINITY, bad = 0.f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      v[e] = TR::bits_to_float((uint16_t)(u[e >> 1] >> (16 * (e & 1))));
+      lo = fminf(lo, v[e]);
+      hi = fmaxf(hi, v[e]);
+      bad = fmaf(v[e], 0.f, bad);   // NaN as soon as one value is NaN or infinite
+    }
+#pragma unroll
+    for (int o = 1; o < 8; o <<= 1) {
+      lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+      hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+      bad += __shfl_xor_sync(0xffffffffu, bad, o);
+    }
+    // IEEE divisions and subnormals: the codes are defined to the last bit (this file is compiled without fast math)
+    const T scale_t = TR::from_float(__fadd_rn(__fsub_rn(__fdiv_rn(hi, 15.f), __fdiv_rn(lo, 15.f)), bad));
+    const T bias_t = TR::from_float(__fadd_rn(lo, bad));
+    const float scale = TR::to_float(scale_t), bias = TR::to_float(bias_t);
+    uint32_t word = 0;
+    if (scale > 0.f) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float q = rintf(__fdiv_rn(__fsub_rn(v[e], bias), scale));
+        word |= (uint32_t)fminf(fmaxf(q, 0.f), 15.f) << (4 * e);
+      }
+    }
+    if (pos[i] >= 0) {
+      c.codes[bb[i] * c.codes_batch_stride + hh[i] * c.codes_head_stride + (long long)pos[i] * (D / 8) + j] = word;
+      if ((j & 7) == 0) {
+        const long long in_row = (long long)pos[i] * (D / kGroup) + (j >> 3);
+        ((T*)c.scales)[bb[i] * c.scales_batch_stride + hh[i] * c.scales_head_stride + in_row] = scale_t;
+        ((T*)c.biases)[bb[i] * c.biases_batch_stride + hh[i] * c.biases_head_stride + in_row] = bias_t;
+      }
+    }
+  }
+}
+
+// ---- read --------------------------------------------------------------------------------------------------------------
+struct ReadArgs {
+  dflash_kv4_cache c[2];
+  void* out[2];
+  const int* starts;
+  int start, Hk, T, capacity;
+  long long rows;
+};
+
+// The same split as the write: a lane unpacks one word into 16 bytes of output.
+template <typename T, int D, int kRows>
+__global__ void __launch_bounds__(128) kv4_read_kernel(const ReadArgs a) {
+  using TR = MmaTraits<T>;
+  constexpr int kLanes = D / 8, kPer = 32 / kLanes;
+  pdl_wait();
+  pdl_trigger();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, side = blockIdx.y;
+  const int j = lane % kLanes;
+  const long long row0 = ((long long)blockIdx.x * 4 + warp) * (kPer * kRows) + lane / kLanes;
+  const dflash_kv4_cache c = a.c[side];
+  uint32_t word[kRows];
+  float scale[kRows], bias[kRows];
+#pragma unroll
+  for (int i = 0; i < kRows; ++i) {
+    const long long row = row0 + (long long)i * kPer;
+    word[i] = 0;
+    scale[i] = bias[i] = 0.f;
+    if (row < a.rows) {
+      const int t = (int)(row % a.T), bh = (int)(row / a.T), b = bh / a.Hk, h = bh % a.Hk;
+      const long long p = (long long)(a.starts ? a.starts[b] : a.start) + t;
+      if (p >= 0 && p < a.capacity) {
+        const long long in_row = p * (D / kGroup) + (j >> 3);
+        word[i] = c.codes[b * c.codes_batch_stride + h * c.codes_head_stride + p * (D / 8) + j];
+        scale[i] = TR::to_float(((const T*)c.scales)[b * c.scales_batch_stride + h * c.scales_head_stride + in_row]);
+        bias[i] = TR::to_float(((const T*)c.biases)[b * c.biases_batch_stride + h * c.biases_head_stride + in_row]);
+      }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < kRows; ++i) {
+    const long long row = row0 + (long long)i * kPer;
+    if (row < a.rows) {
+      uint4 o;
+      uint32_t* po = (uint32_t*)&o;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        // code * scale is exact in fp32 (4 + 11 bits), so there is one rounding in the sum and one to the output type
+        const T x0 = TR::from_float(fmaf((float)((word[i] >> (8 * e)) & 15u), scale[i], bias[i]));
+        const T x1 = TR::from_float(fmaf((float)((word[i] >> (8 * e + 4)) & 15u), scale[i], bias[i]));
+        po[e] = (uint32_t) * (const uint16_t*)&x0 | ((uint32_t) * (const uint16_t*)&x1 << 16);
+      }
+      *(uint4*)((T*)a.out[side] + row * D + 8 * j) = o;
+    }
+  }
+}
+
+// ---- attention, few rows per KV head -----------------------------------------------------------------------------------
+// One warp works on 16 keys at a time, on its own: codes and scales of its next tiles arrive by cp.async in a ring of
+// kStages shared-memory buffers that only this warp touches, so there is no block-wide barrier in the loop.  Both products
+// have the KEYS' codes (or their transpose) as the 16-row operand and 8 query rows as the 8 columns, so one decoded token of a
+// grouped model (Hq/Hk <= 8 rows) wastes nothing:
+//   S^T [16 keys, 8 rows] += K codes [16, 16 channels] x Q^T : a thread unpacks the two words of its quarter of a group; the
+//       16 channels of an MMA step are any 16 of one group (Q is laid out to match), so a group's sum ends in its own
+//       accumulator and takes its scale there.
+//   O^T [16 channels, 8 rows] += V codes^T [16, 16 keys] x P' : P' = p * sv in fp16 (sv brought into fp16's range by a power of
+//       two per warp that is undone at the end).  Nibble t and 4 + t of a word are rows r and r + 8 of MMA t, so a thread's
+//       words serve four MMAs without crossing lanes.
+// Codes become code - 8 by OR-ing the nibble into a constant and one exact packed subtraction: centred integers keep the
+// fp32 sums small (with the constant left in, a score's sum carries 136 or 1032 times sum |q|, which costs digits).
+// The running maximum moves only when a score exceeds it by 8 octaves (p <= 256 otherwise), so the accumulators are rarely
+// rescaled.  The warps of a block and then the splits of the key range are merged with fp32 partials.
+constexpr int kWarps = 8;
+constexpr float kMaxStep = 5.545177444f;   // 8 ln 2
+
+template <int D>
+struct Tile {
+  static constexpr int kG = D / kGroup;                 // groups of a row
+  static constexpr int kCodeBytes = 16 * D / 2;         // 16 keys or values
+  static constexpr int kScaleBytes = 16 * kG * 2;
+  static constexpr int kBytes = 2 * kCodeBytes + 4 * kScaleBytes;
+};
+
+__device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool valid) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(valid ? 16 : 0) : "memory");
+}
+template <int N>
+__device__ __forceinline__ void cp_small(uint32_t dst, const void* src, bool valid) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(dst), "l"(src), "n"(N), "r"(valid ? N : 0) : "memory");
+}
+__device__ __forceinline__ uint32_t movm(uint32_t x) {   // transpose of an 8x8 matrix of 16-bit elements held by the warp
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+// Codes of nibbles i and 4 + i of a word, minus 8, as pair i.  (1024 + c) - 1032, (1024 + 16 c) / 16 - 72 and (128 + c) - 136 are
+// exact.
+template <typename T> __device__ __forceinline__ void unpack(uint32_t w, uint32_t (&out)[4]);
+template <> __device__ __forceinline__ void unpack<__half>(uint32_t w, uint32_t (&out)[4]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t u = lop3_and_or(i < 2 ? w : w >> 8, (i & 1) ? 0x00F000F0u : 0x000F000Fu, 0x64006400u);
+    __half2 v = *(const __half2*)&u;
+    if (i & 1) v = __hfma2(v, __float2half2_rn(0.0625f), __float2half2_rn(-72.f));
+    else v = __hadd2(v, __float2half2_rn(-1032.f));
+    out[i] = *(const uint32_t*)&v;
+  }
+}
+template <> __device__ __forceinline__ void unpack<__nv_bfloat16>(uint32_t w, uint32_t (&out)[4]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t u = lop3_and_or(w >> (4 * i), 0x000F000Fu, 0x43004300u);
+    const __nv_bfloat162 v = __hadd2(*(const __nv_bfloat162*)&u, __float2bfloat162_rn(-136.f));
+    out[i] = *(const uint32_t*)&v;
+  }
+}
+// Where 16-byte chunk `ch` of row `r` goes: rows that are read together fall into different banks (K: rows 0..3 at a time,
+// V: rows 0, 2, 4, 6 at a time; with D = 128 two rows share 128 bytes, and V keeps a two-way conflict).
+template <int D>
+__device__ __forceinline__ int k_chunk(int r, int ch) { return ch ^ (D == 256 ? ((r & 3) << 1) : (((r >> 1) & 1) << 1)); }
+template <int D>
+__device__ __forceinline__ int v_chunk(int r, int ch) { return ch ^ (D == 256 ? (((r >> 1) & 3) << 1) : (((r >> 1) & 1) << 1)); }
+
+template <typename T, int D, int NT, bool kMask>
+__global__ void __launch_bounds__(kWarps * 32) kv4_sdpa_kernel(const SdpaArgs a, int stages) {
+  using TR = MmaTraits<T>;
+  using H = MmaTraits<__half>;
+  constexpr int G = D / kGroup, CPR = D / 32, KS = D / 16;   // groups, 16-byte chunks of a row's codes, MMA steps of Q K^T
+  using TL = Tile<D>;
+  extern __shared__ __align__(128) uint8_t smem[];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3;
+  uint2* sQ = (uint2*)smem;                                   // [NT][KS][32] fragments of Q^T
+  float* sQs = (float*)(smem + NT * KS * 32 * 8);             // [NT][G][8] sums of q over a group
+  uint8_t* ring = smem + NT * KS * 32 * 8 + NT * G * 8 * 4 + warp * stages * TL::kBytes;
+  const uint32_t uring = smem_u32(ring);
+  pdl_wait();
+  pdl_trigger();
+  const int split = blockIdx.x, bhk = blockIdx.z, b = bhk / a.Hk, hk = bhk % a.Hk, row0 = blockIdx.y * 8 * NT;
+  const int len = a.lengths ? a.lengths[b] : a.max_length;
+  const int t_last = min(row0 + 8 * NT, a.rows) - 1;
+  // one past the last position any row of this block sees
+  const int hi = min(min(len, a.max_length), len - a.T + t_last / a.gqa + 1);
+  const int tiles = hi > 0 ? (hi + 15) >> 4 : 0;
+  const int per = (tiles + a.splits - 1) / a.splits;
+  const int tile1 = min(tiles, (split + 1) * per);
+  int tile = split * per + warp;
+
+  const uint8_t* kc = (const uint8_t*)(a.k.codes + b * a.k.codes_batch_stride + hk * a.k.codes_head_stride);
+  const uint8_t* vc = (const uint8_t*)(a.v.codes + b * a.v.codes_batch_stride + hk * a.v.codes_head_stride);
+  const T* ksc = (const T*)a.k.scales + b * a.k.scales_batch_stride + hk * a.k.scales_head_stride;
+  const T* kbi = (const T*)a.k.biases + b * a.k.biases_batch_stride + hk * a.k.biases_head_stride;
+  const T* vsc = (const T*)a.v.scales + b * a.v.scales_batch_stride + hk * a.v.scales_head_stride;
+  const T* vbi = (const T*)a.v.biases + b * a.v.biases_batch_stride + hk * a.v.biases_head_stride;
+  auto fetch = [&](int tl, int stage) {
+    if (tl < tile1) {
+      const uint32_t dst = uring + stage * TL::kBytes;
+      const int n0 = tl * 16;
+#pragma unroll
+      for (int i = 0; i < 16 * CPR / 32; ++i) {
+        const int at = lane + 32 * i, row = at / CPR, ch = at % CPR;
+        const bool ok = n0 + row < hi;
+        const size_t from = (size_t)(ok ? n0 + row : 0) * (D / 2) + ch * 16;
+        cp16(dst + row * (D / 2) + k_chunk<D>(row, ch) * 16, kc + from, ok);
+        cp16(dst + TL::kCodeBytes + row * (D / 2) + v_chunk<D>(row, ch) * 16, vc + from, ok);
+      }
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {   // lane -> (array, key)
+        const int which = 2 * i + (lane >> 4), row = lane & 15;
+        const bool ok = n0 + row < hi;
+        const T* base = which == 0 ? ksc : which == 1 ? kbi : which == 2 ? vsc : vbi;
+        cp_small<2 * G>(dst + 2 * TL::kCodeBytes + which * TL::kScaleBytes + row * 2 * G, base + (size_t)(ok ? n0 + row : 0) * G, ok);
+      }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  for (int s = 0; s < stages - 1; ++s) fetch(tile + s * kWarps, s);
+
+  // Q^T fragments: lane (r, c) holds query row r; step ks of group g covers the nibble pairs of words 8g+2c and 8g+2c+1
+  for (int i = threadIdx.x; i < NT * KS * 32; i += kWarps * 32) {
+    const int ln = i & 31, ks = (i >> 5) % KS, nt = (i >> 5) / KS;
+    const int row = row0 + nt * 8 + (ln >> 2), g = ks >> 2, s = ks & 3;
+    uint2 f = make_uint2(0, 0);
+    if (row < a.rows) {
+      const int t = row / a.gqa, h = hk * a.gqa + row % a.gqa;
+      const uint16_t* q = (const uint16_t*)a.q + b * a.q_sb + h * a.q_sh + t * a.q_st + 64 * g + 8 * (2 * (ln & 3) + (s >> 1));
+      const int p = 2 * (s & 1);
+      f.x = (uint32_t)q[p] | ((uint32_t)q[p + 4] << 16);
+      f.y = (uint32_t)q[p + 1] | ((uint32_t)q[p + 5] << 16);
+    }
+    sQ[i] = f;
+  }
+  for (int i = threadIdx.x; i < NT * G * 8; i += kWarps * 32) {
+    const int row = row0 + (i / (G * 8)) * 8 + (i & 7), g = (i >> 3) % G;
+    float s = 0.f;
+    if (row < a.rows) {
+      const int t = row / a.gqa, h = hk * a.gqa + row % a.gqa;
+      const uint4* q = (const uint4*)((const T*)a.q + b * a.q_sb + h * a.q_sh + t * a.q_st + 64 * g);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const uint4 w = q[e];
+        const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+        for (int x = 0; x < 4; ++x) s += TR::bits_to_float((uint16_t)u[x]) + TR::bits_to_float((uint16_t)(u[x] >> 16));
+      }
+    }
+    sQs[i] = s;
+  }
+  __syncthreads();
+
+  float o[D / 16][NT][4], ob[G][NT][2], m[NT][2], l[NT][2];
+  int lim[NT][2];
+  long long mat[NT][2];
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      m[nt][e] = -INFINITY;
+      l[nt][e] = 0.f;
+      const int row = row0 + nt * 8 + 2 * c + e;
+      const int t = row / a.gqa;
+      lim[nt][e] = row < a.rows ? min(len - a.T + t, hi - 1) : -1;   // last key the row sees
+      mat[nt][e] = kMask && row < a.rows ? b * a.m_sb + (hk * a.gqa + row % a.gqa) * a.m_sh + t * a.m_st : 0;
+#pragma unroll
+      for (int g = 0; g < G; ++g) ob[g][nt][e] = 0.f;
+    }
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i) o[i][nt][0] = o[i][nt][1] = o[i][nt][2] = o[i][nt][3] = 0.f;
+  }
+  float sv_mul = 0x1p126f;   // power of two that brings this warp's value scales into fp16's range
+
+  int stage = 0;
+  for (; tile < tile1; tile += kWarps) {
+    {
+      int ahead = stage + stages - 1;
+      if (ahead >= stages) ahead -= stages;
+      fetch(tile + (stages - 1) * kWarps, ahead);
+    }
+    // this tile is the oldest of `stages` groups in flight
+    if (stages == 4) asm volatile("cp.async.wait_group 3;" ::: "memory");
+    else if (stages == 3) asm volatile("cp.async.wait_group 2;" ::: "memory");
+    else asm volatile("cp.async.wait_group 1;" ::: "memory");
+    __syncwarp();
+    const uint8_t* st = ring + stage * TL::kBytes;
+    const int n0 = tile * 16;
+    // scales of keys r and r + 8
+    float sk[2][G], bk[2][G], sv[2][G], bv[2][G];
+    float bad[2] = {0.f, 0.f};
+    float big = 0.f;
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const uint16_t* sc = (const uint16_t*)(st + 2 * TL::kCodeBytes) + (r + 8 * e) * G;
+      uint16_t h[4][G];
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        if (G == 4) *(uint2*)h[w] = *(const uint2*)(sc + w * 16 * G);
+        else *(uint32_t*)h[w] = *(const uint32_t*)(sc + w * 16 * G);
+      }
+#pragma unroll
+      for (int g = 0; g < G; ++g) {
+        sk[e][g] = TR::bits_to_float(h[0][g]);
+        bk[e][g] = fmaf(sk[e][g], 8.f, TR::bits_to_float(h[1][g]));
+        sv[e][g] = TR::bits_to_float(h[2][g]);
+        const float bb = TR::bits_to_float(h[3][g]);
+        bad[e] = fmaf(sv[e][g], 0.f, fmaf(bb, 0.f, bad[e]));   // NaN when a scale or bias of the value is not finite
+        bv[e][g] = fmaf(sv[e][g], 8.f, bb);
+        big = fmaxf(big, fabsf(sv[e][g]));
+      }
+    }
+    if (__any_sync(0xffffffffu, !(bad[0] == 0.f) || !(bad[1] == 0.f))) {
+      // keep such a value out of the products (0 * NaN would reach rows that do not see it); rows that do see it get NaN
+      // through their scores below
+      big = 0.f;
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+#pragma unroll
+        for (int g = 0; g < G; ++g) {
+          if (!(bad[e] == 0.f)) sv[e][g] = bv[e][g] = 0.f;
+          big = fmaxf(big, fabsf(sv[e][g]));
+        }
+    }
+    // ---- S^T = K Q^T ----
+    float s[NT][4];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.f;
+#pragma unroll
+    for (int g = 0; g < G; ++g) {
+      const uint2 w0 = *(const uint2*)(st + r * (D / 2) + k_chunk<D>(r, 2 * g + (c >> 1)) * 16 + (c & 1) * 8);
+      const uint2 w1 = *(const uint2*)(st + (r + 8) * (D / 2) + k_chunk<D>(r + 8, 2 * g + (c >> 1)) * 16 + (c & 1) * 8);
+      float acc[NT][4];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) acc[nt][0] = acc[nt][1] = acc[nt][2] = acc[nt][3] = 0.f;
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        uint32_t u0[4], u1[4];
+        unpack<T>(half ? w0.y : w0.x, u0);
+        unpack<T>(half ? w1.y : w1.x, u1);
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            const uint2 f = sQ[(nt * KS + 4 * g + 2 * half + ks) * 32 + lane];
+            TR::mma(acc[nt], u0[2 * ks], u1[2 * ks], u0[2 * ks + 1], u1[2 * ks + 1], f.x, f.y);
+          }
+      }
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        const float2 qs = *(const float2*)(sQs + (nt * G + g) * 8 + 2 * c);
+        s[nt][0] = fmaf(sk[0][g], acc[nt][0], fmaf(bk[0][g], qs.x, s[nt][0]));
+        s[nt][1] = fmaf(sk[0][g], acc[nt][1], fmaf(bk[0][g], qs.y, s[nt][1]));
+        s[nt][2] = fmaf(sk[1][g], acc[nt][2], fmaf(bk[1][g], qs.x, s[nt][2]));
+        s[nt][3] = fmaf(sk[1][g], acc[nt][3], fmaf(bk[1][g], qs.y, s[nt][3]));
+      }
+    }
+    // ---- visibility, running maximum ----
+    bool grow = big * sv_mul > 64.f;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        const int n = n0 + r + ((x >> 1) << 3), e = x & 1;
+        float t = fmaf(s[nt][x], a.scale, bad[x >> 1]);
+        const bool seen = n <= lim[nt][e];
+        if (kMask) {
+          if (seen) t = apply_mask<T>(a, t, mat[nt][e] + n * a.m_sn);
+        }
+        t = seen ? t : -INFINITY;
+        s[nt][x] = t;
+        grow |= t > m[nt][e] + kMaxStep;
+      }
+    if (__any_sync(0xffffffffu, grow)) {
+      float top = big;
+#pragma unroll
+      for (int w = 4; w < 32; w <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
+      float ratio = 1.f;
+      if (top * sv_mul > 64.f) {
+        const int ex = max((int)(__float_as_uint(top) >> 23) - 127, -100);
+        const float next = __uint_as_float((uint32_t)(127 + 5 - ex) << 23);   // top * next in [32, 64)
+        ratio = next / sv_mul;
+        sv_mul = next;
+      }
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        float f[2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          float x = fmaxf(m[nt][e], fmaxf(s[nt][e], s[nt][2 + e]));
+#pragma unroll
+          for (int w = 4; w < 32; w <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, w));
+          f[e] = x == -INFINITY ? 1.f : ex2((m[nt][e] - x) * kLog2e);   // nothing seen yet: the sums are zero
+          m[nt][e] = x;
+          l[nt][e] *= f[e];
+#pragma unroll
+          for (int g = 0; g < G; ++g) ob[g][nt][e] *= f[e];
+          f[e] *= ratio;
+        }
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i) {
+          o[i][nt][0] *= f[0]; o[i][nt][1] *= f[1];
+          o[i][nt][2] *= f[0]; o[i][nt][3] *= f[1];
+        }
+      }
+    }
+    // ---- p, and O^T += V^T P' per group ----
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        const float ref = m[nt][x & 1] == -INFINITY ? 0.f : m[nt][x & 1];
+        const float p = ex2((s[nt][x] - ref) * kLog2e);
+        s[nt][x] = p;
+        l[nt][x & 1] += p;
+      }
+    const uint8_t* sV = st + TL::kCodeBytes;
+#pragma unroll
+    for (int g = 0; g < G; ++g) {
+      uint32_t pb[NT][2];
+      const float s0 = sv[0][g] * sv_mul, s1 = sv[1][g] * sv_mul;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        const __half2 h0 = __floats2half2_rn(s[nt][0] * s0, s[nt][1] * s0), h1 = __floats2half2_rn(s[nt][2] * s1, s[nt][3] * s1);
+        pb[nt][0] = movm(*(const uint32_t*)&h0);
+        pb[nt][1] = movm(*(const uint32_t*)&h1);
+        ob[g][nt][0] = fmaf(s[nt][0], bv[0][g], fmaf(s[nt][2], bv[1][g], ob[g][nt][0]));
+        ob[g][nt][1] = fmaf(s[nt][1], bv[0][g], fmaf(s[nt][3], bv[1][g], ob[g][nt][1]));
+      }
+      uint32_t w[4];   // word 8g + r of keys 2c, 2c+1, 2c+8, 2c+9
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int key = 2 * c + (i & 1) + 8 * (i >> 1);
+        w[i] = *(const uint32_t*)(sV + key * (D / 2) + v_chunk<D>(key, 2 * g + (r >> 2)) * 16 + (r & 3) * 4);
+      }
+      // nibbles 0..3 / 4..7 of two keys side by side
+      uint32_t lo01[4], hi01[4], lo89[4], hi89[4];
+      unpack<__half>(prmt(w[0], w[1], 0x5410), lo01);
+      unpack<__half>(prmt(w[0], w[1], 0x7632), hi01);
+      unpack<__half>(prmt(w[2], w[3], 0x5410), lo89);
+      unpack<__half>(prmt(w[2], w[3], 0x7632), hi89);
+#pragma unroll
+      for (int t = 0; t < 4; ++t)
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) H::mma(o[4 * g + t][nt], lo01[t], hi01[t], lo89[t], hi89[t], pb[nt][0], pb[nt][1]);
+    }
+    if (++stage == stages) stage = 0;
+    __syncwarp();   // the buffer is refilled by the next iteration's fetch
+  }
+  asm volatile("cp.async.wait_group 0;" ::: "memory");
+  __syncthreads();   // the rings become the merge buffers
+
+  // ---- merge the warps: O [warp][8 NT][D], m and l [warp][8 NT] ----
+  float* mO = (float*)(smem + NT * KS * 32 * 8 + NT * G * 8 * 4);
+  float* mM = mO + kWarps * 8 * NT * D;
+  float* mL = mM + kWarps * 8 * NT;
+  const float undo = 1.f / sv_mul;
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      float x = l[nt][e];
+#pragma unroll
+      for (int w = 4; w < 32; w <<= 1) x += __shfl_xor_sync(0xffffffffu, x, w);
+      const int row = nt * 8 + 2 * c + e;
+      if (r == 0) {
+        mM[warp * 8 * NT + row] = m[nt][e];
+        mL[warp * 8 * NT + row] = x;
+      }
+      float* po = mO + ((size_t)warp * 8 * NT + row) * D;
+#pragma unroll
+      for (int g = 0; g < G; ++g) {
+        float y = ob[g][nt][e];
+#pragma unroll
+        for (int w = 4; w < 32; w <<= 1) y += __shfl_xor_sync(0xffffffffu, y, w);
+        float4 v0, v1;   // channels 64g + 8r + 0..3 and + 4..7
+        v0.x = fmaf(o[4 * g][nt][e], undo, y); v0.y = fmaf(o[4 * g + 1][nt][e], undo, y);
+        v0.z = fmaf(o[4 * g + 2][nt][e], undo, y); v0.w = fmaf(o[4 * g + 3][nt][e], undo, y);
+        v1.x = fmaf(o[4 * g][nt][2 + e], undo, y); v1.y = fmaf(o[4 * g + 1][nt][2 + e], undo, y);
+        v1.z = fmaf(o[4 * g + 2][nt][2 + e], undo, y); v1.w = fmaf(o[4 * g + 3][nt][2 + e], undo, y);
+        *(float4*)(po + 64 * g + 8 * r) = v0;
+        *(float4*)(po + 64 * g + 8 * r + 4) = v1;
+      }
+    }
+  __syncthreads();
+  const int nrows = min(8 * NT, a.rows - row0);
+  for (int i = threadIdx.x; i < nrows * (D / 4); i += kWarps * 32) {
+    const int row = i / (D / 4), d = (i % (D / 4)) * 4;
+    float mx = -INFINITY, den = 0.f;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) mx = fmaxf(mx, mM[w * 8 * NT + row]);
+    const float ref = mx == -INFINITY ? 0.f : mx;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      const float f = ex2((mM[w * 8 * NT + row] - ref) * kLog2e);
+      const float4 v = *(const float4*)(mO + ((size_t)w * 8 * NT + row) * D + d);
+      den = fmaf(f, mL[w * 8 * NT + row], den);
+      acc.x = fmaf(f, v.x, acc.x); acc.y = fmaf(f, v.y, acc.y);
+      acc.z = fmaf(f, v.z, acc.z); acc.w = fmaf(f, v.w, acc.w);
+    }
+    if (a.splits == 1) {
+      const float inv = den == 0.f ? 1.f : 1.f / den;   // a row that sees nothing yields zeros; NaN stays
+      const T y[4] = {TR::from_float(acc.x * inv), TR::from_float(acc.y * inv), TR::from_float(acc.z * inv), TR::from_float(acc.w * inv)};
+      const float nan = den * 0.f;                       // a NaN sum reaches channels whose own products are finite
+      T z[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) z[e] = nan == 0.f ? y[e] : TR::from_float(nan);
+      *(uint2*)((T*)a.out + out_row(a, b, hk, row0 + row) * D + d) = *(const uint2*)z;
+    } else {
+      const size_t at = ((size_t)bhk * a.rows + row0 + row) * a.splits + split;
+      *(float4*)(a.part_o + at * D + d) = acc;
+      if (d == 0) {
+        a.part_m[at] = mx;
+        a.part_l[at] = den;
+      }
+    }
+  }
+}
+
+// out = sum_s w_s O_s / sum_s w_s l_s, w_s = exp(m_s - max m): one block per row.
+template <typename T, int D>
+__global__ void __launch_bounds__(D / 4 < 64 ? 64 : D / 4) kv4_combine_kernel(const SdpaArgs a) {
+  using TR = MmaTraits<T>;
+  constexpr int kThreads = D / 4 < 64 ? 64 : D / 4, kPer = kThreads / (D / 4);   // key ranges read side by side
+  __shared__ float sw[1024];
+  __shared__ float red[kThreads / 32];
+  __shared__ float4 part[kPer][D / 4];
+  pdl_wait();
+  pdl_trigger();
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const size_t row = (size_t)blockIdx.y * a.rows + blockIdx.x;
+  const float* pm = a.part_m + row * a.splits;
+  const float* pl = a.part_l + row * a.splits;
+  float mx = -INFINITY;
+  for (int s = tid; s < a.splits; s += kThreads) mx = fmaxf(mx, pm[s]);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+  if (lane == 0) red[warp] = mx;
+  __syncthreads();
+  mx = red[0];
+#pragma unroll
+  for (int i = 1; i < kThreads / 32; ++i) mx = fmaxf(mx, red[i]);
+  __syncthreads();
+  const float ref = mx == -INFINITY ? 0.f : mx;
+  float den = 0.f;
+  for (int s = tid; s < a.splits; s += kThreads) {
+    const float w = ex2((pm[s] - ref) * kLog2e);
+    sw[s] = w;
+    den = fmaf(w, pl[s], den);
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) den += __shfl_xor_sync(0xffffffffu, den, o);
+  if (lane == 0) red[warp] = den;
+  __syncthreads();
+  den = red[0];
+#pragma unroll
+  for (int i = 1; i < kThreads / 32; ++i) den += red[i];
+  const int d4 = tid % (D / 4), s0 = tid / (D / 4);
+  const float4* po = (const float4*)(a.part_o + row * a.splits * D) + d4;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+  for (int s = s0; s < a.splits; s += kPer) {
+    const float4 v = po[(size_t)s * (D / 4)];
+    const float w = sw[s];
+    acc.x = fmaf(w, v.x, acc.x); acc.y = fmaf(w, v.y, acc.y);
+    acc.z = fmaf(w, v.z, acc.z); acc.w = fmaf(w, v.w, acc.w);
+  }
+  if (kPer > 1) {
+    part[s0][d4] = acc;
+    __syncthreads();
+    if (s0 != 0) return;
+#pragma unroll
+    for (int i = 1; i < kPer; ++i) {
+      const float4 v = part[i][d4];
+      acc.x += v.x; acc.y += v.y; acc.z += v.z; acc.w += v.w;
+    }
+  }
+  const float inv = den == 0.f ? 1.f : 1.f / den, nan = den * 0.f;
+  const float v[4] = {acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv};
+  T z[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) z[e] = TR::from_float(nan == 0.f ? v[e] : nan);
+  const int b = blockIdx.y / a.Hk, hk = blockIdx.y % a.Hk;
+  *(uint2*)((T*)a.out + out_row(a, b, hk, blockIdx.x) * D + 4 * d4) = *(const uint2*)z;
+}
+
+// ---- host side ---------------------------------------------------------------------------------------------------------
+int row_tile(int rows) { return rows <= 8 ? 1 : 2; }   // 8-row columns of the MMA tile: 16 query rows share one pass
+
+int choose_splits(int units, int max_length, int device, int requested) {
+  // a split is worth its partials from about one 16-key tile per warp on
+  const int most = (max_length + 16 * kWarps - 1) / (16 * kWarps);
+  int s = requested > 0 ? requested : sm_count(device) / (units > 0 ? units : 1);
+  if (s > most) s = most;
+  if (s > 1024) s = 1024;
+  return s < 1 ? 1 : s;
+}
+
+template <typename T, int D, int NT>
+int launch_sdpa(SdpaArgs a, cudaStream_t st, int device) {
+  using TL = Tile<D>;
+  constexpr size_t fixed = (size_t)NT * (D / 16) * 32 * 8 + (size_t)NT * (D / kGroup) * 8 * 4;
+  constexpr size_t merge = (size_t)kWarps * 8 * NT * (D + 2) * 4;
+  constexpr int stages = 3;
+  constexpr size_t ring = (size_t)kWarps * stages * TL::kBytes;
+  constexpr size_t smem = fixed + (ring > merge ? ring : merge);
+  static_assert(smem <= 227 * 1024, "shared memory");
+  auto kern = a.mask_kind ? kv4_sdpa_kernel<T, D, NT, true> : kv4_sdpa_kernel<T, D, NT, false>;
+  static std::mutex mu;
+  static bool done[64][2] = {};
+  {
+    std::lock_guard<std::mutex> lk(mu);
+    bool& d = done[device & 63][a.mask_kind ? 1 : 0];
+    if (!d) {
+      cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+      if (e != cudaSuccess) return fail(DFLASH_ERR_LAUNCH, "kv4_sdpa: cudaFuncSetAttribute: %s", cudaGetErrorString(e));
+      d = true;
+    }
+  }
+  const int row_tiles = (a.rows + 8 * NT - 1) / (8 * NT);
+  cudaError_t e = launch_kernel(kern, dim3(a.splits, row_tiles, a.B * a.Hk), dim3(kWarps * 32), smem, st, a, stages);
+  if (e == cudaSuccess) e = cudaGetLastError();
+  if (e != cudaSuccess) return fail(DFLASH_ERR_LAUNCH, "kv4_sdpa launch: %s", cudaGetErrorString(e));
+  if (a.splits > 1) {
+    e = launch_kernel(kv4_combine_kernel<T, D>, dim3(a.rows, a.B * a.Hk), dim3(D / 4 < 64 ? 64 : D / 4), 0, st, a);
+    if (e == cudaSuccess) e = cudaGetLastError();
+    if (e != cudaSuccess) return fail(DFLASH_ERR_LAUNCH, "kv4_sdpa combine launch: %s", cudaGetErrorString(e));
+  }
+  return DFLASH_OK;
+}
+
+template <typename T>
+int launch_typed(const SdpaArgs& a, int D, cudaStream_t st, int device) {
+  if (row_tile(a.rows) == 1) return D == 128 ? launch_sdpa<T, 128, 1>(a, st, device) : launch_sdpa<T, 256, 1>(a, st, device);
+  return D == 128 ? launch_sdpa<T, 128, 2>(a, st, device) : launch_sdpa<T, 256, 2>(a, st, device);
+}
+
+int check_cache(const char* who, const dflash_kv4_cache* c, int D) {
+  if (!c || !c->codes || !c->scales || !c->biases) return fail(DFLASH_ERR_BAD_ARG, "%s: null cache array", who);
+  const int row = D / kGroup;
+  if (((uintptr_t)c->codes & 15) || ((uintptr_t)c->scales & (2 * row - 1)) || ((uintptr_t)c->biases & (2 * row - 1)) ||
+      (c->codes_batch_stride & 3) || (c->codes_head_stride & 3) || c->scales_batch_stride % row || c->scales_head_stride % row ||
+      c->biases_batch_stride % row || c->biases_head_stride % row)
+    return fail(DFLASH_ERR_MISALIGNED, "%s: cache arrays must be aligned to 16 bytes (codes) and to a row (scales, biases)", who);
+  return DFLASH_OK;
+}
+
+int check_sizes(const char* who, int B, int Hk, int T, int D, int capacity, int dtype) {
+  if (B < 0 || Hk < 1 || T < 0) return fail(DFLASH_ERR_BAD_SHAPE, "%s: bad sizes B=%d Hk=%d T=%d", who, B, Hk, T);
+  if (D != 128 && D != 256) return fail(DFLASH_ERR_BAD_SHAPE, "%s: D=%d not in {128,256}", who, D);
+  if (capacity < 1) return fail(DFLASH_ERR_BAD_SHAPE, "%s: capacity %d", who, capacity);
+  if (dtype != DFLASH_BF16 && dtype != DFLASH_F16) return fail(DFLASH_ERR_BAD_ARG, "%s: dtype %d (want bf16 or f16)", who, dtype);
+  return DFLASH_OK;
+}
+
+bool aligned_rows(const void* p, const long long* s) {
+  return !((uintptr_t)p & 15) && s[0] % 8 == 0 && s[1] % 8 == 0 && s[2] % 8 == 0;
+}
+
+// Rows of a warp at once: one while the blocks do not fill the SMs (latency), four for long inputs (loads in flight).
+constexpr int kManyRows = 4;
+
+}  // namespace
+}  // namespace kv4
+}  // namespace dflash
+
+using namespace dflash;
+using namespace dflash::kv4;
+
+extern "C" int dflash_kv4_write(const void* keys, const long long* key_strides, const void* values,
+                                const long long* value_strides, const dflash_kv4_cache* k_cache,
+                                const dflash_kv4_cache* v_cache, const int* offsets, const int* counts, int B, int Hk, int T,
+                                int D, int capacity, int dtype, void* stream) {
+  int rc = check_sizes("kv4_write", B, Hk, T, D, capacity, dtype);
+  if (rc) return rc;
+  if (B == 0 || T == 0) return DFLASH_OK;
+  if (!keys || !values || !key_strides || !value_strides || !offsets) return fail(DFLASH_ERR_BAD_ARG, "kv4_write: null operand");
+  if ((rc = check_cache("kv4_write", k_cache, D)) || (rc = check_cache("kv4_write", v_cache, D))) return rc;
+  if (!aligned_rows(keys, key_strides) || !aligned_rows(values, value_strides))
+    return fail(DFLASH_ERR_MISALIGNED, "kv4_write: keys and values need 16-byte aligned rows");
+  WriteArgs a{};
+  a.x[0] = keys; a.x[1] = values;
+  for (int i = 0; i < 2; ++i) {
+    const long long* s = i ? value_strides : key_strides;
+    a.sb[i] = s[0]; a.sh[i] = s[1]; a.st[i] = s[2];
+    a.c[i] = i ? *v_cache : *k_cache;
+  }
+  a.offsets = offsets; a.counts = counts; a.Hk = Hk; a.T = T; a.capacity = capacity;
+  a.rows = (long long)B * Hk * T;
+  int device = 0;
+  cudaGetDevice(&device);
+  int* err = device_error_word(device);
+  if (!err) return fail(DFLASH_ERR_LAUNCH, "kv4_write: no device error word");
+  const int per = D == 128 ? 8 : 4;   // rows of a block of four warps
+  const bool many = a.rows >= (long long)per * kManyRows * sm_count(device);
+  const long long blocks = (a.rows + (long long)per * (many ? kManyRows : 1) - 1) / (per * (many ? kManyRows : 1));
+  if (blocks > 0x7fffffffll) return fail(DFLASH_ERR_BAD_SHAPE, "kv4_write: too many rows");
+  const dim3 grid((unsigned)blocks, 2), block(128);
+  cudaStream_t st = (cudaStream_t)stream;
+  auto go = [&](auto one, auto four) { return many ? launch_kernel(four, grid, block, 0, st, a, err) : launch_kernel(one, grid, block, 0, st, a, err); };
+  cudaError_t e;
+  if (dtype == DFLASH_BF16)
+    e = D == 128 ? go(kv4_write_kernel<__nv_bfloat16, 128, 1>, kv4_write_kernel<__nv_bfloat16, 128, kManyRows>)
+                 : go(kv4_write_kernel<__nv_bfloat16, 256, 1>, kv4_write_kernel<__nv_bfloat16, 256, kManyRows>);
+  else
+    e = D == 128 ? go(kv4_write_kernel<__half, 128, 1>, kv4_write_kernel<__half, 128, kManyRows>)
+                 : go(kv4_write_kernel<__half, 256, 1>, kv4_write_kernel<__half, 256, kManyRows>);
+  if (e == cudaSuccess) e = cudaGetLastError();
+  return e == cudaSuccess ? DFLASH_OK : fail(DFLASH_ERR_LAUNCH, "kv4_write launch: %s", cudaGetErrorString(e));
+}
+
+extern "C" int dflash_kv4_read(const dflash_kv4_cache* k_cache, const dflash_kv4_cache* v_cache, void* keys_out,
+                               void* values_out, const int* starts, int start, int B, int Hk, int T, int D, int capacity,
+                               int dtype, void* stream) {
+  int rc = check_sizes("kv4_read", B, Hk, T, D, capacity, dtype);
+  if (rc) return rc;
+  if (B == 0 || T == 0) return DFLASH_OK;
+  if (!keys_out) return fail(DFLASH_ERR_BAD_ARG, "kv4_read: null operand");
+  if ((rc = check_cache("kv4_read", k_cache, D)) || (values_out && (rc = check_cache("kv4_read", v_cache, D)))) return rc;
+  if (((uintptr_t)keys_out & 15) || ((uintptr_t)values_out & 15)) return fail(DFLASH_ERR_MISALIGNED, "kv4_read: outputs must be 16-byte aligned");
+  ReadArgs a{};
+  a.c[0] = *k_cache;
+  if (values_out) a.c[1] = *v_cache;
+  a.out[0] = keys_out; a.out[1] = values_out;
+  a.starts = starts; a.start = start; a.Hk = Hk; a.T = T; a.capacity = capacity;
+  a.rows = (long long)B * Hk * T;
+  int device = 0;
+  cudaGetDevice(&device);
+  const int per = D == 128 ? 8 : 4;
+  const bool many = a.rows >= (long long)per * kManyRows * sm_count(device);
+  const long long blocks = (a.rows + (long long)per * (many ? kManyRows : 1) - 1) / (per * (many ? kManyRows : 1));
+  if (blocks > 0x7fffffffll) return fail(DFLASH_ERR_BAD_SHAPE, "kv4_read: too many rows");
+  const dim3 grid((unsigned)blocks, values_out ? 2 : 1), block(128);
+  cudaStream_t st = (cudaStream_t)stream;
+  auto go = [&](auto one, auto four) { return many ? launch_kernel(four, grid, block, 0, st, a) : launch_kernel(one, grid, block, 0, st, a); };
+  cudaError_t e;
+  if (dtype == DFLASH_BF16)
+    e = D == 128 ? go(kv4_read_kernel<__nv_bfloat16, 128, 1>, kv4_read_kernel<__nv_bfloat16, 128, kManyRows>)
+                 : go(kv4_read_kernel<__nv_bfloat16, 256, 1>, kv4_read_kernel<__nv_bfloat16, 256, kManyRows>);
+  else
+    e = D == 128 ? go(kv4_read_kernel<__half, 128, 1>, kv4_read_kernel<__half, 128, kManyRows>)
+                 : go(kv4_read_kernel<__half, 256, 1>, kv4_read_kernel<__half, 256, kManyRows>);
+  if (e == cudaSuccess) e = cudaGetLastError();
+  return e == cudaSuccess ? DFLASH_OK : fail(DFLASH_ERR_LAUNCH, "kv4_read launch: %s", cudaGetErrorString(e));
+}
+
+static int kv4_splits(int B, int Hk, long long rows, int max_length, int device, int num_splits) {
+  const long long units = (long long)B * Hk * ((rows + 8 * row_tile((int)rows) - 1) / (8 * row_tile((int)rows)));
+  return choose_splits((int)(units > 65535 ? 65535 : units), max_length, device, num_splits);
+}
+
+extern "C" size_t dflash_kv4_sdpa_workspace_bytes(int B, int Hq, int Hk, int T, int D, int max_length, int num_splits) {
+  if (B < 1 || Hq < 1 || Hk < 1 || T < 1 || D < 1 || max_length < 1 || Hq % Hk != 0 || (long long)(Hq / Hk) * T > 0x7fffffffll) return 0;
+  int device = 0;
+  cudaGetDevice(&device);
+  const long long rows = (long long)(Hq / Hk) * T;
+  const int splits = kv4_splits(B, Hk, rows, max_length, device, num_splits);
+  return splits > 1 ? (size_t)B * Hk * rows * splits * (D + 2) * sizeof(float) : 0;
+}
+
+extern "C" int dflash_kv4_sdpa(const void* q, const long long* q_strides, const dflash_kv4_cache* k_cache,
+                               const dflash_kv4_cache* v_cache, const void* mask, int mask_kind, const long long* mask_strides,
+                               void* out, const int* lengths, int B, int Hq, int Hk, int T, int D, int capacity, int max_length,
+                               float scale, int dtype, int num_splits, void* workspace, size_t workspace_bytes, void* stream) {
+  int rc = check_sizes("kv4_sdpa", B, Hk, T, D, capacity, dtype);
+  if (rc) return rc;
+  if (Hq < 1 || Hq % Hk != 0) return fail(DFLASH_ERR_BAD_SHAPE, "kv4_sdpa: %d query heads on %d KV heads", Hq, Hk);
+  if (max_length < 0 || max_length > capacity) return fail(DFLASH_ERR_BAD_SHAPE, "kv4_sdpa: max_length %d outside 0..%d", max_length, capacity);
+  if (B == 0 || T == 0) return DFLASH_OK;
+  if (!q || !q_strides || !out) return fail(DFLASH_ERR_BAD_ARG, "kv4_sdpa: null operand");
+  if (mask_kind < 0 || mask_kind > 3 || (mask_kind != 0) != (mask != nullptr) || (mask_kind && !mask_strides))
+    return fail(DFLASH_ERR_BAD_ARG, "kv4_sdpa: mask and mask_kind %d do not agree", mask_kind);
+  if ((rc = check_cache("kv4_sdpa", k_cache, D)) || (rc = check_cache("kv4_sdpa", v_cache, D))) return rc;
+  if (!aligned_rows(q, q_strides) || ((uintptr_t)out & 15)) return fail(DFLASH_ERR_MISALIGNED, "kv4_sdpa: q and out need 16-byte aligned rows");
+  const long long rows = (long long)(Hq / Hk) * T;
+  if ((long long)B * Hk > 65535 || rows > 1000000) return fail(DFLASH_ERR_BAD_SHAPE, "kv4_sdpa: B*Hk=%lld or rows per KV head %lld too large", (long long)B * Hk, rows);
+  int device = 0;
+  cudaGetDevice(&device);
+  SdpaArgs a{};
+  a.q = q; a.q_sb = q_strides[0]; a.q_sh = q_strides[1]; a.q_st = q_strides[2];
+  a.k = *k_cache; a.v = *v_cache;
+  a.mask = mask; a.mask_kind = mask_kind;
+  if (mask_kind) { a.m_sb = mask_strides[0]; a.m_sh = mask_strides[1]; a.m_st = mask_strides[2]; a.m_sn = mask_strides[3]; }
+  a.out = out; a.lengths = lengths;
+  a.B = B; a.Hq = Hq; a.Hk = Hk; a.gqa = Hq / Hk; a.T = T; a.rows = (int)rows;
+  a.max_length = max_length; a.scale = scale;
+  a.splits = kv4_splits(B, Hk, rows, max_length > 0 ? max_length : 1, device, num_splits);
+  if (a.splits > 1) {
+    const size_t n = (size_t)B * Hk * rows * a.splits, need = n * (D + 2) * sizeof(float);
+    if (!workspace || workspace_bytes < need) return fail(DFLASH_ERR_WORKSPACE, "kv4_sdpa needs %zu workspace bytes, got %zu", need, workspace_bytes);
+    if ((uintptr_t)workspace & 15) return fail(DFLASH_ERR_MISALIGNED, "kv4_sdpa workspace must be 16-byte aligned");
+    a.part_o = (float*)workspace;
+    a.part_m = a.part_o + n * D;
+    a.part_l = a.part_m + n;
+  }
+  cudaStream_t st = (cudaStream_t)stream;
+  return dtype == DFLASH_BF16 ? launch_typed<__nv_bfloat16>(a, D, st, device) : launch_typed<__half>(a, D, st, device);
+}

@@ -1,0 +1,362 @@
+// Log-probabilities of given tokens, entropy and the top alternatives of every row of logits, in one pass over the logits.
+//
+//   m = max x,  L = sum exp((x - m) / T),  W = sum (x - m) exp((x - m) / T)
+//   log p[token] = (x[token] - m) / T - ln L,   entropy = ln L - W / (L T)
+// Every thread sums relative to the maximum of its own elements and the (m, L, W) triples are merged in a fixed tree
+// (L' = L exp((m - m') / T), W' = (W + (m - m') L) exp((m - m') / T)), so the result does not depend on timing.
+//
+// Top alternatives: 64 groups of threads give 64 maxima; at least top_k elements are >= the top_k-th largest of them, and only
+// those (a few dozen of tens of thousands) are collected and ranked by counting.  Keys are (value, lower index first) and
+// therefore unique.  When more are collected than the list holds (a row of equal values, sorted logits) the top_k-th largest key is
+// found bit by bit instead.
+//
+// One row per thread-block cluster: every block keeps its share of the row in registers (16-byte loads, all issued before the
+// first is used), the first block merges the triples and the blocks' lists through distributed shared memory.  Bound by HBM
+// for many rows; one row is bound by the launch, one memory round trip and the merges.
+#include <cooperative_groups.h>
+
+#include <mutex>
+
+#include "common.cuh"
+
+namespace dflash {
+namespace lp {
+namespace {
+
+constexpr int kThreads = 512, kGroups = 64, kMaxK = 32, kList = 1024;
+constexpr float kLog2e = 1.4426950408889634f;
+
+struct Args {
+  const void* logits;
+  long long ld;
+  const int* tokens;
+  const uint8_t* suppress;
+  float* token_logprob;
+  float* entropy;
+  float* top_logprobs;
+  int* top_ids;
+  float temperature, scale;   // scale = log2(e) / temperature
+  int V, k;
+};
+
+template <typename T> struct Elem;
+template <> struct Elem<float> {
+  static constexpr int kPer = 4, kSlots = 10;
+  static constexpr uint32_t kNegInf = 0xFF800000u;
+  __device__ static __forceinline__ float get(const uint32_t (&w)[4], int e) { return __uint_as_float(w[e]); }
+  __device__ static __forceinline__ void hide(uint32_t (&w)[4], int e) { w[e] = kNegInf; }
+  __device__ static __forceinline__ void put(uint32_t (&w)[4], int e, const float* p) { w[e] = __float_as_uint(*p); }
+  __device__ static __forceinline__ float load(const float* p) { return *p; }
+};
+template <typename T, uint32_t kInf> struct Elem16 {
+  static constexpr int kPer = 8, kSlots = 5;
+  __device__ static __forceinline__ float get(const uint32_t (&w)[4], int e) {
+    return MmaTraits<T>::bits_to_float((uint16_t)(w[e >> 1] >> (16 * (e & 1))));
+  }
+  __device__ static __forceinline__ void put_bits(uint32_t (&w)[4], int e, uint32_t bits) {
+    w[e >> 1] = (e & 1) ? ((w[e >> 1] & 0xFFFFu) | (bits << 16)) : ((w[e >> 1] & 0xFFFF0000u) | bits);
+  }
+  __device__ static __forceinline__ void hide(uint32_t (&w)[4], int e) { put_bits(w, e, kInf); }
+  __device__ static __forceinline__ void put(uint32_t (&w)[4], int e, const T* p) { put_bits(w, e, *(const uint16_t*)p); }
+  __device__ static __forceinline__ float load(const T* p) { return MmaTraits<T>::to_float(*p); }
+};
+template <> struct Elem<__nv_bfloat16> : Elem16<__nv_bfloat16, 0xFF80u> {};
+template <> struct Elem<__half> : Elem16<__half, 0xFC00u> {};
+
+struct Sums { float m, l, w; };
+__device__ __forceinline__ Sums merge(const Sums& a, const Sums& b, float scale) {
+  Sums s;
+  s.m = fmaxf(a.m, b.m);
+  // a side without a maximum has sums of zero (or NaN, which stays): it needs no factor
+  const float da = a.m == -INFINITY ? 0.f : a.m - s.m, db = b.m == -INFINITY ? 0.f : b.m - s.m;
+  const float fa = exp2f(da * scale), fb = exp2f(db * scale);
+  s.l = a.l * fa + b.l * fb;
+  // a vanished side must not turn an infinite distance into NaN
+  s.w = (fa == 0.f ? 0.f : fmaf(da, a.l, a.w) * fa) + (fb == 0.f ? 0.f : fmaf(db, b.l, b.w) * fb);
+  return s;
+}
+__device__ __forceinline__ unsigned long long key_of(float v, int index) {
+  const uint32_t u = __float_as_uint(__fadd_rn(v, 0.f));   // -0 and +0 are one value
+  const uint32_t o = u ^ ((u >> 31) ? 0xFFFFFFFFu : 0x80000000u);
+  return ((unsigned long long)o << 32) | (uint32_t)~(uint32_t)index;
+}
+__device__ __forceinline__ float key_value(unsigned long long k) {
+  const uint32_t o = (uint32_t)(k >> 32);
+  return __uint_as_float(o ^ ((o >> 31) ? 0x80000000u : 0xFFFFFFFFu));
+}
+__device__ __forceinline__ int key_index(unsigned long long k) { return (int)~(uint32_t)k; }
+
+struct Shared {
+  Sums warp_sums[kThreads / 32];
+  Sums block_sums;
+  float group_max[kGroups];
+  float tau;
+  int count;
+  unsigned long long list[kList];
+  unsigned long long top[kMaxK];                  // this block's best, highest first; 0 = none
+  unsigned long long gathered[8 * kMaxK];         // first block of a cluster: every block's `top`
+  int counts[2][kThreads / 32];
+};
+
+// The `k` largest of list[0..n) in order; keys are unique, 0 marks an empty place and is skipped.
+__device__ __forceinline__ void rank_into(unsigned long long* top, const unsigned long long* list, int n, int k) {
+  for (int i = threadIdx.x; i < n; i += kThreads) {
+    const unsigned long long mine = list[i];
+    if (mine == 0) continue;
+    int rank = 0;
+    for (int j = 0; j < n && rank < k; ++j) rank += list[j] > mine;
+    if (rank < k) top[rank] = mine;
+  }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads, 2) token_logprobs_kernel(const Args a) {
+  namespace cg = cooperative_groups;
+  using E = Elem<T>;
+  constexpr int kPer = E::kPer, kSlots = E::kSlots;
+  __shared__ Shared sh;
+  cg::cluster_group cluster = cg::this_cluster();
+  const int blocks = (int)cluster.num_blocks(), me = (int)cluster.block_rank();
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const long long row = blockIdx.x / blocks;
+  pdl_wait();
+  pdl_trigger();
+  const T* x = (const T*)a.logits + row * a.ld;
+  // 16-byte vectors from the aligned address at or before the row; the first and last are loaded element by element
+  const int skew = (int)(((uintptr_t)x & 15) / sizeof(T));
+  const int vecs = (skew + a.V + kPer - 1) / kPer;
+  const int share = (vecs + blocks - 1) / blocks;
+  const int v0 = me * share, v1 = min(vecs, v0 + share);
+  Sums sums = {-INFINITY, 0.f, 0.f};
+  if (tid < kMaxK) sh.top[tid] = 0;
+  for (int base = v0; base < v1; base += kThreads * kSlots) {
+    uint32_t raw[kSlots][4];
+#pragma unroll
+    for (int s = 0; s < kSlots; ++s) {
+      const int v = base + s * kThreads + tid;
+      const int i0 = v * kPer - skew;
+      if (v < v1 && i0 >= 0 && i0 + kPer <= a.V) {
+        const uint4 u = __ldcs((const uint4*)(x + i0));
+        raw[s][0] = u.x; raw[s][1] = u.y; raw[s][2] = u.z; raw[s][3] = u.w;
+      } else {
+#pragma unroll
+        for (int e = 0; e < kPer; ++e) {
+          if (v < v1 && i0 + e >= 0 && i0 + e < a.V) E::put(raw[s], e, x + i0 + e);
+          else E::hide(raw[s], e);
+        }
+      }
+    }
+    if (a.suppress != nullptr) {
+#pragma unroll
+      for (int s = 0; s < kSlots; ++s) {
+        const int v = base + s * kThreads + tid;
+        const int i0 = v * kPer - skew;
+        if (v < v1) {
+#pragma unroll
+          for (int e = 0; e < kPer; ++e)
+            if (i0 + e >= 0 && i0 + e < a.V && a.suppress[i0 + e]) E::hide(raw[s], e);
+        }
+      }
+    }
+    Sums mine = {-INFINITY, 0.f, 0.f};
+#pragma unroll
+    for (int s = 0; s < kSlots; ++s)
+#pragma unroll
+      for (int e = 0; e < kPer; ++e) mine.m = fmaxf(mine.m, E::get(raw[s], e));
+    const float ref = mine.m == -INFINITY ? 0.f : mine.m;
+#pragma unroll
+    for (int s = 0; s < kSlots; ++s)
+#pragma unroll
+      for (int e = 0; e < kPer; ++e) {
+        const float d = E::get(raw[s], e) - ref;
+        const float p = exp2f(d * a.scale);
+        mine.l += p;
+        mine.w = fmaf(fmaxf(d, -1e30f), p, mine.w);   // a hidden element adds 0, not -inf * 0; NaN stays through p
+      }
+    if (a.k > 0) {
+      // ---- candidates of this pass: everything >= the k-th largest group maximum ----
+      float g = mine.m;
+#pragma unroll
+      for (int o = 1; o < 8; o <<= 1) g = fmaxf(g, __shfl_xor_sync(0xffffffffu, g, o));
+      if ((lane & 7) == 0) sh.group_max[warp * 4 + (lane >> 3)] = g;
+      if (tid == 0) sh.count = 0;
+      __syncthreads();
+      if (warp == 0) {
+        const float g0 = sh.group_max[lane], g1 = sh.group_max[lane + 32];
+        int r0 = 0, r1 = 0;
+#pragma unroll 8
+        for (int i = 0; i < kGroups; ++i) {
+          const float o = sh.group_max[i];
+          r0 += o > g0 || (o == g0 && i < lane);
+          r1 += o > g1 || (o == g1 && i < lane + 32);
+        }
+        if (r0 == a.k - 1) sh.tau = g0;
+        if (r1 == a.k - 1) sh.tau = g1;
+      }
+      __syncthreads();
+      const float tau = sh.tau;
+      // NaN elements count as the largest; a thread whose own maximum is below tau can only hold NaN beyond it
+      if (mine.m >= tau || !(mine.l == mine.l)) {
+#pragma unroll
+        for (int s = 0; s < kSlots; ++s)
+#pragma unroll
+          for (int e = 0; e < kPer; ++e) {
+            const float v = E::get(raw[s], e);
+            const int i = (base + s * kThreads + tid) * kPer - skew + e;
+            if (!(v < tau) && base + s * kThreads + tid < v1 && i >= 0 && i < a.V) {
+              const int at = atomicAdd(&sh.count, 1);
+              if (at < kList - kMaxK) sh.list[at] = key_of(v, i);
+            }
+          }
+      }
+      __syncthreads();
+      const int n = sh.count;
+      if (n <= kList - kMaxK) {
+        if (tid < kMaxK) {   // the best of the earlier passes compete again
+          sh.list[n + tid] = sh.top[tid];
+        }
+        __syncthreads();
+        if (tid < kMaxK) sh.top[tid] = 0;
+        __syncthreads();
+        rank_into(sh.top, sh.list, n + kMaxK, a.k);
+      } else {
+        // too many at or above tau (ties, sorted logits): the k-th largest key bit by bit, then exactly the keys from it on
+        const unsigned long long earlier = tid < kMaxK ? sh.top[tid] : 0ull;
+        unsigned long long kth = 0;
+#pragma unroll 1
+        for (int bit = 63; bit >= 0; --bit) {
+          const unsigned long long t = kth | (1ull << bit);
+          int n_at = earlier >= t;
+#pragma unroll
+          for (int s = 0; s < kSlots; ++s)
+#pragma unroll
+            for (int e = 0; e < kPer; ++e) {
+              const int v = base + s * kThreads + tid, i = v * kPer - skew + e;
+              n_at += v < v1 && i >= 0 && i < a.V && key_of(E::get(raw[s], e), i) >= t;
+            }
+          n_at = __reduce_add_sync(0xffffffffu, n_at);
+          if (lane == 0) sh.counts[bit & 1][warp] = n_at;
+          __syncthreads();
+          n_at = __reduce_add_sync(0xffffffffu, lane < kThreads / 32 ? sh.counts[bit & 1][lane] : 0);
+          if (n_at >= a.k) kth = t;
+        }
+        if (tid == 0) sh.count = 0;
+        if (tid < kMaxK) sh.top[tid] = 0;
+        __syncthreads();
+        // kth = 0: fewer than k elements so far, all of them stay
+        if (earlier >= kth && earlier != 0) sh.list[atomicAdd(&sh.count, 1)] = earlier;
+#pragma unroll
+        for (int s = 0; s < kSlots; ++s)
+#pragma unroll
+          for (int e = 0; e < kPer; ++e) {
+            const int v = base + s * kThreads + tid, i = v * kPer - skew + e;
+            if (v < v1 && i >= 0 && i < a.V) {
+              const unsigned long long q = key_of(E::get(raw[s], e), i);
+              if (q >= kth) sh.list[atomicAdd(&sh.count, 1)] = q;
+            }
+          }
+        __syncthreads();
+        rank_into(sh.top, sh.list, sh.count, a.k);
+      }
+      __syncthreads();
+    }
+    sums = merge(sums, mine, a.scale);
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    const Sums other = {__shfl_xor_sync(0xffffffffu, sums.m, o), __shfl_xor_sync(0xffffffffu, sums.l, o),
+                        __shfl_xor_sync(0xffffffffu, sums.w, o)};
+    // the lower lane's triple first: both partners then compute the same bits
+    sums = (lane & o) ? merge(other, sums, a.scale) : merge(sums, other, a.scale);
+  }
+  if (lane == 0) sh.warp_sums[warp] = sums;
+  __syncthreads();
+  if (tid == 0) {
+    Sums all = sh.warp_sums[0];
+    for (int i = 1; i < kThreads / 32; ++i) all = merge(all, sh.warp_sums[i], a.scale);
+    sh.block_sums = all;
+  }
+  cluster.sync();
+  if (me == 0) {
+    Sums all = sh.block_sums;
+    for (int i = 1; i < blocks; ++i) all = merge(all, *cluster.map_shared_rank(&sh.block_sums, i), a.scale);
+    if (a.k > 0) {
+      for (int i = tid; i < blocks * kMaxK; i += kThreads)
+        sh.gathered[i] = cluster.map_shared_rank(&sh.top[0], i / kMaxK)[i % kMaxK];
+      __syncthreads();
+      if (blocks > 1) {
+        rank_into(sh.list, sh.gathered, blocks * kMaxK, a.k);   // list: free again
+        __syncthreads();
+      } else {
+        if (tid < kMaxK) sh.list[tid] = sh.top[tid];
+        __syncthreads();
+      }
+    }
+    const bool empty = all.m == -INFINITY && all.l == 0.f;   // nothing but -inf
+    if (tid <= a.k) {
+      // tid 0: the given token and the entropy; tid 1..k: an alternative each.  ln L in double: a peaked row has L = 1 + eps
+      const double log_l = log((double)all.l);
+      float value;
+      bool in_range = true;
+      if (tid == 0) {
+        const int token = a.tokens[row];
+        in_range = token >= 0 && token < a.V;
+        value = !in_range || (a.suppress != nullptr && a.suppress[token]) ? -INFINITY : E::load(x + token);
+      } else {
+        value = key_value(sh.list[tid - 1]);
+      }
+      float out = empty ? -INFINITY : (float)((double)(value - all.m) / (double)a.temperature - log_l);
+      if (!in_range) out = __int_as_float(0x7FC00000);
+      if (tid == 0) {
+        a.token_logprob[row] = out;
+        if (a.entropy != nullptr)
+          a.entropy[row] = empty ? 0.f : (float)(log_l - (double)all.w / ((double)all.l * (double)a.temperature));
+      } else {
+        a.top_logprobs[row * a.k + tid - 1] = out;
+        a.top_ids[row * a.k + tid - 1] = key_index(sh.list[tid - 1]);
+      }
+    }
+  }
+  cluster.sync();   // the first block has read the others' shared memory
+}
+
+template <typename T>
+int launch(const Args& a, int R, cudaStream_t st, int device) {
+  // a block holds kThreads * kSlots vectors at once; with few rows the cluster grows while a block keeps 2048 elements
+  const int hold = kThreads * Elem<T>::kSlots * Elem<T>::kPer;
+  int c = 1;
+  while (c < 8 && ((long long)c * hold < a.V || ((long long)R * c < sm_count(device) && a.V >= 2 * c * 2048))) c <<= 1;
+  if ((long long)R * c > 0x7fffffffll) return fail(DFLASH_ERR_BAD_SHAPE, "token_logprobs: too many rows");
+  cudaError_t e = launch_kernel_cluster(token_logprobs_kernel<T>, dim3((unsigned)R * c), dim3(kThreads), c, 0, st, a);
+  if (e == cudaSuccess) e = cudaGetLastError();
+  return e == cudaSuccess ? DFLASH_OK : fail(DFLASH_ERR_LAUNCH, "token_logprobs launch: %s", cudaGetErrorString(e));
+}
+
+}  // namespace
+}  // namespace lp
+}  // namespace dflash
+
+using namespace dflash;
+
+extern "C" int dflash_token_logprobs(const void* logits, long long ld, const int* tokens, const uint8_t* suppress, float temperature,
+                                     float* token_logprob, float* entropy, float* top_logprobs, int* top_ids, int R, int V,
+                                     int top_k, int dtype, void* stream) {
+  if (R < 0 || V < 1 || ld < V) return fail(DFLASH_ERR_BAD_SHAPE, "token_logprobs: R=%d V=%d ld=%lld", R, V, ld);
+  if (V > 0x7fffffff - 64 * 1024) return fail(DFLASH_ERR_BAD_SHAPE, "token_logprobs: V=%d too large", V);
+  if (top_k < 0 || top_k > lp::kMaxK || top_k > V) return fail(DFLASH_ERR_BAD_SHAPE, "token_logprobs: top_k=%d outside 0..min(%d, V)", top_k, lp::kMaxK);
+  if (!(temperature > 0.f) || !(temperature <= 3.0e38f)) return fail(DFLASH_ERR_BAD_ARG, "token_logprobs: temperature must be positive and finite");
+  if (R == 0) return DFLASH_OK;
+  if (!logits || !tokens || !token_logprob || (top_k > 0 && (!top_logprobs || !top_ids))) return fail(DFLASH_ERR_BAD_ARG, "token_logprobs: null operand");
+  const int size = dtype == DFLASH_F32 ? 4 : 2;
+  if ((uintptr_t)logits % size) return fail(DFLASH_ERR_MISALIGNED, "token_logprobs: logits are not aligned to their type");
+  lp::Args a{logits, ld, tokens, suppress, token_logprob, entropy, top_logprobs, top_ids, temperature, lp::kLog2e / temperature, V, top_k};
+  int device = 0;
+  cudaGetDevice(&device);
+  cudaStream_t st = (cudaStream_t)stream;
+  switch (dtype) {
+    case DFLASH_BF16: return lp::launch<__nv_bfloat16>(a, R, st, device);
+    case DFLASH_F16: return lp::launch<__half>(a, R, st, device);
+    case DFLASH_F32: return lp::launch<float>(a, R, st, device);
+  }
+  return fail(DFLASH_ERR_BAD_ARG, "token_logprobs: dtype %d", dtype);
+}

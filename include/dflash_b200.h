@@ -383,6 +383,75 @@ DFLASH_API int dflash_moe_qmm_fused(const void* x, const void* w_q, const void* 
                                     void* workspace, size_t workspace_bytes, void* stream);
 
 /* ---------------------------------------------------------------------------------------------
+ * 4-bit KV cache: quantising keys and values as they are written, reading them back, and attention over the codes.
+ * The layout is that of the packed weights above and of mlx-lm's quantised cache (the cache class the reference tests
+ * for, dflash_mlx/runtime.py:671-676): per position and KV head the D channels are D/8 words (nibble i of word j is
+ * channel 8j+i) with one scale and one bias per 64 channels; a channel stands for code * scale + bias.
+ * One struct describes the keys' or the values' side.  Element (b,h,n) of an array starts at b*batch_stride +
+ * h*head_stride + n*row, row = D/8 words or D/64 scales; strides in words (codes) or elements (scales, biases).
+ * Codes are 16-byte aligned with strides that are multiples of 4 words; scales and biases are aligned to a row (D/64
+ * elements), strides multiples of it. */
+typedef struct dflash_kv4_cache {
+  uint32_t* codes;
+  void* scales;
+  void* biases;
+  long long codes_batch_stride, codes_head_stride;
+  long long scales_batch_stride, scales_head_stride;
+  long long biases_batch_stride, biases_head_stride;
+} dflash_kv4_cache;
+/* Quantises T new rows per sequence and KV head and stores them at positions offsets[b] + t (offsets: device int[B]).
+ *   keys, values  dtype; element (b,h,t,d) at b*strides[0] + h*strides[1] + t*strides[2] + d, strides in elements and
+ *                 multiples of 8, bases 16-byte aligned
+ *   counts        device int[B] or NULL: only the first counts[b] rows of sequence b are stored (clamped to 0..T)
+ *   scale = dtype(max/15 - min/15), bias = min, code = clamp(round((x - bias) / scale), 0, 15) per 64 channels (ties to
+ *   even; scale 0: code 0).  A group that holds a NaN or an infinity is stored as scale = bias = NaN, code 0: it reads back as
+ *   NaN.  A row whose position is outside [0, capacity) is NOT stored and sets device error 61 | (t << 8).
+ *   D in {128,256}; dtype bf16 or f16.  B = 0 or T = 0 does nothing. */
+DFLASH_API int dflash_kv4_write(const void* keys, const long long* key_strides, const void* values,
+                                const long long* value_strides, const dflash_kv4_cache* k_cache,
+                                const dflash_kv4_cache* v_cache, const int* offsets, const int* counts, int B, int Hk, int T,
+                                int D, int capacity, int dtype, void* stream);
+/* Reads positions start[b] .. start[b]+T-1 back: keys_out / values_out dtype [B,Hk,T,D] contiguous, 16-byte aligned,
+ * = dtype(code * scale + bias).  starts: device int[B], or NULL for the same `start` in every sequence.  Positions outside
+ * [0, capacity) read as zero.  `values_out` (with v_cache) may be NULL. */
+DFLASH_API int dflash_kv4_read(const dflash_kv4_cache* k_cache, const dflash_kv4_cache* v_cache, void* keys_out,
+                               void* values_out, const int* starts, int start, int B, int Hk, int T, int D, int capacity,
+                               int dtype, void* stream);
+/* Softmax attention of T query positions per sequence over the cache, T >= 1.
+ *   q        dtype, element (b,h,t,d) at b*strides[0] + h*strides[1] + t*strides[2] + d (multiples of 8, 16-byte aligned)
+ *   out      dtype [B,Hq,T,D] contiguous, 16-byte aligned;  head hq reads KV head hq / (Hq/Hk)
+ *   lengths  device int[B] = positions sequence b holds, the T queries' own among them, or NULL: max_length for all.
+ *            Row t of sequence b sees position n iff n <= lengths[b] - T + t, n < lengths[b], n < max_length.
+ *   max_length <= capacity bounds the lengths (the launch geometry and the workspace are those of max_length, so one
+ *            captured graph serves every length up to it); positions from max_length on are never read.
+ *   mask     element (b,h,t,n) at the four strides (elements; 0 broadcasts); mask_kind 0 = none, 1 = bytes (0 hides),
+ *            2 = additive in dtype, 3 = additive f32.  -inf hides; a finite value, however low, is added.
+ *   A row that sees nothing yields zeros.  Keys and values that a row does not see never reach it, NaN and infinities
+ *   included; a visible value row with a non-finite scale or bias makes the whole output row NaN.
+ *   num_splits: 0 = chosen from the SM count.  workspace: dflash_kv4_sdpa_workspace_bytes() bytes of device memory, 16-byte
+ *   aligned, contents irrelevant, not shared by calls that can overlap. */
+DFLASH_API size_t dflash_kv4_sdpa_workspace_bytes(int B, int Hq, int Hk, int T, int D, int max_length, int num_splits);
+DFLASH_API int dflash_kv4_sdpa(const void* q, const long long* q_strides, const dflash_kv4_cache* k_cache,
+                               const dflash_kv4_cache* v_cache, const void* mask, int mask_kind, const long long* mask_strides,
+                               void* out, const int* lengths, int B, int Hq, int Hk, int T, int D, int capacity, int max_length,
+                               float scale, int dtype, int num_splits, void* workspace, size_t workspace_bytes, void* stream);
+
+/* ---------------------------------------------------------------------------------------------
+ * Log-probabilities of given tokens, with the entropy and the most likely alternatives of every row of logits: what a
+ * server reports beside the greedy token (greedy_tokens_with_mask, dflash_mlx/runtime.py:90-98).
+ *   logits    dtype (bf16, f16 or f32) [R,V], rows `ld` elements apart;  x = logits / temperature, p = softmax(x)
+ *   tokens    device int[R]; token_logprob[r] = log p[tokens[r]] (NaN for a token outside [0,V))
+ *   suppress  uint8[V] or NULL: tokens with suppress != 0 have probability 0 (log-probability -inf)
+ *   entropy[r] = -sum p log p in nats (may be NULL)
+ *   top_logprobs f32[R,top_k], top_ids int[R,top_k]: the top_k tokens by logit, highest first, ties to the lower index;
+ *             0 <= top_k <= min(32, V); both NULL when top_k = 0
+ *   A row with nothing but -inf: log-probabilities -inf, entropy 0.  A row with a NaN or +inf: NaN (ids still in range).
+ * One launch, no workspace; sums in f32. */
+DFLASH_API int dflash_token_logprobs(const void* logits, long long ld, const int* tokens, const uint8_t* suppress, float temperature,
+                                     float* token_logprob, float* entropy, float* top_logprobs, int* top_ids, int R, int V,
+                                     int top_k, int dtype, void* stream);
+
+/* ---------------------------------------------------------------------------------------------
  * Tensor-parallel reduction over peer-mapped memory, fused with the residual add and RMSNorm that consume it.
  * Generalises the reference's single collective, `mx.distributed.all_sum` after the GatedDeltaNet out_proj
  * (dflash_mlx/runtime.py:449-450), to every row-parallel projection of the step:
