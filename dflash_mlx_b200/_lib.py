@@ -78,6 +78,31 @@ def lib():
     return _lib
 
 
+_native = None
+
+
+def native():
+    """The C++ binding (csrc/binding.cpp), bound to this library's functions; built first if absent."""
+    global _native
+    if _native is None:
+        handle = lib()
+        with _lock:
+            if _native is None:
+                import importlib.util
+
+                from .csrc.build import BINDING, build_binding
+                if not BINDING.exists():
+                    build_binding()
+                spec = importlib.util.spec_from_file_location("dflash_mlx_b200._native", BINDING)
+                module = importlib.util.module_from_spec(spec)
+                spec.loader.exec_module(module)
+                names = ("dflash_kv4_write", "dflash_kv4_read", "dflash_kv4_sdpa_workspace_bytes", "dflash_kv4_sdpa",
+                         "dflash_token_logprobs", "dflash_last_error_string")
+                module.bind(DFlashError, *[ctypes.cast(getattr(handle, n), ctypes.c_void_p).value for n in names])
+                _native = module
+    return _native
+
+
 def check(status: int, what: str = "") -> None:
     if status < 0:
         msg = lib().dflash_last_error_string().decode("utf-8", "replace")

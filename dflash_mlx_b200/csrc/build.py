@@ -5,11 +5,13 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 from pathlib import Path
 
 CSRC = Path(__file__).resolve().parent
 PKG = CSRC.parent
 LIB = PKG / "libdflash_b200.so"
+BINDING = PKG / "_native.so"
 SOURCES = ["runtime.cu", "qmm.cu", "qmm_tc.cu", "gdn.cu", "gdn_layer.cu", "sdpa.cu", "sdpa_tc.cu", "glue.cu", "peer.cu", "kv4.cu",
            "logprobs.cu"]
 FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17", "--use_fast_math",
@@ -30,6 +32,25 @@ def _stale(obj: Path, src: Path) -> bool:
         return True
     newest = max(p.stat().st_mtime for p in [src, *CSRC.glob("*.cuh"), PKG.parent / "include" / "dflash_b200.h"])
     return obj.stat().st_mtime < newest
+
+
+def build_binding(force: bool = False) -> Path:
+    """The C++ binding of the operators in quantized_kv.py and logprobs.py, against the installed torch."""
+    src = CSRC / "binding.cpp"
+    if not force and not _stale(BINDING, src):
+        return BINDING
+    import torch
+    base = Path(torch.__file__).resolve().parent
+    cuda = Path(_nvcc()).resolve().parent.parent
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", f"-I{base}/include",
+           f"-I{base}/include/torch/csrc/api/include", f"-I{cuda}/include", f"-I{sysconfig.get_paths()['include']}", str(src), "-o",
+           str(BINDING), f"-L{base}/lib", "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_python"]
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if res.returncode != 0:
+        sys.stderr.write(res.stderr)
+        raise RuntimeError("g++ failed on binding.cpp")
+    return BINDING
 
 
 def build(force: bool = False, verbose: bool = False) -> Path:
@@ -60,6 +81,7 @@ def build(force: bool = False, verbose: bool = False) -> Path:
         if res.returncode != 0:
             sys.stderr.write(res.stderr)
             raise RuntimeError("link of libdflash_b200.so failed")
+    build_binding(force)
     return LIB
 
 

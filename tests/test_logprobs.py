@@ -1,4 +1,6 @@
 """Token log-probabilities without a GPU: what the entry points refuse."""
+import ctypes
+
 import pytest
 import torch
 
@@ -11,7 +13,8 @@ def test_refuses_cpu_tensors():
 
 
 def test_c_entry_refuses_before_any_launch():
-    logprobs._ensure_declared()
+    vp, i32 = ctypes.c_void_p, ctypes.c_int
+    _lib.declare("dflash_token_logprobs", i32, [vp, ctypes.c_longlong, vp, vp, ctypes.c_float] + [vp] * 4 + [i32] * 4 + [vp])
     lib = _lib.lib()
 
     def call(x=0x1000, ld=100, tokens=0x1000, t=1.0, lp=0x1000, tops=0x1000, ids=0x1000, R=1, V=100, k=4, dtype=0):

@@ -39,28 +39,48 @@ def test_refuses_cpu_tensors():
 
 def test_refuses_bad_caches():
     k, v = qkv.allocate(1, 2, 64, 128, device="cpu")
+    check = lambda one, other=v: _lib.native().check_cache(*one, *other)  # noqa: E731
+    check(k)
     with pytest.raises(ValueError, match="D=64"):
-        qkv._side((k.codes[..., :8], k.scales, k.biases), "k")
+        check((k.codes[..., :8], k.scales, k.biases))
     with pytest.raises(ValueError, match="int32"):
-        qkv._side((k.codes.long(), k.scales, k.biases), "k")
+        check((k.codes.long(), k.scales, k.biases))
     with pytest.raises(ValueError, match="scales must be"):
-        qkv._side((k.codes, k.scales[..., :1], k.biases), "k")
+        check((k.codes, k.scales[..., :1], k.biases))
     with pytest.raises(ValueError, match="share"):
-        qkv._side((k.codes, k.scales, k.biases.half()), "k")
+        check((k.codes, k.scales, k.biases.half()))
     with pytest.raises(ValueError, match="share"):
-        qkv._side((k.codes, k.scales.float(), k.biases.float()), "k")
+        check((k.codes, k.scales.float(), k.biases.float()))
     with pytest.raises(ValueError, match="contiguous"):
-        qkv._side((k.codes[:, :, ::2], k.scales[:, :, ::2], k.biases[:, :, ::2]), "k")
+        check((k.codes[:, :, ::2], k.scales[:, :, ::2], k.biases[:, :, ::2]))
     with pytest.raises(ValueError, match="differ"):
-        qkv._sides(k, qkv.allocate(1, 2, 32, 128, device="cpu")[1])
+        check(k, qkv.allocate(1, 2, 32, 128, device="cpu")[1])
     with pytest.raises(ValueError, match="D=96"):
         qkv.allocate(1, 1, 8, 96, device="cpu")
     with pytest.raises(ValueError, match="dtype"):
         qkv.allocate(1, 1, 8, 128, dtype=torch.float32, device="cpu")
 
 
+_ll, _vp, _i32 = ctypes.c_longlong, ctypes.c_void_p, ctypes.c_int
+
+
+class _Cache(ctypes.Structure):
+    """``dflash_kv4_cache`` of the C ABI."""
+    _fields_ = [("codes", _vp), ("scales", _vp), ("biases", _vp), ("codes_b", _ll), ("codes_h", _ll), ("scales_b", _ll),
+                ("scales_h", _ll), ("biases_b", _ll), ("biases_h", _ll)]
+
+
+def _declare():
+    cp, sp = ctypes.POINTER(_Cache), ctypes.POINTER(_ll)
+    _lib.declare("dflash_kv4_write", _i32, [_vp, sp, _vp, sp, cp, cp, _vp, _vp] + [_i32] * 6 + [_vp])
+    _lib.declare("dflash_kv4_read", _i32, [cp, cp, _vp, _vp, _vp] + [_i32] * 7 + [_vp])
+    _lib.declare("dflash_kv4_sdpa_workspace_bytes", ctypes.c_size_t, [_i32] * 7)
+    _lib.declare("dflash_kv4_sdpa", _i32, [_vp, sp, cp, cp, _vp, _i32, sp, _vp, _vp] + [_i32] * 7 +
+                 [ctypes.c_float, _i32, _i32, _vp, ctypes.c_size_t, _vp])
+
+
 def _cache_struct(base=0x1000, **kw):
-    s = qkv._Cache(base, base, base, 1024, 512, 128, 64, 128, 64)
+    s = _Cache(base, base, base, 1024, 512, 128, 64, 128, 64)
     for name, value in kw.items():
         setattr(s, name, value)
     return s
@@ -72,7 +92,7 @@ def _write(lib, k, v, B=1, Hk=2, T=1, D=128, cap=32, dtype=0, keys=0x1000, strid
 
 
 def test_c_entries_refuse_before_any_launch():
-    qkv._ensure_declared()
+    _declare()
     lib = _lib.lib()
     ok = _cache_struct()
     assert _write(lib, ok, ok, T=0) == 0 and _write(lib, ok, ok, B=0) == 0      # nothing to do
