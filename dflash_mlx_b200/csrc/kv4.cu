@@ -21,7 +21,7 @@ constexpr float kLog2e = 1.4426950408889634f;
 // ---- write -------------------------------------------------------------------------------------------------------------
 // A lane owns the eight channels of one word, eight lanes a group: minimum and maximum in three shuffles, no shared memory.
 // Bound by HBM (prompts) or by the launch (single tokens): kRows rows per warp are loaded before the first is used, so that a
-// warp has 16 * kRows bytes a lane in flight.
+// warp has 16 * kRows bytes a lane in flight.  blockIdx.x is (sequence, head), so no lane divides.
 struct WriteArgs {
   const void* x[2];
   long long sb[2], sh[2], st[2];
@@ -29,80 +29,82 @@ struct WriteArgs {
   const int* offsets;
   const int* counts;
   int Hk, T, capacity;
-  long long rows;   // B * Hk * T
 };
+
+// round((v - bias) / scale) by a reciprocal; where that lands within 1e-4 of a border between two codes (its own error is below
+// 1e-5, codes being at most 16) or the reciprocal is not finite, by the division that defines the code.
+__device__ __forceinline__ uint32_t code_of(float v, float bias, float scale, float inv) {
+  const float y = __fsub_rn(v, bias);
+  const float q = y * inv;
+  float n = rintf(q);
+  if (!(fabsf(q - n) < 0.4999f)) n = rintf(__fdiv_rn(y, scale));
+  return (uint32_t)fminf(fmaxf(n, 0.f), 15.f);
+}
 
 template <typename T, int D, int kRows>
 __global__ void __launch_bounds__(128) kv4_write_kernel(const WriteArgs a, int* __restrict__ err) {
   using TR = MmaTraits<T>;
   constexpr int kLanes = D / 8, kPer = 32 / kLanes;   // lanes of a row, rows of a warp at once
+  constexpr int kBlock = 4 * kPer * kRows;            // rows of a block
   pdl_wait();
   pdl_trigger();
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, side = blockIdx.y;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, side = blockIdx.z;
   const int j = lane % kLanes;
-  const long long row0 = ((long long)blockIdx.x * 4 + warp) * (kPer * kRows) + lane / kLanes;
-  const T* x = (const T*)a.x[side];
+  const int b = blockIdx.x / a.Hk, h = blockIdx.x % a.Hk;
+  const int n = min(a.counts ? a.counts[b] : a.T, a.T);
+  const long long at = a.offsets[b];
+  const T* x = (const T*)a.x[side] + b * a.sb[side] + h * a.sh[side] + 8 * j;
   const dflash_kv4_cache c = a.c[side];
-  uint4 raw[kRows];
-  int pos[kRows], bb[kRows], hh[kRows];
+  uint32_t* codes = c.codes + b * c.codes_batch_stride + h * c.codes_head_stride + j;
+  T* scales = (T*)c.scales + b * c.scales_batch_stride + h * c.scales_head_stride + (j >> 3);
+  T* biases = (T*)c.biases + b * c.biases_batch_stride + h * c.biases_head_stride + (j >> 3);
+  for (int t0 = blockIdx.y * kBlock; t0 < n; t0 += gridDim.y * kBlock) {
+    uint4 raw[kRows];
+    bool ok[kRows];
 #pragma unroll
-  for (int i = 0; i < kRows; ++i) {
-    const long long row = row0 + (long long)i * kPer;
-    pos[i] = -1;
-    raw[i] = make_uint4(0, 0, 0, 0);
-    bb[i] = hh[i] = 0;
-    if (row < a.rows) {
-      const int t = (int)(row % a.T), bh = (int)(row / a.T);
-      bb[i] = bh / a.Hk;
-      hh[i] = bh % a.Hk;
-      const int n = a.counts ? a.counts[bb[i]] : a.T;
-      if (t < n) {
-        const long long p = (long long)a.offsets[bb[i]] + t;
-        if (p >= 0 && p < a.capacity) {
-          pos[i] = (int)p;
-          raw[i] = *(const uint4*)(x + bb[i] * a.sb[side] + hh[i] * a.sh[side] + t * a.st[side] + 8 * j);
-        } else if (j == 0) {
-          atomicCAS(err, 0, 61 | ((t & 0x7FFFFF) << 8));
-        }
-      }
-    }
-  }
-#pragma unroll
-  for (int i = 0; i < kRows; ++i) {
-    float v[8];
-    const uint32_t u[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
-    float lo = INFINITY, hi = -INFINITY, bad = 0.f;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      v[e] = TR::bits_to_float((uint16_t)(u[e >> 1] >> (16 * (e & 1))));
-      lo = fminf(lo, v[e]);
-      hi = fmaxf(hi, v[e]);
-      bad = fmaf(v[e], 0.f, bad);   // NaN as soon as one value is NaN or infinite
+    for (int i = 0; i < kRows; ++i) {
+      const int t = t0 + (warp * kRows + i) * kPer + lane / kLanes;
+      const long long p = at + t;
+      ok[i] = t < n && p >= 0 && p < a.capacity;
+      raw[i] = make_uint4(0, 0, 0, 0);
+      if (ok[i]) raw[i] = *(const uint4*)(x + t * a.st[side]);
+      else if (t < n && j == 0) atomicCAS(err, 0, 61 | ((t & 0x7FFFFF) << 8));
     }
 #pragma unroll
-    for (int o = 1; o < 8; o <<= 1) {
-      lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-      hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
-      bad += __shfl_xor_sync(0xffffffffu, bad, o);
-    }
-    // IEEE divisions and subnormals: the codes are defined to the last bit (this file is compiled without fast math)
-    const T scale_t = TR::from_float(__fadd_rn(__fsub_rn(__fdiv_rn(hi, 15.f), __fdiv_rn(lo, 15.f)), bad));
-    const T bias_t = TR::from_float(__fadd_rn(lo, bad));
-    const float scale = TR::to_float(scale_t), bias = TR::to_float(bias_t);
-    uint32_t word = 0;
-    if (scale > 0.f) {
+    for (int i = 0; i < kRows; ++i) {
+      float v[8];
+      const uint32_t u[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+      float lo = INFINITY, hi = -INFINITY, bad = 0.f;
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        const float q = rintf(__fdiv_rn(__fsub_rn(v[e], bias), scale));
-        word |= (uint32_t)fminf(fmaxf(q, 0.f), 15.f) << (4 * e);
+        v[e] = TR::bits_to_float((uint16_t)(u[e >> 1] >> (16 * (e & 1))));
+        lo = fminf(lo, v[e]);
+        hi = fmaxf(hi, v[e]);
+        bad = fmaf(v[e], 0.f, bad);   // NaN as soon as one value is NaN or infinite
       }
-    }
-    if (pos[i] >= 0) {
-      c.codes[bb[i] * c.codes_batch_stride + hh[i] * c.codes_head_stride + (long long)pos[i] * (D / 8) + j] = word;
-      if ((j & 7) == 0) {
-        const long long in_row = (long long)pos[i] * (D / kGroup) + (j >> 3);
-        ((T*)c.scales)[bb[i] * c.scales_batch_stride + hh[i] * c.scales_head_stride + in_row] = scale_t;
-        ((T*)c.biases)[bb[i] * c.biases_batch_stride + hh[i] * c.biases_head_stride + in_row] = bias_t;
+#pragma unroll
+      for (int o = 1; o < 8; o <<= 1) {
+        lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+        hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+        bad += __shfl_xor_sync(0xffffffffu, bad, o);
+      }
+      // IEEE divisions and subnormals: the codes are defined to the last bit (this file is compiled without fast math)
+      const T scale_t = TR::from_float(__fadd_rn(__fsub_rn(__fdiv_rn(hi, 15.f), __fdiv_rn(lo, 15.f)), bad));
+      const T bias_t = TR::from_float(__fadd_rn(lo, bad));
+      const float scale = TR::to_float(scale_t), bias = TR::to_float(bias_t);
+      uint32_t word = 0;
+      if (scale > 0.f) {
+        const float inv = __frcp_rn(scale);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) word |= code_of(v[e], bias, scale, inv) << (4 * e);
+      }
+      if (ok[i]) {
+        const long long p = at + t0 + (warp * kRows + i) * kPer + lane / kLanes;
+        codes[p * (D / 8)] = word;
+        if ((j & 7) == 0) {
+          scales[p * (D / kGroup)] = scale_t;
+          biases[p * (D / kGroup)] = bias_t;
+        }
       }
     }
   }
@@ -114,52 +116,55 @@ struct ReadArgs {
   void* out[2];
   const int* starts;
   int start, Hk, T, capacity;
-  long long rows;
 };
 
 // The same split as the write: a lane unpacks one word into 16 bytes of output.
 template <typename T, int D, int kRows>
 __global__ void __launch_bounds__(128) kv4_read_kernel(const ReadArgs a) {
   using TR = MmaTraits<T>;
-  constexpr int kLanes = D / 8, kPer = 32 / kLanes;
+  constexpr int kLanes = D / 8, kPer = 32 / kLanes, kBlock = 4 * kPer * kRows;
   pdl_wait();
   pdl_trigger();
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, side = blockIdx.y;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, side = blockIdx.z;
   const int j = lane % kLanes;
-  const long long row0 = ((long long)blockIdx.x * 4 + warp) * (kPer * kRows) + lane / kLanes;
+  const int b = blockIdx.x / a.Hk, h = blockIdx.x % a.Hk;
+  const long long at = a.starts ? a.starts[b] : a.start;
   const dflash_kv4_cache c = a.c[side];
-  uint32_t word[kRows];
-  float scale[kRows], bias[kRows];
+  const uint32_t* codes = c.codes + b * c.codes_batch_stride + h * c.codes_head_stride + j;
+  const T* scales = (const T*)c.scales + b * c.scales_batch_stride + h * c.scales_head_stride + (j >> 3);
+  const T* biases = (const T*)c.biases + b * c.biases_batch_stride + h * c.biases_head_stride + (j >> 3);
+  T* out = (T*)a.out[side] + (long long)blockIdx.x * a.T * D + 8 * j;
+  for (int t0 = blockIdx.y * kBlock; t0 < a.T; t0 += gridDim.y * kBlock) {
+    uint32_t word[kRows];
+    T scale[kRows], bias[kRows];
 #pragma unroll
-  for (int i = 0; i < kRows; ++i) {
-    const long long row = row0 + (long long)i * kPer;
-    word[i] = 0;
-    scale[i] = bias[i] = 0.f;
-    if (row < a.rows) {
-      const int t = (int)(row % a.T), bh = (int)(row / a.T), b = bh / a.Hk, h = bh % a.Hk;
-      const long long p = (long long)(a.starts ? a.starts[b] : a.start) + t;
-      if (p >= 0 && p < a.capacity) {
-        const long long in_row = p * (D / kGroup) + (j >> 3);
-        word[i] = c.codes[b * c.codes_batch_stride + h * c.codes_head_stride + p * (D / 8) + j];
-        scale[i] = TR::to_float(((const T*)c.scales)[b * c.scales_batch_stride + h * c.scales_head_stride + in_row]);
-        bias[i] = TR::to_float(((const T*)c.biases)[b * c.biases_batch_stride + h * c.biases_head_stride + in_row]);
+    for (int i = 0; i < kRows; ++i) {
+      const int t = t0 + (warp * kRows + i) * kPer + lane / kLanes;
+      const long long p = at + t;
+      word[i] = 0;
+      scale[i] = bias[i] = TR::from_float(0.f);
+      if (t < a.T && p >= 0 && p < a.capacity) {
+        word[i] = codes[p * (D / 8)];
+        scale[i] = scales[p * (D / kGroup)];
+        bias[i] = biases[p * (D / kGroup)];
       }
     }
-  }
 #pragma unroll
-  for (int i = 0; i < kRows; ++i) {
-    const long long row = row0 + (long long)i * kPer;
-    if (row < a.rows) {
-      uint4 o;
-      uint32_t* po = (uint32_t*)&o;
+    for (int i = 0; i < kRows; ++i) {
+      const int t = t0 + (warp * kRows + i) * kPer + lane / kLanes;
+      if (t < a.T) {
+        const float s = TR::to_float(scale[i]), z = TR::to_float(bias[i]);
+        uint4 o;
+        uint32_t* po = (uint32_t*)&o;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        // code * scale is exact in fp32 (4 + 11 bits), so there is one rounding in the sum and one to the output type
-        const T x0 = TR::from_float(fmaf((float)((word[i] >> (8 * e)) & 15u), scale[i], bias[i]));
-        const T x1 = TR::from_float(fmaf((float)((word[i] >> (8 * e + 4)) & 15u), scale[i], bias[i]));
-        po[e] = (uint32_t) * (const uint16_t*)&x0 | ((uint32_t) * (const uint16_t*)&x1 << 16);
+        for (int e = 0; e < 4; ++e) {
+          // code * scale is exact in fp32 (4 + 11 bits), so there is one rounding in the sum and one to the output type
+          const T x0 = TR::from_float(fmaf((float)((word[i] >> (8 * e)) & 15u), s, z));
+          const T x1 = TR::from_float(fmaf((float)((word[i] >> (8 * e + 4)) & 15u), s, z));
+          po[e] = (uint32_t) * (const uint16_t*)&x0 | ((uint32_t) * (const uint16_t*)&x1 << 16);
+        }
+        *(uint4*)(out + (long long)t * D) = o;
       }
-      *(uint4*)((T*)a.out[side] + row * D + 8 * j) = o;
     }
   }
 }
@@ -179,7 +184,9 @@ __global__ void __launch_bounds__(128) kv4_read_kernel(const ReadArgs a) {
 // fp32 sums small (with the constant left in, a score's sum carries 136 or 1032 times sum |q|, which costs digits).
 // The running maximum moves only when a score exceeds it by 8 octaves (p <= 256 otherwise), so the accumulators are rarely
 // rescaled.  The warps of a block and then the splits of the key range are merged with fp32 partials.
-constexpr int kWarps = 8;
+// Warps of a block, one block per SM: as many as the registers allow (the loop is bound by instruction issue: unpacking, scales
+// and softmax next to the MMAs).
+template <int D, int NT> constexpr int kWarpsOf = NT == 2 ? (D == 256 ? 8 : 12) : (D == 256 ? 12 : 16);
 constexpr float kMaxStep = 5.545177444f;   // 8 ln 2
 
 template <int D>
@@ -231,7 +238,8 @@ template <int D>
 __device__ __forceinline__ int v_chunk(int r, int ch) { return ch ^ (D == 256 ? (((r >> 1) & 3) << 1) : (((r >> 1) & 1) << 1)); }
 
 template <typename T, int D, int NT, bool kMask>
-__global__ void __launch_bounds__(kWarps * 32) kv4_sdpa_kernel(const SdpaArgs a, int stages) {
+__global__ void __launch_bounds__((kWarpsOf<D, NT>) * 32) kv4_sdpa_kernel(const SdpaArgs a, int stages) {
+  constexpr int kWarps = (kWarpsOf<D, NT>);
   using TR = MmaTraits<T>;
   using H = MmaTraits<__half>;
   constexpr int G = D / kGroup, CPR = D / 32, KS = D / 16;   // groups, 16-byte chunks of a row's codes, MMA steps of Q K^T
@@ -653,17 +661,20 @@ __global__ void __launch_bounds__(D / 4 < 64 ? 64 : D / 4) kv4_combine_kernel(co
 // ---- host side ---------------------------------------------------------------------------------------------------------
 int row_tile(int rows) { return rows <= 8 ? 1 : 2; }   // 8-row columns of the MMA tile: 16 query rows share one pass
 
-int choose_splits(int units, int max_length, int device, int requested) {
+// Key ranges per (sequence, KV head, row tile).  One sequence: one block per SM, equal shares.  Several sequences may differ in
+// length (the host does not know them), and their blocks in work: four waves of smaller ranges let the SMs even it out.
+int choose_splits(long long units, int B, int max_length, int device, int requested) {
   // a split is worth its partials from about one 16-key tile per warp on
-  const int most = (max_length + 16 * kWarps - 1) / (16 * kWarps);
-  int s = requested > 0 ? requested : sm_count(device) / (units > 0 ? units : 1);
+  const int most = (max_length + 127) / 128;
+  long long s = requested > 0 ? requested : (B > 1 ? 4ll : 1ll) * sm_count(device) / units;
   if (s > most) s = most;
   if (s > 1024) s = 1024;
-  return s < 1 ? 1 : s;
+  return s < 1 ? 1 : (int)s;
 }
 
 template <typename T, int D, int NT>
 int launch_sdpa(SdpaArgs a, cudaStream_t st, int device) {
+  constexpr int kWarps = (kWarpsOf<D, NT>);
   using TL = Tile<D>;
   constexpr size_t fixed = (size_t)NT * (D / 16) * 32 * 8 + (size_t)NT * (D / kGroup) * 8 * 4;
   constexpr size_t merge = (size_t)kWarps * 8 * NT * (D + 2) * 4;
@@ -715,6 +726,8 @@ int check_sizes(const char* who, int B, int Hk, int T, int D, int capacity, int 
   if (B < 0 || Hk < 1 || T < 0) return fail(DFLASH_ERR_BAD_SHAPE, "%s: bad sizes B=%d Hk=%d T=%d", who, B, Hk, T);
   if (D != 128 && D != 256) return fail(DFLASH_ERR_BAD_SHAPE, "%s: D=%d not in {128,256}", who, D);
   if (capacity < 1) return fail(DFLASH_ERR_BAD_SHAPE, "%s: capacity %d", who, capacity);
+  if ((long long)B * Hk > 0x7fffffffll) return fail(DFLASH_ERR_BAD_SHAPE, "%s: B*Hk too large", who);
+  if (T > 0x7fffffff - (1 << 20)) return fail(DFLASH_ERR_BAD_SHAPE, "%s: T=%d too large", who, T);
   if (dtype != DFLASH_BF16 && dtype != DFLASH_F16) return fail(DFLASH_ERR_BAD_ARG, "%s: dtype %d (want bf16 or f16)", who, dtype);
   return DFLASH_OK;
 }
@@ -723,8 +736,17 @@ bool aligned_rows(const void* p, const long long* s) {
   return !((uintptr_t)p & 15) && s[0] % 8 == 0 && s[1] % 8 == 0 && s[2] % 8 == 0;
 }
 
-// Rows of a warp at once: one while the blocks do not fill the SMs (latency), four for long inputs (loads in flight).
-constexpr int kManyRows = 4;
+// Rows of a warp at once: one while the blocks do not fill the SMs (latency), more for long inputs (loads in flight).
+constexpr int kManyRows = 8;
+// Grid of a write or read: (sequence, head) x blocks of rows x sides; true: kManyRows rows a warp.
+bool row_grid(int B, int Hk, int T, int D, int sides, int device, dim3* grid) {
+  const int per = D == 128 ? 8 : 4;   // rows of a block of four warps, one each
+  const long long heads = (long long)B * Hk;
+  const bool many = heads * T * sides >= 8ll * per * kManyRows * sm_count(device);
+  const long long y = ((long long)T + per * (many ? kManyRows : 1) - 1) / (per * (many ? kManyRows : 1));
+  *grid = dim3((unsigned)heads, (unsigned)(y < 65535 ? y : 65535), (unsigned)sides);
+  return many;
+}
 
 }  // namespace
 }  // namespace kv4
@@ -752,16 +774,13 @@ extern "C" int dflash_kv4_write(const void* keys, const long long* key_strides, 
     a.c[i] = i ? *v_cache : *k_cache;
   }
   a.offsets = offsets; a.counts = counts; a.Hk = Hk; a.T = T; a.capacity = capacity;
-  a.rows = (long long)B * Hk * T;
   int device = 0;
   cudaGetDevice(&device);
   int* err = device_error_word(device);
   if (!err) return fail(DFLASH_ERR_LAUNCH, "kv4_write: no device error word");
-  const int per = D == 128 ? 8 : 4;   // rows of a block of four warps
-  const bool many = a.rows >= (long long)per * kManyRows * sm_count(device);
-  const long long blocks = (a.rows + (long long)per * (many ? kManyRows : 1) - 1) / (per * (many ? kManyRows : 1));
-  if (blocks > 0x7fffffffll) return fail(DFLASH_ERR_BAD_SHAPE, "kv4_write: too many rows");
-  const dim3 grid((unsigned)blocks, 2), block(128);
+  dim3 grid;
+  const bool many = row_grid(B, Hk, T, D, 2, device, &grid);
+  const dim3 block(128);
   cudaStream_t st = (cudaStream_t)stream;
   auto go = [&](auto one, auto four) { return many ? launch_kernel(four, grid, block, 0, st, a, err) : launch_kernel(one, grid, block, 0, st, a, err); };
   cudaError_t e;
@@ -789,14 +808,11 @@ extern "C" int dflash_kv4_read(const dflash_kv4_cache* k_cache, const dflash_kv4
   if (values_out) a.c[1] = *v_cache;
   a.out[0] = keys_out; a.out[1] = values_out;
   a.starts = starts; a.start = start; a.Hk = Hk; a.T = T; a.capacity = capacity;
-  a.rows = (long long)B * Hk * T;
   int device = 0;
   cudaGetDevice(&device);
-  const int per = D == 128 ? 8 : 4;
-  const bool many = a.rows >= (long long)per * kManyRows * sm_count(device);
-  const long long blocks = (a.rows + (long long)per * (many ? kManyRows : 1) - 1) / (per * (many ? kManyRows : 1));
-  if (blocks > 0x7fffffffll) return fail(DFLASH_ERR_BAD_SHAPE, "kv4_read: too many rows");
-  const dim3 grid((unsigned)blocks, values_out ? 2 : 1), block(128);
+  dim3 grid;
+  const bool many = row_grid(B, Hk, T, D, values_out ? 2 : 1, device, &grid);
+  const dim3 block(128);
   cudaStream_t st = (cudaStream_t)stream;
   auto go = [&](auto one, auto four) { return many ? launch_kernel(four, grid, block, 0, st, a) : launch_kernel(one, grid, block, 0, st, a); };
   cudaError_t e;
@@ -812,7 +828,7 @@ extern "C" int dflash_kv4_read(const dflash_kv4_cache* k_cache, const dflash_kv4
 
 static int kv4_splits(int B, int Hk, long long rows, int max_length, int device, int num_splits) {
   const long long units = (long long)B * Hk * ((rows + 8 * row_tile((int)rows) - 1) / (8 * row_tile((int)rows)));
-  return choose_splits((int)(units > 65535 ? 65535 : units), max_length, device, num_splits);
+  return choose_splits(units, B, max_length, device, num_splits);
 }
 
 extern "C" size_t dflash_kv4_sdpa_workspace_bytes(int B, int Hq, int Hk, int T, int D, int max_length, int num_splits) {

@@ -47,7 +47,17 @@ template <> struct Elem<float> {
   __device__ static __forceinline__ void hide(uint32_t (&w)[4], int e) { w[e] = kNegInf; }
   __device__ static __forceinline__ void put(uint32_t (&w)[4], int e, const float* p) { w[e] = __float_as_uint(*p); }
   __device__ static __forceinline__ float load(const float* p) { return *p; }
+  __device__ static __forceinline__ float max_of(const uint32_t (&w)[kSlots][4]) {   // NaN is passed over
+    float m = -INFINITY;
+#pragma unroll
+    for (int s = 0; s < kSlots; ++s)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) m = fmaxf(m, __uint_as_float(w[s][i]));
+    return m;
+  }
 };
+__device__ __forceinline__ __nv_bfloat162 as_pair(uint32_t u, __nv_bfloat16) { return *(const __nv_bfloat162*)&u; }
+__device__ __forceinline__ __half2 as_pair(uint32_t u, __half) { return *(const __half2*)&u; }
 template <typename T, uint32_t kInf> struct Elem16 {
   static constexpr int kPer = 8, kSlots = 5;
   __device__ static __forceinline__ float get(const uint32_t (&w)[4], int e) {
@@ -59,6 +69,12 @@ template <typename T, uint32_t kInf> struct Elem16 {
   __device__ static __forceinline__ void hide(uint32_t (&w)[4], int e) { put_bits(w, e, kInf); }
   __device__ static __forceinline__ void put(uint32_t (&w)[4], int e, const T* p) { put_bits(w, e, *(const uint16_t*)p); }
   __device__ static __forceinline__ float load(const T* p) { return MmaTraits<T>::to_float(*p); }
+  __device__ static __forceinline__ float max_of(const uint32_t (&w)[kSlots][4]) {   // packed; NaN is passed over
+    auto m = as_pair(w[0][0], T());
+#pragma unroll
+    for (int i = 1; i < 4 * kSlots; ++i) m = __hmax2(m, as_pair(w[i >> 2][i & 3], T()));
+    return fmaxf(fmaxf(MmaTraits<T>::to_float(m.x), MmaTraits<T>::to_float(m.y)), -INFINITY);
+  }
 };
 template <> struct Elem<__nv_bfloat16> : Elem16<__nv_bfloat16, 0xFF80u> {};
 template <> struct Elem<__half> : Elem16<__half, 0xFC00u> {};
@@ -90,7 +106,7 @@ struct Shared {
   Sums warp_sums[kThreads / 32];
   Sums block_sums;
   float group_max[kGroups];
-  float tau;
+  float tau;                                      // only elements from here on (the first pass) or beyond (later ones) matter
   int count;
   unsigned long long list[kList];
   unsigned long long top[kMaxK];                  // this block's best, highest first; 0 = none
@@ -102,11 +118,19 @@ struct Shared {
 __device__ __forceinline__ void rank_into(unsigned long long* top, const unsigned long long* list, int n, int k) {
   for (int i = threadIdx.x; i < n; i += kThreads) {
     const unsigned long long mine = list[i];
-    if (mine == 0) continue;
     int rank = 0;
-    for (int j = 0; j < n && rank < k; ++j) rank += list[j] > mine;
-    if (rank < k) top[rank] = mine;
+#pragma unroll 8
+    for (int j = 0; j < n; ++j) rank += list[j] > mine;
+    if (rank < k && mine != 0) top[rank] = mine;
   }
+}
+
+// raw[s] for an s that is not known at compile time (registers cannot be indexed).
+template <int N>
+__device__ __forceinline__ void slot(const uint32_t (&raw)[N][4], int s, uint32_t (&w)[4]) {
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+    if (i == s) { w[0] = raw[i][0]; w[1] = raw[i][1]; w[2] = raw[i][2]; w[3] = raw[i][3]; }
 }
 
 template <typename T>
@@ -147,22 +171,29 @@ __global__ void __launch_bounds__(kThreads, 2) token_logprobs_kernel(const Args 
       }
     }
     if (a.suppress != nullptr) {
+      // eight bytes at once where the vectors start on a multiple of eight of them
+      const bool packed = kPer == 8 && skew == 0 && ((uintptr_t)a.suppress & 7) == 0;
 #pragma unroll
       for (int s = 0; s < kSlots; ++s) {
         const int v = base + s * kThreads + tid;
         const int i0 = v * kPer - skew;
         if (v < v1) {
+          if (packed && i0 + 8 <= a.V) {
+            const uint2 u = *(const uint2*)(a.suppress + i0);
+            if (u.x | u.y) {
 #pragma unroll
-          for (int e = 0; e < kPer; ++e)
-            if (i0 + e >= 0 && i0 + e < a.V && a.suppress[i0 + e]) E::hide(raw[s], e);
+              for (int e = 0; e < kPer; ++e)
+                if ((e < 4 ? u.x >> (8 * (e & 3)) : u.y >> (8 * (e & 3))) & 0xFFu) E::hide(raw[s], e);
+            }
+          } else {
+#pragma unroll
+            for (int e = 0; e < kPer; ++e)
+              if (i0 + e >= 0 && i0 + e < a.V && a.suppress[i0 + e]) E::hide(raw[s], e);
+          }
         }
       }
     }
-    Sums mine = {-INFINITY, 0.f, 0.f};
-#pragma unroll
-    for (int s = 0; s < kSlots; ++s)
-#pragma unroll
-      for (int e = 0; e < kPer; ++e) mine.m = fmaxf(mine.m, E::get(raw[s], e));
+    Sums mine = {E::max_of(raw), 0.f, 0.f};
     const float ref = mine.m == -INFINITY ? 0.f : mine.m;
 #pragma unroll
     for (int s = 0; s < kSlots; ++s)
@@ -174,51 +205,70 @@ __global__ void __launch_bounds__(kThreads, 2) token_logprobs_kernel(const Args 
         mine.w = fmaf(fmaxf(d, -1e30f), p, mine.w);   // a hidden element adds 0, not -inf * 0; NaN stays through p
       }
     if (a.k > 0) {
-      // ---- candidates of this pass: everything >= the k-th largest group maximum ----
-      float g = mine.m;
+      // ---- candidates of this pass ----
+      const bool first = base == v0;
+      if (first) {   // everything >= the k-th largest group maximum
+        float g = mine.m;
 #pragma unroll
-      for (int o = 1; o < 8; o <<= 1) g = fmaxf(g, __shfl_xor_sync(0xffffffffu, g, o));
-      if ((lane & 7) == 0) sh.group_max[warp * 4 + (lane >> 3)] = g;
-      if (tid == 0) sh.count = 0;
-      __syncthreads();
-      if (warp == 0) {
+        for (int o = 1; o < 8; o <<= 1) g = fmaxf(g, __shfl_xor_sync(0xffffffffu, g, o));
+        if ((lane & 7) == 0) sh.group_max[warp * 4 + (lane >> 3)] = g;
+        if (tid == 0) sh.count = 0;
+        __syncthreads();
         const float g0 = sh.group_max[lane], g1 = sh.group_max[lane + 32];
-        int r0 = 0, r1 = 0;
-#pragma unroll 8
-        for (int i = 0; i < kGroups; ++i) {
-          const float o = sh.group_max[i];
-          r0 += o > g0 || (o == g0 && i < lane);
-          r1 += o > g1 || (o == g1 && i < lane + 32);
-        }
-        if (r0 == a.k - 1) sh.tau = g0;
-        if (r1 == a.k - 1) sh.tau = g1;
-      }
-      __syncthreads();
-      const float tau = sh.tau;
-      // NaN elements count as the largest; a thread whose own maximum is below tau can only hold NaN beyond it
-      if (mine.m >= tau || !(mine.l == mine.l)) {
 #pragma unroll
-        for (int s = 0; s < kSlots; ++s)
+        for (int i = 0; i < kGroups / (kThreads / 32); ++i) {   // every warp ranks its own groups, ties by number
+          const int j = warp * (kGroups / (kThreads / 32)) + i;
+          const float v = sh.group_max[j];
+          const int rank = __popc(__ballot_sync(0xffffffffu, g0 > v || (g0 == v && lane < j))) +
+                           __popc(__ballot_sync(0xffffffffu, g1 > v || (g1 == v && lane + 32 < j)));
+          if (rank == a.k - 1 && lane == 0) sh.tau = v;
+        }
+        __syncthreads();
+      }
+      const float tau = sh.tau;
+      // NaN elements count as the largest; a thread whose own maximum does not reach tau can only hold NaN beyond it
+      if ((first ? mine.m >= tau : !(mine.m <= tau)) || !(mine.l == mine.l)) {
+#pragma unroll 1
+        for (int s = 0; s < kSlots; ++s) {
+          uint32_t w[4];
+          slot(raw, s, w);
+          const int v = base + s * kThreads + tid, i0 = v * kPer - skew;
+          uint32_t hits = 0;
 #pragma unroll
           for (int e = 0; e < kPer; ++e) {
-            const float v = E::get(raw[s], e);
-            const int i = (base + s * kThreads + tid) * kPer - skew + e;
-            if (!(v < tau) && base + s * kThreads + tid < v1 && i >= 0 && i < a.V) {
+            const float f = E::get(w, e);
+            hits |= (uint32_t)(first ? !(f < tau) : !(f <= tau)) << e;
+          }
+          if (v >= v1) hits = 0;
+          while (hits) {
+            const int e = __ffs(hits) - 1;
+            hits &= hits - 1;
+            float f = 0.f;
+#pragma unroll
+            for (int ee = 0; ee < kPer; ++ee)
+              if (ee == e) f = E::get(w, ee);
+            if (i0 + e >= 0 && i0 + e < a.V) {
               const int at = atomicAdd(&sh.count, 1);
-              if (at < kList - kMaxK) sh.list[at] = key_of(v, i);
+              if (at < kList - kMaxK) sh.list[at] = key_of(f, i0 + e);
             }
           }
+        }
       }
       __syncthreads();
       const int n = sh.count;
-      if (n <= kList - kMaxK) {
-        if (tid < kMaxK) {   // the best of the earlier passes compete again
-          sh.list[n + tid] = sh.top[tid];
+      if (n == 0) {
+        // nothing new (later passes, mostly)
+      } else if (n <= kList - kMaxK) {
+        int all = n;
+        if (!first) {   // the best of the earlier passes compete again
+          if (tid < a.k) {
+            sh.list[n + tid] = sh.top[tid];
+            sh.top[tid] = 0;
+          }
+          all += a.k;
+          __syncthreads();
         }
-        __syncthreads();
-        if (tid < kMaxK) sh.top[tid] = 0;
-        __syncthreads();
-        rank_into(sh.top, sh.list, n + kMaxK, a.k);
+        rank_into(sh.top, sh.list, all, a.k);
       } else {
         // too many at or above tau (ties, sorted logits): the k-th largest key bit by bit, then exactly the keys from it on
         const unsigned long long earlier = tid < kMaxK ? sh.top[tid] : 0ull;
@@ -227,13 +277,15 @@ __global__ void __launch_bounds__(kThreads, 2) token_logprobs_kernel(const Args 
         for (int bit = 63; bit >= 0; --bit) {
           const unsigned long long t = kth | (1ull << bit);
           int n_at = earlier >= t;
+#pragma unroll 1
+          for (int s = 0; s < kSlots; ++s) {
+            uint32_t w[4];
+            slot(raw, s, w);
+            const int v = base + s * kThreads + tid, i0 = v * kPer - skew;
 #pragma unroll
-          for (int s = 0; s < kSlots; ++s)
-#pragma unroll
-            for (int e = 0; e < kPer; ++e) {
-              const int v = base + s * kThreads + tid, i = v * kPer - skew + e;
-              n_at += v < v1 && i >= 0 && i < a.V && key_of(E::get(raw[s], e), i) >= t;
-            }
+            for (int e = 0; e < kPer; ++e)
+              n_at += v < v1 && i0 + e >= 0 && i0 + e < a.V && key_of(E::get(w, e), i0 + e) >= t;
+          }
           n_at = __reduce_add_sync(0xffffffffu, n_at);
           if (lane == 0) sh.counts[bit & 1][warp] = n_at;
           __syncthreads();
@@ -245,18 +297,26 @@ __global__ void __launch_bounds__(kThreads, 2) token_logprobs_kernel(const Args 
         __syncthreads();
         // kth = 0: fewer than k elements so far, all of them stay
         if (earlier >= kth && earlier != 0) sh.list[atomicAdd(&sh.count, 1)] = earlier;
+#pragma unroll 1
+        for (int s = 0; s < kSlots; ++s) {
+          uint32_t w[4];
+          slot(raw, s, w);
+          const int v = base + s * kThreads + tid, i0 = v * kPer - skew;
 #pragma unroll
-        for (int s = 0; s < kSlots; ++s)
-#pragma unroll
-          for (int e = 0; e < kPer; ++e) {
-            const int v = base + s * kThreads + tid, i = v * kPer - skew + e;
-            if (v < v1 && i >= 0 && i < a.V) {
-              const unsigned long long q = key_of(E::get(raw[s], e), i);
+          for (int e = 0; e < kPer; ++e)
+            if (v < v1 && i0 + e >= 0 && i0 + e < a.V) {
+              const unsigned long long q = key_of(E::get(w, e), i0 + e);
               if (q >= kth) sh.list[atomicAdd(&sh.count, 1)] = q;
             }
-          }
+        }
         __syncthreads();
         rank_into(sh.top, sh.list, sh.count, a.k);
+      }
+      __syncthreads();
+      // the next pass: only what beats the k-th best (its own index is lower); -inf while there are fewer than k
+      if (tid == 0) {
+        sh.count = 0;
+        sh.tau = sh.top[a.k - 1] == 0 ? -INFINITY : key_value(sh.top[a.k - 1]);
       }
       __syncthreads();
     }
@@ -281,11 +341,11 @@ __global__ void __launch_bounds__(kThreads, 2) token_logprobs_kernel(const Args 
     Sums all = sh.block_sums;
     for (int i = 1; i < blocks; ++i) all = merge(all, *cluster.map_shared_rank(&sh.block_sums, i), a.scale);
     if (a.k > 0) {
-      for (int i = tid; i < blocks * kMaxK; i += kThreads)
-        sh.gathered[i] = cluster.map_shared_rank(&sh.top[0], i / kMaxK)[i % kMaxK];
-      __syncthreads();
       if (blocks > 1) {
-        rank_into(sh.list, sh.gathered, blocks * kMaxK, a.k);   // list: free again
+        for (int i = tid; i < blocks * a.k; i += kThreads)
+          sh.gathered[i] = cluster.map_shared_rank(&sh.top[0], i / a.k)[i % a.k];
+        __syncthreads();
+        rank_into(sh.list, sh.gathered, blocks * a.k, a.k);   // list: free again
         __syncthreads();
       } else {
         if (tid < kMaxK) sh.list[tid] = sh.top[tid];
@@ -322,10 +382,10 @@ __global__ void __launch_bounds__(kThreads, 2) token_logprobs_kernel(const Args 
 
 template <typename T>
 int launch(const Args& a, int R, cudaStream_t st, int device) {
-  // a block holds kThreads * kSlots vectors at once; with few rows the cluster grows while a block keeps 2048 elements
-  const int hold = kThreads * Elem<T>::kSlots * Elem<T>::kPer;
+  // rows alone fill the SMs: a block per row passes over it, most passes finding no new candidate; few rows: the cluster grows
+  // while a block keeps 2048 elements
   int c = 1;
-  while (c < 8 && ((long long)c * hold < a.V || ((long long)R * c < sm_count(device) && a.V >= 2 * c * 2048))) c <<= 1;
+  while (c < 8 && (long long)R * c < sm_count(device) && a.V >= 2 * c * 2048) c <<= 1;
   if ((long long)R * c > 0x7fffffffll) return fail(DFLASH_ERR_BAD_SHAPE, "token_logprobs: too many rows");
   cudaError_t e = launch_kernel_cluster(token_logprobs_kernel<T>, dim3((unsigned)R * c), dim3(kThreads), c, 0, st, a);
   if (e == cudaSuccess) e = cudaGetLastError();
