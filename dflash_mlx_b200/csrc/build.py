@@ -13,11 +13,11 @@ PKG = CSRC.parent
 LIB = PKG / "libdflash_b200.so"
 BINDING = PKG / "_native.so"
 SOURCES = ["runtime.cu", "qmm.cu", "qmm_tc.cu", "gdn.cu", "gdn_layer.cu", "sdpa.cu", "sdpa_tc.cu", "glue.cu", "peer.cu", "kv4.cu",
-           "logprobs.cu"]
+           "kv4_tc.cu", "logprobs.cu"]
 FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17", "--use_fast_math",
          "-Xcompiler", "-fPIC", "-Xcompiler", "-fvisibility=hidden", "-Xptxas", "-v"]
 # Sources whose results are defined to the last bit, subnormals included: IEEE division and no flush to zero.
-IEEE_SOURCES = {"kv4.cu"}
+IEEE_SOURCES = {"kv4.cu", "kv4_tc.cu"}
 
 
 def _nvcc() -> str:

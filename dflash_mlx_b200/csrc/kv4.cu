@@ -661,15 +661,26 @@ __global__ void __launch_bounds__(D / 4 < 64 ? 64 : D / 4) kv4_combine_kernel(co
 // ---- host side ---------------------------------------------------------------------------------------------------------
 int row_tile(int rows) { return rows <= 8 ? 1 : 2; }   // 8-row columns of the MMA tile: 16 query rows share one pass
 
-// Key ranges per (sequence, KV head, row tile).  One sequence: one block per SM, equal shares.  Several sequences may differ in
-// length (the host does not know them), and their blocks in work: four waves of smaller ranges let the SMs even it out.
+// Key ranges per (sequence, KV head, row tile), one block per SM at a time.  A block costs its keys and about kOverhead keys'
+// worth of start-up and merging.  Equal sequences run in whole waves; sequences of different lengths (several of them: the host
+// does not know) fill the SMs as blocks end, behind the longest of which the launch waits: half of each estimate.
+constexpr int kOverhead = 320;
 int choose_splits(long long units, int B, int max_length, int device, int requested) {
-  // a split is worth its partials from about one 16-key tile per warp on
-  const int most = (max_length + 127) / 128;
-  long long s = requested > 0 ? requested : (B > 1 ? 4ll : 1ll) * sm_count(device) / units;
-  if (s > most) s = most;
-  if (s > 1024) s = 1024;
-  return s < 1 ? 1 : (int)s;
+  const int most = (max_length + 127) / 128;   // a 16-key tile per warp
+  if (requested > 0) return requested < most ? requested : most;
+  const int sms = sm_count(device);
+  int best = 1;
+  double least = 1e300;
+  for (int s = 1; s <= most && s <= 1024 && units * s <= 8ll * sms; ++s) {
+    const double keys = (double)max_length / s + kOverhead;
+    double cost = (double)((units * s + sms - 1) / sms) * keys;
+    if (B > 1) cost = 0.5 * cost + 0.5 * ((double)(units * s) / sms * (0.6 * max_length / s + kOverhead) + 0.5 * keys);
+    if (cost < least) {
+      least = cost;
+      best = s;
+    }
+  }
+  return best;
 }
 
 template <typename T, int D, int NT>
@@ -698,18 +709,24 @@ int launch_sdpa(SdpaArgs a, cudaStream_t st, int device) {
   cudaError_t e = launch_kernel(kern, dim3(a.splits, row_tiles, a.B * a.Hk), dim3(kWarps * 32), smem, st, a, stages);
   if (e == cudaSuccess) e = cudaGetLastError();
   if (e != cudaSuccess) return fail(DFLASH_ERR_LAUNCH, "kv4_sdpa launch: %s", cudaGetErrorString(e));
-  if (a.splits > 1) {
-    e = launch_kernel(kv4_combine_kernel<T, D>, dim3(a.rows, a.B * a.Hk), dim3(D / 4 < 64 ? 64 : D / 4), 0, st, a);
-    if (e == cudaSuccess) e = cudaGetLastError();
-    if (e != cudaSuccess) return fail(DFLASH_ERR_LAUNCH, "kv4_sdpa combine launch: %s", cudaGetErrorString(e));
-  }
   return DFLASH_OK;
 }
 
+template <typename T, int D>
+int launch_combine(const SdpaArgs& a, cudaStream_t st) {
+  cudaError_t e = launch_kernel(kv4_combine_kernel<T, D>, dim3(a.rows, a.B * a.Hk), dim3(D / 4 < 64 ? 64 : D / 4), 0, st, a);
+  if (e == cudaSuccess) e = cudaGetLastError();
+  return e == cudaSuccess ? DFLASH_OK : fail(DFLASH_ERR_LAUNCH, "kv4_sdpa combine launch: %s", cudaGetErrorString(e));
+}
+
 template <typename T>
-int launch_typed(const SdpaArgs& a, int D, cudaStream_t st, int device) {
-  if (row_tile(a.rows) == 1) return D == 128 ? launch_sdpa<T, 128, 1>(a, st, device) : launch_sdpa<T, 256, 1>(a, st, device);
-  return D == 128 ? launch_sdpa<T, 128, 2>(a, st, device) : launch_sdpa<T, 256, 2>(a, st, device);
+int launch_typed(const SdpaArgs& a, int dtype, int D, cudaStream_t st, int device) {
+  int rc;
+  if (a.rows > kFewRows) rc = launch_partials_tc(a, dtype, D, st, device);
+  else if (row_tile(a.rows) == 1) rc = D == 128 ? launch_sdpa<T, 128, 1>(a, st, device) : launch_sdpa<T, 256, 1>(a, st, device);
+  else rc = D == 128 ? launch_sdpa<T, 128, 2>(a, st, device) : launch_sdpa<T, 256, 2>(a, st, device);
+  if (rc || a.splits == 1) return rc;
+  return D == 128 ? launch_combine<T, 128>(a, st) : launch_combine<T, 256>(a, st);
 }
 
 int check_cache(const char* who, const dflash_kv4_cache* c, int D) {
@@ -827,7 +844,8 @@ extern "C" int dflash_kv4_read(const dflash_kv4_cache* k_cache, const dflash_kv4
 }
 
 static int kv4_splits(int B, int Hk, long long rows, int max_length, int device, int num_splits) {
-  const long long units = (long long)B * Hk * ((rows + 8 * row_tile((int)rows) - 1) / (8 * row_tile((int)rows)));
+  const int tile = rows > kFewRows ? kTcRows : 8 * row_tile((int)rows);
+  const long long units = (long long)B * Hk * ((rows + tile - 1) / tile);
   return choose_splits(units, B, max_length, device, num_splits);
 }
 
@@ -876,5 +894,5 @@ extern "C" int dflash_kv4_sdpa(const void* q, const long long* q_strides, const 
     a.part_l = a.part_m + n;
   }
   cudaStream_t st = (cudaStream_t)stream;
-  return dtype == DFLASH_BF16 ? launch_typed<__nv_bfloat16>(a, D, st, device) : launch_typed<__half>(a, D, st, device);
+  return dtype == DFLASH_BF16 ? launch_typed<__nv_bfloat16>(a, dtype, D, st, device) : launch_typed<__half>(a, dtype, D, st, device);
 }

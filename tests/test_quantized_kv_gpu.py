@@ -36,6 +36,13 @@ def ints(*v):
 TOL = {torch.bfloat16: 2.0 ** -8 + 2.0 ** -9 + 5e-4, torch.float16: 2.0 ** -11 + 2.0 ** -9 + 5e-4}
 
 
+@pytest.fixture(autouse=True)
+def no_device_error():
+    """A bounded wait that ran out is a failure even where the values are right."""
+    yield
+    assert _lib.lib().dflash_device_error(0) == 0
+
+
 def check_rows(got, want, dtype):
     assert torch.equal(torch.isnan(got.double()), torch.isnan(want))
     err = (got.double() - want).nan_to_num(0).norm(dim=-1)
