@@ -593,9 +593,9 @@ __global__ void __launch_bounds__((kWarpsOf<D, NT>) * 32) kv4_sdpa_kernel(const 
 
 // out = sum_s w_s O_s / sum_s w_s l_s, w_s = exp(m_s - max m): one block per row.
 template <typename T, int D>
-__global__ void __launch_bounds__(D / 4 < 64 ? 64 : D / 4) kv4_combine_kernel(const SdpaArgs a) {
+__global__ void __launch_bounds__(256) kv4_combine_kernel(const SdpaArgs a) {
   using TR = MmaTraits<T>;
-  constexpr int kThreads = D / 4 < 64 ? 64 : D / 4, kPer = kThreads / (D / 4);   // key ranges read side by side
+  constexpr int kThreads = 256, kPer = kThreads / (D / 4);   // key ranges read side by side
   __shared__ float sw[1024];
   __shared__ float red[kThreads / 32];
   __shared__ float4 part[kPer][D / 4];
@@ -639,15 +639,13 @@ __global__ void __launch_bounds__(D / 4 < 64 ? 64 : D / 4) kv4_combine_kernel(co
     acc.x = fmaf(w, v.x, acc.x); acc.y = fmaf(w, v.y, acc.y);
     acc.z = fmaf(w, v.z, acc.z); acc.w = fmaf(w, v.w, acc.w);
   }
-  if (kPer > 1) {
-    part[s0][d4] = acc;
-    __syncthreads();
-    if (s0 != 0) return;
+  part[s0][d4] = acc;
+  __syncthreads();
+  if (s0 != 0) return;
 #pragma unroll
-    for (int i = 1; i < kPer; ++i) {
-      const float4 v = part[i][d4];
-      acc.x += v.x; acc.y += v.y; acc.z += v.z; acc.w += v.w;
-    }
+  for (int i = 1; i < kPer; ++i) {
+    const float4 v = part[i][d4];
+    acc.x += v.x; acc.y += v.y; acc.z += v.z; acc.w += v.w;
   }
   const float inv = den == 0.f ? 1.f : 1.f / den, nan = den * 0.f;
   const float v[4] = {acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv};
@@ -714,7 +712,7 @@ int launch_sdpa(SdpaArgs a, cudaStream_t st, int device) {
 
 template <typename T, int D>
 int launch_combine(const SdpaArgs& a, cudaStream_t st) {
-  cudaError_t e = launch_kernel(kv4_combine_kernel<T, D>, dim3(a.rows, a.B * a.Hk), dim3(D / 4 < 64 ? 64 : D / 4), 0, st, a);
+  cudaError_t e = launch_kernel(kv4_combine_kernel<T, D>, dim3(a.rows, a.B * a.Hk), dim3(256), 0, st, a);
   if (e == cudaSuccess) e = cudaGetLastError();
   return e == cudaSuccess ? DFLASH_OK : fail(DFLASH_ERR_LAUNCH, "kv4_sdpa combine launch: %s", cudaGetErrorString(e));
 }

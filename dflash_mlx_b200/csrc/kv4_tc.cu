@@ -2,14 +2,15 @@
 // grouped model, a chunk of a prompt); the contract and the formulas are those of kv4.cu.
 //
 // One block = 128 query rows (row = position * heads-per-KV-head + head, the TMEM lanes of an M128 tile) and a range of keys,
-// in tiles of 64.  Keys and values are unpacked to fp16 into 128B-swizzled shared memory, a ring of buffers that alternate
-// K(0) V(0) K(1) V(1) ...; both have rows of keys with 64 channels (one quantisation group) each 128 bytes, which is K-major for
-// S = Q K^T and MN-major for O = P V.
-//   warps 0-3  softmax, a thread per row: S from tensor memory, P back over it, O rescaled in place when the maximum moved
-//   next 2 * (D/64) warps unpack: a thread owns the 64 channels of one key and group, i.e. one scale and one 128-byte row
-//   last warp  one thread issues the MMAs in the order QK(0) QK(1) PV(0) QK(2) PV(1) ..., so that a tile's softmax runs under
-//              the next tile's scores
-// Q sits in tensor memory too (A operand of QK), so that the tensor pipe reads only K and V from shared memory.
+// in tiles of 128: two score tiles and the output fill tensor memory (2 x 128 + 256 columns; narrower score tiles ran at half
+// rate, an M128 N64 MMA taking as long as N128).  Keys and values are unpacked to fp16 into 128B-swizzled shared memory: a slab
+// per 64 channels (one quantisation group), rows of keys of 128 bytes, which is K-major for S = Q K^T and MN-major for O = P V.
+//   warps 0-3   softmax, a thread per row: S from tensor memory, P back over it, O rescaled in place when the maximum moved
+//   warps 4-7   unpack keys, 8-11 values: a thread owns a key, a group at a time
+//   warp 12     one thread issues the MMAs in the order QK(0) QK(1) PV(0) QK(2) PV(1) ..., so that a tile's softmax runs under
+//               the next tile's scores
+// One tile of keys and one of values are enough: a slab of keys is free as soon as its four steps of QK(i) are done and is
+// refilled under PV(i-1), values (in blocks of 32 keys) the other way round.
 //
 // Unpacking costs 9 instructions for 8 codes: a nibble left in place is an fp16 subnormal, code * 2^-24 (or * 2^-20), and one packed
 // fma turns two of them into code * scale + bias with a single rounding to fp16 (2^-11; the cache's scales carry 8 or 11 bits,
@@ -27,29 +28,24 @@ namespace kv4 {
 namespace {
 
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
-constexpr int kRows = 128, kKeys = 64;
+constexpr int kRows = 128, kKeys = 128;
+constexpr int kThreads = 13 * 32, kKeyWarp = 4, kValueWarp = 8, kIssuer = 12;
 constexpr float kMaxStep = 8 * kLn2;   // natural units
 constexpr float kPShift = 6.f;         // P = p * 2^6 (p <= 2^8): further from fp16's subnormals
-
-template <int D>
-struct Shape {
-  static constexpr int kG = D / kGroup;
-  static constexpr int kUnpackWarps = 2 * kG;
-  static constexpr int kThreads = (4 + kUnpackWarps + 1) * 32;
-  static constexpr int kSlots = D == 256 ? 6 : 8;
-  static constexpr int kSlab = kKeys * 128;            // 64 keys x 64 channels
-  static constexpr int kBuf = kG * kSlab;
-  static constexpr uint32_t kQCol = 0, kSCol = D / 2, kOCol = 256, kCols = 512;
-};
+constexpr int kSlab = kKeys * 128;     // 128 rows x 64 channels: Q, K or V
+constexpr uint32_t kOCol = 256, kCols = 512;   // S / P of tile i at 128 * (i & 1)
 
 // What softmax needs to know about a tile: per 32 keys the power of two of K, the exponent of V, and keys whose value is not
 // finite.
 struct Meta {
-  float k_factor[2];
-  int v_exp[2];
-  uint32_t bad[2];
+  float k_factor[4];
+  int v_exp[4];
+  uint32_t bad[4];
 };
-constexpr int kMeta = 8;   // tiles in flight are at most 4
+constexpr int kMeta = 4;   // keys are unpacked at most two tiles ahead of the softmax
+
+// mbarriers, 8 bytes each
+enum { kBarKFull = 0, kBarKEmpty = 4, kBarVFull = 8, kBarVEmpty = 12, kBarS = 16, kBarP = 18, kBarO = 20, kBarVMeta = 22, kBarQ = 24, kBars = 26 };
 
 __device__ __forceinline__ bool wait_bar(uint32_t bar, uint32_t parity) {
   for (uint32_t i = 0; i < (1u << 16); ++i) {   // hardware-suspended polls of up to a microsecond
@@ -71,6 +67,14 @@ __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::be
 __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void commit(uint32_t bar) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+// D (+)= A (shared memory descriptor) * B (shared memory descriptor)
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accum) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accum)
+      : "memory");
 }
 // D (+)= A (tensor memory) * B (shared memory descriptor)
 __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc, uint32_t accum) {
@@ -118,8 +122,8 @@ __device__ __forceinline__ float pow2(int e) { return __uint_as_float((uint32_t)
 __device__ __forceinline__ bool finite(float x) { return (__float_as_uint(x) & 0x7F800000u) != 0x7F800000u; }
 
 template <int D>
-struct Raw {   // one key's codes of one group, and its scales and biases of every group
-  uint4 c0, c1;
+struct Raw {   // one key: codes, scales and biases of every group
+  uint4 c[D / 32];
   uint32_t s[D / 128], b[D / 128];
 };
 
@@ -170,11 +174,11 @@ __device__ __forceinline__ bool wide_range(const float (&s)[G], const float (&b)
 }
 // 64 codes -> a swizzled 128-byte row; the eight codes of a word land in the order 0 4 1 5 2 6 3 7.  Narrow: the nibbles are
 // fp16 subnormals and one fma makes the value (9 instructions a word); wide: the nibbles become whole numbers first (13).
-template <int D, bool kWide>
-__device__ __forceinline__ void unpack_row(const Raw<D>& r, float scale, float bias, int e, uint32_t row, int key) {
+template <bool kWide>
+__device__ __forceinline__ void unpack_row(const uint4& c0, const uint4& c1, float scale, float bias, int e, uint32_t row, int key) {
   const float sx = scale * pow2(kWide ? -e : min(24 - e, 127));   // e >= -100
   const uint32_t s0 = splat(sx), s1 = splat(sx * 0.0625f), z = splat(bias * pow2(-e));
-  const uint32_t w[8] = {r.c0.x, r.c0.y, r.c0.z, r.c0.w, r.c1.x, r.c1.y, r.c1.z, r.c1.w};
+  const uint32_t w[8] = {c0.x, c0.y, c0.z, c0.w, c1.x, c1.y, c1.z, c1.w};
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     uint32_t v[4];
@@ -196,35 +200,118 @@ __device__ __forceinline__ void unpack_row(const Raw<D>& r, float scale, float b
   }
 }
 
+// The keys (kV = false) or values of a block's range, by the four warps of a side: thread = key of the tile.
+template <typename T, int D, bool kV>
+__device__ __forceinline__ void unpack_side(const dflash_kv4_cache& c, int b, int hk, int k0, int hi, int tiles, uint8_t* buf, uint32_t bar0,
+                                            Meta* meta, int* err) {
+  constexpr int G = D / kGroup;
+  const int w = (threadIdx.x >> 5) & 3, lane = threadIdx.x & 31, key = w * 32 + lane;
+  const uint8_t* codes = (const uint8_t*)(c.codes + b * c.codes_batch_stride + hk * c.codes_head_stride);
+  const T* scales = (const T*)c.scales + b * c.scales_batch_stride + hk * c.scales_head_stride;
+  const T* biases = (const T*)c.biases + b * c.biases_batch_stride + hk * c.biases_head_stride;
+  auto load = [&](int tile, Raw<D>& r) {
+    const int n = k0 + tile * kKeys + key;
+    if (tile < tiles && n < hi) {
+      const uint4* p = (const uint4*)(codes + (size_t)n * (D / 2));
+#pragma unroll
+      for (int i = 0; i < D / 32; ++i) r.c[i] = __ldg(p + i);
+      const T *ps = scales + (size_t)n * G, *pb = biases + (size_t)n * G;
+      if (G == 4) {
+        const uint2 s = *(const uint2*)ps, z = *(const uint2*)pb;
+        r.s[0] = s.x; r.s[G / 2 - 1] = s.y;
+        r.b[0] = z.x; r.b[G / 2 - 1] = z.y;
+      } else {
+        r.s[0] = *(const uint32_t*)ps;
+        r.b[0] = *(const uint32_t*)pb;
+      }
+    } else {   // behind the range: zeros, which no row sees
+#pragma unroll
+      for (int i = 0; i < D / 32; ++i) r.c[i] = make_uint4(0, 0, 0, 0);
+#pragma unroll
+      for (int i = 0; i < D / 128; ++i) r.s[i] = r.b[i] = 0;
+    }
+  };
+  auto done = [&](uint32_t bar) {
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // the tensor pipe reads what was stored
+    __syncwarp();
+    if (lane == 0) mbar_arrive(bar);
+  };
+  Raw<D> cur, next;
+  load(0, next);
+  bool ok = true;
+  for (int t = 0; t < tiles && ok; ++t) {
+    cur = next;
+    load(t + 1, next);   // in flight under this tile's unpacking and waits
+    float s[G], z[G];
+    scales_of<T, D>(cur, s, z);
+    int e;
+    bool wide = false;
+    if (kV) wide = wide_range(s, z, &e);
+    if (!wide) e = block_exponent(s, z);
+    Meta& m = meta[t & (kMeta - 1)];
+    if (kV) {
+      bool bad = false;
+#pragma unroll
+      for (int g = 0; g < G; ++g) bad |= !finite(s[g]) || !finite(z[g]);
+      if (bad) {   // out of the products; rows that see it get NaN through its score
+#pragma unroll
+        for (int g = 0; g < G; ++g) s[g] = z[g] = 0.f;
+      }
+      const uint32_t bads = __ballot_sync(0xffffffffu, bad);
+      if (lane == 0) {
+        m.v_exp[w] = e;
+        m.bad[w] = bads;
+        mbar_arrive(bar0 + 8 * (kBarVMeta + (t & 1)));
+      }
+      // this warp's keys are one block of the values' buffer
+      if (!wait_warp(bar0 + 8 * (kBarVEmpty + w), (t & 1) ^ 1)) { atomicCAS(err, 0, 62 | (1 << 8)); ok = false; break; }
+    } else if (lane == 0) {
+      m.k_factor[w] = pow2(e);
+    }
+#pragma unroll
+    for (int g = 0; g < G; ++g) {
+      if (!kV && !wait_warp(bar0 + 8 * (kBarKEmpty + g), (t & 1) ^ 1)) { atomicCAS(err, 0, 62 | (2 << 8)); ok = false; break; }
+      const uint32_t row = smem_u32(buf + g * kSlab + key * 128);
+      if (kV && wide) unpack_row<true>(cur.c[2 * g], cur.c[2 * g + 1], s[g], z[g], e, row, key);
+      else unpack_row<false>(cur.c[2 * g], cur.c[2 * g + 1], s[g], z[g], e, row, key);
+      if (!kV) done(bar0 + 8 * (kBarKFull + g));
+    }
+    if (kV) done(bar0 + 8 * (kBarVFull + w));
+  }
+}
+
 template <typename T, int D, bool kMask>
-__global__ void __launch_bounds__(Shape<D>::kThreads, 1) kv4_sdpa_tc_kernel(const SdpaArgs a, int* __restrict__ err) {
-  using S = Shape<D>;
+__global__ void __launch_bounds__(kThreads, 1) kv4_sdpa_tc_kernel(const SdpaArgs a, int* __restrict__ err) {
   using TR = MmaTraits<T>;
-  constexpr int G = S::kG;
+  constexpr int G = D / kGroup;
   extern __shared__ __align__(1024) uint8_t smem[];
-  uint8_t* ring = smem;
-  uint64_t* bars = (uint64_t*)(smem + S::kSlots * S::kBuf);
-  Meta* meta = (Meta*)(bars + 2 * S::kSlots + 8);
-  uint32_t* holder = (uint32_t*)(meta + kMeta);
-  const uint32_t bar_full = smem_u32(bars), bar_empty = bar_full + 8 * S::kSlots, bar_q = bar_empty + 8 * S::kSlots;
-  const uint32_t bar_s = bar_q + 8, bar_p = bar_s + 16, bar_o = bar_p + 16;
+  uint8_t* sQ = smem;
+  uint8_t* sK = sQ + G * kSlab;
+  uint8_t* sV = sK + G * kSlab;
+  uint64_t* bars = (uint64_t*)(sV + G * kSlab);
+  Meta* meta = (Meta*)(bars + kBars);
+  int* sE = (int*)(meta + kMeta);                 // exponent of each query row
+  uint32_t* holder = (uint32_t*)(sE + kRows);
+  const uint32_t bar0 = smem_u32(bars);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  constexpr int kIssuer = 4 + S::kUnpackWarps;
   if (threadIdx.x == 0) {
-    for (int i = 0; i < S::kSlots; ++i) {
-      mbar_init(bar_full + 8 * i, S::kUnpackWarps);
-      mbar_init(bar_empty + 8 * i, 1);
+    for (int i = 0; i < 4; ++i) {
+      mbar_init(bar0 + 8 * (kBarKFull + i), 4);
+      mbar_init(bar0 + 8 * (kBarKEmpty + i), 1);
+      mbar_init(bar0 + 8 * (kBarVFull + i), 1);
+      mbar_init(bar0 + 8 * (kBarVEmpty + i), 1);
     }
-    mbar_init(bar_q, 4);
     for (int i = 0; i < 2; ++i) {
-      mbar_init(bar_s + 8 * i, 1);
-      mbar_init(bar_p + 8 * i, 4);
-      mbar_init(bar_o + 8 * i, 1);
+      mbar_init(bar0 + 8 * (kBarS + i), 1);
+      mbar_init(bar0 + 8 * (kBarP + i), 4);
+      mbar_init(bar0 + 8 * (kBarO + i), 1);
+      mbar_init(bar0 + 8 * (kBarVMeta + i), 4);
     }
+    mbar_init(bar0 + 8 * kBarQ, 4);
     mbar_fence_init();
   }
   if (warp == kIssuer) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(holder)), "r"(S::kCols) : "memory");
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(holder)), "r"(kCols) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
   fence_before();
@@ -243,225 +330,159 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) kv4_sdpa_tc_kernel(cons
   const int k0 = split * per * kKeys;
   const int tiles = max(0, min(tiles_all - split * per, per));
 
-  if (warp >= 4 && warp < kIssuer) {
-    // ---------------- unpack ----------------
-    const int dw = warp - 4, half = dw & 1, g = dw >> 1, key = half * 32 + lane;
-    const dflash_kv4_cache* sides[2] = {&a.k, &a.v};
-    const uint8_t* codes[2];
-    const T *scales[2], *biases[2];
-#pragma unroll
-    for (int v = 0; v < 2; ++v) {
-      codes[v] = (const uint8_t*)(sides[v]->codes + b * sides[v]->codes_batch_stride + hk * sides[v]->codes_head_stride) + 32 * g;
-      scales[v] = (const T*)sides[v]->scales + b * sides[v]->scales_batch_stride + hk * sides[v]->scales_head_stride;
-      biases[v] = (const T*)sides[v]->biases + b * sides[v]->biases_batch_stride + hk * sides[v]->biases_head_stride;
-    }
-    auto load = [&](int tile, int v, Raw<D>& r) {
-      const int n = k0 + tile * kKeys + key;
-      if (tile < tiles && n < hi) {
-        const uint4* p = (const uint4*)(codes[v] + (size_t)n * (D / 2));
-        r.c0 = __ldg(p);
-        r.c1 = __ldg(p + 1);
-        const T *ps = scales[v] + (size_t)n * G, *pb = biases[v] + (size_t)n * G;
-        if (G == 4) {
-          const uint2 s = *(const uint2*)ps, z = *(const uint2*)pb;
-          r.s[0] = s.x; r.s[G / 2 - 1] = s.y;
-          r.b[0] = z.x; r.b[G / 2 - 1] = z.y;
-        } else {
-          r.s[0] = *(const uint32_t*)ps;
-          r.b[0] = *(const uint32_t*)pb;
-        }
-      } else {   // behind the range: zeros, which no row sees
-        r.c0 = r.c1 = make_uint4(0, 0, 0, 0);
-#pragma unroll
-        for (int i = 0; i < D / 128; ++i) r.s[i] = r.b[i] = 0;
-      }
-    };
-    constexpr int kAhead = 2;   // tiles in registers: about a memory latency of unpacking
-    Raw<D> rk[kAhead], rv[kAhead];
-#pragma unroll
-    for (int i = 0; i < kAhead; ++i) {
-      load(i, 0, rk[i]);
-      load(i, 1, rv[i]);
-    }
-    bool ok = true;
-    int slot = 0;
-    uint32_t phase = 1;   // the first pass over the ring does not wait
-    for (int t0 = 0; t0 < tiles && ok; t0 += kAhead) {
-#pragma unroll
-      for (int u = 0; u < kAhead; ++u) {
-        const int t = t0 + u;
-        if (t < tiles && ok) {
-          float s[G], z[G], sv[G], zv[G];
-          scales_of<T, D>(rk[u], s, z);
-          scales_of<T, D>(rv[u], sv, zv);
-          const int ek = block_exponent(s, z);
-          int ev;
-          const bool wide = wide_range(sv, zv, &ev);
-          if (!wide) ev = block_exponent(sv, zv);
-          bool bad = false;
-#pragma unroll
-          for (int i = 0; i < G; ++i) bad |= !finite(sv[i]) || !finite(zv[i]);
-          const uint32_t bads = __ballot_sync(0xffffffffu, bad);
-          if (g == 0 && lane == 0) {
-            Meta& m = meta[t & (kMeta - 1)];
-            m.k_factor[half] = pow2(ek);
-            m.v_exp[half] = ev;
-            m.bad[half] = bads;
-          }
-          float mine_s = s[0], mine_z = z[0], mine_sv = sv[0], mine_zv = zv[0];
-#pragma unroll
-          for (int i = 1; i < G; ++i)
-            if (i == g) { mine_s = s[i]; mine_z = z[i]; mine_sv = sv[i]; mine_zv = zv[i]; }
-          if (bad) mine_sv = mine_zv = 0.f;   // out of the products; rows that see it get NaN through its score
-#pragma unroll
-          for (int v = 0; v < 2; ++v) {
-            if (!wait_warp(bar_empty + 8 * slot, phase)) { atomicCAS(err, 0, 62 | (1 << 8)); ok = false; break; }
-            const uint32_t row = smem_u32(ring + slot * S::kBuf + g * S::kSlab + key * 128);
-            if (v == 0) {
-              unpack_row<D, false>(rk[u], mine_s, mine_z, ek, row, key);
-              load(t + kAhead, 0, rk[u]);
-            } else {
-              if (wide) unpack_row<D, true>(rv[u], mine_sv, mine_zv, ev, row, key);
-              else unpack_row<D, false>(rv[u], mine_sv, mine_zv, ev, row, key);
-              load(t + kAhead, 1, rv[u]);
-            }
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // the tensor pipe reads what was stored
-            __syncwarp();
-            if (lane == 0) mbar_arrive(bar_full + 8 * slot);
-            if (++slot == S::kSlots) { slot = 0; phase ^= 1; }
-          }
-        }
-      }
-    }
+  if (warp >= kKeyWarp && warp < kValueWarp) {
+    unpack_side<T, D, false>(a.k, b, hk, k0, hi, tiles, sK, bar0, meta, err);
+  } else if (warp >= kValueWarp && warp < kIssuer) {
+    unpack_side<T, D, true>(a.v, b, hk, k0, hi, tiles, sV, bar0, meta, err);
   } else if (warp == kIssuer) {
     // ---------------- MMA issue ----------------
-    if (lane == 0 && tiles > 0) {
-      bool ok = wait_bar(bar_q, 0);
-      if (!ok) atomicCAS(err, 0, 62 | (2 << 8));
-      fence_after();
-      for (int i = 0; i <= tiles && ok; ++i) {
+    if (lane == 0) {
+      bool ok = wait_bar(bar0 + 8 * kBarQ, 0);
+      if (!ok) atomicCAS(err, 0, 62 | (9 << 8));
+      for (int i = 0; i <= tiles && ok && tiles > 0; ++i) {
         if (i < tiles) {   // S(i) = Q K(i)^T
-          const int seq = 2 * i, slot = seq % S::kSlots;
-          if (!wait_bar(bar_full + 8 * slot, (seq / S::kSlots) & 1)) { atomicCAS(err, 0, 62 | (3 << 8)); ok = false; break; }
-          fence_after();
-          const uint32_t d = tmem + S::kSCol + 64u * (i & 1);
+          const uint32_t d = tmem + 128u * (i & 1);
+          for (int g = 0; g < G && ok; ++g) {
+            if (!wait_bar(bar0 + 8 * (kBarKFull + g), i & 1)) { atomicCAS(err, 0, 62 | (3 << 8)); ok = false; break; }
+            fence_after();
+            const uint64_t da = desc_k(smem_u32(sQ + g * kSlab)), db = desc_k(smem_u32(sK + g * kSlab));
 #pragma unroll
-          for (int ks = 0; ks < D / 16; ++ks)
-            mma_ts(d, tmem + S::kQCol + 8u * ks, desc_k(smem_u32(ring + slot * S::kBuf + (ks >> 2) * S::kSlab)) + 2 * (ks & 3),
-                   idesc(kKeys, false), ks ? 1u : 0u);
-          commit(bar_empty + 8 * slot);
-          commit(bar_s + 8 * (i & 1));
+            for (int j = 0; j < 4; ++j) mma_ss(d, da + 2 * j, db + 2 * j, idesc(kKeys, false), (g | j) ? 1u : 0u);
+            commit(bar0 + 8 * (kBarKEmpty + g));
+          }
+          if (!ok) break;
+          commit(bar0 + 8 * (kBarS + (i & 1)));
         }
-        if (i > 0) {       // O += P(j) V(j)
-          const int j = i - 1, seq = 2 * j + 1, slot = seq % S::kSlots;
-          if (!wait_bar(bar_p + 8 * (j & 1), (j >> 1) & 1)) { atomicCAS(err, 0, 62 | (4 << 8)); ok = false; break; }
-          if (!wait_bar(bar_full + 8 * slot, (seq / S::kSlots) & 1)) { atomicCAS(err, 0, 62 | (5 << 8)); ok = false; break; }
-          fence_after();
-          const uint64_t dv = desc_mn(smem_u32(ring + slot * S::kBuf), S::kSlab);
+        if (i > 0) {       // O += P(n) V(n); the score tile after next, which takes P(n)'s columns, is issued behind it
+          const int n = i - 1;
+          if (!wait_bar(bar0 + 8 * (kBarP + (n & 1)), (n >> 1) & 1)) { atomicCAS(err, 0, 62 | (4 << 8)); ok = false; break; }
+          for (int blk = 0; blk < 4 && ok; ++blk) {
+            if (!wait_bar(bar0 + 8 * (kBarVFull + blk), n & 1)) { atomicCAS(err, 0, 62 | (5 << 8)); ok = false; break; }
+            fence_after();
+            const uint64_t dv = desc_mn(smem_u32(sV + blk * 32 * 128), kSlab);
 #pragma unroll
-          for (int ks = 0; ks < kKeys / 16; ++ks)   // 16 keys = two 1024-byte groups; P: 8 columns (16 fp16)
-            mma_ts(tmem + S::kOCol, tmem + S::kSCol + 64u * (j & 1) + 8u * ks, dv + (uint64_t)(ks * (2048 >> 4)), idesc(D, true),
-                   (j | ks) ? 1u : 0u);
-          commit(bar_empty + 8 * slot);
-          commit(bar_o + 8 * (j & 1));
+            for (int j = 0; j < 2; ++j)   // 16 keys = two 1024-byte groups; P: 8 columns (16 fp16)
+              mma_ts(tmem + kOCol, tmem + 128u * (n & 1) + 8u * (2 * blk + j), dv + (uint64_t)(j * (2048 >> 4)), idesc(D, true),
+                     (n | blk | j) ? 1u : 0u);
+            commit(bar0 + 8 * (kBarVEmpty + blk));
+          }
+          if (!ok) break;
+          commit(bar0 + 8 * (kBarO + (n & 1)));
         }
       }
     }
     __syncwarp();
   } else {
     // ---------------- softmax: thread = query row ----------------
-    const int row = row0 + warp * 32 + lane;
+    const int r = warp * 32 + lane, row = row0 + r;
     const bool row_ok = row < a.rows;
+    const bool live = row0 + warp * 32 < a.rows;
     const uint32_t lanes = (uint32_t)(warp * 32) << 16;
     const int t = row_ok ? row / a.gqa : 0, h = hk * a.gqa + (row_ok ? row % a.gqa : 0);
-    // Q: the row's largest exponent, then fp16 in the channel order of unpack_row
-    const uint4* q = (const uint4*)((const T*)a.q + b * a.q_sb + h * a.q_sh + t * a.q_st);
-    float big = 0.f;
-    for (int i = 0; i < D / 8; ++i) {
-      const uint4 x = row_ok ? q[i] : make_uint4(0, 0, 0, 0);
-      const uint32_t u[4] = {x.x, x.y, x.z, x.w};
+    // Q: a row per D / 8 lanes, brought to fp16 by a power of two (its largest element to [2^7, 2^8)) in unpack_row's channel order;
+    // the scale's sign goes with it, so that scores grow with their products
+    {
+      constexpr int kLanes = D / 8, kPer = 32 / kLanes, kBatch = 16;
+      const int j = lane % kLanes;
+#pragma unroll 1
+      for (int r0 = warp * 32; r0 < warp * 32 + 32; r0 += kBatch * kPer) {
+        uint4 x[kBatch];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float f = TR::bits_to_float((uint16_t)(u[e >> 1] >> (16 * (e & 1))));
-        big = fmaxf(big, finite(f) ? fabsf(f) : 0.f);
-      }
-    }
-    const int eq = min(max((int)(__float_as_uint(big) >> 23) - 127 - 7, -100), 126);   // largest element in [2^7, 2^8)
-    const float to_q = a.scale < 0.f ? -pow2(-eq) : pow2(-eq);   // the scale's sign goes with q: scores then grow with their products
-    for (int i0 = 0; i0 < D / 8; i0 += 4) {
-      uint32_t w[16];
+        for (int i = 0; i < kBatch; ++i) {
+          const int row = row0 + r0 + i * kPer + lane / kLanes;
+          x[i] = make_uint4(0, 0, 0, 0);
+          if (row < a.rows) {
+            const int t = row / a.gqa, h = hk * a.gqa + row % a.gqa;
+            x[i] = *(const uint4*)((const T*)a.q + b * a.q_sb + h * a.q_sh + t * a.q_st + 8 * j);
+          }
+        }
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const uint4 x = row_ok ? q[i0 + i] : make_uint4(0, 0, 0, 0);
-        const uint32_t u[4] = {x.x, x.y, x.z, x.w};
-        float f[8];
+        for (int i = 0; i < kBatch; ++i) {
+          const int r = r0 + i * kPer + lane / kLanes;
+          const uint32_t u[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+          float f[8], big = 0.f;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) f[e] = TR::bits_to_float((uint16_t)(u[e >> 1] >> (16 * (e & 1)))) * to_q;
+          for (int e = 0; e < 8; ++e) {
+            f[e] = TR::bits_to_float((uint16_t)(u[e >> 1] >> (16 * (e & 1))));
+            big = fmaxf(big, finite(f[e]) ? fabsf(f[e]) : 0.f);
+          }
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const __half2 p = __floats2half2_rn(f[e], f[4 + e]);
-          w[4 * i + e] = *(const uint32_t*)&p;
+          for (int o = 1; o < kLanes; o <<= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, o));
+          const int eq = min(max((int)(__float_as_uint(big) >> 23) - 127 - 7, -100), 126);
+          const float to_q = a.scale < 0.f ? -pow2(-eq) : pow2(-eq);
+          uint32_t p[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const __half2 hh = __floats2half2_rn(f[e] * to_q, f[4 + e] * to_q);
+            p[e] = *(const uint32_t*)&hh;
+          }
+          *(uint4*)(sQ + (j >> 3) * kSlab + r * 128 + (((j & 7) ^ (r & 7)) << 4)) = make_uint4(p[0], p[1], p[2], p[3]);
+          if (j == 0) sE[r] = eq;
         }
       }
-      st16(tmem + lanes + S::kQCol + 4 * i0, w);
     }
-    wait_st();
-    fence_before();
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     __syncwarp();
-    if (lane == 0) mbar_arrive(bar_q);
-
-    const float c_row = fabsf(a.scale) * pow2(eq);
+    if (lane == 0) mbar_arrive(bar0 + 8 * kBarQ);
+    const float c_row = fabsf(a.scale) * pow2(sE[r]);
     // last key the row sees; rows behind the last one compute what nobody reads
     const int lim = row_ok ? min(len - a.T + t, hi - 1) : (kMask ? -1 : 0x7FFFFFFF);
-    const bool live = row0 + warp * 32 < a.rows;
     const long long mat = kMask && row_ok ? b * a.m_sb + h * a.m_sh + t * a.m_st : 0;
     float m = -INFINITY, l = 0.f;
     int ev = -200;   // exponent that O carries
     bool ok = true;
     for (int i = 0; i < tiles; ++i) {
-      if (!wait_warp(bar_s + 8 * (i & 1), (i >> 1) & 1)) { atomicCAS(err, 0, 62 | (6 << 8)); ok = false; break; }
+      if (!wait_warp(bar0 + 8 * (kBarS + (i & 1)), (i >> 1) & 1) || !wait_warp(bar0 + 8 * (kBarVMeta + (i & 1)), (i >> 1) & 1)) {
+        atomicCAS(err, 0, 62 | (6 << 8));
+        ok = false;
+        break;
+      }
       fence_after();
       if (!live) {   // P is whatever is there: lanes of their own
         fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(bar_p + 8 * (i & 1));
+        if (lane == 0) mbar_arrive(bar0 + 8 * (kBarP + (i & 1)));
         continue;
       }
-      const uint32_t s_col = tmem + lanes + S::kSCol + 64u * (i & 1);
-      uint32_t v[64];
-      ld32(s_col, v);
-      ld32(s_col + 32, v + 32);
-      const Meta mt = meta[i & (kMeta - 1)];
+      const uint32_t s_col = tmem + lanes + 128u * (i & 1);
+      const Meta& mt = meta[i & (kMeta - 1)];
       const int n0 = k0 + i * kKeys;
-      wait_ld();
-      float c[2] = {c_row * mt.k_factor[0], c_row * mt.k_factor[1]};
-      const bool plain = !kMask && (mt.bad[0] | mt.bad[1]) == 0 && __all_sync(0xffffffffu, n0 + kKeys - 1 <= lim);
+      const bool plain = !kMask && (mt.bad[0] | mt.bad[1] | mt.bad[2] | mt.bad[3]) == 0 && __all_sync(0xffffffffu, n0 + kKeys - 1 <= lim);
       float top = -INFINITY;
-      if (plain) {
-        float t0 = -INFINITY, t1 = -INFINITY;
 #pragma unroll
-        for (int e = 0; e < 32; ++e) {
-          t0 = fmaxf(t0, __uint_as_float(v[e]));
-          t1 = fmaxf(t1, __uint_as_float(v[32 + e]));
-        }
-        top = fmaxf(t0 * c[0], t1 * c[1]);
-      } else {
+      for (int q0 = 0; q0 < 4; q0 += 2) {   // 64 keys at a time
+        uint32_t v[64];
+        ld32(s_col + 32 * q0, v);
+        ld32(s_col + 32 * q0 + 32, v + 32);
+        wait_ld();
+        if (plain) {
+          float t0 = -INFINITY, t1 = -INFINITY;
 #pragma unroll
-        for (int e = 0; e < 64; ++e) {
-          const int n = n0 + e;
-          float x = __uint_as_float(v[e]) * c[e >> 5];
-          if ((mt.bad[e >> 5] >> (e & 31)) & 1) x = __int_as_float(0x7FC00000);
-          if (n <= lim) {
-            if (kMask) x = apply_mask<T>(a, x, mat + n * a.m_sn);
-          } else {
-            x = -INFINITY;
+          for (int e = 0; e < 32; ++e) {
+            t0 = fmaxf(t0, __uint_as_float(v[e]));
+            t1 = fmaxf(t1, __uint_as_float(v[32 + e]));
           }
-          top = fmaxf(top, x);
-          v[e] = __float_as_uint(x);
+          top = fmaxf(top, fmaxf(t0 * (c_row * mt.k_factor[q0]), t1 * (c_row * mt.k_factor[q0 + 1])));
+        } else {   // scores as the row sees them, back into their columns
+#pragma unroll
+          for (int e = 0; e < 64; ++e) {
+            const int n = n0 + 32 * q0 + e;
+            float x = __uint_as_float(v[e]) * (c_row * mt.k_factor[q0 + (e >> 5)]);
+            if ((mt.bad[q0 + (e >> 5)] >> (e & 31)) & 1) x = __int_as_float(0x7FC00000);
+            if (n <= lim) {
+              if (kMask) x = apply_mask<T>(a, x, mat + n * a.m_sn);
+            } else {
+              x = -INFINITY;
+            }
+            top = fmaxf(top, x);
+            v[e] = __float_as_uint(x);
+          }
+#pragma unroll
+          for (int e = 0; e < 64; e += 16) st16(s_col + 32 * q0 + e, v + e);
+          wait_st();
         }
-        c[0] = c[1] = 1.f;
       }
-      const int ev_tile = max(mt.v_exp[0], mt.v_exp[1]);
+      const int ev_tile = max(max(mt.v_exp[0], mt.v_exp[1]), max(mt.v_exp[2], mt.v_exp[3]));
       if (__any_sync(0xffffffffu, top > m + kMaxStep) || ev_tile > ev) {
         const float m_new = fmaxf(m, top);
         const int ev_new = max(ev, ev_tile);
@@ -470,16 +491,16 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) kv4_sdpa_tc_kernel(cons
         l *= f;
         m = m_new;
         if (i > 0) {
-          if (!wait_warp(bar_o + 8 * ((i - 1) & 1), ((i - 1) >> 1) & 1)) { atomicCAS(err, 0, 62 | (7 << 8)); ok = false; break; }
+          if (!wait_warp(bar0 + 8 * (kBarO + ((i - 1) & 1)), ((i - 1) >> 1) & 1)) { atomicCAS(err, 0, 62 | (7 << 8)); ok = false; break; }
           fence_after();
           for (int c0 = 0; c0 < D; c0 += 32) {
             uint32_t o[32];
-            ld32(tmem + lanes + S::kOCol + c0, o);
+            ld32(tmem + lanes + kOCol + c0, o);
             wait_ld();
 #pragma unroll
             for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * fo);
-            st16(tmem + lanes + S::kOCol + c0, o);
-            st16(tmem + lanes + S::kOCol + c0 + 16, o + 16);
+            st16(tmem + lanes + kOCol + c0, o);
+            st16(tmem + lanes + kOCol + c0 + 16, o + 16);
           }
           wait_st();
         }
@@ -487,14 +508,17 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) kv4_sdpa_tc_kernel(cons
       }
       const float ref = m == -INFINITY ? 0.f : m;
 #pragma unroll
-      for (int hf = 0; hf < 2; ++hf) {
-        const float shift = kPShift + (float)max(mt.v_exp[hf] - ev, -100);   // P carries V's power of two
-        const float cl = c[hf] * kLog2e, off = shift - ref * kLog2e;
+      for (int q = 0; q < 4; ++q) {
+        uint32_t v[32];
+        ld32(s_col + 32 * q, v);
+        wait_ld();
+        const float shift = kPShift + (float)max(mt.v_exp[q] - ev, -100);   // P carries V's power of two
+        const float cl = plain ? c_row * mt.k_factor[q] * kLog2e : kLog2e, off = shift - ref * kLog2e;
         float sum0 = 0.f, sum1 = 0.f;
         uint32_t w[16];
 #pragma unroll
         for (int e = 0; e < 32; e += 2) {
-          const float x0 = __uint_as_float(v[32 * hf + e]), x1 = __uint_as_float(v[32 * hf + e + 1]);
+          const float x0 = __uint_as_float(v[e]), x1 = __uint_as_float(v[e + 1]);
           float p0, p1;
           if (kMask) {   // scores may be the lowest finite value: their difference first
             p0 = ex2(fmaf(x0 - ref, kLog2e, shift));
@@ -509,63 +533,71 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) kv4_sdpa_tc_kernel(cons
           w[e >> 1] = *(const uint32_t*)&p;
         }
         l = fmaf(sum0 + sum1, ex2(-shift), l);
-        st16(s_col + 16 * hf, w);   // over scores that are in registers
+        st16(s_col + 16 * q, w);   // over columns that have been read
       }
       wait_st();
       fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(bar_p + 8 * (i & 1));
+      if (lane == 0) mbar_arrive(bar0 + 8 * (kBarP + (i & 1)));
     }
-    // ---- epilogue ----
+    // ---- epilogue: the row goes through shared memory (all of Q, K and V is spent), so that it leaves as one bulk copy ----
     // the last product; the one two before it is done (its successor's scores were), so the phase cannot be mistaken
-    if (tiles > 0 && ok && !wait_warp(bar_o + 8 * ((tiles - 1) & 1), ((tiles - 1) >> 1) & 1)) { atomicCAS(err, 0, 62 | (8 << 8)); ok = false; }
+    if (tiles > 0 && ok && !wait_warp(bar0 + 8 * (kBarO + ((tiles - 1) & 1)), ((tiles - 1) >> 1) & 1)) { atomicCAS(err, 0, 62 | (8 << 8)); ok = false; }
     fence_after();
     const bool have = tiles > 0 && ok;
-    const float undo = pow2(min(max(ev - (int)kPShift, -126), 127));
-    const bool last = a.splits == 1;
-    const float inv = l == 0.f ? 1.f : 1.f / l, nan = l * 0.f;   // a row that sees nothing yields zeros; NaN reaches the whole row
-    const size_t at = ((size_t)bhk * a.rows + row) * a.splits + split;
-    for (int c0 = 0; c0 < D; c0 += 32) {
-      uint32_t o[32];
-      if (have) {
-        ld32(tmem + lanes + S::kOCol + c0, o);
-        wait_ld();
-      }
-      float y[32];   // back to the channels' order
+    if (live) {
+      const float undo = pow2(min(max(ev - (int)kPShift, -126), 127));
+      const bool last = a.splits == 1;
+      const float inv = l == 0.f ? 1.f : 1.f / l, nan = l * 0.f;   // a row that sees nothing yields zeros; NaN reaches the whole row
+      const size_t at = ((size_t)bhk * a.rows + row) * a.splits + split;
+      uint8_t* stage = smem + r * (D * 4 + 16);   // rows 16 bytes apart modulo 128: no bank conflicts
+      for (int c0 = 0; c0 < D; c0 += 32) {
+        uint32_t o[32];
+        if (have) {
+          ld32(tmem + lanes + kOCol + c0, o);
+          wait_ld();
+        }
+        float y[32];   // back to the channels' order
 #pragma unroll
-      for (int e = 0; e < 32; ++e) y[(e & ~7) + ((e & 1) << 2) + ((e & 7) >> 1)] = have ? __uint_as_float(o[e]) * undo : 0.f;
-      if (row_ok) {
+        for (int e = 0; e < 32; ++e) y[(e & ~7) + ((e & 1) << 2) + ((e & 7) >> 1)] = have ? __uint_as_float(o[e]) * undo : 0.f;
         if (last) {
-          T* dst = (T*)a.out + out_row(a, b, hk, row) * D + c0;
 #pragma unroll
           for (int e = 0; e < 32; e += 8) {
             T z[8];
 #pragma unroll
             for (int x = 0; x < 8; ++x) z[x] = TR::from_float(nan == 0.f ? y[e + x] * inv : nan);
-            *(uint4*)(dst + e) = *(const uint4*)z;
+            *(uint4*)(stage + (c0 + e) * 2) = *(const uint4*)z;
           }
         } else {
-          float4* dst = (float4*)(a.part_o + at * D + c0);
 #pragma unroll
-          for (int e = 0; e < 32; e += 4) dst[e >> 2] = make_float4(y[e], y[e + 1], y[e + 2], y[e + 3]);
+          for (int e = 0; e < 32; e += 4) *(float4*)(stage + (c0 + e) * 4) = make_float4(y[e], y[e + 1], y[e + 2], y[e + 3]);
         }
       }
-    }
-    if (row_ok && !last) {
-      a.part_m[at] = m;
-      a.part_l[at] = l;
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      if (row_ok) {
+        const void* dst = last ? (const void*)((T*)a.out + out_row(a, b, hk, row) * D) : (const void*)(a.part_o + at * D);
+        asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(dst), "r"(smem_u32(stage)), "r"(last ? D * 2 : D * 4)
+                     : "memory");
+        if (!last) {
+          a.part_m[at] = m;
+          a.part_l[at] = l;
+        }
+      }
+      asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+      asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
     }
   }
   fence_before();
   __syncthreads();
   if (warp == kIssuer)
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(S::kCols) : "memory");
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kCols) : "memory");
 }
 
 template <typename T, int D>
 int launch(const SdpaArgs& a, cudaStream_t st, int device) {
-  using S = Shape<D>;
-  constexpr size_t smem = (size_t)S::kSlots * S::kBuf + (2 * S::kSlots + 8) * 8 + kMeta * sizeof(Meta) + 16;
+  constexpr size_t tiles = (size_t)3 * (D / kGroup) * kSlab, rest = kBars * 8 + kMeta * sizeof(Meta) + kRows * 4 + 16;
+  static_assert(kRows * (D * 4 + 16) <= tiles, "the epilogue's rows fit where Q, K and V were");
+  constexpr size_t smem = tiles + rest;
   static_assert(smem <= 227 * 1024, "shared memory");
   auto kern = a.mask_kind ? kv4_sdpa_tc_kernel<T, D, true> : kv4_sdpa_tc_kernel<T, D, false>;
   static std::mutex mu;
@@ -582,7 +614,7 @@ int launch(const SdpaArgs& a, cudaStream_t st, int device) {
   int* err = device_error_word(device);
   if (!err) return fail(DFLASH_ERR_LAUNCH, "kv4_sdpa: no device error word");
   const dim3 grid(a.splits, (a.rows + kRows - 1) / kRows, a.B * a.Hk);
-  cudaError_t e = launch_kernel(kern, grid, dim3(S::kThreads), smem, st, a, err);
+  cudaError_t e = launch_kernel(kern, grid, dim3(kThreads), smem, st, a, err);
   if (e == cudaSuccess) e = cudaGetLastError();
   return e == cudaSuccess ? DFLASH_OK : fail(DFLASH_ERR_LAUNCH, "kv4_sdpa (tcgen05) launch: %s", cudaGetErrorString(e));
 }
