@@ -5,12 +5,15 @@
 // in tiles of 128: two score tiles and the output fill tensor memory (2 x 128 + 256 columns; narrower score tiles ran at half
 // rate, an M128 N64 MMA taking as long as N128).  Keys and values are unpacked to fp16 into 128B-swizzled shared memory: a slab
 // per 64 channels (one quantisation group), rows of keys of 128 bytes, which is K-major for S = Q K^T and MN-major for O = P V.
-//   warps 0-3   softmax, a thread per row: S from tensor memory, P back over it, O rescaled in place when the maximum moved
-//   warps 4-7   unpack keys, 8-11 values: a thread owns a key, a group at a time
-//   warp 12     one thread issues the MMAs in the order QK(0) QK(1) PV(0) QK(2) PV(1) ..., so that a tile's softmax runs under
-//               the next tile's scores
-// One tile of keys and one of values are enough: a slab of keys is free as soon as its four steps of QK(i) are done and is
-// refilled under PV(i-1), values (in blocks of 32 keys) the other way round.
+//   warps 0-7    softmax, a thread per row: S from tensor memory, P back over it, O rescaled in place when the maximum moved.  Warps
+//                0-3 take the even tiles and 4-7 the odd ones (one warp per SM sub-partition left the softmax latency bound:
+//                4300 clocks a tile); a row's reference maximum is handed from one to the other right after a tile's maxima
+//   warps 8-11   unpack keys, 12-15 values: a thread owns a key, a group at a time
+//   warp 16      one thread issues S(i) = Q K(i)^T, warp 17 O += P(i) V(i): issuing an MMA blocks until the pipe has room and a
+//                satisfied wait costs about 100 cycles of it, so each thread waits under the other one's MMAs
+// Two score tiles are in flight: a tile's softmax runs under the next one's scores.  One tile of keys and one of values are
+// enough: a slab of keys is free as soon as its four steps of QK(i) are done and is refilled under PV(i-1), values (in blocks of
+// 32 keys) the other way round.
 //
 // Unpacking costs 9 instructions for 8 codes: a nibble left in place is an fp16 subnormal, code * 2^-24 (or * 2^-20), and one packed
 // fma turns two of them into code * scale + bias with a single rounding to fp16 (2^-11; the cache's scales carry 8 or 11 bits,
@@ -29,7 +32,7 @@ namespace {
 
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr int kRows = 128, kKeys = 128;
-constexpr int kThreads = 13 * 32, kKeyWarp = 4, kValueWarp = 8, kIssuer = 12;
+constexpr int kThreads = 18 * 32, kKeyWarp = 8, kValueWarp = 12, kIssuer = 16;   // kIssuer: scores; the next warp: output
 constexpr float kMaxStep = 8 * kLn2;   // natural units
 constexpr float kPShift = 6.f;         // P = p * 2^6 (p <= 2^8): further from fp16's subnormals
 constexpr int kSlab = kKeys * 128;     // 128 rows x 64 channels: Q, K or V
@@ -42,10 +45,12 @@ struct Meta {
   int v_exp[4];
   uint32_t bad[4];
 };
-constexpr int kMeta = 4;   // keys are unpacked at most two tiles ahead of the softmax
+constexpr int kMeta = 4;   // scales are looked at no more than three tiles ahead of the softmax
 
-// mbarriers, 8 bytes each
-enum { kBarKFull = 0, kBarKEmpty = 4, kBarVFull = 8, kBarVEmpty = 12, kBarS = 16, kBarP = 18, kBarO = 20, kBarVMeta = 22, kBarQ = 24, kBars = 26 };
+// mbarriers, 8 bytes each.  kBarVMeta: a tile's exponents of V are known; kBarM: a row reference handed on, per tile
+// parity and 32 rows
+enum { kBarKFull = 0, kBarVFull = 1, kBarQ = 2, kBarKEmpty = 4, kBarVEmpty = 8, kBarS = 12, kBarP = 14, kBarO = 16, kBarM = 18,
+       kBarVMeta = 26, kBars = 30 };
 
 __device__ __forceinline__ bool wait_bar(uint32_t bar, uint32_t parity) {
   for (uint32_t i = 0; i < (1u << 16); ++i) {   // hardware-suspended polls of up to a microsecond
@@ -121,19 +126,11 @@ __device__ __forceinline__ constexpr uint32_t idesc(int n, bool b_mn) {
 __device__ __forceinline__ float pow2(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }   // -126 <= e <= 127
 __device__ __forceinline__ bool finite(float x) { return (__float_as_uint(x) & 0x7F800000u) != 0x7F800000u; }
 
-template <int D>
-struct Raw {   // one key: codes, scales and biases of every group
-  uint4 c[D / 32];
-  uint32_t s[D / 128], b[D / 128];
-};
-
+// Scales (or biases) of one key from their packed pairs.
 template <typename T, int D>
-__device__ __forceinline__ void scales_of(const Raw<D>& r, float (&s)[D / kGroup], float (&b)[D / kGroup]) {
+__device__ __forceinline__ void scales_of(const uint32_t (&r)[D / 128], float (&s)[D / kGroup]) {
 #pragma unroll
-  for (int g = 0; g < D / kGroup; ++g) {
-    s[g] = MmaTraits<T>::bits_to_float((uint16_t)(r.s[g >> 1] >> (16 * (g & 1))));
-    b[g] = MmaTraits<T>::bits_to_float((uint16_t)(r.b[g >> 1] >> (16 * (g & 1))));
-  }
+  for (int g = 0; g < D / kGroup; ++g) s[g] = MmaTraits<T>::bits_to_float((uint16_t)(r[g >> 1] >> (16 * (g & 1))));
 }
 // Exponent e shared by the warp's 32 keys: scale * 2^-e < 2^-9 and |bias| * 2^-e < 2^14 for the finite ones.
 template <int G>
@@ -172,6 +169,60 @@ __device__ __forceinline__ bool wide_range(const float (&s)[G], const float (&b)
   *e = min(max(hi - 127 - 13, -100), 126);
   return hi - lo > 6 && lo < 255;
 }
+// fp32 pairs: one instruction for two lanes of arithmetic
+__device__ __forceinline__ uint64_t pair(float x, float y) {
+  uint64_t d;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(x), "f"(y));
+  return d;
+}
+__device__ __forceinline__ void unpair(uint64_t d, float& x, float& y) { asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(d)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t x, uint64_t y, uint64_t z) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(x), "l"(y), "l"(z));
+  return d;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t x, uint64_t y) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(x), "l"(y));
+  return d;
+}
+// Bit e: byte mask entry of key n0 + e is not 0, for the bits set in `want` (others are not read).
+__device__ __forceinline__ uint32_t mask_bits(const SdpaArgs& a, long long at, int n0, uint32_t want) {
+  const uint8_t* p = (const uint8_t*)a.mask + at + (long long)n0 * a.m_sn;
+  uint32_t bits = 0;
+  if (want == 0xFFFFFFFFu && a.m_sn == 1 && ((uintptr_t)p & 3) == 0) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      uint32_t x = *(const uint32_t*)(p + 4 * i);
+      x = __vcmpne4(x, 0) & 0x08040201u;              // a bit of its own per byte
+      bits |= (((x * 0x01010101u) >> 24) & 15u) << (4 * i);
+    }
+  } else if (want) {
+#pragma unroll 8
+    for (int e = 0; e < 32; ++e)
+      if ((want >> e) & 1) bits |= (uint32_t)(p[e * a.m_sn] != 0) << e;
+  }
+  return bits;
+}
+// Keys n0 .. n0 + 31 that a row sees: up to `lim`, and where a byte mask lets it.
+template <int kMask>
+__device__ __forceinline__ uint32_t seen_bits(const SdpaArgs& a, long long at, int n0, int lim) {
+  const int left = lim - n0;   // below 0: none, from 31: all
+  const uint32_t seen = left < 0 ? 0u : left >= 31 ? 0xFFFFFFFFu : (2u << left) - 1u;
+  return kMask == 1 ? mask_bits(a, at, n0, seen) : seen;
+}
+// Per half, the larger magnitude of two pairs (the sign bits are to be ignored).
+template <typename T> __device__ __forceinline__ uint32_t abs_max(uint32_t x, uint32_t y);
+template <> __device__ __forceinline__ uint32_t abs_max<__nv_bfloat16>(uint32_t x, uint32_t y) {
+  x &= 0x7FFF7FFFu; y &= 0x7FFF7FFFu;
+  const __nv_bfloat162 m = __hmax2(*(const __nv_bfloat162*)&x, *(const __nv_bfloat162*)&y);
+  return *(const uint32_t*)&m;
+}
+template <> __device__ __forceinline__ uint32_t abs_max<__half>(uint32_t x, uint32_t y) {
+  x &= 0x7FFF7FFFu; y &= 0x7FFF7FFFu;
+  const __half2 m = __hmax2(*(const __half2*)&x, *(const __half2*)&y);
+  return *(const uint32_t*)&m;
+}
 // 64 codes -> a swizzled 128-byte row; the eight codes of a word land in the order 0 4 1 5 2 6 3 7.  Narrow: the nibbles are
 // fp16 subnormals and one fma makes the value (9 instructions a word); wide: the nibbles become whole numbers first (13).
 template <bool kWide>
@@ -201,34 +252,51 @@ __device__ __forceinline__ void unpack_row(const uint4& c0, const uint4& c1, flo
 }
 
 // The keys (kV = false) or values of a block's range, by the four warps of a side: thread = key of the tile.
-template <typename T, int D, bool kV>
-__device__ __forceinline__ void unpack_side(const dflash_kv4_cache& c, int b, int hk, int k0, int hi, int tiles, uint8_t* buf, uint32_t bar0,
-                                            Meta* meta, int* err) {
+template <int D>
+__device__ __forceinline__ int raw_chunk(int r, int ch) { return D == 256 ? ch ^ (r & 7) : ch ^ ((r >> 1) & 3); }
+template <typename T, int D, bool kV, typename F>
+__device__ __forceinline__ void unpack_side(const dflash_kv4_cache& c, int b, int hk, int k0, int hi, int tiles, uint8_t* buf, uint8_t* raw,
+                                            uint32_t bar0, Meta* meta, int* err, F query_rows) {
   constexpr int G = D / kGroup;
   const int w = (threadIdx.x >> 5) & 3, lane = threadIdx.x & 31, key = w * 32 + lane;
   const uint8_t* codes = (const uint8_t*)(c.codes + b * c.codes_batch_stride + hk * c.codes_head_stride);
   const T* scales = (const T*)c.scales + b * c.scales_batch_stride + hk * c.scales_head_stride;
   const T* biases = (const T*)c.biases + b * c.biases_batch_stride + hk * c.biases_head_stride;
-  auto load = [&](int tile, Raw<D>& r) {
-    const int n = k0 + tile * kKeys + key;
-    if (tile < tiles && n < hi) {
-      const uint4* p = (const uint4*)(codes + (size_t)n * (D / 2));
+  constexpr int kChunks = D / 32, kRowsAtOnce = 32 / kChunks;   // 16-byte chunks of a key, keys of one load
+  raw += w * 32 * (D / 2);
+  const uint32_t uraw = smem_u32(raw);
+  // This warp's 32 keys of a tile: codes by coalesced asynchronous copies (a lane loading its own key's row would touch 32 lines
+  // with every instruction, which measured as the kernel's bound), swizzled so that a lane then reads its row without bank
+  // conflicts; scales and biases to registers.  Behind the range: zeros, which no row sees.
+  auto load = [&](int tile) {
+    const int n0 = k0 + tile * kKeys + w * 32;
+    const bool in = tile < tiles;
+    if (in) {
 #pragma unroll
-      for (int i = 0; i < D / 32; ++i) r.c[i] = __ldg(p + i);
+      for (int i = 0; i < kChunks; ++i) {
+        const int r = i * kRowsAtOnce + lane / kChunks, ch = lane % kChunks;
+        const bool ok = n0 + r < hi;
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(uraw + r * (D / 2) + raw_chunk<D>(r, ch) * 16),
+                     "l"(codes + (size_t)(ok ? n0 + r : 0) * (D / 2) + ch * 16), "r"(ok ? 16 : 0)
+                     : "memory");
+      }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  auto load_scales = [&](int tile, uint32_t (&s)[D / 128], uint32_t (&z)[D / 128]) {
+    const int n = k0 + tile * kKeys + key;
+#pragma unroll
+    for (int i = 0; i < D / 128; ++i) s[i] = z[i] = 0;
+    if (tile < tiles && n < hi) {
       const T *ps = scales + (size_t)n * G, *pb = biases + (size_t)n * G;
       if (G == 4) {
-        const uint2 s = *(const uint2*)ps, z = *(const uint2*)pb;
-        r.s[0] = s.x; r.s[G / 2 - 1] = s.y;
-        r.b[0] = z.x; r.b[G / 2 - 1] = z.y;
+        const uint2 x = *(const uint2*)ps, y = *(const uint2*)pb;
+        s[0] = x.x; s[G / 2 - 1] = x.y;
+        z[0] = y.x; z[G / 2 - 1] = y.y;
       } else {
-        r.s[0] = *(const uint32_t*)ps;
-        r.b[0] = *(const uint32_t*)pb;
+        s[0] = *(const uint32_t*)ps;
+        z[0] = *(const uint32_t*)pb;
       }
-    } else {   // behind the range: zeros, which no row sees
-#pragma unroll
-      for (int i = 0; i < D / 32; ++i) r.c[i] = make_uint4(0, 0, 0, 0);
-#pragma unroll
-      for (int i = 0; i < D / 128; ++i) r.s[i] = r.b[i] = 0;
     }
   };
   auto done = [&](uint32_t bar) {
@@ -236,19 +304,18 @@ __device__ __forceinline__ void unpack_side(const dflash_kv4_cache& c, int b, in
     __syncwarp();
     if (lane == 0) mbar_arrive(bar);
   };
-  Raw<D> cur, next;
-  load(0, next);
-  bool ok = true;
-  for (int t = 0; t < tiles && ok; ++t) {
-    cur = next;
-    load(t + 1, next);   // in flight under this tile's unpacking and waits
-    float s[G], z[G];
-    scales_of<T, D>(cur, s, z);
-    int e;
-    bool wide = false;
+  // Scales of a tile, a tile ahead of its codes: what they say about the tile is published before the codes' buffer is free.
+  uint32_t ns[D / 128], nz[D / 128];
+  float s[G], z[G];
+  int e = 0;
+  bool wide = false;
+  auto prepare = [&](int tile) {
+    scales_of<T, D>(ns, s);
+    scales_of<T, D>(nz, z);
+    wide = false;
     if (kV) wide = wide_range(s, z, &e);
     if (!wide) e = block_exponent(s, z);
-    Meta& m = meta[t & (kMeta - 1)];
+    Meta& m = meta[tile & (kMeta - 1)];
     if (kV) {
       bool bad = false;
 #pragma unroll
@@ -258,29 +325,60 @@ __device__ __forceinline__ void unpack_side(const dflash_kv4_cache& c, int b, in
         for (int g = 0; g < G; ++g) s[g] = z[g] = 0.f;
       }
       const uint32_t bads = __ballot_sync(0xffffffffu, bad);
-      if (lane == 0) {
+      if (lane == 0 && tile < tiles) {
         m.v_exp[w] = e;
         m.bad[w] = bads;
-        mbar_arrive(bar0 + 8 * (kBarVMeta + (t & 1)));
+        mbar_arrive(bar0 + 8 * (kBarVMeta + (tile & (kMeta - 1))));
       }
-      // this warp's keys are one block of the values' buffer
-      if (!wait_warp(bar0 + 8 * (kBarVEmpty + w), (t & 1) ^ 1)) { atomicCAS(err, 0, 62 | (1 << 8)); ok = false; break; }
-    } else if (lane == 0) {
+    } else if (lane == 0 && tile < tiles) {
       m.k_factor[w] = pow2(e);
     }
+  };
+  load(0);
+  load_scales(0, ns, nz);
+  query_rows();   // the block's queries, while the first keys and values are on their way
+  prepare(0);
+  load_scales(1, ns, nz);
+  for (int t = 0; t < tiles; ++t) {
+    float cs[G], cz[G];
 #pragma unroll
+    for (int g = 0; g < G; ++g) { cs[g] = s[g]; cz[g] = z[g]; }
+    const int ce = e;
+    const bool cwide = wide;
+    if (kV) {
+      prepare(t + 1);
+      load_scales(t + 2, ns, nz);
+    }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+    __syncwarp();
+    // this warp's keys are one block of the values' buffer
+    if (kV && !wait_warp(bar0 + 8 * (kBarVEmpty + w), (t & 1) ^ 1)) { atomicCAS(err, 0, 62 | (1 << 8)); break; }
+    bool ok = true;
+#pragma unroll 1
     for (int g = 0; g < G; ++g) {
       if (!kV && !wait_warp(bar0 + 8 * (kBarKEmpty + g), (t & 1) ^ 1)) { atomicCAS(err, 0, 62 | (2 << 8)); ok = false; break; }
+      const uint4 c0 = *(const uint4*)(raw + lane * (D / 2) + raw_chunk<D>(lane, 2 * g) * 16);
+      const uint4 c1 = *(const uint4*)(raw + lane * (D / 2) + raw_chunk<D>(lane, 2 * g + 1) * 16);
+      float sg = cs[0], zg = cz[0];
+#pragma unroll
+      for (int i = 1; i < G; ++i)
+        if (i == g) { sg = cs[i]; zg = cz[i]; }
       const uint32_t row = smem_u32(buf + g * kSlab + key * 128);
-      if (kV && wide) unpack_row<true>(cur.c[2 * g], cur.c[2 * g + 1], s[g], z[g], e, row, key);
-      else unpack_row<false>(cur.c[2 * g], cur.c[2 * g + 1], s[g], z[g], e, row, key);
-      if (!kV) done(bar0 + 8 * (kBarKFull + g));
+      if (kV && cwide) unpack_row<true>(c0, c1, sg, zg, ce, row, key);
+      else unpack_row<false>(c0, c1, sg, zg, ce, row, key);
     }
-    if (kV) done(bar0 + 8 * (kBarVFull + w));
+    if (!ok) break;
+    done(bar0 + 8 * (kV ? kBarVFull : kBarKFull));
+    load(t + 1);
+    if (!kV) {   // a tile's factor is published with its codes: nothing waits for it before
+      prepare(t + 1);
+      load_scales(t + 2, ns, nz);
+    }
   }
+  asm volatile("cp.async.wait_group 0;" ::: "memory");
 }
 
-template <typename T, int D, bool kMask>
+template <typename T, int D, int kMask>   // 0 = no mask, 1 = bytes, 2 = additive
 __global__ void __launch_bounds__(kThreads, 1) kv4_sdpa_tc_kernel(const SdpaArgs a, int* __restrict__ err) {
   using TR = MmaTraits<T>;
   constexpr int G = D / kGroup;
@@ -288,26 +386,31 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_sdpa_tc_kernel(const SdpaArgs
   uint8_t* sQ = smem;
   uint8_t* sK = sQ + G * kSlab;
   uint8_t* sV = sK + G * kSlab;
-  uint64_t* bars = (uint64_t*)(sV + G * kSlab);
+  uint8_t* sRaw = sV + G * kSlab;                 // codes of the next tile: keys, then values
+  uint64_t* bars = (uint64_t*)(sRaw + kKeys * D);
   Meta* meta = (Meta*)(bars + kBars);
   int* sE = (int*)(meta + kMeta);                 // exponent of each query row
-  uint32_t* holder = (uint32_t*)(sE + kRows);
+  float* sRef = (float*)(sE + kRows);             // [2][128] reference maximum of a row after a tile
+  int* sEv = (int*)(sRef + 2 * kRows);            // [2][4] exponent that O carries
+  uint32_t* holder = (uint32_t*)(sEv + 8);
+  float2* sEnd = (float2*)sRaw;                   // [2][128] reference and sum of either half of the softmax, at the end
   const uint32_t bar0 = smem_u32(bars);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     for (int i = 0; i < 4; ++i) {
-      mbar_init(bar0 + 8 * (kBarKFull + i), 4);
       mbar_init(bar0 + 8 * (kBarKEmpty + i), 1);
-      mbar_init(bar0 + 8 * (kBarVFull + i), 1);
       mbar_init(bar0 + 8 * (kBarVEmpty + i), 1);
+      mbar_init(bar0 + 8 * (kBarVMeta + i), 4);
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(bar0 + 8 * (kBarS + i), 1);
       mbar_init(bar0 + 8 * (kBarP + i), 4);
       mbar_init(bar0 + 8 * (kBarO + i), 1);
-      mbar_init(bar0 + 8 * (kBarVMeta + i), 4);
     }
-    mbar_init(bar0 + 8 * kBarQ, 4);
+    for (int i = 0; i < 8; ++i) mbar_init(bar0 + 8 * (kBarM + i), 1);
+    mbar_init(bar0 + 8 * kBarQ, kIssuer);
+    mbar_init(bar0 + 8 * kBarKFull, 4);
+    mbar_init(bar0 + 8 * kBarVFull, 4);
     mbar_fence_init();
   }
   if (warp == kIssuer) {
@@ -330,92 +433,46 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_sdpa_tc_kernel(const SdpaArgs
   const int k0 = split * per * kKeys;
   const int tiles = max(0, min(tiles_all - split * per, per));
 
-  if (warp >= kKeyWarp && warp < kValueWarp) {
-    unpack_side<T, D, false>(a.k, b, hk, k0, hi, tiles, sK, bar0, meta, err);
-  } else if (warp >= kValueWarp && warp < kIssuer) {
-    unpack_side<T, D, true>(a.v, b, hk, k0, hi, tiles, sV, bar0, meta, err);
-  } else if (warp == kIssuer) {
-    // ---------------- MMA issue ----------------
-    if (lane == 0) {
-      bool ok = wait_bar(bar0 + 8 * kBarQ, 0);
-      if (!ok) atomicCAS(err, 0, 62 | (9 << 8));
-      for (int i = 0; i <= tiles && ok && tiles > 0; ++i) {
-        if (i < tiles) {   // S(i) = Q K(i)^T
-          const uint32_t d = tmem + 128u * (i & 1);
-          for (int g = 0; g < G && ok; ++g) {
-            if (!wait_bar(bar0 + 8 * (kBarKFull + g), i & 1)) { atomicCAS(err, 0, 62 | (3 << 8)); ok = false; break; }
-            fence_after();
-            const uint64_t da = desc_k(smem_u32(sQ + g * kSlab)), db = desc_k(smem_u32(sK + g * kSlab));
+  // Q: a row per D / 8 lanes, brought to fp16 by a power of two (its largest element to [2^7, 2^8)) in unpack_row's channel order;
+  // the scale's sign goes with it, so that scores grow with their products.  Sixteen warps, every sixteenth row each.
+  auto query_rows = [&]() {
+    constexpr int kLanes = D / 8, kPer = 32 / kLanes, kBatch = 4;
+    const int j = lane % kLanes;
+#pragma unroll 1
+    for (int i0 = 0; i0 * kIssuer * kPer < kRows; i0 += kBatch) {
+      uint4 x[kBatch];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) mma_ss(d, da + 2 * j, db + 2 * j, idesc(kKeys, false), (g | j) ? 1u : 0u);
-            commit(bar0 + 8 * (kBarKEmpty + g));
-          }
-          if (!ok) break;
-          commit(bar0 + 8 * (kBarS + (i & 1)));
-        }
-        if (i > 0) {       // O += P(n) V(n); the score tile after next, which takes P(n)'s columns, is issued behind it
-          const int n = i - 1;
-          if (!wait_bar(bar0 + 8 * (kBarP + (n & 1)), (n >> 1) & 1)) { atomicCAS(err, 0, 62 | (4 << 8)); ok = false; break; }
-          for (int blk = 0; blk < 4 && ok; ++blk) {
-            if (!wait_bar(bar0 + 8 * (kBarVFull + blk), n & 1)) { atomicCAS(err, 0, 62 | (5 << 8)); ok = false; break; }
-            fence_after();
-            const uint64_t dv = desc_mn(smem_u32(sV + blk * 32 * 128), kSlab);
-#pragma unroll
-            for (int j = 0; j < 2; ++j)   // 16 keys = two 1024-byte groups; P: 8 columns (16 fp16)
-              mma_ts(tmem + kOCol, tmem + 128u * (n & 1) + 8u * (2 * blk + j), dv + (uint64_t)(j * (2048 >> 4)), idesc(D, true),
-                     (n | blk | j) ? 1u : 0u);
-            commit(bar0 + 8 * (kBarVEmpty + blk));
-          }
-          if (!ok) break;
-          commit(bar0 + 8 * (kBarO + (n & 1)));
+      for (int i = 0; i < kBatch; ++i) {
+        const int r = ((i0 + i) * kIssuer + warp) * kPer + lane / kLanes, row = row0 + r;
+        x[i] = make_uint4(0, 0, 0, 0);
+        if (r < kRows && row < a.rows) {
+          const int t = row / a.gqa, h = hk * a.gqa + row % a.gqa;
+          x[i] = *(const uint4*)((const T*)a.q + b * a.q_sb + h * a.q_sh + t * a.q_st + 8 * j);
         }
       }
-    }
-    __syncwarp();
-  } else {
-    // ---------------- softmax: thread = query row ----------------
-    const int r = warp * 32 + lane, row = row0 + r;
-    const bool row_ok = row < a.rows;
-    const bool live = row0 + warp * 32 < a.rows;
-    const uint32_t lanes = (uint32_t)(warp * 32) << 16;
-    const int t = row_ok ? row / a.gqa : 0, h = hk * a.gqa + (row_ok ? row % a.gqa : 0);
-    // Q: a row per D / 8 lanes, brought to fp16 by a power of two (its largest element to [2^7, 2^8)) in unpack_row's channel order;
-    // the scale's sign goes with it, so that scores grow with their products
-    {
-      constexpr int kLanes = D / 8, kPer = 32 / kLanes, kBatch = 16;
-      const int j = lane % kLanes;
-#pragma unroll 1
-      for (int r0 = warp * 32; r0 < warp * 32 + 32; r0 += kBatch * kPer) {
-        uint4 x[kBatch];
 #pragma unroll
-        for (int i = 0; i < kBatch; ++i) {
-          const int row = row0 + r0 + i * kPer + lane / kLanes;
-          x[i] = make_uint4(0, 0, 0, 0);
-          if (row < a.rows) {
-            const int t = row / a.gqa, h = hk * a.gqa + row % a.gqa;
-            x[i] = *(const uint4*)((const T*)a.q + b * a.q_sb + h * a.q_sh + t * a.q_st + 8 * j);
-          }
+      for (int i = 0; i < kBatch; ++i) {
+        const int r = ((i0 + i) * kIssuer + warp) * kPer + lane / kLanes;
+        const uint32_t u[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+        // largest magnitude of the row, NaN passed over (an infinity makes the row NaN whatever its scale)
+        uint32_t top = abs_max<T>(abs_max<T>(u[0], u[1]), abs_max<T>(u[2], u[3]));
+        top = __float_as_uint(fmaxf(TR::bits_to_float((uint16_t)(top & 0x7FFFu)), TR::bits_to_float((uint16_t)((top >> 16) & 0x7FFFu))));
+        if (kLanes == 32) {
+          top = __reduce_max_sync(0xffffffffu, top);
+        } else {
+#pragma unroll
+          for (int o = 1; o < kLanes; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
         }
+        const int eq = min(max((int)(top >> 23) - 127 - 7, -100), 126);
+        const float to_q = a.scale < 0.f ? -pow2(-eq) : pow2(-eq);
+        uint32_t p[4];
 #pragma unroll
-        for (int i = 0; i < kBatch; ++i) {
-          const int r = r0 + i * kPer + lane / kLanes;
-          const uint32_t u[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
-          float f[8], big = 0.f;
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            f[e] = TR::bits_to_float((uint16_t)(u[e >> 1] >> (16 * (e & 1))));
-            big = fmaxf(big, finite(f[e]) ? fabsf(f[e]) : 0.f);
-          }
-#pragma unroll
-          for (int o = 1; o < kLanes; o <<= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, o));
-          const int eq = min(max((int)(__float_as_uint(big) >> 23) - 127 - 7, -100), 126);
-          const float to_q = a.scale < 0.f ? -pow2(-eq) : pow2(-eq);
-          uint32_t p[4];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const __half2 hh = __floats2half2_rn(f[e] * to_q, f[4 + e] * to_q);
-            p[e] = *(const uint32_t*)&hh;
-          }
+        for (int e = 0; e < 4; ++e) {
+          const float f0 = TR::bits_to_float((uint16_t)(u[e >> 1] >> (16 * (e & 1)))), f1 = TR::bits_to_float((uint16_t)(u[2 + (e >> 1)] >> (16 * (e & 1))));
+          const __half2 hh = __floats2half2_rn(f0 * to_q, f1 * to_q);
+          p[e] = *(const uint32_t*)&hh;
+        }
+        if (r < kRows) {
           *(uint4*)(sQ + (j >> 3) * kSlab + r * 128 + (((j & 7) ^ (r & 7)) << 4)) = make_uint4(p[0], p[1], p[2], p[3]);
           if (j == 0) sE[r] = eq;
         }
@@ -424,63 +481,133 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_sdpa_tc_kernel(const SdpaArgs
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     __syncwarp();
     if (lane == 0) mbar_arrive(bar0 + 8 * kBarQ);
+  };
+
+  if (warp >= kKeyWarp && warp < kValueWarp) {
+    unpack_side<T, D, false>(a.k, b, hk, k0, hi, tiles, sK, sRaw, bar0, meta, err, query_rows);
+  } else if (warp >= kValueWarp && warp < kIssuer) {
+    unpack_side<T, D, true>(a.v, b, hk, k0, hi, tiles, sV, sRaw + kKeys * D / 2, bar0, meta, err, query_rows);
+  } else if (warp == kIssuer) {
+    // ---------------- scores ----------------
+    if (lane == 0) {
+      bool ok = wait_bar(bar0 + 8 * kBarQ, 0);
+      if (!ok) atomicCAS(err, 0, 62 | (9 << 8));
+      const uint64_t da = desc_k(smem_u32(sQ)), db = desc_k(smem_u32(sK));
+      for (int i = 0; i < tiles && ok; ++i) {
+        // the columns hold P(i - 2) until its product is done
+        if (i >= 2 && !wait_bar(bar0 + 8 * (kBarO + (i & 1)), ((i - 2) >> 1) & 1)) { atomicCAS(err, 0, 62 | (11 << 8)); break; }
+        if (!wait_bar(bar0 + 8 * kBarKFull, i & 1)) { atomicCAS(err, 0, 62 | (3 << 8)); break; }
+        fence_after();
+        const uint32_t d = tmem + 128u * (i & 1);
+#pragma unroll 1
+        for (int g = 0; g < G; ++g) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const uint64_t step = (uint64_t)(g * (kSlab >> 4) + 2 * j);
+            mma_ss(d, da + step, db + step, idesc(kKeys, false), (g | j) ? 1u : 0u);
+          }
+          commit(bar0 + 8 * (kBarKEmpty + g));
+        }
+        commit(bar0 + 8 * (kBarS + (i & 1)));
+      }
+    }
+    __syncwarp();
+  } else if (warp == kIssuer + 1) {
+    // ---------------- output ----------------
+    if (lane == 0) {
+      const uint64_t dv = desc_mn(smem_u32(sV), kSlab);
+      for (int i = 0; i < tiles; ++i) {
+        if (!wait_bar(bar0 + 8 * kBarVFull, i & 1)) { atomicCAS(err, 0, 62 | (5 << 8)); break; }
+        if (!wait_bar(bar0 + 8 * (kBarP + (i & 1)), (i >> 1) & 1)) { atomicCAS(err, 0, 62 | (4 << 8)); break; }
+        fence_after();
+        const uint32_t pc = tmem + 128u * (i & 1);
+#pragma unroll 1
+        for (int blk = 0; blk < 4; ++blk) {
+#pragma unroll
+          for (int j = 0; j < 2; ++j)   // 16 keys = two 1024-byte groups; P: 8 columns (16 fp16)
+            mma_ts(tmem + kOCol, pc + 8u * (2 * blk + j), dv + (uint64_t)((2 * blk + j) * (2048 >> 4)), idesc(D, true),
+                   (blk | j) ? 1u : (i ? 1u : 0u));
+          commit(bar0 + 8 * (kBarVEmpty + blk));
+        }
+        commit(bar0 + 8 * (kBarO + (i & 1)));
+      }
+    }
+    __syncwarp();
+  } else {
+    // ---------------- softmax: thread = query row ----------------
+    const int group = warp >> 2, part = warp & 3, r = part * 32 + lane, row = row0 + r;
+    const bool row_ok = row < a.rows;
+    const bool live = row0 + part * 32 < a.rows;
+    const uint32_t lanes = (uint32_t)(part * 32) << 16;
+    const int t = row_ok ? row / a.gqa : 0, h = hk * a.gqa + (row_ok ? row % a.gqa : 0);
+    query_rows();
+    bool ok = wait_warp(bar0 + 8 * kBarQ, 0);
+    if (!ok) atomicCAS(err, 0, 62 | (10 << 8));
     const float c_row = fabsf(a.scale) * pow2(sE[r]);
     // last key the row sees; rows behind the last one compute what nobody reads
     const int lim = row_ok ? min(len - a.T + t, hi - 1) : (kMask ? -1 : 0x7FFFFFFF);
     const long long mat = kMask && row_ok ? b * a.m_sb + h * a.m_sh + t * a.m_st : 0;
-    float m = -INFINITY, l = 0.f;
-    int ev = -200;   // exponent that O carries
-    bool ok = true;
-    for (int i = 0; i < tiles; ++i) {
-      if (!wait_warp(bar0 + 8 * (kBarS + (i & 1)), (i >> 1) & 1) || !wait_warp(bar0 + 8 * (kBarVMeta + (i & 1)), (i >> 1) & 1)) {
-        atomicCAS(err, 0, 62 | (6 << 8));
-        ok = false;
-        break;
-      }
+    const uint32_t s_col = tmem + lanes + 128u * group;
+    float m_l = -INFINITY, l = 0.f;   // this half's sum and the reference it is relative to
+    for (int i = group; i < tiles && ok; i += 2) {
+      if (!wait_warp(bar0 + 8 * (kBarS + group), (i >> 1) & 1)) { atomicCAS(err, 0, 62 | (6 << 8)); ok = false; break; }
       fence_after();
       if (!live) {   // P is whatever is there: lanes of their own
         fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(bar0 + 8 * (kBarP + (i & 1)));
+        if (lane == 0) mbar_arrive(bar0 + 8 * (kBarP + group));
         continue;
       }
-      const uint32_t s_col = tmem + lanes + 128u * (i & 1);
       const Meta& mt = meta[i & (kMeta - 1)];
       const int n0 = k0 + i * kKeys;
-      const bool plain = !kMask && (mt.bad[0] | mt.bad[1] | mt.bad[2] | mt.bad[3]) == 0 && __all_sync(0xffffffffu, n0 + kKeys - 1 <= lim);
+      // every key of the tile seen by every row of the warp, and no mask
+      const bool plain = !kMask && __all_sync(0xffffffffu, n0 + kKeys - 1 <= lim);
       float top = -INFINITY;
-#pragma unroll
-      for (int q0 = 0; q0 < 4; q0 += 2) {   // 64 keys at a time
-        uint32_t v[64];
-        ld32(s_col + 32 * q0, v);
-        ld32(s_col + 32 * q0 + 32, v + 32);
+      // (loops over 32 keys stay rolled: the roles' code together has to fit the instruction cache, whose misses were a quarter
+      // of the warps' time with everything unrolled)
+#pragma unroll 1
+      for (int q = 0; q < 4; ++q) {
+        uint32_t v[32];
+        ld32(s_col + 32 * q, v);
+        const float c = c_row * mt.k_factor[q];
+        const uint32_t seen = plain ? 0xFFFFFFFFu : seen_bits<kMask>(a, mat, n0 + 32 * q, lim);
         wait_ld();
-        if (plain) {
-          float t0 = -INFINITY, t1 = -INFINITY;
+        if (kMask == 2) {   // scores as the row sees them, back into their columns
 #pragma unroll
           for (int e = 0; e < 32; ++e) {
-            t0 = fmaxf(t0, __uint_as_float(v[e]));
-            t1 = fmaxf(t1, __uint_as_float(v[32 + e]));
-          }
-          top = fmaxf(top, fmaxf(t0 * (c_row * mt.k_factor[q0]), t1 * (c_row * mt.k_factor[q0 + 1])));
-        } else {   // scores as the row sees them, back into their columns
-#pragma unroll
-          for (int e = 0; e < 64; ++e) {
-            const int n = n0 + 32 * q0 + e;
-            float x = __uint_as_float(v[e]) * (c_row * mt.k_factor[q0 + (e >> 5)]);
-            if ((mt.bad[q0 + (e >> 5)] >> (e & 31)) & 1) x = __int_as_float(0x7FC00000);
-            if (n <= lim) {
-              if (kMask) x = apply_mask<T>(a, x, mat + n * a.m_sn);
-            } else {
-              x = -INFINITY;
-            }
+            float x = __uint_as_float(v[e]) * c;
+            x = (seen >> e) & 1 ? apply_mask<T>(a, x, mat + (n0 + 32 * q + e) * a.m_sn) : -INFINITY;
             top = fmaxf(top, x);
             v[e] = __float_as_uint(x);
           }
-#pragma unroll
-          for (int e = 0; e < 64; e += 16) st16(s_col + 32 * q0 + e, v + e);
+          st16(s_col + 32 * q, v);
+          st16(s_col + 32 * q + 16, v + 16);
           wait_st();
+        } else {
+          if (!plain) {
+#pragma unroll
+            for (int e = 0; e < 32; ++e)
+              if (!((seen >> e) & 1)) v[e] = 0xFF800000u;
+          }
+          float t0 = -INFINITY, t1 = -INFINITY;
+#pragma unroll
+          for (int e = 0; e < 32; e += 4) {
+            t0 = fmaxf(fmaxf(t0, __uint_as_float(v[e])), __uint_as_float(v[e + 1]));
+            t1 = fmaxf(fmaxf(t1, __uint_as_float(v[e + 2])), __uint_as_float(v[e + 3]));
+          }
+          t0 = fmaxf(t0, t1);
+          top = fmaxf(top, t0 == -INFINITY ? t0 : t0 * c);   // c may be 0
         }
+      }
+      if (!wait_warp(bar0 + 8 * (kBarVMeta + (i & (kMeta - 1))), (i / kMeta) & 1)) { atomicCAS(err, 0, 62 | (13 << 8)); ok = false; break; }
+      const bool bads = (mt.bad[0] | mt.bad[1] | mt.bad[2] | mt.bad[3]) != 0;
+      // ---- the row's reference: what the tile before left, moved when this tile exceeds it by 8 octaves ----
+      float m = -INFINITY;
+      int ev = -200;
+      if (i > 0) {
+        if (!wait_warp(bar0 + 8 * (kBarM + 4 * (group ^ 1) + part), ((i - 1) >> 1) & 1)) { atomicCAS(err, 0, 62 | (12 << 8)); ok = false; break; }
+        m = sRef[(group ^ 1) * kRows + r];
+        ev = sEv[(group ^ 1) * 4 + part];
       }
       const int ev_tile = max(max(mt.v_exp[0], mt.v_exp[1]), max(mt.v_exp[2], mt.v_exp[3]));
       if (__any_sync(0xffffffffu, top > m + kMaxStep) || ev_tile > ev) {
@@ -488,11 +615,11 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_sdpa_tc_kernel(const SdpaArgs
         const int ev_new = max(ev, ev_tile);
         const float f = m_new == -INFINITY ? 1.f : ex2((m - m_new) * kLog2e);
         const float fo = f * pow2(max(ev - ev_new, -126));
-        l *= f;
         m = m_new;
         if (i > 0) {
-          if (!wait_warp(bar0 + 8 * (kBarO + ((i - 1) & 1)), ((i - 1) >> 1) & 1)) { atomicCAS(err, 0, 62 | (7 << 8)); ok = false; break; }
+          if (!wait_warp(bar0 + 8 * (kBarO + (group ^ 1)), ((i - 1) >> 1) & 1)) { atomicCAS(err, 0, 62 | (7 << 8)); ok = false; break; }
           fence_after();
+#pragma unroll 1
           for (int c0 = 0; c0 < D; c0 += 32) {
             uint32_t o[32];
             ld32(tmem + lanes + kOCol + c0, o);
@@ -506,52 +633,88 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_sdpa_tc_kernel(const SdpaArgs
         }
         ev = ev_new;
       }
+      sRef[group * kRows + r] = m;
+      if (lane == 0) sEv[group * 4 + part] = ev;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar0 + 8 * (kBarM + 4 * group + part));
+      if (m != m_l) {
+        if (m_l != -INFINITY) l *= ex2((m_l - m) * kLog2e);
+        m_l = m;
+      }
+      // ---- P ----
       const float ref = m == -INFINITY ? 0.f : m;
-#pragma unroll
+#pragma unroll 1
       for (int q = 0; q < 4; ++q) {
         uint32_t v[32];
         ld32(s_col + 32 * q, v);
-        wait_ld();
         const float shift = kPShift + (float)max(mt.v_exp[q] - ev, -100);   // P carries V's power of two
-        const float cl = plain ? c_row * mt.k_factor[q] * kLog2e : kLog2e, off = shift - ref * kLog2e;
-        float sum0 = 0.f, sum1 = 0.f;
+        const float cl = kMask == 2 ? kLog2e : c_row * mt.k_factor[q] * kLog2e, off = shift - ref * kLog2e;
+        const uint64_t cl2 = pair(cl, cl), off2 = pair(off, off);
+        uint64_t sum = 0;
         uint32_t w[16];
+        uint32_t seen = 0xFFFFFFFFu;
+        if (kMask != 2 && !plain) seen = seen_bits<kMask>(a, mat, n0 + 32 * q, lim);
+        wait_ld();
+        if (bads) {   // a value that is not finite makes the rows NaN that see its key
+#pragma unroll
+          for (int e = 0; e < 32; ++e)
+            if (((mt.bad[q] >> e) & 1) && !(kMask == 2 && v[e] == 0xFF800000u)) v[e] = 0x7FC00000u;
+        }
+        if (kMask != 2 && !plain) {
+#pragma unroll
+          for (int e = 0; e < 32; ++e)
+            if (!((seen >> e) & 1)) v[e] = 0xFF800000u;
+        }
 #pragma unroll
         for (int e = 0; e < 32; e += 2) {
-          const float x0 = __uint_as_float(v[e]), x1 = __uint_as_float(v[e + 1]);
           float p0, p1;
-          if (kMask) {   // scores may be the lowest finite value: their difference first
-            p0 = ex2(fmaf(x0 - ref, kLog2e, shift));
-            p1 = ex2(fmaf(x1 - ref, kLog2e, shift));
+          if (kMask == 2) {   // scores may be the lowest finite value: their difference first
+            p0 = fmaf(__uint_as_float(v[e]) - ref, kLog2e, shift);
+            p1 = fmaf(__uint_as_float(v[e + 1]) - ref, kLog2e, shift);
           } else {
-            p0 = ex2(fmaf(x0, cl, off));
-            p1 = ex2(fmaf(x1, cl, off));
+            unpair(fma2(pair(__uint_as_float(v[e]), __uint_as_float(v[e + 1])), cl2, off2), p0, p1);
           }
-          sum0 += p0;
-          sum1 += p1;
+          p0 = ex2(p0);
+          p1 = ex2(p1);
+          sum = add2(sum, pair(p0, p1));
           const __half2 p = __floats2half2_rn(p0, p1);
           w[e >> 1] = *(const uint32_t*)&p;
         }
+        float sum0, sum1;
+        unpair(sum, sum0, sum1);
         l = fmaf(sum0 + sum1, ex2(-shift), l);
         st16(s_col + 16 * q, w);   // over columns that have been read
       }
       wait_st();
       fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(bar0 + 8 * (kBarP + (i & 1)));
+      if (lane == 0) mbar_arrive(bar0 + 8 * (kBarP + group));
     }
-    // ---- epilogue: the row goes through shared memory (all of Q, K and V is spent), so that it leaves as one bulk copy ----
-    // the last product; the one two before it is done (its successor's scores were), so the phase cannot be mistaken
+    // ---- epilogue: either half of the softmax takes half of the channels; the rows go through shared memory (all of Q, K and V is
+    // spent), so that they leave as bulk copies ----
+    // the last product; the one two before it is done (the last scores took its columns), so the phase cannot be mistaken
     if (tiles > 0 && ok && !wait_warp(bar0 + 8 * (kBarO + ((tiles - 1) & 1)), ((tiles - 1) >> 1) & 1)) { atomicCAS(err, 0, 62 | (8 << 8)); ok = false; }
     fence_after();
+    sEnd[group * kRows + r] = make_float2(m_l, l);
+    named_bar_sync(1, 256);
     const bool have = tiles > 0 && ok;
     if (live) {
+      const float m = tiles > 0 ? sRef[((tiles - 1) & 1) * kRows + r] : -INFINITY;
+      const int ev = tiles > 0 ? sEv[((tiles - 1) & 1) * 4 + part] : 0;
+      l = 0.f;
+#pragma unroll
+      for (int g = 0; g < 2; ++g) {
+        const float2 x = sEnd[g * kRows + r];
+        l = fmaf(x.y, x.x == -INFINITY ? 1.f : ex2((x.x - m) * kLog2e), l);
+      }
       const float undo = pow2(min(max(ev - (int)kPShift, -126), 127));
       const bool last = a.splits == 1;
       const float inv = l == 0.f ? 1.f : 1.f / l, nan = l * 0.f;   // a row that sees nothing yields zeros; NaN reaches the whole row
       const size_t at = ((size_t)bhk * a.rows + row) * a.splits + split;
       uint8_t* stage = smem + r * (D * 4 + 16);   // rows 16 bytes apart modulo 128: no bank conflicts
-      for (int c0 = 0; c0 < D; c0 += 32) {
+      const int c_first = group * (D / 2);
+#pragma unroll 1
+      for (int c0 = c_first; c0 < c_first + D / 2; c0 += 32) {
         uint32_t o[32];
         if (have) {
           ld32(tmem + lanes + kOCol + c0, o);
@@ -575,16 +738,18 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_sdpa_tc_kernel(const SdpaArgs
       }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       if (row_ok) {
-        const void* dst = last ? (const void*)((T*)a.out + out_row(a, b, hk, row) * D) : (const void*)(a.part_o + at * D);
-        asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(dst), "r"(smem_u32(stage)), "r"(last ? D * 2 : D * 4)
+        const int size = last ? 2 : 4;
+        const uint8_t* dst = last ? (const uint8_t*)((T*)a.out + out_row(a, b, hk, row) * D) : (const uint8_t*)(a.part_o + at * D);
+        asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(dst + c_first * size),
+                     "r"(smem_u32(stage) + c_first * size), "r"(D / 2 * size)
                      : "memory");
-        if (!last) {
+        if (!last && group == 0) {
           a.part_m[at] = m;
           a.part_l[at] = l;
         }
       }
       asm volatile("cp.async.bulk.commit_group;" ::: "memory");
-      asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+      asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
     }
   }
   fence_before();
@@ -595,16 +760,17 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_sdpa_tc_kernel(const SdpaArgs
 
 template <typename T, int D>
 int launch(const SdpaArgs& a, cudaStream_t st, int device) {
-  constexpr size_t tiles = (size_t)3 * (D / kGroup) * kSlab, rest = kBars * 8 + kMeta * sizeof(Meta) + kRows * 4 + 16;
+  constexpr size_t tiles = (size_t)3 * (D / kGroup) * kSlab, rest = (size_t)kKeys * D + kBars * 8 + kMeta * sizeof(Meta) + kRows * 12 + 48;
   static_assert(kRows * (D * 4 + 16) <= tiles, "the epilogue's rows fit where Q, K and V were");
   constexpr size_t smem = tiles + rest;
   static_assert(smem <= 227 * 1024, "shared memory");
-  auto kern = a.mask_kind ? kv4_sdpa_tc_kernel<T, D, true> : kv4_sdpa_tc_kernel<T, D, false>;
+  const int mask = a.mask_kind == 0 ? 0 : a.mask_kind == 1 ? 1 : 2;
+  auto kern = mask == 0 ? kv4_sdpa_tc_kernel<T, D, 0> : mask == 1 ? kv4_sdpa_tc_kernel<T, D, 1> : kv4_sdpa_tc_kernel<T, D, 2>;
   static std::mutex mu;
-  static bool done[64][2] = {};
+  static bool done[64][3] = {};
   {
     std::lock_guard<std::mutex> lk(mu);
-    bool& d = done[device & 63][a.mask_kind ? 1 : 0];
+    bool& d = done[device & 63][mask];
     if (!d) {
       cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
       if (e != cudaSuccess) return fail(DFLASH_ERR_LAUNCH, "kv4_sdpa: cudaFuncSetAttribute: %s", cudaGetErrorString(e));
