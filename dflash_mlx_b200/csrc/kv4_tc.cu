@@ -73,20 +73,22 @@ __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::aft
 __device__ __forceinline__ void commit(uint32_t bar) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
 }
-// D (+)= A (shared memory descriptor) * B (shared memory descriptor)
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accum) {
+// D (+)= A (shared memory descriptor) * B (shared memory descriptor); descriptors as their two halves, of which a step through
+// shared memory changes the lower one only
+template <bool kAccum>
+__device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a_lo, uint32_t a_hi, uint32_t b_lo, uint32_t b_hi, uint32_t idesc) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accum)
+      "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\tsetp.ne.u32 p, %6, 0;\n\tmov.b64 a, {%1, %2};\n\tmov.b64 b, {%3, %4};\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %5, p;\n\t}" ::"r"(d),
+      "r"(a_lo), "r"(a_hi), "r"(b_lo), "r"(b_hi), "r"(idesc), "n"(kAccum ? 1 : 0)
       : "memory");
 }
 // D (+)= A (tensor memory) * B (shared memory descriptor)
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc, uint32_t accum) {
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a_tmem, uint32_t b_lo, uint32_t b_hi, uint32_t idesc, uint32_t accum) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
-      "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accum)
+      "{\n\t.reg .pred p;\n\t.reg .b64 b;\n\tsetp.ne.u32 p, %5, 0;\n\tmov.b64 b, {%2, %3};\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %4, p;\n\t}" ::"r"(d),
+      "r"(a_tmem), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(accum)
       : "memory");
 }
 __device__ __forceinline__ void ld32(uint32_t taddr, uint32_t* r) {
@@ -168,23 +170,6 @@ __device__ __forceinline__ bool wide_range(const float (&s)[G], const float (&b)
   const int hi = (int)__reduce_max_sync(0xffffffffu, u), lo = (int)__reduce_min_sync(0xffffffffu, mine == 0.f ? 255u : u);
   *e = min(max(hi - 127 - 13, -100), 126);
   return hi - lo > 6 && lo < 255;
-}
-// fp32 pairs: one instruction for two lanes of arithmetic
-__device__ __forceinline__ uint64_t pair(float x, float y) {
-  uint64_t d;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(x), "f"(y));
-  return d;
-}
-__device__ __forceinline__ void unpair(uint64_t d, float& x, float& y) { asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(d)); }
-__device__ __forceinline__ uint64_t fma2(uint64_t x, uint64_t y, uint64_t z) {
-  uint64_t d;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(x), "l"(y), "l"(z));
-  return d;
-}
-__device__ __forceinline__ uint64_t add2(uint64_t x, uint64_t y) {
-  uint64_t d;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(x), "l"(y));
-  return d;
 }
 // Bit e: byte mask entry of key n0 + e is not 0, for the bits set in `want` (others are not read).
 __device__ __forceinline__ uint32_t mask_bits(const SdpaArgs& a, long long at, int n0, uint32_t want) {
@@ -492,19 +477,20 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_sdpa_tc_kernel(const SdpaArgs
     if (lane == 0) {
       bool ok = wait_bar(bar0 + 8 * kBarQ, 0);
       if (!ok) atomicCAS(err, 0, 62 | (9 << 8));
-      const uint64_t da = desc_k(smem_u32(sQ)), db = desc_k(smem_u32(sK));
+      const uint32_t da = (uint32_t)desc_k(smem_u32(sQ)), db = (uint32_t)desc_k(smem_u32(sK)), hi32 = (uint32_t)(desc_k(0) >> 32);
       for (int i = 0; i < tiles && ok; ++i) {
         // the columns hold P(i - 2) until its product is done
         if (i >= 2 && !wait_bar(bar0 + 8 * (kBarO + (i & 1)), ((i - 2) >> 1) & 1)) { atomicCAS(err, 0, 62 | (11 << 8)); break; }
         if (!wait_bar(bar0 + 8 * kBarKFull, i & 1)) { atomicCAS(err, 0, 62 | (3 << 8)); break; }
         fence_after();
         const uint32_t d = tmem + 128u * (i & 1);
-#pragma unroll 1
+#pragma unroll
         for (int g = 0; g < G; ++g) {
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            const uint64_t step = (uint64_t)(g * (kSlab >> 4) + 2 * j);
-            mma_ss(d, da + step, db + step, idesc(kKeys, false), (g | j) ? 1u : 0u);
+            const uint32_t step = g * (kSlab >> 4) + 2 * j;
+            if ((g | j) == 0) mma_ss<false>(d, da, hi32, db, hi32, idesc(kKeys, false));
+            else mma_ss<true>(d, da + step, hi32, db + step, hi32, idesc(kKeys, false));
           }
           commit(bar0 + 8 * (kBarKEmpty + g));
         }
@@ -515,18 +501,18 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_sdpa_tc_kernel(const SdpaArgs
   } else if (warp == kIssuer + 1) {
     // ---------------- output ----------------
     if (lane == 0) {
-      const uint64_t dv = desc_mn(smem_u32(sV), kSlab);
+      const uint32_t dv = (uint32_t)desc_mn(smem_u32(sV), kSlab), hi32 = (uint32_t)(desc_mn(0, 0) >> 32);
       for (int i = 0; i < tiles; ++i) {
         if (!wait_bar(bar0 + 8 * kBarVFull, i & 1)) { atomicCAS(err, 0, 62 | (5 << 8)); break; }
         if (!wait_bar(bar0 + 8 * (kBarP + (i & 1)), (i >> 1) & 1)) { atomicCAS(err, 0, 62 | (4 << 8)); break; }
         fence_after();
         const uint32_t pc = tmem + 128u * (i & 1);
-#pragma unroll 1
+#pragma unroll
         for (int blk = 0; blk < 4; ++blk) {
 #pragma unroll
           for (int j = 0; j < 2; ++j)   // 16 keys = two 1024-byte groups; P: 8 columns (16 fp16)
-            mma_ts(tmem + kOCol, pc + 8u * (2 * blk + j), dv + (uint64_t)((2 * blk + j) * (2048 >> 4)), idesc(D, true),
-                   (blk | j) ? 1u : (i ? 1u : 0u));
+            mma_ts(tmem + kOCol, pc + 8u * (2 * blk + j), dv + (uint32_t)((2 * blk + j) * (2048 >> 4)), hi32, idesc(D, true),
+                   (blk | j) ? 1u : (uint32_t)i);
           commit(bar0 + 8 * (kBarVEmpty + blk));
         }
         commit(bar0 + 8 * (kBarO + (i & 1)));

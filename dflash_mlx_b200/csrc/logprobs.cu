@@ -23,7 +23,7 @@ namespace dflash {
 namespace lp {
 namespace {
 
-constexpr int kThreads = 512, kGroups = 64, kMaxK = 32, kList = 1024;
+constexpr int kThreads = 256, kGroups = 64, kMaxK = 32, kList = 1024;
 constexpr float kLog2e = 1.4426950408889634f;
 
 struct Args {
@@ -41,10 +41,17 @@ struct Args {
 
 template <typename T> struct Elem;
 template <> struct Elem<float> {
-  static constexpr int kPer = 4, kSlots = 10;
+  static constexpr int kPer = 4, kSlots = 4;
   static constexpr uint32_t kNegInf = 0xFF800000u;
   __device__ static __forceinline__ float get(const uint32_t (&w)[4], int e) { return __uint_as_float(w[e]); }
   __device__ static __forceinline__ void hide(uint32_t (&w)[4], int e) { w[e] = kNegInf; }
+  // hides the elements whose byte in `bytes` (as many as elements, from address p) is not 0
+  __device__ static __forceinline__ void hide_by(uint32_t (&w)[4], const uint8_t* p) {
+    const uint32_t u = *(const uint32_t*)p;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if ((u >> (8 * e)) & 0xFFu) w[e] = kNegInf;
+  }
   __device__ static __forceinline__ void put(uint32_t (&w)[4], int e, const float* p) { w[e] = __float_as_uint(*p); }
   __device__ static __forceinline__ float load(const float* p) { return *p; }
   __device__ static __forceinline__ float max_of(const uint32_t (&w)[kSlots][4]) {   // NaN is passed over
@@ -59,7 +66,7 @@ template <> struct Elem<float> {
 __device__ __forceinline__ __nv_bfloat162 as_pair(uint32_t u, __nv_bfloat16) { return *(const __nv_bfloat162*)&u; }
 __device__ __forceinline__ __half2 as_pair(uint32_t u, __half) { return *(const __half2*)&u; }
 template <typename T, uint32_t kInf> struct Elem16 {
-  static constexpr int kPer = 8, kSlots = 5;
+  static constexpr int kPer = 8, kSlots = 4;
   __device__ static __forceinline__ float get(const uint32_t (&w)[4], int e) {
     return MmaTraits<T>::bits_to_float((uint16_t)(w[e >> 1] >> (16 * (e & 1))));
   }
@@ -67,6 +74,15 @@ template <typename T, uint32_t kInf> struct Elem16 {
     w[e >> 1] = (e & 1) ? ((w[e >> 1] & 0xFFFFu) | (bits << 16)) : ((w[e >> 1] & 0xFFFF0000u) | bits);
   }
   __device__ static __forceinline__ void hide(uint32_t (&w)[4], int e) { put_bits(w, e, kInf); }
+  __device__ static __forceinline__ void hide_by(uint32_t (&w)[4], const uint8_t* p) {
+    const uint2 u = *(const uint2*)p;
+    const uint32_t t[2] = {__vcmpne4(u.x, 0), __vcmpne4(u.y, 0)};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t m = prmt(t[i >> 1], 0, (i & 1) ? 0x3322 : 0x1100);   // a byte for each half
+      w[i] = (w[i] & ~m) | ((kInf | (kInf << 16)) & m);
+    }
+  }
   __device__ static __forceinline__ void put(uint32_t (&w)[4], int e, const T* p) { put_bits(w, e, *(const uint16_t*)p); }
   __device__ static __forceinline__ float load(const T* p) { return MmaTraits<T>::to_float(*p); }
   __device__ static __forceinline__ float max_of(const uint32_t (&w)[kSlots][4]) {   // packed; NaN is passed over
@@ -134,7 +150,7 @@ __device__ __forceinline__ void slot(const uint32_t (&raw)[N][4], int s, uint32_
 }
 
 template <typename T>
-__global__ void __launch_bounds__(kThreads, 2) token_logprobs_kernel(const Args a) {
+__global__ void __launch_bounds__(kThreads, 3) token_logprobs_kernel(const Args a) {
   namespace cg = cooperative_groups;
   using E = Elem<T>;
   constexpr int kPer = E::kPer, kSlots = E::kSlots;
@@ -153,8 +169,9 @@ __global__ void __launch_bounds__(kThreads, 2) token_logprobs_kernel(const Args 
   const int v0 = me * share, v1 = min(vecs, v0 + share);
   Sums sums = {-INFINITY, 0.f, 0.f};
   if (tid < kMaxK) sh.top[tid] = 0;
-  for (int base = v0; base < v1; base += kThreads * kSlots) {
-    uint32_t raw[kSlots][4];
+  if (tid == 0) sh.count = 0;
+  const bool packed = a.suppress != nullptr && skew == 0 && ((uintptr_t)a.suppress & (kPer - 1)) == 0;
+  auto load = [&](int base, uint32_t (&raw)[kSlots][4]) {
 #pragma unroll
     for (int s = 0; s < kSlots; ++s) {
       const int v = base + s * kThreads + tid;
@@ -170,21 +187,24 @@ __global__ void __launch_bounds__(kThreads, 2) token_logprobs_kernel(const Args 
         }
       }
     }
+  };
+  uint32_t next[kSlots][4];
+  if (v0 < v1) load(v0, next);
+  for (int base = v0; base < v1; base += kThreads * kSlots) {
+    uint32_t raw[kSlots][4];
+#pragma unroll
+    for (int s = 0; s < kSlots; ++s)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) raw[s][i] = next[s][i];
+    if (base + kThreads * kSlots < v1) load(base + kThreads * kSlots, next);   // in flight under this pass
     if (a.suppress != nullptr) {
-      // eight bytes at once where the vectors start on a multiple of eight of them
-      const bool packed = kPer == 8 && skew == 0 && ((uintptr_t)a.suppress & 7) == 0;
 #pragma unroll
       for (int s = 0; s < kSlots; ++s) {
         const int v = base + s * kThreads + tid;
         const int i0 = v * kPer - skew;
         if (v < v1) {
-          if (packed && i0 + 8 <= a.V) {
-            const uint2 u = *(const uint2*)(a.suppress + i0);
-            if (u.x | u.y) {
-#pragma unroll
-              for (int e = 0; e < kPer; ++e)
-                if ((e < 4 ? u.x >> (8 * (e & 3)) : u.y >> (8 * (e & 3))) & 0xFFu) E::hide(raw[s], e);
-            }
+          if (packed && i0 + kPer <= a.V) {   // the vector's bytes at once
+            E::hide_by(raw[s], a.suppress + i0);
           } else {
 #pragma unroll
             for (int e = 0; e < kPer; ++e)
@@ -195,24 +215,36 @@ __global__ void __launch_bounds__(kThreads, 2) token_logprobs_kernel(const Args 
     }
     Sums mine = {E::max_of(raw), 0.f, 0.f};
     const float ref = mine.m == -INFINITY ? 0.f : mine.m;
+    const uint64_t ref2 = pair(-ref, -ref), scale2 = pair(a.scale, a.scale);
+    uint64_t l2 = 0, w2 = 0;
 #pragma unroll
     for (int s = 0; s < kSlots; ++s)
 #pragma unroll
-      for (int e = 0; e < kPer; ++e) {
-        const float d = E::get(raw[s], e) - ref;
-        const float p = exp2f(d * a.scale);
-        mine.l += p;
-        mine.w = fmaf(fmaxf(d, -1e30f), p, mine.w);   // a hidden element adds 0, not -inf * 0; NaN stays through p
+      for (int e = 0; e < kPer; e += 2) {
+        const uint64_t d2 = add2(pair(E::get(raw[s], e), E::get(raw[s], e + 1)), ref2);
+        float d0, d1, p0, p1;
+        unpair(d2, d0, d1);
+        unpair(mul2(d2, scale2), p0, p1);
+        const uint64_t p2 = pair(exp2f(p0), exp2f(p1));
+        l2 = add2(l2, p2);
+        // a hidden element adds 0, not -inf * 0; NaN stays through p
+        w2 = fma2(pair(fmaxf(d0, -1e30f), fmaxf(d1, -1e30f)), p2, w2);
       }
+    {
+      float x0, x1;
+      unpair(l2, x0, x1);
+      mine.l = x0 + x1;
+      unpair(w2, x0, x1);
+      mine.w = x0 + x1;
+    }
     if (a.k > 0) {
       // ---- candidates of this pass ----
       const bool first = base == v0;
       if (first) {   // everything >= the k-th largest group maximum
         float g = mine.m;
 #pragma unroll
-        for (int o = 1; o < 8; o <<= 1) g = fmaxf(g, __shfl_xor_sync(0xffffffffu, g, o));
-        if ((lane & 7) == 0) sh.group_max[warp * 4 + (lane >> 3)] = g;
-        if (tid == 0) sh.count = 0;
+        for (int o = 1; o < kThreads / kGroups; o <<= 1) g = fmaxf(g, __shfl_xor_sync(0xffffffffu, g, o));
+        if ((lane & (kThreads / kGroups - 1)) == 0) sh.group_max[tid / (kThreads / kGroups)] = g;
         __syncthreads();
         const float g0 = sh.group_max[lane], g1 = sh.group_max[lane + 32];
 #pragma unroll
@@ -227,7 +259,12 @@ __global__ void __launch_bounds__(kThreads, 2) token_logprobs_kernel(const Args 
       }
       const float tau = sh.tau;
       // NaN elements count as the largest; a thread whose own maximum does not reach tau can only hold NaN beyond it
-      if ((first ? mine.m >= tau : !(mine.m <= tau)) || !(mine.l == mine.l)) {
+      const bool has = (first ? mine.m >= tau : !(mine.m <= tau)) || !(mine.l == mine.l);
+      if (!__syncthreads_or(has)) {   // later passes, mostly
+        sums = merge(sums, mine, a.scale);
+        continue;
+      }
+      if (has) {
 #pragma unroll 1
         for (int s = 0; s < kSlots; ++s) {
           uint32_t w[4];
@@ -256,9 +293,7 @@ __global__ void __launch_bounds__(kThreads, 2) token_logprobs_kernel(const Args 
       }
       __syncthreads();
       const int n = sh.count;
-      if (n == 0) {
-        // nothing new (later passes, mostly)
-      } else if (n <= kList - kMaxK) {
+      if (n <= kList - kMaxK) {
         int all = n;
         if (!first) {   // the best of the earlier passes compete again
           if (tid < a.k) {
@@ -355,7 +390,7 @@ __global__ void __launch_bounds__(kThreads, 2) token_logprobs_kernel(const Args 
     const bool empty = all.m == -INFINITY && all.l == 0.f;   // nothing but -inf
     if (tid <= a.k) {
       // tid 0: the given token and the entropy; tid 1..k: an alternative each.  ln L in double: a peaked row has L = 1 + eps
-      const double log_l = log((double)all.l);
+      const double log_l = log((double)all.l), inv_t = 1.0 / (double)a.temperature;
       float value;
       bool in_range = true;
       if (tid == 0) {
@@ -365,12 +400,12 @@ __global__ void __launch_bounds__(kThreads, 2) token_logprobs_kernel(const Args 
       } else {
         value = key_value(sh.list[tid - 1]);
       }
-      float out = empty ? -INFINITY : (float)((double)(value - all.m) / (double)a.temperature - log_l);
+      float out = empty ? -INFINITY : (float)((double)(value - all.m) * inv_t - log_l);
       if (!in_range) out = __int_as_float(0x7FC00000);
       if (tid == 0) {
         a.token_logprob[row] = out;
         if (a.entropy != nullptr)
-          a.entropy[row] = empty ? 0.f : (float)(log_l - (double)all.w / ((double)all.l * (double)a.temperature));
+          a.entropy[row] = empty ? 0.f : (float)(log_l - (double)all.w * inv_t / (double)all.l);
       } else {
         a.top_logprobs[row * a.k + tid - 1] = out;
         a.top_ids[row * a.k + tid - 1] = key_index(sh.list[tid - 1]);
