@@ -4,7 +4,7 @@
 // scale and one bias per 64 channels; a channel stands for code * scale + bias.
 //
 // Attention over the codes, per KV head with rows = (Hq/Hk) * T query rows r and keys n, group g = 64 channels:
-//   S[r,n] = scale * sum_g ( sk[n,g] * sum_{d in g} q[r,d] (ck[n,d] - 8)  +  (bk[n,g] + 8 sk[n,g]) * sum_{d in g} q[r,d] )
+//   S[r,n] = scale * sum_g ( sk[n,g] * sum_{d in g} q[r,d] ck[n,d]  +  bk[n,g] * sum_{d in g} q[r,d] )
 //   O[r,d] = sum_n p[r,n] sv[n,g] (cv[n,d] - 8)  +  sum_n p[r,n] (bv[n,g] + 8 sv[n,g])          (g the group of d)
 // The codes enter both products as exact small integers; scales and biases are applied in fp32 around them, so the only
 // rounding besides fp32 sums is that of p * sv to fp16 (11 bits; the cache's values themselves are never rounded).
@@ -180,13 +180,16 @@ __global__ void __launch_bounds__(128) kv4_read_kernel(const ReadArgs a) {
 //   O^T [16 channels, 8 rows] += V codes^T [16, 16 keys] x P' : P' = p * sv in fp16 (sv brought into fp16's range by a power of
 //       two per warp that is undone at the end).  Nibble t and 4 + t of a word are rows r and r + 8 of MMA t, so a thread's
 //       words serve four MMAs without crossing lanes.
-// Codes become code - 8 by OR-ing the nibble into a constant and one exact packed subtraction: centred integers keep the
-// fp32 sums small (with the constant left in, a score's sum carries 136 or 1032 times sum |q|, which costs digits).
+// Codes become exact fp16 integers by OR-ing the nibble into 1024 and one packed operation that takes the constant away again
+// (left in, a sum would carry 1024 times sum |q| or sum P', which costs digits); values are centred as code - 8, which halves
+// what the rounding of P' is multiplied with.  q is brought to fp16 by a power of two per row: bf16's 8 bits are exact in it
+// down to 2^-28 of the row's largest element.
 // The running maximum moves only when a score exceeds it by 8 octaves (p <= 256 otherwise), so the accumulators are rarely
 // rescaled.  The warps of a block and then the splits of the key range are merged with fp32 partials.
-// Warps of a block, one block per SM: as many as the registers allow (the loop is bound by instruction issue: unpacking, scales
-// and softmax next to the MMAs).
-template <int D, int NT> constexpr int kWarpsOf = NT == 2 ? (D == 256 ? 8 : 12) : (D == 256 ? 12 : 16);
+// Warps of a block.  Two blocks share an SM, so that one starts or merges while the other streams; as many warps as the registers
+// allow (the loop is bound by instruction issue: unpacking, scales and softmax next to the MMAs).
+constexpr int kStages = 3;   // tiles of a warp in shared memory
+template <int D, int NT> constexpr int kWarpsOf = NT == 2 ? (D == 256 ? 4 : 6) : (D == 256 ? 6 : 8);
 constexpr float kMaxStep = 5.545177444f;   // 8 ln 2
 
 template <int D>
@@ -209,24 +212,16 @@ __device__ __forceinline__ uint32_t movm(uint32_t x) {   // transpose of an 8x8 
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
   return y;
 }
-// Codes of nibbles i and 4 + i of a word, minus 8, as pair i.  (1024 + c) - 1032, (1024 + 16 c) / 16 - 72 and (128 + c) - 136 are
+// Codes of nibbles i and 4 + i of a word, minus kMinus, as pair i: (1024 + c) - 1024 - kMinus and (1024 + 16 c) / 16 - 64 - kMinus are
 // exact.
-template <typename T> __device__ __forceinline__ void unpack(uint32_t w, uint32_t (&out)[4]);
-template <> __device__ __forceinline__ void unpack<__half>(uint32_t w, uint32_t (&out)[4]) {
+template <int kMinus>
+__device__ __forceinline__ void unpack(uint32_t w, uint32_t (&out)[4]) {
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const uint32_t u = lop3_and_or(i < 2 ? w : w >> 8, (i & 1) ? 0x00F000F0u : 0x000F000Fu, 0x64006400u);
     __half2 v = *(const __half2*)&u;
-    if (i & 1) v = __hfma2(v, __float2half2_rn(0.0625f), __float2half2_rn(-72.f));
-    else v = __hadd2(v, __float2half2_rn(-1032.f));
-    out[i] = *(const uint32_t*)&v;
-  }
-}
-template <> __device__ __forceinline__ void unpack<__nv_bfloat16>(uint32_t w, uint32_t (&out)[4]) {
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const uint32_t u = lop3_and_or(w >> (4 * i), 0x000F000Fu, 0x43004300u);
-    const __nv_bfloat162 v = __hadd2(*(const __nv_bfloat162*)&u, __float2bfloat162_rn(-136.f));
+    if (i & 1) v = __hfma2(v, __float2half2_rn(0.0625f), __float2half2_rn(-64.f - kMinus));
+    else v = __hadd2(v, __float2half2_rn(-1024.f - kMinus));
     out[i] = *(const uint32_t*)&v;
   }
 }
@@ -238,7 +233,8 @@ template <int D>
 __device__ __forceinline__ int v_chunk(int r, int ch) { return ch ^ (D == 256 ? (((r >> 1) & 3) << 1) : (((r >> 1) & 1) << 1)); }
 
 template <typename T, int D, int NT, bool kMask>
-__global__ void __launch_bounds__((kWarpsOf<D, NT>) * 32) kv4_sdpa_kernel(const SdpaArgs a, int stages) {
+__global__ void __launch_bounds__((kWarpsOf<D, NT>) * 32, 2) kv4_sdpa_kernel(const SdpaArgs a) {
+  constexpr int stages = kStages;
   constexpr int kWarps = (kWarpsOf<D, NT>);
   using TR = MmaTraits<T>;
   using H = MmaTraits<__half>;
@@ -248,7 +244,8 @@ __global__ void __launch_bounds__((kWarpsOf<D, NT>) * 32) kv4_sdpa_kernel(const 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3;
   uint2* sQ = (uint2*)smem;                                   // [NT][KS][32] fragments of Q^T
   float* sQs = (float*)(smem + NT * KS * 32 * 8);             // [NT][G][8] sums of q over a group
-  uint8_t* ring = smem + NT * KS * 32 * 8 + NT * G * 8 * 4 + warp * stages * TL::kBytes;
+  float* sC = sQs + NT * G * 8;                               // [NT][8] what brings a row's products back to scores
+  uint8_t* ring = smem + NT * KS * 32 * 8 + NT * (G + 1) * 8 * 4 + warp * stages * TL::kBytes;
   const uint32_t uring = smem_u32(ring);
   pdl_wait();
   pdl_trigger();
@@ -268,63 +265,74 @@ __global__ void __launch_bounds__((kWarpsOf<D, NT>) * 32) kv4_sdpa_kernel(const 
   const T* kbi = (const T*)a.k.biases + b * a.k.biases_batch_stride + hk * a.k.biases_head_stride;
   const T* vsc = (const T*)a.v.scales + b * a.v.scales_batch_stride + hk * a.v.scales_head_stride;
   const T* vbi = (const T*)a.v.biases + b * a.v.biases_batch_stride + hk * a.v.biases_head_stride;
+  // A lane's places: chunk lane % CPR of row lane / CPR + 32 / CPR * i of the codes; key lane & 15 of two of the four scale arrays.
+  const uint8_t* kl = kc + lane * 16;
+  const uint8_t* vl = vc + lane * 16;
+  const T* sl[2] = {((lane & 16) ? kbi : ksc) + (lane & 15) * G, ((lane & 16) ? vbi : vsc) + (lane & 15) * G};
   auto fetch = [&](int tl, int stage) {
     if (tl < tile1) {
       const uint32_t dst = uring + stage * TL::kBytes;
       const int n0 = tl * 16;
+      const bool whole = n0 + 16 <= hi;
+      const size_t from = (size_t)n0 * (D / 2);
 #pragma unroll
       for (int i = 0; i < 16 * CPR / 32; ++i) {
-        const int at = lane + 32 * i, row = at / CPR, ch = at % CPR;
-        const bool ok = n0 + row < hi;
-        const size_t from = (size_t)(ok ? n0 + row : 0) * (D / 2) + ch * 16;
-        cp16(dst + row * (D / 2) + k_chunk<D>(row, ch) * 16, kc + from, ok);
-        cp16(dst + TL::kCodeBytes + row * (D / 2) + v_chunk<D>(row, ch) * 16, vc + from, ok);
+        const int row = lane / CPR + 32 / CPR * i, ch = lane % CPR;
+        const bool ok = whole || n0 + row < hi;
+        const size_t at = ok ? from + 512 * i : 0;   // 32 chunks of 16 bytes a step
+        cp16(dst + row * (D / 2) + k_chunk<D>(row, ch) * 16, kl + at, ok);
+        cp16(dst + TL::kCodeBytes + row * (D / 2) + v_chunk<D>(row, ch) * 16, vl + at, ok);
       }
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {   // lane -> (array, key)
-        const int which = 2 * i + (lane >> 4), row = lane & 15;
-        const bool ok = n0 + row < hi;
-        const T* base = which == 0 ? ksc : which == 1 ? kbi : which == 2 ? vsc : vbi;
-        cp_small<2 * G>(dst + 2 * TL::kCodeBytes + which * TL::kScaleBytes + row * 2 * G, base + (size_t)(ok ? n0 + row : 0) * G, ok);
+      for (int i = 0; i < 2; ++i) {
+        const bool ok = whole || n0 + (lane & 15) < hi;
+        cp_small<2 * G>(dst + 2 * TL::kCodeBytes + (2 * i + (lane >> 4)) * TL::kScaleBytes + (lane & 15) * 2 * G, sl[i] + (ok ? (size_t)n0 * G : 0), ok);
       }
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
   for (int s = 0; s < stages - 1; ++s) fetch(tile + s * kWarps, s);
 
-  // Q^T fragments: lane (r, c) holds query row r; step ks of group g covers the nibble pairs of words 8g+2c and 8g+2c+1
-  for (int i = threadIdx.x; i < NT * KS * 32; i += kWarps * 32) {
-    const int ln = i & 31, ks = (i >> 5) % KS, nt = (i >> 5) / KS;
-    const int row = row0 + nt * 8 + (ln >> 2), g = ks >> 2, s = ks & 3;
-    uint2 f = make_uint2(0, 0);
-    if (row < a.rows) {
-      const int t = row / a.gqa, h = hk * a.gqa + row % a.gqa;
-      const uint16_t* q = (const uint16_t*)a.q + b * a.q_sb + h * a.q_sh + t * a.q_st + 64 * g + 8 * (2 * (ln & 3) + (s >> 1));
-      const int p = 2 * (s & 1);
-      f.x = (uint32_t)q[p] | ((uint32_t)q[p + 4] << 16);
-      f.y = (uint32_t)q[p + 1] | ((uint32_t)q[p + 5] << 16);
+  // Q^T fragments: a warp per row, a lane per octet j of channels.  In an MMA step lane (r, c) holds row r and the nibble pairs of
+  // words 8g + 2c (steps 0 and 1 of group g) and 8g + 2c + 1 (steps 2 and 3).
+  for (int row = warp; row < 8 * NT; row += kWarps) {
+    uint4 x = make_uint4(0, 0, 0, 0);
+    if (row0 + row < a.rows && lane < D / 8) {
+      const int t = (row0 + row) / a.gqa, h = hk * a.gqa + (row0 + row) % a.gqa;
+      x = *(const uint4*)((const T*)a.q + b * a.q_sb + h * a.q_sh + t * a.q_st + 8 * lane);
     }
-    sQ[i] = f;
-  }
-  for (int i = threadIdx.x; i < NT * G * 8; i += kWarps * 32) {
-    const int row = row0 + (i / (G * 8)) * 8 + (i & 7), g = (i >> 3) % G;
-    float s = 0.f;
-    if (row < a.rows) {
-      const int t = row / a.gqa, h = hk * a.gqa + row % a.gqa;
-      const uint4* q = (const uint4*)((const T*)a.q + b * a.q_sb + h * a.q_sh + t * a.q_st + 64 * g);
+    const uint32_t u[4] = {x.x, x.y, x.z, x.w};
+    float f[8], big = 0.f;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const uint4 w = q[e];
-        const uint32_t u[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-        for (int x = 0; x < 4; ++x) s += TR::bits_to_float((uint16_t)u[x]) + TR::bits_to_float((uint16_t)(u[x] >> 16));
-      }
+    for (int e = 0; e < 8; ++e) {
+      f[e] = TR::bits_to_float((uint16_t)(u[e >> 1] >> (16 * (e & 1))));
+      big = fmaxf(big, fabsf(f[e]));   // NaN is passed over; an infinity makes the row NaN whatever its scale
     }
-    sQs[i] = s;
+    const int eq = max((int)(__reduce_max_sync(0xffffffffu, __float_as_uint(big)) >> 23) - 127 - 14, -100);
+    const float to_q = __uint_as_float((uint32_t)(127 - eq) << 23);
+    float sum = 0.f;
+    uint32_t p[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const __half2 hh = __floats2half2_rn(f[e] * to_q, f[4 + e] * to_q);
+      p[e] = *(const uint32_t*)&hh;
+      sum += __low2float(hh) + __high2float(hh);
+    }
+#pragma unroll
+    for (int w = 1; w < 8; w <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, w);
+    const int nt = row >> 3, rr = row & 7, g = lane >> 3;
+    if (lane < D / 8) {
+      uint2* dst = sQ + (nt * KS + 4 * g + 2 * (lane & 1)) * 32 + rr * 4 + ((lane & 7) >> 1);
+      dst[0] = make_uint2(p[0], p[1]);
+      dst[32] = make_uint2(p[2], p[3]);
+      if ((lane & 7) == 0) sQs[(nt * G + g) * 8 + rr] = sum;
+    }
+    if (lane == 0) sC[row] = a.scale * __uint_as_float((uint32_t)(127 + eq) << 23);
   }
   __syncthreads();
 
-  float o[D / 16][NT][4], ob[G][NT][2], m[NT][2], l[NT][2];
+  float o[D / 16][NT][4], m[NT][2], l[NT][2], cs[NT][2];
+  uint64_t ob[G][NT];   // the rows 2c and 2c + 1 side by side, as in s
   int lim[NT][2];
   long long mat[NT][2];
 #pragma unroll
@@ -337,9 +345,10 @@ __global__ void __launch_bounds__((kWarpsOf<D, NT>) * 32) kv4_sdpa_kernel(const 
       const int t = row / a.gqa;
       lim[nt][e] = row < a.rows ? min(len - a.T + t, hi - 1) : -1;   // last key the row sees
       mat[nt][e] = kMask && row < a.rows ? b * a.m_sb + (hk * a.gqa + row % a.gqa) * a.m_sh + t * a.m_st : 0;
-#pragma unroll
-      for (int g = 0; g < G; ++g) ob[g][nt][e] = 0.f;
+      cs[nt][e] = sC[nt * 8 + 2 * c + e];
     }
+#pragma unroll
+    for (int g = 0; g < G; ++g) ob[g][nt] = 0;
 #pragma unroll
     for (int i = 0; i < D / 16; ++i) o[i][nt][0] = o[i][nt][1] = o[i][nt][2] = o[i][nt][3] = 0.f;
   }
@@ -353,9 +362,7 @@ __global__ void __launch_bounds__((kWarpsOf<D, NT>) * 32) kv4_sdpa_kernel(const 
       fetch(tile + (stages - 1) * kWarps, ahead);
     }
     // this tile is the oldest of `stages` groups in flight
-    if (stages == 4) asm volatile("cp.async.wait_group 3;" ::: "memory");
-    else if (stages == 3) asm volatile("cp.async.wait_group 2;" ::: "memory");
-    else asm volatile("cp.async.wait_group 1;" ::: "memory");
+    asm volatile("cp.async.wait_group %0;" ::"n"(stages - 1) : "memory");
     __syncwarp();
     const uint8_t* st = ring + stage * TL::kBytes;
     const int n0 = tile * 16;
@@ -375,7 +382,7 @@ __global__ void __launch_bounds__((kWarpsOf<D, NT>) * 32) kv4_sdpa_kernel(const 
 #pragma unroll
       for (int g = 0; g < G; ++g) {
         sk[e][g] = TR::bits_to_float(h[0][g]);
-        bk[e][g] = fmaf(sk[e][g], 8.f, TR::bits_to_float(h[1][g]));
+        bk[e][g] = TR::bits_to_float(h[1][g]);
         sv[e][g] = TR::bits_to_float(h[2][g]);
         const float bb = TR::bits_to_float(h[3][g]);
         bad[e] = fmaf(sv[e][g], 0.f, fmaf(bb, 0.f, bad[e]));   // NaN when a scale or bias of the value is not finite
@@ -396,9 +403,9 @@ __global__ void __launch_bounds__((kWarpsOf<D, NT>) * 32) kv4_sdpa_kernel(const 
         }
     }
     // ---- S^T = K Q^T ----
-    float s[NT][4];
+    uint64_t s2[NT][2];   // key r, then r + 8; rows 2c and 2c + 1 side by side
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.f;
+    for (int nt = 0; nt < NT; ++nt) s2[nt][0] = s2[nt][1] = 0;
 #pragma unroll
     for (int g = 0; g < G; ++g) {
       const uint2 w0 = *(const uint2*)(st + r * (D / 2) + k_chunk<D>(r, 2 * g + (c >> 1)) * 16 + (c & 1) * 8);
@@ -409,24 +416,29 @@ __global__ void __launch_bounds__((kWarpsOf<D, NT>) * 32) kv4_sdpa_kernel(const 
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
         uint32_t u0[4], u1[4];
-        unpack<T>(half ? w0.y : w0.x, u0);
-        unpack<T>(half ? w1.y : w1.x, u1);
+        unpack<0>(half ? w0.y : w0.x, u0);
+        unpack<0>(half ? w1.y : w1.x, u1);
 #pragma unroll
         for (int ks = 0; ks < 2; ++ks)
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
             const uint2 f = sQ[(nt * KS + 4 * g + 2 * half + ks) * 32 + lane];
-            TR::mma(acc[nt], u0[2 * ks], u1[2 * ks], u0[2 * ks + 1], u1[2 * ks + 1], f.x, f.y);
+            H::mma(acc[nt], u0[2 * ks], u1[2 * ks], u0[2 * ks + 1], u1[2 * ks + 1], f.x, f.y);
           }
       }
+      const uint64_t sk0 = pair(sk[0][g], sk[0][g]), sk1 = pair(sk[1][g], sk[1][g]), bk0 = pair(bk[0][g], bk[0][g]), bk1 = pair(bk[1][g], bk[1][g]);
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
-        const float2 qs = *(const float2*)(sQs + (nt * G + g) * 8 + 2 * c);
-        s[nt][0] = fmaf(sk[0][g], acc[nt][0], fmaf(bk[0][g], qs.x, s[nt][0]));
-        s[nt][1] = fmaf(sk[0][g], acc[nt][1], fmaf(bk[0][g], qs.y, s[nt][1]));
-        s[nt][2] = fmaf(sk[1][g], acc[nt][2], fmaf(bk[1][g], qs.x, s[nt][2]));
-        s[nt][3] = fmaf(sk[1][g], acc[nt][3], fmaf(bk[1][g], qs.y, s[nt][3]));
+        const uint64_t qs = *(const uint64_t*)(sQs + (nt * G + g) * 8 + 2 * c);
+        s2[nt][0] = fma2(sk0, pair(acc[nt][0], acc[nt][1]), fma2(bk0, qs, s2[nt][0]));
+        s2[nt][1] = fma2(sk1, pair(acc[nt][2], acc[nt][3]), fma2(bk1, qs, s2[nt][1]));
       }
+    }
+    float s[NT][4];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      unpair(s2[nt][0], s[nt][0], s[nt][1]);
+      unpair(s2[nt][1], s[nt][2], s[nt][3]);
     }
     // ---- visibility, running maximum ----
     bool grow = big * sv_mul > 64.f;
@@ -435,7 +447,7 @@ __global__ void __launch_bounds__((kWarpsOf<D, NT>) * 32) kv4_sdpa_kernel(const 
 #pragma unroll
       for (int x = 0; x < 4; ++x) {
         const int n = n0 + r + ((x >> 1) << 3), e = x & 1;
-        float t = fmaf(s[nt][x], a.scale, bad[x >> 1]);
+        float t = fmaf(s[nt][x], cs[nt][e], bad[x >> 1]);
         const bool seen = n <= lim[nt][e];
         if (kMask) {
           if (seen) t = apply_mask<T>(a, t, mat[nt][e] + n * a.m_sn);
@@ -466,10 +478,11 @@ __global__ void __launch_bounds__((kWarpsOf<D, NT>) * 32) kv4_sdpa_kernel(const 
           f[e] = x == -INFINITY ? 1.f : ex2((m[nt][e] - x) * kLog2e);   // nothing seen yet: the sums are zero
           m[nt][e] = x;
           l[nt][e] *= f[e];
-#pragma unroll
-          for (int g = 0; g < G; ++g) ob[g][nt][e] *= f[e];
-          f[e] *= ratio;
         }
+#pragma unroll
+        for (int g = 0; g < G; ++g) ob[g][nt] = mul2(ob[g][nt], pair(f[0], f[1]));
+        f[0] *= ratio;
+        f[1] *= ratio;
 #pragma unroll
         for (int i = 0; i < D / 16; ++i) {
           o[i][nt][0] *= f[0]; o[i][nt][1] *= f[1];
@@ -492,13 +505,17 @@ __global__ void __launch_bounds__((kWarpsOf<D, NT>) * 32) kv4_sdpa_kernel(const 
     for (int g = 0; g < G; ++g) {
       uint32_t pb[NT][2];
       const float s0 = sv[0][g] * sv_mul, s1 = sv[1][g] * sv_mul;
+      const uint64_t bv0 = pair(bv[0][g], bv[0][g]), bv1 = pair(bv[1][g], bv[1][g]);
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
-        const __half2 h0 = __floats2half2_rn(s[nt][0] * s0, s[nt][1] * s0), h1 = __floats2half2_rn(s[nt][2] * s1, s[nt][3] * s1);
+        const uint64_t p0 = pair(s[nt][0], s[nt][1]), p1 = pair(s[nt][2], s[nt][3]);
+        float x0, x1, x2, x3;
+        unpair(mul2(p0, pair(s0, s0)), x0, x1);
+        unpair(mul2(p1, pair(s1, s1)), x2, x3);
+        const __half2 h0 = __floats2half2_rn(x0, x1), h1 = __floats2half2_rn(x2, x3);
         pb[nt][0] = movm(*(const uint32_t*)&h0);
         pb[nt][1] = movm(*(const uint32_t*)&h1);
-        ob[g][nt][0] = fmaf(s[nt][0], bv[0][g], fmaf(s[nt][2], bv[1][g], ob[g][nt][0]));
-        ob[g][nt][1] = fmaf(s[nt][1], bv[0][g], fmaf(s[nt][3], bv[1][g], ob[g][nt][1]));
+        ob[g][nt] = fma2(p0, bv0, fma2(p1, bv1, ob[g][nt]));
       }
       uint32_t w[4];   // word 8g + r of keys 2c, 2c+1, 2c+8, 2c+9
 #pragma unroll
@@ -508,10 +525,10 @@ __global__ void __launch_bounds__((kWarpsOf<D, NT>) * 32) kv4_sdpa_kernel(const 
       }
       // nibbles 0..3 / 4..7 of two keys side by side
       uint32_t lo01[4], hi01[4], lo89[4], hi89[4];
-      unpack<__half>(prmt(w[0], w[1], 0x5410), lo01);
-      unpack<__half>(prmt(w[0], w[1], 0x7632), hi01);
-      unpack<__half>(prmt(w[2], w[3], 0x5410), lo89);
-      unpack<__half>(prmt(w[2], w[3], 0x7632), hi89);
+      unpack<8>(prmt(w[0], w[1], 0x5410), lo01);
+      unpack<8>(prmt(w[0], w[1], 0x7632), hi01);
+      unpack<8>(prmt(w[2], w[3], 0x5410), lo89);
+      unpack<8>(prmt(w[2], w[3], 0x7632), hi89);
 #pragma unroll
       for (int t = 0; t < 4; ++t)
 #pragma unroll
@@ -524,7 +541,7 @@ __global__ void __launch_bounds__((kWarpsOf<D, NT>) * 32) kv4_sdpa_kernel(const 
   __syncthreads();   // the rings become the merge buffers
 
   // ---- merge the warps: O [warp][8 NT][D], m and l [warp][8 NT] ----
-  float* mO = (float*)(smem + NT * KS * 32 * 8 + NT * G * 8 * 4);
+  float* mO = (float*)(smem + NT * KS * 32 * 8 + NT * (G + 1) * 8 * 4);
   float* mM = mO + kWarps * 8 * NT * D;
   float* mL = mM + kWarps * 8 * NT;
   const float undo = 1.f / sv_mul;
@@ -543,7 +560,9 @@ __global__ void __launch_bounds__((kWarpsOf<D, NT>) * 32) kv4_sdpa_kernel(const 
       float* po = mO + ((size_t)warp * 8 * NT + row) * D;
 #pragma unroll
       for (int g = 0; g < G; ++g) {
-        float y = ob[g][nt][e];
+        float y, other;
+        if (e == 0) unpair(ob[g][nt], y, other);
+        else unpair(ob[g][nt], other, y);
 #pragma unroll
         for (int w = 4; w < 32; w <<= 1) y += __shfl_xor_sync(0xffffffffu, y, w);
         float4 v0, v1;   // channels 64g + 8r + 0..3 and + 4..7
@@ -659,17 +678,17 @@ __global__ void __launch_bounds__(256) kv4_combine_kernel(const SdpaArgs a) {
 // ---- host side ---------------------------------------------------------------------------------------------------------
 int row_tile(int rows) { return rows <= 8 ? 1 : 2; }   // 8-row columns of the MMA tile: 16 query rows share one pass
 
-// Key ranges per (sequence, KV head, row tile), one block per SM at a time.  A block costs its keys and about kOverhead keys'
+// Key ranges per (sequence, KV head, row tile), per_sm blocks on an SM at a time.  A block costs its keys and about kOverhead keys'
 // worth of start-up and merging.  Equal sequences run in whole waves; sequences of different lengths (several of them: the host
 // does not know) fill the SMs as blocks end, behind the longest of which the launch waits: half of each estimate.
 constexpr int kOverhead = 320;
-int choose_splits(long long units, int B, int max_length, int device, int requested) {
-  const int most = (max_length + 127) / 128;   // a 16-key tile per warp
+int choose_splits(long long units, int B, int max_length, int device, int requested, int per_sm) {
+  const int most = (max_length + 127) / 128;
   if (requested > 0) return requested < most ? requested : most;
-  const int sms = sm_count(device);
+  const int sms = per_sm * sm_count(device);   // blocks at a time
   int best = 1;
   double least = 1e300;
-  for (int s = 1; s <= most && s <= 1024 && units * s <= 8ll * sms; ++s) {
+  for (int s = 1; s <= most && s <= 1024 && units * s <= 4ll * sms; ++s) {
     const double keys = (double)max_length / s + kOverhead;
     double cost = (double)((units * s + sms - 1) / sms) * keys;
     if (B > 1) cost = 0.5 * cost + 0.5 * ((double)(units * s) / sms * (0.6 * max_length / s + kOverhead) + 0.5 * keys);
@@ -685,12 +704,11 @@ template <typename T, int D, int NT>
 int launch_sdpa(SdpaArgs a, cudaStream_t st, int device) {
   constexpr int kWarps = (kWarpsOf<D, NT>);
   using TL = Tile<D>;
-  constexpr size_t fixed = (size_t)NT * (D / 16) * 32 * 8 + (size_t)NT * (D / kGroup) * 8 * 4;
+  constexpr size_t fixed = (size_t)NT * (D / 16) * 32 * 8 + (size_t)NT * (D / kGroup + 1) * 8 * 4;
   constexpr size_t merge = (size_t)kWarps * 8 * NT * (D + 2) * 4;
-  constexpr int stages = 3;
-  constexpr size_t ring = (size_t)kWarps * stages * TL::kBytes;
+  constexpr size_t ring = (size_t)kWarps * kStages * TL::kBytes;
   constexpr size_t smem = fixed + (ring > merge ? ring : merge);
-  static_assert(smem <= 227 * 1024, "shared memory");
+  static_assert(smem <= 113 * 1024, "two blocks of an SM share its memory");
   auto kern = a.mask_kind ? kv4_sdpa_kernel<T, D, NT, true> : kv4_sdpa_kernel<T, D, NT, false>;
   static std::mutex mu;
   static bool done[64][2] = {};
@@ -704,7 +722,7 @@ int launch_sdpa(SdpaArgs a, cudaStream_t st, int device) {
     }
   }
   const int row_tiles = (a.rows + 8 * NT - 1) / (8 * NT);
-  cudaError_t e = launch_kernel(kern, dim3(a.splits, row_tiles, a.B * a.Hk), dim3(kWarps * 32), smem, st, a, stages);
+  cudaError_t e = launch_kernel(kern, dim3(a.splits, row_tiles, a.B * a.Hk), dim3(kWarps * 32), smem, st, a);
   if (e == cudaSuccess) e = cudaGetLastError();
   if (e != cudaSuccess) return fail(DFLASH_ERR_LAUNCH, "kv4_sdpa launch: %s", cudaGetErrorString(e));
   return DFLASH_OK;
@@ -844,7 +862,7 @@ extern "C" int dflash_kv4_read(const dflash_kv4_cache* k_cache, const dflash_kv4
 static int kv4_splits(int B, int Hk, long long rows, int max_length, int device, int num_splits) {
   const int tile = rows > kFewRows ? kTcRows : 8 * row_tile((int)rows);
   const long long units = (long long)B * Hk * ((rows + tile - 1) / tile);
-  return choose_splits(units, B, max_length, device, num_splits);
+  return choose_splits(units, B, max_length, device, num_splits, rows > kFewRows ? 1 : 2);
 }
 
 extern "C" size_t dflash_kv4_sdpa_workspace_bytes(int B, int Hq, int Hk, int T, int D, int max_length, int num_splits) {
