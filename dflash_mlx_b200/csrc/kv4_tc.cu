@@ -2,18 +2,17 @@
 // grouped model, a chunk of a prompt); the contract and the formulas are those of kv4.cu.
 //
 // One block = 128 query rows (row = position * heads-per-KV-head + head, the TMEM lanes of an M128 tile) and a range of keys,
-// in tiles of 128: two score tiles and the output fill tensor memory (2 x 128 + 256 columns; narrower score tiles ran at half
-// rate, an M128 N64 MMA taking as long as N128).  Keys and values are unpacked to fp16 into 128B-swizzled shared memory: a slab
-// per 64 channels (one quantisation group), rows of keys of 128 bytes, which is K-major for S = Q K^T and MN-major for O = P V.
+// in pairs of 64-key tiles: two pairs of score tiles and the output fill tensor memory (2 x 128 + 256 columns).  Keys and values are
+// unpacked to fp16 into 128B-swizzled shared memory: a slab per 64 channels (one quantisation group), rows of keys of 128 bytes,
+// which is K-major for S = Q K^T and MN-major for O = P V.  Scores are multiplied by pairs (an M128 N64 MMA takes 55 clocks, N128 64),
+// softmax and output go tile by tile.
 //   warps 0-7    softmax, a thread per row: S from tensor memory, P back over it, O rescaled in place when the maximum moved.  Warps
-//                0-3 take the even tiles and 4-7 the odd ones (one warp per SM sub-partition left the softmax latency bound:
-//                4300 clocks a tile); a row's reference maximum is handed from one to the other right after a tile's maxima
+//                0-3 take the even tiles and 4-7 the odd ones; a row's reference maximum is handed from one to the other right
+//                after a tile's maxima
 //   warps 8-11   unpack keys, 12-15 values: a thread owns a key, a group at a time
-//   warp 16      one thread issues S(i) = Q K(i)^T, warp 17 O += P(i) V(i): issuing an MMA blocks until the pipe has room and a
-//                satisfied wait costs about 100 cycles of it, so each thread waits under the other one's MMAs
-// Two score tiles are in flight: a tile's softmax runs under the next one's scores.  One tile of keys and one of values are
-// enough: a slab of keys is free as soon as its four steps of QK(i) are done and is refilled under PV(i-1), values (in blocks of
-// 32 keys) the other way round.
+//   warp 16      one thread issues S = Q K^T, warp 17 O += P V: issuing an MMA blocks until the pipe has room and a satisfied wait
+//                costs about 100 cycles of it, so each thread waits under the other one's MMAs
+// A slab of keys is refilled as soon as its steps are done, either half of the values while the other one is multiplied.
 //
 // Unpacking costs 9 instructions for 8 codes: a nibble left in place is an fp16 subnormal, code * 2^-24 (or * 2^-20), and one packed
 // fma turns two of them into code * scale + bias with a single rounding to fp16 (2^-11; the cache's scales carry 8 or 11 bits,
@@ -31,14 +30,14 @@ namespace kv4 {
 namespace {
 
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
-constexpr int kRows = 128, kKeys = 128;
+constexpr int kRows = 128, kKeys = 128, kTile = 64;   // keys are unpacked by 128, multiplied by 64
 constexpr int kThreads = 18 * 32, kKeyWarp = 8, kValueWarp = 12, kIssuer = 16;   // kIssuer: scores; the next warp: output
 constexpr float kMaxStep = 8 * kLn2;   // natural units
 constexpr float kPShift = 6.f;         // P = p * 2^6 (p <= 2^8): further from fp16's subnormals
 constexpr int kSlab = kKeys * 128;     // 128 rows x 64 channels: Q, K or V
-constexpr uint32_t kOCol = 256, kCols = 512;   // S / P of tile i at 128 * (i & 1)
+constexpr uint32_t kOCol = 256, kCols = 512;   // S / P of tile i at 64 * (i & 3)
 
-// What softmax needs to know about a tile: per 32 keys the power of two of K, the exponent of V, and keys whose value is not
+// What softmax needs to know about 128 keys: per 32 of them the power of two of K, the exponent of V, and keys whose value is not
 // finite.
 struct Meta {
   float k_factor[4];
@@ -47,10 +46,11 @@ struct Meta {
 };
 constexpr int kMeta = 4;   // scales are looked at no more than three tiles ahead of the softmax
 
-// mbarriers, 8 bytes each.  kBarVMeta: a tile's exponents of V are known; kBarM: a row reference handed on, per tile
-// parity and 32 rows
-enum { kBarKFull = 0, kBarVFull = 1, kBarQ = 2, kBarKEmpty = 4, kBarVEmpty = 8, kBarS = 12, kBarP = 14, kBarO = 16, kBarM = 18,
-       kBarVMeta = 26, kBars = 30 };
+// mbarriers, 8 bytes each.  kBarKEmpty: per slab; V full and empty: per half of the buffer (64 keys); kBarS: per pair of score tiles;
+// P, O: per tile in flight; kBarM: a row reference handed on, per tile parity and 32 rows; kBarVMeta: the values' exponents of 128
+// keys are known
+enum { kBarKFull = 0, kBarQ = 1, kBarVFull = 2, kBarKEmpty = 4, kBarVEmpty = 8, kBarS = 10, kBarP = 12, kBarO = 16, kBarM = 20,
+       kBarVMeta = 28, kBars = 32 };
 
 __device__ __forceinline__ bool wait_bar(uint32_t bar, uint32_t parity) {
   for (uint32_t i = 0; i < (1u << 16); ++i) {   // hardware-suspended polls of up to a microsecond
@@ -102,6 +102,19 @@ __device__ __forceinline__ void ld32(uint32_t taddr, uint32_t* r) {
       : "r"(taddr)
       : "memory");
 }
+__device__ __forceinline__ void ld16(uint32_t taddr, uint32_t* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr)
+      : "memory");
+}
+__device__ __forceinline__ void st8(uint32_t taddr, const uint32_t* r) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(taddr), "r"(r[0]), "r"(r[1]),
+               "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+               : "memory");
+}
 __device__ __forceinline__ void wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void st16(uint32_t taddr, const uint32_t* r) {
@@ -134,18 +147,13 @@ __device__ __forceinline__ void scales_of(const uint32_t (&r)[D / 128], float (&
 #pragma unroll
   for (int g = 0; g < D / kGroup; ++g) s[g] = MmaTraits<T>::bits_to_float((uint16_t)(r[g >> 1] >> (16 * (g & 1))));
 }
-// Exponent e shared by the warp's 32 keys: scale * 2^-e < 2^-9 and |bias| * 2^-e < 2^14 for the finite ones.
+// The largest value a key's scales allow, as bits (15 |scale| + |bias| over its groups): not finite where one of them is not.
 template <int G>
-__device__ __forceinline__ int block_exponent(const float (&s)[G], const float (&b)[G]) {
-  float ms = 0.f, mb = 0.f;
+__device__ __forceinline__ uint32_t largest_bits(const float (&s)[G], const float (&b)[G]) {
+  uint32_t m = 0;
 #pragma unroll
-  for (int g = 0; g < G; ++g) {
-    ms = fmaxf(ms, finite(s[g]) ? fabsf(s[g]) : 0.f);
-    mb = fmaxf(mb, finite(b[g]) ? fabsf(b[g]) : 0.f);
-  }
-  const int es = (int)(__reduce_max_sync(0xffffffffu, __float_as_uint(ms)) >> 23) - 127;
-  const int eb = (int)(__reduce_max_sync(0xffffffffu, __float_as_uint(mb)) >> 23) - 127;
-  return min(max(max(es + 10, eb - 13), -100), 126);
+  for (int g = 0; g < G; ++g) m = max(m, __float_as_uint(fmaf(fabsf(s[g]), 15.f, fabsf(b[g]))) & 0x7FFFFFFFu);
+  return m;
 }
 __device__ __forceinline__ uint32_t hfma2(uint32_t a, uint32_t b, uint32_t c) {
   uint32_t d;
@@ -155,21 +163,6 @@ __device__ __forceinline__ uint32_t hfma2(uint32_t a, uint32_t b, uint32_t c) {
 __device__ __forceinline__ uint32_t splat(float x) {
   const __half2 h = __float2half2_rn(x);
   return *(const uint32_t*)&h;
-}
-// Exponent for unpack_row's wide form: |scale| * 15 + |bias| of every finite key is below 2^14 after it, and whether the keys
-// are too unlike for the narrow form: a key's largest value is more than 6 octaves below the largest of the 32.
-template <int G>
-__device__ __forceinline__ bool wide_range(const float (&s)[G], const float (&b)[G], int* e) {
-  float mine = 0.f;
-#pragma unroll
-  for (int g = 0; g < G; ++g) {
-    const float x = fmaf(fabsf(s[g]), 15.f, fabsf(b[g]));
-    mine = fmaxf(mine, finite(x) ? x : 0.f);
-  }
-  const uint32_t u = __float_as_uint(mine) >> 23;
-  const int hi = (int)__reduce_max_sync(0xffffffffu, u), lo = (int)__reduce_min_sync(0xffffffffu, mine == 0.f ? 255u : u);
-  *e = min(max(hi - 127 - 13, -100), 126);
-  return hi - lo > 6 && lo < 255;
 }
 // Bit e: byte mask entry of key n0 + e is not 0, for the bits set in `want` (others are not read).
 __device__ __forceinline__ uint32_t mask_bits(const SdpaArgs& a, long long at, int n0, uint32_t want) {
@@ -297,14 +290,17 @@ __device__ __forceinline__ void unpack_side(const dflash_kv4_cache& c, int b, in
   auto prepare = [&](int tile) {
     scales_of<T, D>(ns, s);
     scales_of<T, D>(nz, z);
-    wide = false;
-    if (kV) wide = wide_range(s, z, &e);
-    if (!wide) e = block_exponent(s, z);
+    const uint32_t largest = largest_bits(s, z);
+    const bool bad = largest >= 0x7F800000u;
+    const int hi_e = (int)(__reduce_max_sync(0xffffffffu, bad ? 0u : largest) >> 23) - 127;   // values of the 32 keys are below 2^(hi_e + 1)
+    // |scale| is below 2^(hi_e - 2): times 2^-e it is below 2^-9, where an fp16 scale * 2^24 still fits
+    e = min(max(hi_e + 7, -100), 126);
     Meta& m = meta[tile & (kMeta - 1)];
     if (kV) {
-      bool bad = false;
-#pragma unroll
-      for (int g = 0; g < G; ++g) bad |= !finite(s[g]) || !finite(z[g]);
+      // keys whose largest value is more than 6 octaves below: the narrow form would lose their bits
+      const int lo_e = (int)(__reduce_min_sync(0xffffffffu, bad || largest == 0 ? 0x7F7FFFFFu : largest) >> 23) - 127;
+      wide = hi_e - lo_e > 6;
+      if (wide) e = min(max(hi_e - 13, -100), 126);   // values below 2^14
       if (bad) {   // out of the products; rows that see it get NaN through its score
 #pragma unroll
         for (int g = 0; g < G; ++g) s[g] = z[g] = 0.f;
@@ -336,8 +332,8 @@ __device__ __forceinline__ void unpack_side(const dflash_kv4_cache& c, int b, in
     }
     asm volatile("cp.async.wait_group 0;" ::: "memory");
     __syncwarp();
-    // this warp's keys are one block of the values' buffer
-    if (kV && !wait_warp(bar0 + 8 * (kBarVEmpty + w), (t & 1) ^ 1)) { atomicCAS(err, 0, 62 | (1 << 8)); break; }
+    // two warps share a half of the values' buffer
+    if (kV && !wait_warp(bar0 + 8 * (kBarVEmpty + (w >> 1)), (t & 1) ^ 1)) { atomicCAS(err, 0, 62 | (1 << 8)); break; }
     bool ok = true;
 #pragma unroll 1
     for (int g = 0; g < G; ++g) {
@@ -353,7 +349,7 @@ __device__ __forceinline__ void unpack_side(const dflash_kv4_cache& c, int b, in
       else unpack_row<false>(c0, c1, sg, zg, ce, row, key);
     }
     if (!ok) break;
-    done(bar0 + 8 * (kV ? kBarVFull : kBarKFull));
+    done(bar0 + 8 * (kV ? kBarVFull + (w >> 1) : kBarKFull));
     load(t + 1);
     if (!kV) {   // a tile's factor is published with its codes: nothing waits for it before
       prepare(t + 1);
@@ -382,20 +378,20 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_sdpa_tc_kernel(const SdpaArgs
   const uint32_t bar0 = smem_u32(bars);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
+    mbar_init(bar0 + 8 * kBarKFull, 4);
+    mbar_init(bar0 + 8 * kBarQ, kIssuer);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(bar0 + 8 * (kBarVFull + i), 2);
+      mbar_init(bar0 + 8 * (kBarVEmpty + i), 1);
+      mbar_init(bar0 + 8 * (kBarS + i), 1);
+    }
     for (int i = 0; i < 4; ++i) {
       mbar_init(bar0 + 8 * (kBarKEmpty + i), 1);
-      mbar_init(bar0 + 8 * (kBarVEmpty + i), 1);
-      mbar_init(bar0 + 8 * (kBarVMeta + i), 4);
-    }
-    for (int i = 0; i < 2; ++i) {
-      mbar_init(bar0 + 8 * (kBarS + i), 1);
       mbar_init(bar0 + 8 * (kBarP + i), 4);
       mbar_init(bar0 + 8 * (kBarO + i), 1);
+      mbar_init(bar0 + 8 * (kBarVMeta + i), 4);
     }
     for (int i = 0; i < 8; ++i) mbar_init(bar0 + 8 * (kBarM + i), 1);
-    mbar_init(bar0 + 8 * kBarQ, kIssuer);
-    mbar_init(bar0 + 8 * kBarKFull, 4);
-    mbar_init(bar0 + 8 * kBarVFull, 4);
     mbar_fence_init();
   }
   if (warp == kIssuer) {
@@ -416,52 +412,51 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_sdpa_tc_kernel(const SdpaArgs
   const int tiles_all = hi > 0 ? (hi + kKeys - 1) / kKeys : 0;
   const int per = (tiles_all + a.splits - 1) / a.splits;
   const int k0 = split * per * kKeys;
-  const int tiles = max(0, min(tiles_all - split * per, per));
+  const int pairs = max(0, min(tiles_all - split * per, per));                    // 128 keys each
+  const int tiles = (min(pairs * kKeys, hi - k0) + kTile - 1) / kTile;            // 64 keys each; 0 without pairs
 
   // Q: a row per D / 8 lanes, brought to fp16 by a power of two (its largest element to [2^7, 2^8)) in unpack_row's channel order;
   // the scale's sign goes with it, so that scores grow with their products.  Sixteen warps, every sixteenth row each.
   auto query_rows = [&]() {
-    constexpr int kLanes = D / 8, kPer = 32 / kLanes, kBatch = 4;
+    constexpr int kLanes = D / 8, kPer = 32 / kLanes, kSteps = kRows / (kIssuer * kPer);
     const int j = lane % kLanes;
+    // raw into place, all copies in flight at once
+#pragma unroll 2
+    for (int i = 0; i < kSteps; ++i) {
+      const int r = (i * kIssuer + warp) * kPer + lane / kLanes, row = row0 + r;
+      const bool in = row < a.rows;
+      const int t = in ? row / a.gqa : 0, h = hk * a.gqa + (in ? row - t * a.gqa : 0);
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(sQ + (j >> 3) * kSlab + r * 128 + (((j & 7) ^ (r & 7)) << 4))),
+                   "l"((const T*)a.q + b * a.q_sb + h * a.q_sh + t * a.q_st + 8 * j), "r"(in ? 16 : 0)
+                   : "memory");
+    }
+    asm volatile("cp.async.commit_group;\n\tcp.async.wait_group 0;" ::: "memory");   // a lane reads what it copied itself
 #pragma unroll 1
-    for (int i0 = 0; i0 * kIssuer * kPer < kRows; i0 += kBatch) {
-      uint4 x[kBatch];
+    for (int i = 0; i < kSteps; ++i) {
+      const int r = (i * kIssuer + warp) * kPer + lane / kLanes;
+      uint4* place = (uint4*)(sQ + (j >> 3) * kSlab + r * 128 + (((j & 7) ^ (r & 7)) << 4));
+      const uint4 x = *place;
+      const uint32_t u[4] = {x.x, x.y, x.z, x.w};
+      // largest magnitude of the row, NaN passed over (an infinity makes the row NaN whatever its scale)
+      uint32_t top = abs_max<T>(abs_max<T>(u[0], u[1]), abs_max<T>(u[2], u[3]));
+      top = __float_as_uint(fmaxf(TR::bits_to_float((uint16_t)(top & 0x7FFFu)), TR::bits_to_float((uint16_t)((top >> 16) & 0x7FFFu))));
+      if (kLanes == 32) {
+        top = __reduce_max_sync(0xffffffffu, top);
+      } else {
 #pragma unroll
-      for (int i = 0; i < kBatch; ++i) {
-        const int r = ((i0 + i) * kIssuer + warp) * kPer + lane / kLanes, row = row0 + r;
-        x[i] = make_uint4(0, 0, 0, 0);
-        if (r < kRows && row < a.rows) {
-          const int t = row / a.gqa, h = hk * a.gqa + row % a.gqa;
-          x[i] = *(const uint4*)((const T*)a.q + b * a.q_sb + h * a.q_sh + t * a.q_st + 8 * j);
-        }
+        for (int o = 1; o < kLanes; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
       }
+      const int eq = min(max((int)(top >> 23) - 127 - 7, -100), 126);
+      const float to_q = a.scale < 0.f ? -pow2(-eq) : pow2(-eq);
+      uint32_t p[4];
 #pragma unroll
-      for (int i = 0; i < kBatch; ++i) {
-        const int r = ((i0 + i) * kIssuer + warp) * kPer + lane / kLanes;
-        const uint32_t u[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
-        // largest magnitude of the row, NaN passed over (an infinity makes the row NaN whatever its scale)
-        uint32_t top = abs_max<T>(abs_max<T>(u[0], u[1]), abs_max<T>(u[2], u[3]));
-        top = __float_as_uint(fmaxf(TR::bits_to_float((uint16_t)(top & 0x7FFFu)), TR::bits_to_float((uint16_t)((top >> 16) & 0x7FFFu))));
-        if (kLanes == 32) {
-          top = __reduce_max_sync(0xffffffffu, top);
-        } else {
-#pragma unroll
-          for (int o = 1; o < kLanes; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-        }
-        const int eq = min(max((int)(top >> 23) - 127 - 7, -100), 126);
-        const float to_q = a.scale < 0.f ? -pow2(-eq) : pow2(-eq);
-        uint32_t p[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float f0 = TR::bits_to_float((uint16_t)(u[e >> 1] >> (16 * (e & 1)))), f1 = TR::bits_to_float((uint16_t)(u[2 + (e >> 1)] >> (16 * (e & 1))));
-          const __half2 hh = __floats2half2_rn(f0 * to_q, f1 * to_q);
-          p[e] = *(const uint32_t*)&hh;
-        }
-        if (r < kRows) {
-          *(uint4*)(sQ + (j >> 3) * kSlab + r * 128 + (((j & 7) ^ (r & 7)) << 4)) = make_uint4(p[0], p[1], p[2], p[3]);
-          if (j == 0) sE[r] = eq;
-        }
+      for (int e = 0; e < 4; ++e) {
+        const float f0 = TR::bits_to_float((uint16_t)(u[e >> 1] >> (16 * (e & 1)))), f1 = TR::bits_to_float((uint16_t)(u[2 + (e >> 1)] >> (16 * (e & 1))));
+        const __half2 hh = __floats2half2_rn(f0 * to_q, f1 * to_q);
+        p[e] = *(const uint32_t*)&hh;
       }
+      *place = make_uint4(p[0], p[1], p[2], p[3]);
+      if (j == 0) sE[r] = eq;
     }
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     __syncwarp();
@@ -469,18 +464,18 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_sdpa_tc_kernel(const SdpaArgs
   };
 
   if (warp >= kKeyWarp && warp < kValueWarp) {
-    unpack_side<T, D, false>(a.k, b, hk, k0, hi, tiles, sK, sRaw, bar0, meta, err, query_rows);
+    unpack_side<T, D, false>(a.k, b, hk, k0, hi, pairs, sK, sRaw, bar0, meta, err, query_rows);
   } else if (warp >= kValueWarp && warp < kIssuer) {
-    unpack_side<T, D, true>(a.v, b, hk, k0, hi, tiles, sV, sRaw + kKeys * D / 2, bar0, meta, err, query_rows);
+    unpack_side<T, D, true>(a.v, b, hk, k0, hi, pairs, sV, sRaw + kKeys * D / 2, bar0, meta, err, query_rows);
   } else if (warp == kIssuer) {
     // ---------------- scores ----------------
     if (lane == 0) {
       bool ok = wait_bar(bar0 + 8 * kBarQ, 0);
       if (!ok) atomicCAS(err, 0, 62 | (9 << 8));
       const uint32_t da = (uint32_t)desc_k(smem_u32(sQ)), db = (uint32_t)desc_k(smem_u32(sK)), hi32 = (uint32_t)(desc_k(0) >> 32);
-      for (int i = 0; i < tiles && ok; ++i) {
-        // the columns hold P(i - 2) until its product is done
-        if (i >= 2 && !wait_bar(bar0 + 8 * (kBarO + (i & 1)), ((i - 2) >> 1) & 1)) { atomicCAS(err, 0, 62 | (11 << 8)); break; }
+      for (int i = 0; i < pairs && ok; ++i) {
+        // the columns hold P of the pair before last until its products are done (both halves: it was not the last pair)
+        if (i >= 2 && !wait_bar(bar0 + 8 * (kBarO + ((2 * i - 3) & 3)), ((2 * i - 3) >> 2) & 1)) { atomicCAS(err, 0, 62 | (11 << 8)); break; }
         if (!wait_bar(bar0 + 8 * kBarKFull, i & 1)) { atomicCAS(err, 0, 62 | (3 << 8)); break; }
         fence_after();
         const uint32_t d = tmem + 128u * (i & 1);
@@ -503,19 +498,15 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_sdpa_tc_kernel(const SdpaArgs
     if (lane == 0) {
       const uint32_t dv = (uint32_t)desc_mn(smem_u32(sV), kSlab), hi32 = (uint32_t)(desc_mn(0, 0) >> 32);
       for (int i = 0; i < tiles; ++i) {
-        if (!wait_bar(bar0 + 8 * kBarVFull, i & 1)) { atomicCAS(err, 0, 62 | (5 << 8)); break; }
-        if (!wait_bar(bar0 + 8 * (kBarP + (i & 1)), (i >> 1) & 1)) { atomicCAS(err, 0, 62 | (4 << 8)); break; }
+        if (!wait_bar(bar0 + 8 * (kBarVFull + (i & 1)), (i >> 1) & 1)) { atomicCAS(err, 0, 62 | (5 << 8)); break; }
+        if (!wait_bar(bar0 + 8 * (kBarP + (i & 3)), (i >> 2) & 1)) { atomicCAS(err, 0, 62 | (4 << 8)); break; }
         fence_after();
-        const uint32_t pc = tmem + 128u * (i & 1);
+        const uint32_t pc = tmem + 64u * (i & 3), dh = dv + (i & 1) * (kTile * 128 >> 4);
 #pragma unroll
-        for (int blk = 0; blk < 4; ++blk) {
-#pragma unroll
-          for (int j = 0; j < 2; ++j)   // 16 keys = two 1024-byte groups; P: 8 columns (16 fp16)
-            mma_ts(tmem + kOCol, pc + 8u * (2 * blk + j), dv + (uint32_t)((2 * blk + j) * (2048 >> 4)), hi32, idesc(D, true),
-                   (blk | j) ? 1u : (uint32_t)i);
-          commit(bar0 + 8 * (kBarVEmpty + blk));
-        }
-        commit(bar0 + 8 * (kBarO + (i & 1)));
+        for (int j = 0; j < kTile / 16; ++j)   // 16 keys = two 1024-byte groups; P: 8 columns (16 fp16)
+          mma_ts(tmem + kOCol, pc + 8u * j, dh + (uint32_t)(j * (2048 >> 4)), hi32, idesc(D, true), j ? 1u : (uint32_t)i);
+        commit(bar0 + 8 * (kBarVEmpty + (i & 1)));
+        commit(bar0 + 8 * (kBarO + (i & 3)));
       }
     }
     __syncwarp();
@@ -533,60 +524,60 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_sdpa_tc_kernel(const SdpaArgs
     // last key the row sees; rows behind the last one compute what nobody reads
     const int lim = row_ok ? min(len - a.T + t, hi - 1) : (kMask ? -1 : 0x7FFFFFFF);
     const long long mat = kMask && row_ok ? b * a.m_sb + h * a.m_sh + t * a.m_st : 0;
-    const uint32_t s_col = tmem + lanes + 128u * group;
     float m_l = -INFINITY, l = 0.f;   // this half's sum and the reference it is relative to
     for (int i = group; i < tiles && ok; i += 2) {
-      if (!wait_warp(bar0 + 8 * (kBarS + group), (i >> 1) & 1)) { atomicCAS(err, 0, 62 | (6 << 8)); ok = false; break; }
+      if (!wait_warp(bar0 + 8 * (kBarS + ((i >> 1) & 1)), (i >> 2) & 1)) { atomicCAS(err, 0, 62 | (6 << 8)); ok = false; break; }
       fence_after();
       if (!live) {   // P is whatever is there: lanes of their own
         fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(bar0 + 8 * (kBarP + group));
+        if (lane == 0) mbar_arrive(bar0 + 8 * (kBarP + (i & 3)));
         continue;
       }
-      const Meta& mt = meta[i & (kMeta - 1)];
-      const int n0 = k0 + i * kKeys;
+      const uint32_t s_col = tmem + lanes + 64u * (i & 3);
+      const Meta& mt = meta[(i >> 1) & (kMeta - 1)];
+      const int blk = 2 * (i & 1);   // the tile's 32-key blocks in `mt`: blk and blk + 1
+      const int n0 = k0 + i * kTile;
+      uint32_t v[kTile];
+      ld32(s_col, v);
+      ld32(s_col + 32, v + 32);
+      float c[2] = {c_row * mt.k_factor[blk], c_row * mt.k_factor[blk + 1]};
       // every key of the tile seen by every row of the warp, and no mask
-      const bool plain = !kMask && __all_sync(0xffffffffu, n0 + kKeys - 1 <= lim);
-      float top = -INFINITY;
-      // (loops over 32 keys stay rolled: the roles' code together has to fit the instruction cache, whose misses were a quarter
-      // of the warps' time with everything unrolled)
-#pragma unroll 1
-      for (int q = 0; q < 4; ++q) {
-        uint32_t v[32];
-        ld32(s_col + 32 * q, v);
-        const float c = c_row * mt.k_factor[q];
-        const uint32_t seen = plain ? 0xFFFFFFFFu : seen_bits<kMask>(a, mat, n0 + 32 * q, lim);
-        wait_ld();
-        if (kMask == 2) {   // scores as the row sees them, back into their columns
+      const bool plain = !kMask && __all_sync(0xffffffffu, n0 + kTile - 1 <= lim);
+      if (!wait_warp(bar0 + 8 * (kBarVMeta + ((i >> 1) & (kMeta - 1))), (i / (2 * kMeta)) & 1)) { atomicCAS(err, 0, 62 | (13 << 8)); ok = false; }
+      wait_ld();
+      if (!ok) break;
+      if (!plain) {
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+          const uint32_t seen = seen_bits<kMask>(a, mat, n0 + 32 * q, lim);
 #pragma unroll
           for (int e = 0; e < 32; ++e) {
-            float x = __uint_as_float(v[e]) * c;
-            x = (seen >> e) & 1 ? apply_mask<T>(a, x, mat + (n0 + 32 * q + e) * a.m_sn) : -INFINITY;
-            top = fmaxf(top, x);
-            v[e] = __float_as_uint(x);
+            if (kMask == 2) {
+              if ((seen >> e) & 1) v[32 * q + e] = __float_as_uint(apply_mask<T>(a, __uint_as_float(v[32 * q + e]) * c[q], mat + (n0 + 32 * q + e) * a.m_sn));
+            }
+            if (!((seen >> e) & 1)) v[32 * q + e] = 0xFF800000u;
           }
-          st16(s_col + 32 * q, v);
-          st16(s_col + 32 * q + 16, v + 16);
-          wait_st();
-        } else {
-          if (!plain) {
-#pragma unroll
-            for (int e = 0; e < 32; ++e)
-              if (!((seen >> e) & 1)) v[e] = 0xFF800000u;
-          }
-          float t0 = -INFINITY, t1 = -INFINITY;
-#pragma unroll
-          for (int e = 0; e < 32; e += 4) {
-            t0 = fmaxf(fmaxf(t0, __uint_as_float(v[e])), __uint_as_float(v[e + 1]));
-            t1 = fmaxf(fmaxf(t1, __uint_as_float(v[e + 2])), __uint_as_float(v[e + 3]));
-          }
-          t0 = fmaxf(t0, t1);
-          top = fmaxf(top, t0 == -INFINITY ? t0 : t0 * c);   // c may be 0
+          if (kMask == 2) c[q] = 1.f;
         }
       }
-      if (!wait_warp(bar0 + 8 * (kBarVMeta + (i & (kMeta - 1))), (i / kMeta) & 1)) { atomicCAS(err, 0, 62 | (13 << 8)); ok = false; break; }
-      const bool bads = (mt.bad[0] | mt.bad[1] | mt.bad[2] | mt.bad[3]) != 0;
+      if ((mt.bad[blk] | mt.bad[blk + 1]) != 0) {   // a value that is not finite makes the rows NaN that see its key
+#pragma unroll
+        for (int e = 0; e < kTile; ++e)
+          if (((mt.bad[blk + (e >> 5)] >> (e & 31)) & 1) && v[e] != 0xFF800000u) v[e] = 0x7FC00000u;
+      }
+      float top = -INFINITY;
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        float t0 = -INFINITY, t1 = -INFINITY;
+#pragma unroll
+        for (int e = 32 * q; e < 32 * q + 32; e += 4) {
+          t0 = fmaxf(fmaxf(t0, __uint_as_float(v[e])), __uint_as_float(v[e + 1]));
+          t1 = fmaxf(fmaxf(t1, __uint_as_float(v[e + 2])), __uint_as_float(v[e + 3]));
+        }
+        t0 = fmaxf(t0, t1);
+        top = fmaxf(top, t0 == -INFINITY ? t0 : t0 * c[q]);   // c may be 0
+      }
       // ---- the row's reference: what the tile before left, moved when this tile exceeds it by 8 octaves ----
       float m = -INFINITY;
       int ev = -200;
@@ -595,7 +586,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_sdpa_tc_kernel(const SdpaArgs
         m = sRef[(group ^ 1) * kRows + r];
         ev = sEv[(group ^ 1) * 4 + part];
       }
-      const int ev_tile = max(max(mt.v_exp[0], mt.v_exp[1]), max(mt.v_exp[2], mt.v_exp[3]));
+      const int ev0 = mt.v_exp[blk], ev1 = mt.v_exp[blk + 1], ev_tile = max(ev0, ev1);
       if (__any_sync(0xffffffffu, top > m + kMaxStep) || ev_tile > ev) {
         const float m_new = fmaxf(m, top);
         const int ev_new = max(ev, ev_tile);
@@ -603,17 +594,16 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_sdpa_tc_kernel(const SdpaArgs
         const float fo = f * pow2(max(ev - ev_new, -126));
         m = m_new;
         if (i > 0) {
-          if (!wait_warp(bar0 + 8 * (kBarO + (group ^ 1)), ((i - 1) >> 1) & 1)) { atomicCAS(err, 0, 62 | (7 << 8)); ok = false; break; }
+          if (!wait_warp(bar0 + 8 * (kBarO + ((i - 1) & 3)), ((i - 1) >> 2) & 1)) { atomicCAS(err, 0, 62 | (7 << 8)); ok = false; break; }
           fence_after();
 #pragma unroll 1
-          for (int c0 = 0; c0 < D; c0 += 32) {
-            uint32_t o[32];
-            ld32(tmem + lanes + kOCol + c0, o);
+          for (int c0 = 0; c0 < D; c0 += 16) {
+            uint32_t o[16];
+            ld16(tmem + lanes + kOCol + c0, o);
             wait_ld();
 #pragma unroll
-            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * fo);
+            for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * fo);
             st16(tmem + lanes + kOCol + c0, o);
-            st16(tmem + lanes + kOCol + c0 + 16, o + 16);
           }
           wait_st();
         }
@@ -629,57 +619,45 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_sdpa_tc_kernel(const SdpaArgs
       }
       // ---- P ----
       const float ref = m == -INFINITY ? 0.f : m;
-#pragma unroll 1
-      for (int q = 0; q < 4; ++q) {
-        uint32_t v[32];
-        ld32(s_col + 32 * q, v);
-        const float shift = kPShift + (float)max(mt.v_exp[q] - ev, -100);   // P carries V's power of two
-        const float cl = kMask == 2 ? kLog2e : c_row * mt.k_factor[q] * kLog2e, off = shift - ref * kLog2e;
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        const float shift = kPShift + (float)max((q ? ev1 : ev0) - ev, -100);   // P carries V's power of two
+        const float cl = c[q] * kLog2e, off = shift - ref * kLog2e;
         const uint64_t cl2 = pair(cl, cl), off2 = pair(off, off);
         uint64_t sum = 0;
-        uint32_t w[16];
-        uint32_t seen = 0xFFFFFFFFu;
-        if (kMask != 2 && !plain) seen = seen_bits<kMask>(a, mat, n0 + 32 * q, lim);
-        wait_ld();
-        if (bads) {   // a value that is not finite makes the rows NaN that see its key
 #pragma unroll
-          for (int e = 0; e < 32; ++e)
-            if (((mt.bad[q] >> e) & 1) && !(kMask == 2 && v[e] == 0xFF800000u)) v[e] = 0x7FC00000u;
-        }
-        if (kMask != 2 && !plain) {
+        for (int e0 = 32 * q; e0 < 32 * q + 32; e0 += 16) {
+          uint32_t w[8];
 #pragma unroll
-          for (int e = 0; e < 32; ++e)
-            if (!((seen >> e) & 1)) v[e] = 0xFF800000u;
-        }
-#pragma unroll
-        for (int e = 0; e < 32; e += 2) {
-          float p0, p1;
-          if (kMask == 2) {   // scores may be the lowest finite value: their difference first
-            p0 = fmaf(__uint_as_float(v[e]) - ref, kLog2e, shift);
-            p1 = fmaf(__uint_as_float(v[e + 1]) - ref, kLog2e, shift);
-          } else {
-            unpair(fma2(pair(__uint_as_float(v[e]), __uint_as_float(v[e + 1])), cl2, off2), p0, p1);
+          for (int e = 0; e < 16; e += 2) {
+            float p0, p1;
+            if (kMask == 2) {   // scores may be the lowest finite value: their difference first
+              p0 = fmaf(__uint_as_float(v[e0 + e]) - ref, kLog2e, shift);
+              p1 = fmaf(__uint_as_float(v[e0 + e + 1]) - ref, kLog2e, shift);
+            } else {
+              unpair(fma2(pair(__uint_as_float(v[e0 + e]), __uint_as_float(v[e0 + e + 1])), cl2, off2), p0, p1);
+            }
+            p0 = ex2(p0);
+            p1 = ex2(p1);
+            sum = add2(sum, pair(p0, p1));
+            const __half2 p = __floats2half2_rn(p0, p1);
+            w[e >> 1] = *(const uint32_t*)&p;
           }
-          p0 = ex2(p0);
-          p1 = ex2(p1);
-          sum = add2(sum, pair(p0, p1));
-          const __half2 p = __floats2half2_rn(p0, p1);
-          w[e >> 1] = *(const uint32_t*)&p;
+          st8(s_col + (e0 >> 1), w);   // over columns that are in registers
         }
         float sum0, sum1;
         unpair(sum, sum0, sum1);
         l = fmaf(sum0 + sum1, ex2(-shift), l);
-        st16(s_col + 16 * q, w);   // over columns that have been read
       }
       wait_st();
       fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(bar0 + 8 * (kBarP + group));
+      if (lane == 0) mbar_arrive(bar0 + 8 * (kBarP + (i & 3)));
     }
-    // ---- epilogue: either half of the softmax takes half of the channels; the rows go through shared memory (all of Q, K and V is
-    // spent), so that they leave as bulk copies ----
-    // the last product; the one two before it is done (the last scores took its columns), so the phase cannot be mistaken
-    if (tiles > 0 && ok && !wait_warp(bar0 + 8 * (kBarO + ((tiles - 1) & 1)), ((tiles - 1) >> 1) & 1)) { atomicCAS(err, 0, 62 | (8 << 8)); ok = false; }
+    // ---- epilogue: either half of the softmax takes half of the channels; a warp's 32 rows go through shared memory (all of Q, K
+    // and V is spent), so that they leave as whole lines ----
+    // the last product; the one four before it is done (the last scores took its columns), so the phase cannot be mistaken
+    if (tiles > 0 && ok && !wait_warp(bar0 + 8 * (kBarO + ((tiles - 1) & 3)), ((tiles - 1) >> 2) & 1)) { atomicCAS(err, 0, 62 | (8 << 8)); ok = false; }
     fence_after();
     sEnd[group * kRows + r] = make_float2(m_l, l);
     named_bar_sync(1, 256);
@@ -722,20 +700,23 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_sdpa_tc_kernel(const SdpaArgs
           for (int e = 0; e < 32; e += 4) *(float4*)(stage + (c0 + e) * 4) = make_float4(y[e], y[e + 1], y[e + 2], y[e + 3]);
         }
       }
-      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-      if (row_ok) {
-        const int size = last ? 2 : 4;
-        const uint8_t* dst = last ? (const uint8_t*)((T*)a.out + out_row(a, b, hk, row) * D) : (const uint8_t*)(a.part_o + at * D);
-        asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(dst + c_first * size),
-                     "r"(smem_u32(stage) + c_first * size), "r"(D / 2 * size)
-                     : "memory");
-        if (!last && group == 0) {
-          a.part_m[at] = m;
-          a.part_l[at] = l;
-        }
+      if (row_ok && !last && group == 0) {
+        a.part_m[at] = m;
+        a.part_l[at] = l;
       }
-      asm volatile("cp.async.bulk.commit_group;" ::: "memory");
-      asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+      const int bytes = D / 2 * (last ? 2 : 4);   // of half a row: 512, 256 or 128
+      const uint64_t dst = (uint64_t)(last ? (const uint8_t*)((T*)a.out + out_row(a, b, hk, row) * D) : (const uint8_t*)(a.part_o + at * D)) +
+                           group * bytes;
+      const int per = 512 / bytes;                // rows a warp stores at once
+      const int off = lane * 16 & (bytes - 1);
+      __syncwarp();
+#pragma unroll 4
+      for (int r1 = 0; r1 < 32; r1 += per) {
+        const int rr = r1 + lane * 16 / bytes;
+        const uint64_t to = __shfl_sync(0xffffffffu, dst, rr);
+        const uint4 x = *(const uint4*)(smem + (part * 32 + rr) * (D * 4 + 16) + group * bytes + off);
+        if (row0 + part * 32 + rr < a.rows) *(uint4*)(to + off) = x;
+      }
     }
   }
   fence_before();
