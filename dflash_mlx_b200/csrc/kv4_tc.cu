@@ -232,9 +232,9 @@ __device__ __forceinline__ void unpack_row(const uint4& c0, const uint4& c1, flo
 // The keys (kV = false) or values of a block's range, by the four warps of a side: thread = key of the tile.
 template <int D>
 __device__ __forceinline__ int raw_chunk(int r, int ch) { return D == 256 ? ch ^ (r & 7) : ch ^ ((r >> 1) & 3); }
-template <typename T, int D, bool kV, typename F>
+template <typename T, int D, bool kV, typename F, typename H>
 __device__ __forceinline__ void unpack_side(const dflash_kv4_cache& c, int b, int hk, int k0, int hi, int tiles, uint8_t* buf, uint8_t* raw,
-                                            uint32_t bar0, Meta* meta, int* err, F query_rows) {
+                                            uint32_t bar0, Meta* meta, int* err, F query_copy, H query_rows) {
   constexpr int G = D / kGroup;
   const int w = (threadIdx.x >> 5) & 3, lane = threadIdx.x & 31, key = w * 32 + lane;
   const uint8_t* codes = (const uint8_t*)(c.codes + b * c.codes_batch_stride + hk * c.codes_head_stride);
@@ -315,9 +315,12 @@ __device__ __forceinline__ void unpack_side(const dflash_kv4_cache& c, int b, in
       m.k_factor[w] = pow2(e);
     }
   };
+  // the block's queries are converted while the first keys and values are on their way
+  query_copy();
   load(0);
   load_scales(0, ns, nz);
-  query_rows();   // the block's queries, while the first keys and values are on their way
+  asm volatile("cp.async.wait_group 1;" ::: "memory");
+  query_rows();
   prepare(0);
   load_scales(1, ns, nz);
   for (int t = 0; t < tiles; ++t) {
@@ -417,10 +420,9 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_sdpa_tc_kernel(const SdpaArgs
 
   // Q: a row per D / 8 lanes, brought to fp16 by a power of two (its largest element to [2^7, 2^8)) in unpack_row's channel order;
   // the scale's sign goes with it, so that scores grow with their products.  Sixteen warps, every sixteenth row each.
-  auto query_rows = [&]() {
-    constexpr int kLanes = D / 8, kPer = 32 / kLanes, kSteps = kRows / (kIssuer * kPer);
+  constexpr int kLanes = D / 8, kPer = 32 / kLanes, kSteps = kRows / (kIssuer * kPer);
+  auto query_copy = [&]() {   // raw into place, all copies in flight at once
     const int j = lane % kLanes;
-    // raw into place, all copies in flight at once
 #pragma unroll 2
     for (int i = 0; i < kSteps; ++i) {
       const int r = (i * kIssuer + warp) * kPer + lane / kLanes, row = row0 + r;
@@ -430,7 +432,10 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_sdpa_tc_kernel(const SdpaArgs
                    "l"((const T*)a.q + b * a.q_sb + h * a.q_sh + t * a.q_st + 8 * j), "r"(in ? 16 : 0)
                    : "memory");
     }
-    asm volatile("cp.async.commit_group;\n\tcp.async.wait_group 0;" ::: "memory");   // a lane reads what it copied itself
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  auto query_rows = [&]() {   // once they have landed; a lane reads what it copied itself
+    const int j = lane % kLanes;
 #pragma unroll 1
     for (int i = 0; i < kSteps; ++i) {
       const int r = (i * kIssuer + warp) * kPer + lane / kLanes;
@@ -464,9 +469,9 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_sdpa_tc_kernel(const SdpaArgs
   };
 
   if (warp >= kKeyWarp && warp < kValueWarp) {
-    unpack_side<T, D, false>(a.k, b, hk, k0, hi, pairs, sK, sRaw, bar0, meta, err, query_rows);
+    unpack_side<T, D, false>(a.k, b, hk, k0, hi, pairs, sK, sRaw, bar0, meta, err, query_copy, query_rows);
   } else if (warp >= kValueWarp && warp < kIssuer) {
-    unpack_side<T, D, true>(a.v, b, hk, k0, hi, pairs, sV, sRaw + kKeys * D / 2, bar0, meta, err, query_rows);
+    unpack_side<T, D, true>(a.v, b, hk, k0, hi, pairs, sV, sRaw + kKeys * D / 2, bar0, meta, err, query_copy, query_rows);
   } else if (warp == kIssuer) {
     // ---------------- scores ----------------
     if (lane == 0) {
@@ -517,6 +522,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_sdpa_tc_kernel(const SdpaArgs
     const bool live = row0 + part * 32 < a.rows;
     const uint32_t lanes = (uint32_t)(part * 32) << 16;
     const int t = row_ok ? row / a.gqa : 0, h = hk * a.gqa + (row_ok ? row % a.gqa : 0);
+    query_copy();
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
     query_rows();
     bool ok = wait_warp(bar0 + 8 * kBarQ, 0);
     if (!ok) atomicCAS(err, 0, 62 | (10 << 8));
@@ -710,7 +717,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_sdpa_tc_kernel(const SdpaArgs
       const int per = 512 / bytes;                // rows a warp stores at once
       const int off = lane * 16 & (bytes - 1);
       __syncwarp();
-#pragma unroll 4
+#pragma unroll 8
       for (int r1 = 0; r1 < 32; r1 += per) {
         const int rr = r1 + lane * 16 / bytes;
         const uint64_t to = __shfl_sync(0xffffffffu, dst, rr);

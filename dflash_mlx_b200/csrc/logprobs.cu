@@ -1,14 +1,18 @@
 // Log-probabilities of given tokens, entropy and the top alternatives of every row of logits, in one pass over the logits.
 //
-//   m = max x,  L = sum exp((x - m) / T),  W = sum (x - m) exp((x - m) / T)
-//   log p[token] = (x[token] - m) / T - ln L,   entropy = ln L - W / (L T)
-// Every thread sums relative to the maximum of its own elements and the (m, L, W) triples are merged in a fixed tree
-// (L' = L exp((m - m') / T), W' = (W + (m - m') L) exp((m - m') / T)), so the result does not depend on timing.
+//   m = max x,  y = (x - m) log2(e) / T,  L = sum 2^y,  W = sum y 2^y
+//   log p[token] = (x[token] - m) / T - ln L,   entropy = ln L - ln 2 W / L
+// Every thread sums relative to the maximum of its own elements, with one fma for y (the rounding of m log2(e) / T is taken back
+// from the sums afterwards), and the (m, L, W) triples are merged in a fixed tree (L' = L 2^d, W' = (W + d L) 2^d with d = (m - m')
+// log2(e) / T), so the result does not depend on timing.
 //
+// A block passes over its share of the row, 32 (16-bit types) or 16 elements a thread at a time, the next ones on their way.
 // Top alternatives: 64 groups of threads give 64 maxima; at least top_k elements are >= the top_k-th largest of them, and only
 // those (a few dozen of tens of thousands) are collected and ranked by counting.  Keys are (value, lower index first) and
-// therefore unique.  When more are collected than the list holds (a row of equal values, sorted logits) the top_k-th largest key is
-// found bit by bit instead.
+// therefore unique.  The first pass sets the bar that way, later passes collect what beats the k-th best so far; the list is ranked
+// after passes 1, 2, 4, 8 ... and the last, between which nothing waits.  If it overflows there, the row starts over with a
+// ranking after every pass; when one pass alone collects more than the list holds (a row of equal values, sorted logits) the top_k-th largest key is
+// found bit by bit.
 //
 // One row per thread-block cluster: every block keeps its share of the row in registers (16-byte loads, all issued before the
 // first is used), the first block merges the triples and the blocks' lists through distributed shared memory.  Bound by HBM
@@ -52,6 +56,10 @@ template <> struct Elem<float> {
     for (int e = 0; e < 4; ++e)
       if ((u >> (8 * e)) & 0xFFu) w[e] = kNegInf;
   }
+  // whether clamped() keeps a thread's sums right: the clamp is 0 probability next to the maximum m
+  __device__ static __forceinline__ bool can_clamp(float, float) { return false; }
+  __device__ static __forceinline__ uint32_t clamped(uint32_t w) { return w; }
+  __device__ static __forceinline__ void two(uint32_t, float&, float&) {}
   __device__ static __forceinline__ void put(uint32_t (&w)[4], int e, const float* p) { w[e] = __float_as_uint(*p); }
   __device__ static __forceinline__ float load(const float* p) { return *p; }
   __device__ static __forceinline__ float max_of(const uint32_t (&w)[kSlots][4]) {   // NaN is passed over
@@ -76,12 +84,23 @@ template <typename T, uint32_t kInf> struct Elem16 {
   __device__ static __forceinline__ void hide(uint32_t (&w)[4], int e) { put_bits(w, e, kInf); }
   __device__ static __forceinline__ void hide_by(uint32_t (&w)[4], const uint8_t* p) {
     const uint2 u = *(const uint2*)p;
-    const uint32_t t[2] = {__vcmpne4(u.x, 0), __vcmpne4(u.y, 0)};
+    const uint32_t t[2] = {u.x * 255u, u.y * 255u};   // 0 or 1 -> 0 or 255, byte by byte
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const uint32_t m = prmt(t[i >> 1], 0, (i & 1) ? 0x3322 : 0x1100);   // a byte for each half
       w[i] = (w[i] & ~m) | ((kInf | (kInf << 16)) & m);
     }
+  }
+  // whether clamped() keeps a thread's sums right: the clamp (-1e30, fp16: -65504) has probability 0 next to the maximum m
+  __device__ static __forceinline__ bool can_clamp(float m, float scale) { return scale >= 0.01f && scale < 1e6f && m > -40000.f && m < 1e30f; }
+  __device__ static __forceinline__ uint32_t clamped(uint32_t w) {
+    const uint32_t low = kInf == 0xFF80u ? 0xF149F149u : 0xFBFFFBFFu;
+    const auto m = __hmax2_nan(as_pair(w, T()), as_pair(low, T()));
+    return *(const uint32_t*)&m;
+  }
+  __device__ static __forceinline__ void two(uint32_t w, float& x0, float& x1) {
+    x0 = MmaTraits<T>::bits_to_float((uint16_t)w);
+    x1 = MmaTraits<T>::bits_to_float((uint16_t)(w >> 16));
   }
   __device__ static __forceinline__ void put(uint32_t (&w)[4], int e, const T* p) { put_bits(w, e, *(const uint16_t*)p); }
   __device__ static __forceinline__ float load(const T* p) { return MmaTraits<T>::to_float(*p); }
@@ -100,8 +119,8 @@ __device__ __forceinline__ Sums merge(const Sums& a, const Sums& b, float scale)
   Sums s;
   s.m = fmaxf(a.m, b.m);
   // a side without a maximum has sums of zero (or NaN, which stays): it needs no factor
-  const float da = a.m == -INFINITY ? 0.f : a.m - s.m, db = b.m == -INFINITY ? 0.f : b.m - s.m;
-  const float fa = exp2f(da * scale), fb = exp2f(db * scale);
+  const float da = a.m == -INFINITY ? 0.f : (a.m - s.m) * scale, db = b.m == -INFINITY ? 0.f : (b.m - s.m) * scale;
+  const float fa = exp2f(da), fb = exp2f(db);
   s.l = a.l * fa + b.l * fb;
   // a vanished side must not turn an infinite distance into NaN
   s.w = (fa == 0.f ? 0.f : fmaf(da, a.l, a.w) * fa) + (fb == 0.f ? 0.f : fmaf(db, b.l, b.w) * fb);
@@ -188,6 +207,7 @@ __global__ void __launch_bounds__(kThreads, 3) token_logprobs_kernel(const Args 
       }
     }
   };
+  bool careful = false;
   uint32_t next[kSlots][4];
   if (v0 < v1) load(v0, next);
   for (int base = v0; base < v1; base += kThreads * kSlots) {
@@ -214,28 +234,37 @@ __global__ void __launch_bounds__(kThreads, 3) token_logprobs_kernel(const Args 
       }
     }
     Sums mine = {E::max_of(raw), 0.f, 0.f};
-    const float ref = mine.m == -INFINITY ? 0.f : mine.m;
-    const uint64_t ref2 = pair(-ref, -ref), scale2 = pair(a.scale, a.scale);
-    uint64_t l2 = 0, w2 = 0;
+    const float ref = mine.m == -INFINITY ? 0.f : mine.m, top = ref * a.scale;
+    float l0 = 0.f, l1 = 0.f, w0 = 0.f, w1 = 0.f;
+    if (E::can_clamp(mine.m, a.scale)) {   // hidden elements become a finite value of probability 0, two at a time
 #pragma unroll
-    for (int s = 0; s < kSlots; ++s)
-#pragma unroll
-      for (int e = 0; e < kPer; e += 2) {
-        const uint64_t d2 = add2(pair(E::get(raw[s], e), E::get(raw[s], e + 1)), ref2);
-        float d0, d1, p0, p1;
-        unpair(d2, d0, d1);
-        unpair(mul2(d2, scale2), p0, p1);
-        const uint64_t p2 = pair(exp2f(p0), exp2f(p1));
-        l2 = add2(l2, p2);
-        // a hidden element adds 0, not -inf * 0; NaN stays through p
-        w2 = fma2(pair(fmaxf(d0, -1e30f), fmaxf(d1, -1e30f)), p2, w2);
+      for (int i = 0; i < 4 * kSlots; ++i) {
+        float x0, x1;
+        E::two(E::clamped(raw[i >> 2][i & 3]), x0, x1);
+        const float y0 = fmaf(x0, a.scale, -top), y1 = fmaf(x1, a.scale, -top);
+        const float p0 = exp2f(y0), p1 = exp2f(y1);
+        l0 += p0;
+        l1 += p1;
+        w0 = fmaf(y0, p0, w0);
+        w1 = fmaf(y1, p1, w1);
       }
-    {
-      float x0, x1;
-      unpair(l2, x0, x1);
-      mine.l = x0 + x1;
-      unpair(w2, x0, x1);
-      mine.w = x0 + x1;
+      // y was taken from the rounded product: back to the exact one
+      const float off = fmaf(ref, a.scale, -top), z = off * 0.6931471805599453f;
+      const float f = fabsf(z) < 0.01f ? fmaf(z, fmaf(z, 0.5f, -1.f), 1.f) : exp2f(-off);
+      mine.l = (l0 + l1) * f;
+      mine.w = fmaf(-off, l0 + l1, w0 + w1) * f;
+    } else {
+#pragma unroll
+      for (int s = 0; s < kSlots; ++s)
+#pragma unroll
+        for (int e = 0; e < kPer; ++e) {
+          const float y = (E::get(raw[s], e) - ref) * a.scale;
+          const float p = exp2f(y);
+          l0 += p;
+          w0 = fmaf(fmaxf(y, -1e30f), p, w0);   // a hidden element adds 0, not -inf * 0; NaN stays through p
+        }
+      mine.l = l0;
+      mine.w = w0;
     }
     if (a.k > 0) {
       // ---- candidates of this pass ----
@@ -260,10 +289,6 @@ __global__ void __launch_bounds__(kThreads, 3) token_logprobs_kernel(const Args 
       const float tau = sh.tau;
       // NaN elements count as the largest; a thread whose own maximum does not reach tau can only hold NaN beyond it
       const bool has = (first ? mine.m >= tau : !(mine.m <= tau)) || !(mine.l == mine.l);
-      if (!__syncthreads_or(has)) {   // later passes, mostly
-        sums = merge(sums, mine, a.scale);
-        continue;
-      }
       if (has) {
 #pragma unroll 1
         for (int s = 0; s < kSlots; ++s) {
@@ -291,8 +316,23 @@ __global__ void __launch_bounds__(kThreads, 3) token_logprobs_kernel(const Args 
           }
         }
       }
+      const int pass = (base - v0) / (kThreads * kSlots) + 1;
+      if (!careful && (pass & (pass - 1)) != 0 && base + kThreads * kSlots < v1) {
+        sums = merge(sums, mine, a.scale);
+        continue;
+      }
       __syncthreads();
       const int n = sh.count;
+      if (n > kList - kMaxK && !careful && !first) {   // over several passes: once more, ranking after each
+        __syncthreads();
+        careful = true;
+        if (tid < kMaxK) sh.top[tid] = 0;
+        if (tid == 0) sh.count = 0;
+        sums = {-INFINITY, 0.f, 0.f};
+        base = v0 - kThreads * kSlots;
+        load(v0, next);
+        continue;
+      }
       if (n <= kList - kMaxK) {
         int all = n;
         if (!first) {   // the best of the earlier passes compete again
@@ -405,7 +445,7 @@ __global__ void __launch_bounds__(kThreads, 3) token_logprobs_kernel(const Args 
       if (tid == 0) {
         a.token_logprob[row] = out;
         if (a.entropy != nullptr)
-          a.entropy[row] = empty ? 0.f : (float)(log_l - (double)all.w * inv_t / (double)all.l);
+          a.entropy[row] = empty ? 0.f : (float)(log_l - 0.69314718055994531 * (double)all.w / (double)all.l);
       } else {
         a.top_logprobs[row * a.k + tid - 1] = out;
         a.top_ids[row * a.k + tid - 1] = key_index(sh.list[tid - 1]);
@@ -439,7 +479,7 @@ extern "C" int dflash_token_logprobs(const void* logits, long long ld, const int
   if (R < 0 || V < 1 || ld < V) return fail(DFLASH_ERR_BAD_SHAPE, "token_logprobs: R=%d V=%d ld=%lld", R, V, ld);
   if (V > 0x7fffffff - 64 * 1024) return fail(DFLASH_ERR_BAD_SHAPE, "token_logprobs: V=%d too large", V);
   if (top_k < 0 || top_k > lp::kMaxK || top_k > V) return fail(DFLASH_ERR_BAD_SHAPE, "token_logprobs: top_k=%d outside 0..min(%d, V)", top_k, lp::kMaxK);
-  if (!(temperature > 0.f) || !(temperature <= 3.0e38f)) return fail(DFLASH_ERR_BAD_ARG, "token_logprobs: temperature must be positive and finite");
+  if (!(temperature >= 1e-30f) || !(temperature <= 3.0e38f)) return fail(DFLASH_ERR_BAD_ARG, "token_logprobs: temperature must be finite and at least 1e-30");
   if (R == 0) return DFLASH_OK;
   if (!logits || !tokens || !token_logprob || (top_k > 0 && (!top_logprobs || !top_ids))) return fail(DFLASH_ERR_BAD_ARG, "token_logprobs: null operand");
   const int size = dtype == DFLASH_F32 ? 4 : 2;
