@@ -10,7 +10,7 @@
 // Top alternatives: 64 groups of threads give 64 maxima; at least top_k elements are >= the top_k-th largest of them, and only
 // those (a few dozen of tens of thousands) are collected and ranked by counting.  Keys are (value, lower index first) and
 // therefore unique.  The first pass sets the bar that way, later passes collect what beats the k-th best so far; the list is ranked
-// after passes 1, 2, 4, 8 ... and the last, between which nothing waits.  If it overflows there, the row starts over with a
+// after passes 1, 4, 16 ... and the last, between which nothing waits.  If it overflows there, the row starts over with a
 // ranking after every pass; when one pass alone collects more than the list holds (a row of equal values, sorted logits) the top_k-th largest key is
 // found bit by bit.
 //
@@ -39,7 +39,8 @@ struct Args {
   float* entropy;
   float* top_logprobs;
   int* top_ids;
-  float temperature, scale;   // scale = log2(e) / temperature
+  double inv_t;                // 1 / temperature
+  float scale;                 // log2(e) / temperature
   int V, k;
 };
 
@@ -49,12 +50,11 @@ template <> struct Elem<float> {
   static constexpr uint32_t kNegInf = 0xFF800000u;
   __device__ static __forceinline__ float get(const uint32_t (&w)[4], int e) { return __uint_as_float(w[e]); }
   __device__ static __forceinline__ void hide(uint32_t (&w)[4], int e) { w[e] = kNegInf; }
-  // hides the elements whose byte in `bytes` (as many as elements, from address p) is not 0
-  __device__ static __forceinline__ void hide_by(uint32_t (&w)[4], const uint8_t* p) {
-    const uint32_t u = *(const uint32_t*)p;
+  __device__ static __forceinline__ uint2 suppress_bytes(const uint8_t* p) { return make_uint2(*(const uint32_t*)p, 0); }
+  __device__ static __forceinline__ void hide_by(uint32_t (&w)[4], uint2 u) {   // the elements whose byte is not 0
 #pragma unroll
     for (int e = 0; e < 4; ++e)
-      if ((u >> (8 * e)) & 0xFFu) w[e] = kNegInf;
+      if ((u.x >> (8 * e)) & 0xFFu) w[e] = kNegInf;
   }
   // whether clamped() keeps a thread's sums right: the clamp is 0 probability next to the maximum m
   __device__ static __forceinline__ bool can_clamp(float, float) { return false; }
@@ -82,8 +82,8 @@ template <typename T, uint32_t kInf> struct Elem16 {
     w[e >> 1] = (e & 1) ? ((w[e >> 1] & 0xFFFFu) | (bits << 16)) : ((w[e >> 1] & 0xFFFF0000u) | bits);
   }
   __device__ static __forceinline__ void hide(uint32_t (&w)[4], int e) { put_bits(w, e, kInf); }
-  __device__ static __forceinline__ void hide_by(uint32_t (&w)[4], const uint8_t* p) {
-    const uint2 u = *(const uint2*)p;
+  __device__ static __forceinline__ uint2 suppress_bytes(const uint8_t* p) { return *(const uint2*)p; }
+  __device__ static __forceinline__ void hide_by(uint32_t (&w)[4], uint2 u) {
     const uint32_t t[2] = {u.x * 255u, u.y * 255u};   // 0 or 1 -> 0 or 255, byte by byte
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -126,6 +126,11 @@ __device__ __forceinline__ Sums merge(const Sums& a, const Sums& b, float scale)
   s.w = (fa == 0.f ? 0.f : fmaf(da, a.l, a.w) * fa) + (fb == 0.f ? 0.f : fmaf(db, b.l, b.w) * fb);
   return s;
 }
+// With the lane whose number differs in bit o: the lower lane's triple first, so that both compute the same bits.
+__device__ __forceinline__ Sums merge_lanes(const Sums& s, int o, float scale) {
+  const Sums other = {__shfl_xor_sync(0xffffffffu, s.m, o), __shfl_xor_sync(0xffffffffu, s.l, o), __shfl_xor_sync(0xffffffffu, s.w, o)};
+  return (threadIdx.x & o) ? merge(other, s, scale) : merge(s, other, scale);
+}
 __device__ __forceinline__ unsigned long long key_of(float v, int index) {
   const uint32_t u = __float_as_uint(__fadd_rn(v, 0.f));   // -0 and +0 are one value
   const uint32_t o = u ^ ((u >> 31) ? 0xFFFFFFFFu : 0x80000000u);
@@ -147,6 +152,7 @@ struct Shared {
   unsigned long long top[kMaxK];                  // this block's best, highest first; 0 = none
   unsigned long long gathered[8 * kMaxK];         // first block of a cluster: every block's `top`
   int counts[2][kThreads / 32];
+  uint4 stage[4][kThreads];                       // elements of threads that hold candidates, to be picked by number
 };
 
 // The `k` largest of list[0..n) in order; keys are unique, 0 marks an empty place and is skipped.
@@ -190,11 +196,14 @@ __global__ void __launch_bounds__(kThreads, 3) token_logprobs_kernel(const Args 
   if (tid < kMaxK) sh.top[tid] = 0;
   if (tid == 0) sh.count = 0;
   const bool packed = a.suppress != nullptr && skew == 0 && ((uintptr_t)a.suppress & (kPer - 1)) == 0;
+  uint2 bytes[kSlots];   // of `suppress`, for the vectors on their way
   auto load = [&](int base, uint32_t (&raw)[kSlots][4]) {
 #pragma unroll
     for (int s = 0; s < kSlots; ++s) {
       const int v = base + s * kThreads + tid;
       const int i0 = v * kPer - skew;
+      bytes[s] = make_uint2(0, 0);
+      if (packed && v < v1 && i0 + kPer <= a.V) bytes[s] = E::suppress_bytes(a.suppress + i0);
       if (v < v1 && i0 >= 0 && i0 + kPer <= a.V) {
         const uint4 u = __ldcs((const uint4*)(x + i0));
         raw[s][0] = u.x; raw[s][1] = u.y; raw[s][2] = u.z; raw[s][3] = u.w;
@@ -213,26 +222,22 @@ __global__ void __launch_bounds__(kThreads, 3) token_logprobs_kernel(const Args 
   for (int base = v0; base < v1; base += kThreads * kSlots) {
     uint32_t raw[kSlots][4];
 #pragma unroll
-    for (int s = 0; s < kSlots; ++s)
+    for (int s = 0; s < kSlots; ++s) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) raw[s][i] = next[s][i];
-    if (base + kThreads * kSlots < v1) load(base + kThreads * kSlots, next);   // in flight under this pass
-    if (a.suppress != nullptr) {
-#pragma unroll
-      for (int s = 0; s < kSlots; ++s) {
+      if (a.suppress != nullptr) {
         const int v = base + s * kThreads + tid;
         const int i0 = v * kPer - skew;
-        if (v < v1) {
-          if (packed && i0 + kPer <= a.V) {   // the vector's bytes at once
-            E::hide_by(raw[s], a.suppress + i0);
-          } else {
+        if (packed && i0 + kPer <= a.V) {   // the vector's bytes at once
+          E::hide_by(raw[s], bytes[s]);
+        } else if (v < v1) {
 #pragma unroll
-            for (int e = 0; e < kPer; ++e)
-              if (i0 + e >= 0 && i0 + e < a.V && a.suppress[i0 + e]) E::hide(raw[s], e);
-          }
+          for (int e = 0; e < kPer; ++e)
+            if (i0 + e >= 0 && i0 + e < a.V && a.suppress[i0 + e]) E::hide(raw[s], e);
         }
       }
     }
+    if (base + kThreads * kSlots < v1) load(base + kThreads * kSlots, next);   // in flight under this pass
     Sums mine = {E::max_of(raw), 0.f, 0.f};
     const float ref = mine.m == -INFINITY ? 0.f : mine.m, top = ref * a.scale;
     float l0 = 0.f, l1 = 0.f, w0 = 0.f, w1 = 0.f;
@@ -290,34 +295,28 @@ __global__ void __launch_bounds__(kThreads, 3) token_logprobs_kernel(const Args 
       // NaN elements count as the largest; a thread whose own maximum does not reach tau can only hold NaN beyond it
       const bool has = (first ? mine.m >= tau : !(mine.m <= tau)) || !(mine.l == mine.l);
       if (has) {
-#pragma unroll 1
+        uint32_t hits = 0;
+#pragma unroll
         for (int s = 0; s < kSlots; ++s) {
-          uint32_t w[4];
-          slot(raw, s, w);
-          const int v = base + s * kThreads + tid, i0 = v * kPer - skew;
-          uint32_t hits = 0;
+          sh.stage[s][tid] = make_uint4(raw[s][0], raw[s][1], raw[s][2], raw[s][3]);
 #pragma unroll
           for (int e = 0; e < kPer; ++e) {
-            const float f = E::get(w, e);
-            hits |= (uint32_t)(first ? !(f < tau) : !(f <= tau)) << e;
+            const float f = E::get(raw[s], e);
+            hits |= (uint32_t)(first ? !(f < tau) : !(f <= tau)) << (s * kPer + e);
           }
-          if (v >= v1) hits = 0;
-          while (hits) {
-            const int e = __ffs(hits) - 1;
-            hits &= hits - 1;
-            float f = 0.f;
-#pragma unroll
-            for (int ee = 0; ee < kPer; ++ee)
-              if (ee == e) f = E::get(w, ee);
-            if (i0 + e >= 0 && i0 + e < a.V) {
-              const int at = atomicAdd(&sh.count, 1);
-              if (at < kList - kMaxK) sh.list[at] = key_of(f, i0 + e);
-            }
+        }
+        while (hits) {
+          const int at_e = __ffs(hits) - 1, s = at_e / kPer, e = at_e % kPer;
+          hits &= hits - 1;
+          const int v = base + s * kThreads + tid, i = v * kPer - skew + e;
+          if (v < v1 && i >= 0 && i < a.V) {
+            const int at = atomicAdd(&sh.count, 1);
+            if (at < kList - kMaxK) sh.list[at] = key_of(E::load((const T*)&sh.stage[s][tid] + e), i);
           }
         }
       }
       const int pass = (base - v0) / (kThreads * kSlots) + 1;
-      if (!careful && (pass & (pass - 1)) != 0 && base + kThreads * kSlots < v1) {
+      if (!careful && ((pass & (pass - 1)) != 0 || (pass & 0x2AAAAAAA) != 0) && base + kThreads * kSlots < v1) {
         sums = merge(sums, mine, a.scale);
         continue;
       }
@@ -333,9 +332,30 @@ __global__ void __launch_bounds__(kThreads, 3) token_logprobs_kernel(const Args 
         load(v0, next);
         continue;
       }
-      if (n <= kList - kMaxK) {
+      if (n <= 64) {   // one warp ranks them
+        if (warp == 0) {
+          const int all = n + (first ? 0 : a.k);   // the best of the earlier passes compete again
+          if (!first && lane < a.k) sh.list[n + lane] = sh.top[lane];
+          __syncwarp();
+          const unsigned long long none = 0, k0 = lane < all ? sh.list[lane] : none, k1 = lane + 32 < all ? sh.list[lane + 32] : none,
+                                   k2 = lane + 64 < all ? sh.list[lane + 64] : none;
+          sh.top[lane] = 0;
+          int r0 = 0, r1 = 0, r2 = 0;
+#pragma unroll 4
+          for (int j = 0; j < all; ++j) {
+            const unsigned long long q = sh.list[j];
+            r0 += q > k0;
+            r1 += q > k1;
+            r2 += q > k2;
+          }
+          __syncwarp();
+          if (k0 != 0 && r0 < a.k) sh.top[r0] = k0;
+          if (k1 != 0 && r1 < a.k) sh.top[r1] = k1;
+          if (k2 != 0 && r2 < a.k) sh.top[r2] = k2;
+        }
+      } else if (n <= kList - kMaxK) {
         int all = n;
-        if (!first) {   // the best of the earlier passes compete again
+        if (!first) {
           if (tid < a.k) {
             sh.list[n + tid] = sh.top[tid];
             sh.top[tid] = 0;
@@ -387,7 +407,8 @@ __global__ void __launch_bounds__(kThreads, 3) token_logprobs_kernel(const Args 
         __syncthreads();
         rank_into(sh.top, sh.list, sh.count, a.k);
       }
-      __syncthreads();
+      if (n > 64) __syncthreads();
+      else __syncwarp();
       // the next pass: only what beats the k-th best (its own index is lower); -inf while there are fewer than k
       if (tid == 0) {
         sh.count = 0;
@@ -398,23 +419,23 @@ __global__ void __launch_bounds__(kThreads, 3) token_logprobs_kernel(const Args 
     sums = merge(sums, mine, a.scale);
   }
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    const Sums other = {__shfl_xor_sync(0xffffffffu, sums.m, o), __shfl_xor_sync(0xffffffffu, sums.l, o),
-                        __shfl_xor_sync(0xffffffffu, sums.w, o)};
-    // the lower lane's triple first: both partners then compute the same bits
-    sums = (lane & o) ? merge(other, sums, a.scale) : merge(sums, other, a.scale);
-  }
+  for (int o = 16; o > 0; o >>= 1) sums = merge_lanes(sums, o, a.scale);
   if (lane == 0) sh.warp_sums[warp] = sums;
   __syncthreads();
-  if (tid == 0) {
-    Sums all = sh.warp_sums[0];
-    for (int i = 1; i < kThreads / 32; ++i) all = merge(all, sh.warp_sums[i], a.scale);
-    sh.block_sums = all;
+  if (warp == 0) {
+    sums = sh.warp_sums[lane & (kThreads / 32 - 1)];
+#pragma unroll
+    for (int o = kThreads / 64; o > 0; o >>= 1) sums = merge_lanes(sums, o, a.scale);
+    if (lane == 0) sh.block_sums = sums;
   }
-  cluster.sync();
+  if (blocks > 1) cluster.sync();
+  else __syncthreads();
   if (me == 0) {
     Sums all = sh.block_sums;
-    for (int i = 1; i < blocks; ++i) all = merge(all, *cluster.map_shared_rank(&sh.block_sums, i), a.scale);
+    if (blocks > 1) {   // every lane fetches a block's, all at once
+      all = *cluster.map_shared_rank(&sh.block_sums, lane & (blocks - 1));
+      for (int o = blocks / 2; o > 0; o >>= 1) all = merge_lanes(all, o, a.scale);
+    }
     if (a.k > 0) {
       if (blocks > 1) {
         for (int i = tid; i < blocks * a.k; i += kThreads)
@@ -430,7 +451,7 @@ __global__ void __launch_bounds__(kThreads, 3) token_logprobs_kernel(const Args 
     const bool empty = all.m == -INFINITY && all.l == 0.f;   // nothing but -inf
     if (tid <= a.k) {
       // tid 0: the given token and the entropy; tid 1..k: an alternative each.  ln L in double: a peaked row has L = 1 + eps
-      const double log_l = log((double)all.l), inv_t = 1.0 / (double)a.temperature;
+      const double log_l = log((double)all.l);
       float value;
       bool in_range = true;
       if (tid == 0) {
@@ -440,19 +461,19 @@ __global__ void __launch_bounds__(kThreads, 3) token_logprobs_kernel(const Args 
       } else {
         value = key_value(sh.list[tid - 1]);
       }
-      float out = empty ? -INFINITY : (float)((double)(value - all.m) * inv_t - log_l);
+      float out = empty ? -INFINITY : (float)((double)(value - all.m) * a.inv_t - log_l);
       if (!in_range) out = __int_as_float(0x7FC00000);
       if (tid == 0) {
         a.token_logprob[row] = out;
         if (a.entropy != nullptr)
-          a.entropy[row] = empty ? 0.f : (float)(log_l - 0.69314718055994531 * (double)all.w / (double)all.l);
+          a.entropy[row] = empty ? 0.f : (float)(log_l - (double)(0.69314718056f * (all.w / all.l)));
       } else {
         a.top_logprobs[row * a.k + tid - 1] = out;
         a.top_ids[row * a.k + tid - 1] = key_index(sh.list[tid - 1]);
       }
     }
   }
-  cluster.sync();   // the first block has read the others' shared memory
+  if (blocks > 1) cluster.sync();   // the first block has read the others' shared memory
 }
 
 template <typename T>
@@ -484,7 +505,7 @@ extern "C" int dflash_token_logprobs(const void* logits, long long ld, const int
   if (!logits || !tokens || !token_logprob || (top_k > 0 && (!top_logprobs || !top_ids))) return fail(DFLASH_ERR_BAD_ARG, "token_logprobs: null operand");
   const int size = dtype == DFLASH_F32 ? 4 : 2;
   if ((uintptr_t)logits % size) return fail(DFLASH_ERR_MISALIGNED, "token_logprobs: logits are not aligned to their type");
-  lp::Args a{logits, ld, tokens, suppress, token_logprob, entropy, top_logprobs, top_ids, temperature, lp::kLog2e / temperature, V, top_k};
+  lp::Args a{logits, ld, tokens, suppress, token_logprob, entropy, top_logprobs, top_ids, 1.0 / (double)temperature, lp::kLog2e / temperature, V, top_k};
   int device = 0;
   cudaGetDevice(&device);
   cudaStream_t st = (cudaStream_t)stream;
