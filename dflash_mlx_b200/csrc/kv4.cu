@@ -20,32 +20,44 @@ constexpr float kLog2e = 1.4426950408889634f;
 
 // ---- write -------------------------------------------------------------------------------------------------------------
 // A lane owns the eight channels of one word, eight lanes a group: minimum and maximum in three shuffles, no shared memory.
-// Bound by HBM (prompts) or by the launch (single tokens): kRows rows per warp are loaded before the first is used, so that a
-// warp has 16 * kRows bytes a lane in flight.  blockIdx.x is (sequence, head), so no lane divides.
+// Bound by HBM and instruction issue (prompts) or by the launch (single tokens): a warp has its next row on the way under the
+// current one, in a rolled loop (eight rows unrolled missed the instruction cache).  blockIdx.x is (sequence, head), so no lane
+// divides.
 struct WriteArgs {
   const void* x[2];
   long long sb[2], sh[2], st[2];
   dflash_kv4_cache c[2];
   const int* offsets;
   const int* counts;
-  int Hk, T, capacity;
+  int Hk, T, capacity, steps;   // steps: rows of a warp (times 256 / D)
 };
 
-// round((v - bias) / scale) by a reciprocal; where that lands within 1e-4 of a border between two codes (its own error is below
-// 1e-5, codes being at most 16) or the reciprocal is not finite, by the division that defines the code.
-__device__ __forceinline__ uint32_t code_of(float v, float bias, float scale, float inv) {
+// The code as a float, round((v - bias) / scale) in 0..15.  The quotient is that of an IEEE division: by the correctly rounded
+// reciprocal and one correction by the exact residual (Markstein), as long as nothing in it is subnormal (`plain`).  bias is the
+// group's minimum, so there is nothing below 0; a scale that was rounded down far (a subnormal) goes above 15.  Adding and
+// taking away 1.5 * 2^23 rounds to a whole number, ties to even, without the slow conversion instructions.
+__device__ __forceinline__ float code_of(float v, float bias, float scale, float inv, bool plain) {
+  constexpr float kMagic = 12582912.f;
   const float y = __fsub_rn(v, bias);
-  const float q = y * inv;
-  float n = rintf(q);
-  if (!(fabsf(q - n) < 0.4999f)) n = rintf(__fdiv_rn(y, scale));
-  return (uint32_t)fminf(fmaxf(n, 0.f), 15.f);
+  float q = y * inv;
+  if (plain) q = __fmaf_rn(__fmaf_rn(-q, scale, y), inv, q);
+  else q = __fdiv_rn(y, scale);
+  return fminf(__fsub_rn(__fadd_rn(q, kMagic), kMagic), 15.f);
 }
+// x / 15 to the last bit for every value of the two 16-bit types (verified over all of them): the quotient by the rounded
+// reciprocal and one correction by its residual.
+__device__ __forceinline__ float by_15(float x) {
+  constexpr float kInv = 1.f / 15.f;
+  const float q = __fmul_rn(x, kInv);
+  return __fmaf_rn(__fmaf_rn(-15.f, q, x), kInv, q);
+}
+__device__ __forceinline__ __nv_bfloat162 pair_of(uint32_t u, __nv_bfloat16) { return *(const __nv_bfloat162*)&u; }
+__device__ __forceinline__ __half2 pair_of(uint32_t u, __half) { return *(const __half2*)&u; }
 
-template <typename T, int D, int kRows>
+template <typename T, int D>
 __global__ void __launch_bounds__(128) kv4_write_kernel(const WriteArgs a, int* __restrict__ err) {
   using TR = MmaTraits<T>;
   constexpr int kLanes = D / 8, kPer = 32 / kLanes;   // lanes of a row, rows of a warp at once
-  constexpr int kBlock = 4 * kPer * kRows;            // rows of a block
   pdl_wait();
   pdl_trigger();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, side = blockIdx.z;
@@ -58,53 +70,59 @@ __global__ void __launch_bounds__(128) kv4_write_kernel(const WriteArgs a, int* 
   uint32_t* codes = c.codes + b * c.codes_batch_stride + h * c.codes_head_stride + j;
   T* scales = (T*)c.scales + b * c.scales_batch_stride + h * c.scales_head_stride + (j >> 3);
   T* biases = (T*)c.biases + b * c.biases_batch_stride + h * c.biases_head_stride + (j >> 3);
-  for (int t0 = blockIdx.y * kBlock; t0 < n; t0 += gridDim.y * kBlock) {
-    uint4 raw[kRows];
-    bool ok[kRows];
+  const int first = (int)blockIdx.y * 4 * kPer * a.steps + warp * kPer + lane / kLanes;
+  auto inside = [&](int t) { return t < n && at + t >= 0 && at + t < a.capacity; };
+  auto load = [&](int t) { return inside(t) ? *(const uint4*)(x + t * a.st[side]) : make_uint4(0, 0, 0, 0); };
+  uint4 next = load(first);
+#pragma unroll 1
+  for (int s = 0; s < a.steps; ++s) {
+    const int t = first + s * 4 * kPer;
+    const uint4 raw = next;
+    if (s + 1 < a.steps) next = load(t + 4 * kPer);
+    if (__all_sync(0xffffffffu, t >= n)) break;
+    if (t < n && !inside(t) && j == 0) atomicCAS(err, 0, 61 | ((t & 0x7FFFFF) << 8));
+    const uint32_t u[4] = {raw.x, raw.y, raw.z, raw.w};
+    // maximum and minimum in pairs; a NaN wins both
+    const auto hi2 = __hmax2_nan(__hmax2_nan(pair_of(u[0], T()), pair_of(u[1], T())), __hmax2_nan(pair_of(u[2], T()), pair_of(u[3], T())));
+    const auto lo2 = __hmin2_nan(__hmin2_nan(pair_of(u[0], T()), pair_of(u[1], T())), __hmin2_nan(pair_of(u[2], T()), pair_of(u[3], T())));
+    const T hi_t = __hmax_nan(hi2.x, hi2.y), nlo_t = __hneg(__hmin_nan(lo2.x, lo2.y));
+    uint32_t ext = (uint32_t) * (const uint16_t*)&hi_t | ((uint32_t) * (const uint16_t*)&nlo_t << 16);   // maximum, -minimum
 #pragma unroll
-    for (int i = 0; i < kRows; ++i) {
-      const int t = t0 + (warp * kRows + i) * kPer + lane / kLanes;
-      const long long p = at + t;
-      ok[i] = t < n && p >= 0 && p < a.capacity;
-      raw[i] = make_uint4(0, 0, 0, 0);
-      if (ok[i]) raw[i] = *(const uint4*)(x + t * a.st[side]);
-      else if (t < n && j == 0) atomicCAS(err, 0, 61 | ((t & 0x7FFFFF) << 8));
+    for (int o = 1; o < 8; o <<= 1) {
+      const auto m = __hmax2_nan(pair_of(ext, T()), pair_of(__shfl_xor_sync(0xffffffffu, ext, o), T()));
+      ext = *(const uint32_t*)&m;
     }
+    const float hi = TR::bits_to_float((uint16_t)ext), lo = -TR::bits_to_float((uint16_t)(ext >> 16));
+    // NaN as soon as one value is NaN or infinite
+    const float bad = fmaf(hi, 0.f, lo * 0.f);
+    // subnormals count too: the codes are defined to the last bit (this file is compiled without fast math)
+    const T scale_t = TR::from_float(__fadd_rn(__fsub_rn(by_15(hi), by_15(lo)), bad));
+    const T bias_t = TR::from_float(__fadd_rn(lo, bad));
+    const float scale = TR::to_float(scale_t), bias = TR::to_float(bias_t);
+    uint32_t word = 0;
+    if (scale > 0.f) {
+      const float inv = __frcp_rn(scale);
+      float f[2];   // four codes each, as one whole number below 2^16
+      auto codes_of = [&](bool plain) {
 #pragma unroll
-    for (int i = 0; i < kRows; ++i) {
-      float v[8];
-      const uint32_t u[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
-      float lo = INFINITY, hi = -INFINITY, bad = 0.f;
+        for (int w = 0; w < 2; ++w) {
+          float k[4];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        v[e] = TR::bits_to_float((uint16_t)(u[e >> 1] >> (16 * (e & 1))));
-        lo = fminf(lo, v[e]);
-        hi = fmaxf(hi, v[e]);
-        bad = fmaf(v[e], 0.f, bad);   // NaN as soon as one value is NaN or infinite
-      }
-#pragma unroll
-      for (int o = 1; o < 8; o <<= 1) {
-        lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-        hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
-        bad += __shfl_xor_sync(0xffffffffu, bad, o);
-      }
-      // IEEE divisions and subnormals: the codes are defined to the last bit (this file is compiled without fast math)
-      const T scale_t = TR::from_float(__fadd_rn(__fsub_rn(__fdiv_rn(hi, 15.f), __fdiv_rn(lo, 15.f)), bad));
-      const T bias_t = TR::from_float(__fadd_rn(lo, bad));
-      const float scale = TR::to_float(scale_t), bias = TR::to_float(bias_t);
-      uint32_t word = 0;
-      if (scale > 0.f) {
-        const float inv = __frcp_rn(scale);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) word |= code_of(v[e], bias, scale, inv) << (4 * e);
-      }
-      if (ok[i]) {
-        const long long p = at + t0 + (warp * kRows + i) * kPer + lane / kLanes;
-        codes[p * (D / 8)] = word;
-        if ((j & 7) == 0) {
-          scales[p * (D / kGroup)] = scale_t;
-          biases[p * (D / kGroup)] = bias_t;
+          for (int e = 0; e < 4; ++e)
+            k[e] = code_of(TR::bits_to_float((uint16_t)(u[2 * w + (e >> 1)] >> (16 * (e & 1)))), bias, scale, inv, plain);
+          f[w] = fmaf(fmaf(fmaf(k[3], 16.f, k[2]), 16.f, k[1]), 16.f, k[0]) + 8388608.f;
         }
+      };
+      if (scale > 0x1p-80f && scale < 0x1p100f) codes_of(true);
+      else codes_of(false);
+      word = prmt(__float_as_uint(f[0]), __float_as_uint(f[1]), 0x5410);
+    }
+    if (inside(t)) {
+      const long long p = at + t;
+      codes[p * (D / 8)] = word;
+      if ((j & 7) == 0) {
+        scales[p * (D / kGroup)] = scale_t;
+        biases[p * (D / kGroup)] = bias_t;
       }
     }
   }
@@ -812,17 +830,18 @@ extern "C" int dflash_kv4_write(const void* keys, const long long* key_strides, 
   int* err = device_error_word(device);
   if (!err) return fail(DFLASH_ERR_LAUNCH, "kv4_write: no device error word");
   dim3 grid;
-  const bool many = row_grid(B, Hk, T, D, 2, device, &grid);
+  a.steps = row_grid(B, Hk, T, D, 2, device, &grid) ? kManyRows : 1;
+  const long long covered = (long long)grid.y * 4 * (D == 128 ? 2 : 1) * a.steps;
+  if (covered < T) a.steps = (int)((T + covered / a.steps - 1) / (covered / a.steps));   // grid.y at its limit: longer loops
   const dim3 block(128);
   cudaStream_t st = (cudaStream_t)stream;
-  auto go = [&](auto one, auto four) { return many ? launch_kernel(four, grid, block, 0, st, a, err) : launch_kernel(one, grid, block, 0, st, a, err); };
   cudaError_t e;
   if (dtype == DFLASH_BF16)
-    e = D == 128 ? go(kv4_write_kernel<__nv_bfloat16, 128, 1>, kv4_write_kernel<__nv_bfloat16, 128, kManyRows>)
-                 : go(kv4_write_kernel<__nv_bfloat16, 256, 1>, kv4_write_kernel<__nv_bfloat16, 256, kManyRows>);
+    e = D == 128 ? launch_kernel(kv4_write_kernel<__nv_bfloat16, 128>, grid, block, 0, st, a, err)
+                 : launch_kernel(kv4_write_kernel<__nv_bfloat16, 256>, grid, block, 0, st, a, err);
   else
-    e = D == 128 ? go(kv4_write_kernel<__half, 128, 1>, kv4_write_kernel<__half, 128, kManyRows>)
-                 : go(kv4_write_kernel<__half, 256, 1>, kv4_write_kernel<__half, 256, kManyRows>);
+    e = D == 128 ? launch_kernel(kv4_write_kernel<__half, 128>, grid, block, 0, st, a, err)
+                 : launch_kernel(kv4_write_kernel<__half, 256>, grid, block, 0, st, a, err);
   if (e == cudaSuccess) e = cudaGetLastError();
   return e == cudaSuccess ? DFLASH_OK : fail(DFLASH_ERR_LAUNCH, "kv4_write launch: %s", cudaGetErrorString(e));
 }
