@@ -202,6 +202,10 @@ PyObject* py_write(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
   const Cache c = cache(a + 2, &d);
   d.add(&offsets); d.add(counts);
   const Side& k = c.k;
+  for (int i = 2; i < 8; ++i) {
+    const at::Tensor& x = THPVariable_Unpack(a[i]);
+    if ((x.size(0) > 1 && x.stride(0) == 0) || (x.size(1) > 1 && x.stride(1) == 0)) refuse("a cache that is written must not repeat its sequences or heads");
+  }
   if (keys.dim() != 4 || keys.sizes() != values.sizes() || keys.size(0) != k.B || keys.size(1) != k.Hk || keys.size(3) != k.D)
     refuse("keys and values must be [B, Hk, T, D] = [", k.B, ", ", k.Hk, ", T, ", k.D, "], got ", keys.sizes(), " and ", values.sizes());
   if (keys.scalar_type() != k.type || values.scalar_type() != k.type) refuse("keys and values must have the cache's dtype ", k.type);
@@ -270,6 +274,7 @@ PyObject* py_sdpa(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
   const Cache c = cache(a + 1, &d);
   const Side& k = c.k;
   const double scale = number(a[7], "scale");
+  if (!std::isfinite((float)scale)) refuse("scale must be finite, got ", scale);
   if (queries.dim() != 4 || queries.size(0) != k.B || queries.size(3) != k.D || queries.size(1) < 1 || k.Hk < 1 || queries.size(1) % k.Hk)
     refuse("queries must be [B, Hq, T, D] = [", k.B, ", n*", k.Hk, ", T, ", k.D, "], got ", queries.sizes());
   if (queries.scalar_type() != k.type) refuse("queries must have the cache's dtype ", k.type);

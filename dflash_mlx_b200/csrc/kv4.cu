@@ -268,7 +268,7 @@ __global__ void __launch_bounds__((kWarpsOf<D, NT>) * 32, 2) kv4_sdpa_kernel(con
   pdl_wait();
   pdl_trigger();
   const int split = blockIdx.x, bhk = blockIdx.z, b = bhk / a.Hk, hk = bhk % a.Hk, row0 = blockIdx.y * 8 * NT;
-  const int len = a.lengths ? a.lengths[b] : a.max_length;
+  const int len = a.lengths ? max(a.lengths[b], 0) : a.max_length;
   const int t_last = min(row0 + 8 * NT, a.rows) - 1;
   // one past the last position any row of this block sees
   const int hi = min(min(len, a.max_length), len - a.T + t_last / a.gqa + 1);
@@ -900,6 +900,7 @@ extern "C" int dflash_kv4_sdpa(const void* q, const long long* q_strides, const 
   int rc = check_sizes("kv4_sdpa", B, Hk, T, D, capacity, dtype);
   if (rc) return rc;
   if (Hq < 1 || Hq % Hk != 0) return fail(DFLASH_ERR_BAD_SHAPE, "kv4_sdpa: %d query heads on %d KV heads", Hq, Hk);
+  if (!(scale - scale == 0.f)) return fail(DFLASH_ERR_BAD_ARG, "kv4_sdpa: the scale is not finite");
   if (max_length < 0 || max_length > capacity) return fail(DFLASH_ERR_BAD_SHAPE, "kv4_sdpa: max_length %d outside 0..%d", max_length, capacity);
   if (B == 0 || T == 0) return DFLASH_OK;
   if (!q || !q_strides || !out) return fail(DFLASH_ERR_BAD_ARG, "kv4_sdpa: null operand");

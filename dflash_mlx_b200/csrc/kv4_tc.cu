@@ -408,7 +408,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_sdpa_tc_kernel(const SdpaArgs
   pdl_wait();
   pdl_trigger();
   const int split = blockIdx.x, bhk = blockIdx.z, b = bhk / a.Hk, hk = bhk % a.Hk, row0 = blockIdx.y * kRows;
-  const int len = a.lengths ? a.lengths[b] : a.max_length;
+  const int len = a.lengths ? max(a.lengths[b], 0) : a.max_length;
   const int t_last = (min(row0 + kRows, a.rows) - 1) / a.gqa;
   // one past the last position any row of this block sees
   const int hi = min(min(len, a.max_length), len - a.T + t_last + 1);
@@ -548,7 +548,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_sdpa_tc_kernel(const SdpaArgs
       uint32_t v[kTile];
       ld32(s_col, v);
       ld32(s_col + 32, v + 32);
-      float c[2] = {c_row * mt.k_factor[blk], c_row * mt.k_factor[blk + 1]};
+      // never 0 (a scale of 0): a hidden score stays -inf under it
+      float c[2] = {fmaxf(c_row * mt.k_factor[blk], 1e-37f), fmaxf(c_row * mt.k_factor[blk + 1], 1e-37f)};
       // every key of the tile seen by every row of the warp, and no mask
       const bool plain = !kMask && __all_sync(0xffffffffu, n0 + kTile - 1 <= lim);
       if (!wait_warp(bar0 + 8 * (kBarVMeta + ((i >> 1) & (kMeta - 1))), (i / (2 * kMeta)) & 1)) { atomicCAS(err, 0, 62 | (13 << 8)); ok = false; }
@@ -583,7 +584,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_sdpa_tc_kernel(const SdpaArgs
           t1 = fmaxf(fmaxf(t1, __uint_as_float(v[e + 2])), __uint_as_float(v[e + 3]));
         }
         t0 = fmaxf(t0, t1);
-        top = fmaxf(top, t0 == -INFINITY ? t0 : t0 * c[q]);   // c may be 0
+        top = fmaxf(top, t0 * c[q]);
       }
       // ---- the row's reference: what the tile before left, moved when this tile exceeds it by 8 octaves ----
       float m = -INFINITY;

@@ -27,7 +27,7 @@ namespace dflash {
 namespace lp {
 namespace {
 
-constexpr int kThreads = 256, kGroups = 64, kMaxK = 32, kList = 1024;
+constexpr int kThreads = 256, kGroups = 64, kMaxK = 32, kList = 1024, kMaxCluster = 8;
 constexpr float kLog2e = 1.4426950408889634f;
 
 struct Args {
@@ -150,7 +150,7 @@ struct Shared {
   int count;
   unsigned long long list[kList];
   unsigned long long top[kMaxK];                  // this block's best, highest first; 0 = none
-  unsigned long long gathered[8 * kMaxK];         // first block of a cluster: every block's `top`
+  unsigned long long gathered[kMaxCluster * kMaxK];         // first block of a cluster: every block's `top`
   int counts[2][kThreads / 32];
   uint4 stage[4][kThreads];                       // elements of threads that hold candidates, to be picked by number
 };
@@ -198,6 +198,17 @@ __global__ void __launch_bounds__(kThreads, 3) token_logprobs_kernel(const Args 
   const bool packed = a.suppress != nullptr && skew == 0 && ((uintptr_t)a.suppress & (kPer - 1)) == 0;
   uint2 bytes[kSlots];   // of `suppress`, for the vectors on their way
   auto load = [&](int base, uint32_t (&raw)[kSlots][4]) {
+    const int last = base + kThreads * kSlots;
+    if (base * kPer >= skew && last <= v1 && last * kPer - skew <= a.V) {   // the whole pass lies inside the row
+      const T* px = x + (base + tid) * kPer - skew;
+#pragma unroll
+      for (int s = 0; s < kSlots; ++s) {
+        const uint4 u = __ldcs((const uint4*)(px + s * kThreads * kPer));
+        raw[s][0] = u.x; raw[s][1] = u.y; raw[s][2] = u.z; raw[s][3] = u.w;
+        bytes[s] = packed ? E::suppress_bytes(a.suppress + (base + s * kThreads + tid) * kPer) : make_uint2(0, 0);
+      }
+      return;
+    }
 #pragma unroll
     for (int s = 0; s < kSlots; ++s) {
       const int v = base + s * kThreads + tid;
@@ -438,10 +449,25 @@ __global__ void __launch_bounds__(kThreads, 3) token_logprobs_kernel(const Args 
     }
     if (a.k > 0) {
       if (blocks > 1) {
-        for (int i = tid; i < blocks * a.k; i += kThreads)
-          sh.gathered[i] = cluster.map_shared_rank(&sh.top[0], i / a.k)[i % a.k];
+        // a key's rank: its place in its own block's list, and in each other list (sorted, 0 at the end) the number above it
+        static_assert(kMaxCluster * kMaxK == kThreads, "a thread per gathered key");
+        const int from = warp, place = lane;
+        if (from < blocks) sh.gathered[tid] = cluster.map_shared_rank(&sh.top[0], from)[place];
         __syncthreads();
-        rank_into(sh.list, sh.gathered, blocks * a.k, a.k);   // list: free again
+        const unsigned long long mine = from < blocks ? sh.gathered[tid] : 0;
+        if (mine != 0) {
+          int rank = place;
+          for (int o = 0; o < blocks; ++o) {
+            if (o == from) continue;
+            const unsigned long long* other = sh.gathered + o * kMaxK;
+            int above = 0;
+#pragma unroll
+            for (int step = kMaxK / 2; step > 0; step >>= 1)
+              if (other[above + step - 1] > mine) above += step;
+            rank += above + (other[above] > mine);
+          }
+          if (rank < a.k) sh.list[rank] = mine;   // list: free again
+        }
         __syncthreads();
       } else {
         if (tid < kMaxK) sh.list[tid] = sh.top[tid];
@@ -481,7 +507,7 @@ int launch(const Args& a, int R, cudaStream_t st, int device) {
   // rows alone fill the SMs: a block per row passes over it, most passes finding no new candidate; few rows: the cluster grows
   // while a block keeps 2048 elements
   int c = 1;
-  while (c < 8 && (long long)R * c < sm_count(device) && a.V >= 2 * c * 2048) c <<= 1;
+  while (c < kMaxCluster && (long long)R * c < sm_count(device) && a.V >= 2 * c * 2048) c <<= 1;
   if ((long long)R * c > 0x7fffffffll) return fail(DFLASH_ERR_BAD_SHAPE, "token_logprobs: too many rows");
   cudaError_t e = launch_kernel_cluster(token_logprobs_kernel<T>, dim3((unsigned)R * c), dim3(kThreads), c, 0, st, a);
   if (e == cudaSuccess) e = cudaGetLastError();

@@ -419,7 +419,7 @@ DFLASH_API int dflash_kv4_read(const dflash_kv4_cache* k_cache, const dflash_kv4
                                int dtype, void* stream);
 /* Softmax attention of T query positions per sequence over the cache, T >= 1.
  *   q        dtype, element (b,h,t,d) at b*strides[0] + h*strides[1] + t*strides[2] + d (multiples of 8, 16-byte aligned)
- *   out      dtype [B,Hq,T,D] contiguous, 16-byte aligned;  head hq reads KV head hq / (Hq/Hk)
+ *   out      dtype [B,Hq,T,D] contiguous, 16-byte aligned;  head hq reads KV head hq / (Hq/Hk);  scale is finite
  *   lengths  device int[B] = positions sequence b holds, the T queries' own among them, or NULL: max_length for all.
  *            Row t of sequence b sees position n iff n <= lengths[b] - T + t, n < lengths[b], n < max_length.
  *   max_length <= capacity bounds the lengths (the launch geometry and the workspace are those of max_length, so one

@@ -95,6 +95,27 @@ def test_suppressed_and_hidden(V):
     check(x, ints(1, 7, 1, V - 1), 12, suppress=torch.ones(V, dtype=torch.bool, device=DEV))
 
 
+@pytest.mark.parametrize("seed", range(12))
+def test_random_shapes(seed):
+    import random
+    r = random.Random(seed)
+    V = int(2 ** r.uniform(1, 17.3))
+    R = r.choice([1, 3, 17, 200 if V < 20000 else 5])
+    k = r.randint(0, min(32, V))
+    x = logits(R, V, r.choice(TYPES), seed, r.choice([0.1, 2.0, 20.0]))
+    suppress = (torch.rand(V, generator=torch.Generator(device=DEV).manual_seed(seed), device=DEV) < 0.3) if r.random() < 0.5 else None
+    tokens = torch.randint(0, V, (R,), generator=torch.Generator().manual_seed(seed)).to(DEV)
+    check(x, tokens, k, r.choice([1.0, 0.3, 3.0, 400.0]), suppress)
+
+
+@pytest.mark.parametrize("ascending", [False, True])
+def test_rows_that_beat_themselves_again_and_again(ascending):
+    """Many rows, one block each, whose later elements keep beating the earlier ones: the list of candidates overflows."""
+    x = torch.linspace(-9, 9, 60000, device=DEV).expand(200, -1).contiguous()
+    x = x if ascending else x.flip(1).contiguous()
+    check(x[:3].repeat(60, 1)[:160], torch.arange(160, device=DEV), 20)
+
+
 @pytest.mark.parametrize("V", [100, 30000])
 def test_nan_infinity_and_lowest(V):
     x = logits(5, V, torch.float32)

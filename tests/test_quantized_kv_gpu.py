@@ -213,6 +213,9 @@ def test_attention_host_length_and_no_keys():
                 dict(lengths=ints(1, 2).long()), dict(lengths=ints(5, 5), max_length=99)):
         with pytest.raises(ValueError):
             qkv.quantized_kv_sdpa(q, k, v, scale, **bad)
+    for bad in (math.nan, math.inf, 1e39):
+        with pytest.raises(ValueError, match="scale"):
+            qkv.quantized_kv_sdpa(q, k, v, bad, 50)
     for bad in (q[:, :3], q.half(), q[..., :64], q[:1]):
         with pytest.raises(ValueError):
             qkv.quantized_kv_sdpa(bad, k, v, scale, 50)
@@ -335,6 +338,61 @@ def test_results_do_not_change_from_call_to_call():
         first = qkv.quantized_kv_sdpa(q, k, v, 0.06, ints(700, 333))
         for _ in range(5):
             assert torch.equal(qkv.quantized_kv_sdpa(q, k, v, 0.06, ints(700, 333)), first)
+
+
+@pytest.mark.parametrize("seed", range(24))
+def test_attention_random_shapes(seed):
+    """Heads, rows, lengths, masks and types drawn at random, both kernels and their edges."""
+    import random
+    r = random.Random(seed)
+    dtype, D = r.choice(TYPES), r.choice([128, 256])
+    Hk, g = r.choice([1, 2, 3]), r.choice([1, 2, 5, 6, 8])
+    T = r.choice([1, 2, 3, r.randint(4, 16), r.randint(17, 60)])
+    B = r.randint(1, 3)
+    cap = r.randint(max(T, 2), 700)
+    n_max = r.randint(1, cap)
+    lengths = [r.choice([0, T, n_max, r.randint(0, n_max), cap + 5]) for _ in range(B)]
+    mask = None
+    if r.random() < 0.5:
+        dims = r.choice([(B, 1, 1, n_max), (1, g * Hk, T, n_max), (n_max,), (B, 1, T, 1)])
+        keep = torch.rand(dims, generator=gen(seed), device=DEV) < 0.7
+        mask = r.choice([keep, torch.where(keep, torch.randn(dims, generator=gen(seed), device=DEV), -math.inf).to(r.choice([dtype, torch.float32]))])
+    run_sdpa(B, g * Hk, Hk, D, T, lengths, dtype, mask=mask, cap=cap, max_length=n_max, seed=seed, num_splits=r.choice([0, 0, 1, 3]))
+
+
+@pytest.mark.parametrize("T", [2, 40])
+def test_attention_scales_and_nan_queries(T):
+    """Zero and negative scales; a NaN or infinite query stays in its own row."""
+    k, v = make_cache(1, 2, 300, 128, torch.bfloat16)
+    q = states((1, 4, T, 128), torch.bfloat16, 3)
+    for scale in (0.0, -0.1, 1e-30):
+        check_rows(qkv.quantized_kv_sdpa(q, k, v, scale, 300), ref.sdpa(q, k, v, scale, [300]), torch.bfloat16)
+    want = qkv.quantized_kv_sdpa(q, k, v, 0.1, 300)
+    for bad in (math.nan, math.inf):
+        p = q.clone()
+        p[0, 1, 1, 5] = bad
+        got = qkv.quantized_kv_sdpa(p, k, v, 0.1, 300)
+        assert bool(got[0, 1, 1].isnan().all())
+        got[0, 1, 1] = want[0, 1, 1]
+        assert torch.equal(got, want)
+    tiny = q * 1e-30                                       # queries below fp16's range
+    check_rows(qkv.quantized_kv_sdpa(tiny, k, v, 1e29, 300), ref.sdpa(tiny, k, v, 1e29, [300]), torch.bfloat16)
+    big = q * 1e30
+    check_rows(qkv.quantized_kv_sdpa(big, k, v, 1e-31, 300), ref.sdpa(big, k, v, 1e-31, [300]), torch.bfloat16)
+
+
+def test_extreme_lengths_and_shared_caches():
+    k, v = make_cache(1, 2, 64, 128, torch.bfloat16)
+    for T in (2, 40):
+        q = states((3, 4, T, 128), torch.bfloat16, 3)
+        shared = [qkv.QuantizedKV(*[p.expand(3, -1, -1, -1) for p in c]) for c in (k, v)]     # one prefix, three readers
+        lengths = [-2 ** 31, 2 ** 31 - 1, 50]
+        got = qkv.quantized_kv_sdpa(q, *shared, 0.1, ints(*lengths))
+        assert not bool(got[0].any())
+        check_rows(got, ref.sdpa(q, *shared, 0.1, lengths), torch.bfloat16)
+        x = states((3, 2, T, 128), torch.bfloat16, 4)
+        with pytest.raises(ValueError, match="repeat"):
+            qkv.quantized_kv_write(x, x, *shared, ints(0, 0, 0))
 
 
 def test_long_cache_offsets_pass_32_bits():
