@@ -642,6 +642,13 @@ __global__ void __launch_bounds__(256) kv4_combine_kernel(const SdpaArgs a) {
   const size_t row = (size_t)blockIdx.y * a.rows + blockIdx.x;
   const float* pm = a.part_m + row * a.splits;
   const float* pl = a.part_l + row * a.splits;
+  const int d4 = tid % (D / 4), s0 = tid / (D / 4);
+  const float4* po = (const float4*)(a.part_o + row * a.splits * D) + d4;
+  constexpr int kEarly = 8;   // requested before the weights are known
+  float4 early[kEarly];
+#pragma unroll
+  for (int i = 0; i < kEarly; ++i)
+    early[i] = s0 + i * kPer < a.splits ? po[(size_t)(s0 + i * kPer) * (D / 4)] : make_float4(0.f, 0.f, 0.f, 0.f);
   float mx = -INFINITY;
   for (int s = tid; s < a.splits; s += kThreads) mx = fmaxf(mx, pm[s]);
 #pragma unroll
@@ -666,16 +673,16 @@ __global__ void __launch_bounds__(256) kv4_combine_kernel(const SdpaArgs a) {
   den = red[0];
 #pragma unroll
   for (int i = 1; i < kThreads / 32; ++i) den += red[i];
-  const int d4 = tid % (D / 4), s0 = tid / (D / 4);
-  const float4* po = (const float4*)(a.part_o + row * a.splits * D) + d4;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-  for (int s = s0; s < a.splits; s += kPer) {
-    const float4 v = po[(size_t)s * (D / 4)];
-    const float w = sw[s];
+  auto add = [&](float w, const float4& v) {
     acc.x = fmaf(w, v.x, acc.x); acc.y = fmaf(w, v.y, acc.y);
     acc.z = fmaf(w, v.z, acc.z); acc.w = fmaf(w, v.w, acc.w);
-  }
+  };
+#pragma unroll
+  for (int i = 0; i < kEarly; ++i)
+    if (s0 + i * kPer < a.splits) add(sw[s0 + i * kPer], early[i]);
+#pragma unroll 4
+  for (int s = s0 + kEarly * kPer; s < a.splits; s += kPer) add(sw[s], po[(size_t)s * (D / 4)]);
   part[s0][d4] = acc;
   __syncthreads();
   if (s0 != 0) return;
@@ -691,6 +698,47 @@ __global__ void __launch_bounds__(256) kv4_combine_kernel(const SdpaArgs a) {
   for (int e = 0; e < 4; ++e) z[e] = TR::from_float(nan == 0.f ? v[e] : nan);
   const int b = blockIdx.y / a.Hk, hk = blockIdx.y % a.Hk;
   *(uint2*)((T*)a.out + out_row(a, b, hk, blockIdx.x) * D + 4 * d4) = *(const uint2*)z;
+}
+
+// The same for at most kFewSplits key ranges (many rows, as a prompt has): a thread per four channels of a row, which computes the
+// row's weights itself; no block-wide step.
+constexpr int kFewSplits = 8;
+template <typename T, int D>
+__global__ void __launch_bounds__(256) kv4_combine_few_kernel(const SdpaArgs a) {
+  using TR = MmaTraits<T>;
+  pdl_wait();
+  pdl_trigger();
+  constexpr int kLanes = D / 4;
+  const int r = blockIdx.x * (256 / kLanes) + threadIdx.x / kLanes, d4 = threadIdx.x % kLanes;
+  if (r >= a.rows) return;
+  const size_t row = (size_t)blockIdx.y * a.rows + r;
+  const float4* po = (const float4*)(a.part_o + row * a.splits * D) + d4;
+  float4 v[kFewSplits];
+  float m[kFewSplits], l[kFewSplits], mx = -INFINITY;
+#pragma unroll
+  for (int s = 0; s < kFewSplits; ++s) {
+    const bool in = s < a.splits;
+    v[s] = in ? po[(size_t)s * kLanes] : make_float4(0.f, 0.f, 0.f, 0.f);
+    m[s] = in ? a.part_m[row * a.splits + s] : -INFINITY;
+    l[s] = in ? a.part_l[row * a.splits + s] : 0.f;
+    mx = fmaxf(mx, m[s]);
+  }
+  const float ref = mx == -INFINITY ? 0.f : mx;
+  float den = 0.f;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+  for (int s = 0; s < kFewSplits; ++s) {
+    const float w = ex2((m[s] - ref) * kLog2e);
+    den = fmaf(w, l[s], den);
+    acc.x = fmaf(w, v[s].x, acc.x); acc.y = fmaf(w, v[s].y, acc.y);
+    acc.z = fmaf(w, v[s].z, acc.z); acc.w = fmaf(w, v[s].w, acc.w);
+  }
+  const float inv = den == 0.f ? 1.f : 1.f / den, nan = den * 0.f;
+  const float y[4] = {acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv};
+  T z[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) z[e] = TR::from_float(nan == 0.f ? y[e] : nan);
+  *(uint2*)((T*)a.out + out_row(a, blockIdx.y / a.Hk, blockIdx.y % a.Hk, r) * D + 4 * d4) = *(const uint2*)z;
 }
 
 // ---- host side ---------------------------------------------------------------------------------------------------------
@@ -748,7 +796,10 @@ int launch_sdpa(SdpaArgs a, cudaStream_t st, int device) {
 
 template <typename T, int D>
 int launch_combine(const SdpaArgs& a, cudaStream_t st) {
-  cudaError_t e = launch_kernel(kv4_combine_kernel<T, D>, dim3(a.rows, a.B * a.Hk), dim3(256), 0, st, a);
+  constexpr int kRowsAtOnce = 256 / (D / 4);
+  cudaError_t e = a.splits <= kFewSplits
+                      ? launch_kernel(kv4_combine_few_kernel<T, D>, dim3((a.rows + kRowsAtOnce - 1) / kRowsAtOnce, a.B * a.Hk), dim3(256), 0, st, a)
+                      : launch_kernel(kv4_combine_kernel<T, D>, dim3(a.rows, a.B * a.Hk), dim3(256), 0, st, a);
   if (e == cudaSuccess) e = cudaGetLastError();
   return e == cudaSuccess ? DFLASH_OK : fail(DFLASH_ERR_LAUNCH, "kv4_sdpa combine launch: %s", cudaGetErrorString(e));
 }

@@ -18,7 +18,7 @@
 // fma turns two of them into code * scale + bias with a single rounding to fp16 (2^-11; the cache's scales carry 8 or 11 bits,
 // the codes 4).  For that, every 32 keys share a power of two that brings the scales under 2^-8 and that S (for K) or P (for V)
 // takes back.  Values far below the largest of their 32 keys lose bits at 2^-21 of that largest one: nothing to a score, and values
-// of keys that differ by more than 6 octaves are unpacked in 13 instructions with 16 more bits of range.  q is brought
+// of keys that differ by more than 6 octaves are unpacked in 13 instructions with 11 more bits of range.  q is brought
 // to fp16 by a power of two per row, exact down to 2^-22 of the row's largest element.  P is fp16, up to 2^14.
 // The running maximum moves only when a score exceeds it by 8 octaves.  Every wait is bounded (device error code 62).
 #include <mutex>
@@ -232,9 +232,9 @@ __device__ __forceinline__ void unpack_row(const uint4& c0, const uint4& c1, flo
 // The keys (kV = false) or values of a block's range, by the four warps of a side: thread = key of the tile.
 template <int D>
 __device__ __forceinline__ int raw_chunk(int r, int ch) { return D == 256 ? ch ^ (r & 7) : ch ^ ((r >> 1) & 3); }
-template <typename T, int D, bool kV, typename F, typename H>
+template <typename T, int D, bool kV, typename F>
 __device__ __forceinline__ void unpack_side(const dflash_kv4_cache& c, int b, int hk, int k0, int hi, int tiles, uint8_t* buf, uint8_t* raw,
-                                            uint32_t bar0, Meta* meta, int* err, F query_copy, H query_rows) {
+                                            uint32_t bar0, Meta* meta, int* err, F query_rows) {
   constexpr int G = D / kGroup;
   const int w = (threadIdx.x >> 5) & 3, lane = threadIdx.x & 31, key = w * 32 + lane;
   const uint8_t* codes = (const uint8_t*)(c.codes + b * c.codes_batch_stride + hk * c.codes_head_stride);
@@ -300,7 +300,8 @@ __device__ __forceinline__ void unpack_side(const dflash_kv4_cache& c, int b, in
       // keys whose largest value is more than 6 octaves below: the narrow form would lose their bits
       const int lo_e = (int)(__reduce_min_sync(0xffffffffu, bad || largest == 0 ? 0x7F7FFFFFu : largest) >> 23) - 127;
       wide = hi_e - lo_e > 6;
-      if (wide) e = min(max(hi_e - 13, -100), 126);   // values below 2^14
+      // values below 2^5: 19 octaves of full precision for them, and only 11 octaves that P has to make up for next to a narrow block
+      if (wide) e = min(max(hi_e - 4, -100), 126);
       if (bad) {   // out of the products; rows that see it get NaN through its score
 #pragma unroll
         for (int g = 0; g < G; ++g) s[g] = z[g] = 0.f;
@@ -316,7 +317,6 @@ __device__ __forceinline__ void unpack_side(const dflash_kv4_cache& c, int b, in
     }
   };
   // the block's queries are converted while the first keys and values are on their way
-  query_copy();
   load(0);
   load_scales(0, ns, nz);
   asm volatile("cp.async.wait_group 1;" ::: "memory");
@@ -408,16 +408,6 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_sdpa_tc_kernel(const SdpaArgs
   pdl_wait();
   pdl_trigger();
   const int split = blockIdx.x, bhk = blockIdx.z, b = bhk / a.Hk, hk = bhk % a.Hk, row0 = blockIdx.y * kRows;
-  const int len = a.lengths ? max(a.lengths[b], 0) : a.max_length;
-  const int t_last = (min(row0 + kRows, a.rows) - 1) / a.gqa;
-  // one past the last position any row of this block sees
-  const int hi = min(min(len, a.max_length), len - a.T + t_last + 1);
-  const int tiles_all = hi > 0 ? (hi + kKeys - 1) / kKeys : 0;
-  const int per = (tiles_all + a.splits - 1) / a.splits;
-  const int k0 = split * per * kKeys;
-  const int pairs = max(0, min(tiles_all - split * per, per));                    // 128 keys each
-  const int tiles = (min(pairs * kKeys, hi - k0) + kTile - 1) / kTile;            // 64 keys each; 0 without pairs
-
   // Q: a row per D / 8 lanes, brought to fp16 by a power of two (its largest element to [2^7, 2^8)) in unpack_row's channel order;
   // the scale's sign goes with it, so that scores grow with their products.  Sixteen warps, every sixteenth row each.
   constexpr int kLanes = D / 8, kPer = 32 / kLanes, kSteps = kRows / (kIssuer * kPer);
@@ -434,9 +424,19 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_sdpa_tc_kernel(const SdpaArgs
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
+  if (warp < kIssuer) query_copy();   // the length, which everything below needs, is on its way meanwhile
+  const int len = a.lengths ? max(a.lengths[b], 0) : a.max_length;
+  const int t_last = (min(row0 + kRows, a.rows) - 1) / a.gqa;
+  // one past the last position any row of this block sees
+  const int hi = min(min(len, a.max_length), len - a.T + t_last + 1);
+  const int tiles_all = hi > 0 ? (hi + kKeys - 1) / kKeys : 0;
+  const int per = (tiles_all + a.splits - 1) / a.splits;
+  const int k0 = split * per * kKeys;
+  const int pairs = max(0, min(tiles_all - split * per, per));                    // 128 keys each
+  const int tiles = (min(pairs * kKeys, hi - k0) + kTile - 1) / kTile;            // 64 keys each; 0 without pairs
   auto query_rows = [&]() {   // once they have landed; a lane reads what it copied itself
     const int j = lane % kLanes;
-#pragma unroll 1
+#pragma unroll 2
     for (int i = 0; i < kSteps; ++i) {
       const int r = (i * kIssuer + warp) * kPer + lane / kLanes;
       uint4* place = (uint4*)(sQ + (j >> 3) * kSlab + r * 128 + (((j & 7) ^ (r & 7)) << 4));
@@ -469,9 +469,9 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_sdpa_tc_kernel(const SdpaArgs
   };
 
   if (warp >= kKeyWarp && warp < kValueWarp) {
-    unpack_side<T, D, false>(a.k, b, hk, k0, hi, pairs, sK, sRaw, bar0, meta, err, query_copy, query_rows);
+    unpack_side<T, D, false>(a.k, b, hk, k0, hi, pairs, sK, sRaw, bar0, meta, err, query_rows);
   } else if (warp >= kValueWarp && warp < kIssuer) {
-    unpack_side<T, D, true>(a.v, b, hk, k0, hi, pairs, sV, sRaw + kKeys * D / 2, bar0, meta, err, query_copy, query_rows);
+    unpack_side<T, D, true>(a.v, b, hk, k0, hi, pairs, sV, sRaw + kKeys * D / 2, bar0, meta, err, query_rows);
   } else if (warp == kIssuer) {
     // ---------------- scores ----------------
     if (lane == 0) {
@@ -522,7 +522,6 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_sdpa_tc_kernel(const SdpaArgs
     const bool live = row0 + part * 32 < a.rows;
     const uint32_t lanes = (uint32_t)(part * 32) << 16;
     const int t = row_ok ? row / a.gqa : 0, h = hk * a.gqa + (row_ok ? row % a.gqa : 0);
-    query_copy();
     asm volatile("cp.async.wait_group 0;" ::: "memory");
     query_rows();
     bool ok = wait_warp(bar0 + 8 * kBarQ, 0);
@@ -597,7 +596,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_sdpa_tc_kernel(const SdpaArgs
       const int ev0 = mt.v_exp[blk], ev1 = mt.v_exp[blk + 1], ev_tile = max(ev0, ev1);
       if (__any_sync(0xffffffffu, top > m + kMaxStep) || ev_tile > ev) {
         const float m_new = fmaxf(m, top);
-        const int ev_new = max(ev, ev_tile);
+        // two octaves of room: the exponents of a sequence's blocks differ by one or two, and each growth rescales O
+        const int ev_new = ev_tile > ev ? ev_tile + 2 : ev;
         const float f = m_new == -INFINITY ? 1.f : ex2((m - m_new) * kLog2e);
         const float fo = f * pow2(max(ev - ev_new, -126));
         m = m_new;
