@@ -192,7 +192,8 @@ __global__ void __launch_bounds__(kThreads, 3) token_logprobs_kernel(const Args 
   const int vecs = (skew + a.V + kPer - 1) / kPer;
   const int share = (vecs + blocks - 1) / blocks;
   const int v0 = me * share, v1 = min(vecs, v0 + share);
-  Sums sums = {-INFINITY, 0.f, 0.f};
+  Sums sums = {-INFINITY, 0.f, 0.f}, run = sums;   // run: of the passes that can_clamp, relative to run.m, which `at` stands for
+  float at = 0.f;
   if (tid < kMaxK) sh.top[tid] = 0;
   if (tid == 0) sh.count = 0;
   const bool packed = a.suppress != nullptr && skew == 0 && ((uintptr_t)a.suppress & (kPer - 1)) == 0;
@@ -249,44 +250,51 @@ __global__ void __launch_bounds__(kThreads, 3) token_logprobs_kernel(const Args 
       }
     }
     if (base + kThreads * kSlots < v1) load(base + kThreads * kSlots, next);   // in flight under this pass
-    Sums mine = {E::max_of(raw), 0.f, 0.f};
-    const float ref = mine.m == -INFINITY ? 0.f : mine.m, top = ref * a.scale;
-    float l0 = 0.f, l1 = 0.f, w0 = 0.f, w1 = 0.f;
-    if (E::can_clamp(mine.m, a.scale)) {   // hidden elements become a finite value of probability 0, two at a time
+    const float top = E::max_of(raw);   // of this pass's elements; NaN is passed over
+    bool nan = false;                   // whether an element was NaN or +inf
+    if (E::can_clamp(top, a.scale) && run.m < 1e30f) {   // hidden elements become a finite value of probability 0, two at a time
+      if (top > run.m) {                // the thread's reference moves: y' = x scale - at, at = rounded(reference scale)
+        const float to = top * a.scale, d = run.m == -INFINITY ? 0.f : at - to, f = exp2f(d);
+        run.w = fmaf(d, run.l, run.w) * f;
+        run.l *= f;
+        run.m = top;
+        at = to;
+      }
+      float l0 = run.l, l1 = 0.f, w0 = run.w, w1 = 0.f;
 #pragma unroll
       for (int i = 0; i < 4 * kSlots; ++i) {
         float x0, x1;
         E::two(E::clamped(raw[i >> 2][i & 3]), x0, x1);
-        const float y0 = fmaf(x0, a.scale, -top), y1 = fmaf(x1, a.scale, -top);
+        const float y0 = fmaf(x0, a.scale, -at), y1 = fmaf(x1, a.scale, -at);
         const float p0 = exp2f(y0), p1 = exp2f(y1);
         l0 += p0;
         l1 += p1;
         w0 = fmaf(y0, p0, w0);
         w1 = fmaf(y1, p1, w1);
       }
-      // y was taken from the rounded product: back to the exact one
-      const float off = fmaf(ref, a.scale, -top), z = off * 0.6931471805599453f;
-      const float f = fabsf(z) < 0.01f ? fmaf(z, fmaf(z, 0.5f, -1.f), 1.f) : exp2f(-off);
-      mine.l = (l0 + l1) * f;
-      mine.w = fmaf(-off, l0 + l1, w0 + w1) * f;
+      run.l = l0 + l1;
+      run.w = w0 + w1;
+      nan = !(run.l == run.l);
     } else {
+      Sums mine = {top, 0.f, 0.f};
+      const float ref = top == -INFINITY ? 0.f : top;
 #pragma unroll
       for (int s = 0; s < kSlots; ++s)
 #pragma unroll
         for (int e = 0; e < kPer; ++e) {
           const float y = (E::get(raw[s], e) - ref) * a.scale;
           const float p = exp2f(y);
-          l0 += p;
-          w0 = fmaf(fmaxf(y, -1e30f), p, w0);   // a hidden element adds 0, not -inf * 0; NaN stays through p
+          mine.l += p;
+          mine.w = fmaf(fmaxf(y, -1e30f), p, mine.w);   // a hidden element adds 0, not -inf * 0; NaN stays through p
         }
-      mine.l = l0;
-      mine.w = w0;
+      nan = !(mine.l == mine.l);
+      sums = merge(sums, mine, a.scale);
     }
     if (a.k > 0) {
       // ---- candidates of this pass ----
       const bool first = base == v0;
       if (first) {   // everything >= the k-th largest group maximum
-        float g = mine.m;
+        float g = top;
 #pragma unroll
         for (int o = 1; o < kThreads / kGroups; o <<= 1) g = fmaxf(g, __shfl_xor_sync(0xffffffffu, g, o));
         if ((lane & (kThreads / kGroups - 1)) == 0) sh.group_max[tid / (kThreads / kGroups)] = g;
@@ -304,7 +312,7 @@ __global__ void __launch_bounds__(kThreads, 3) token_logprobs_kernel(const Args 
       }
       const float tau = sh.tau;
       // NaN elements count as the largest; a thread whose own maximum does not reach tau can only hold NaN beyond it
-      const bool has = (first ? mine.m >= tau : !(mine.m <= tau)) || !(mine.l == mine.l);
+      const bool has = (first ? top >= tau : !(top <= tau)) || nan;
       if (has) {
         uint32_t hits = 0;
 #pragma unroll
@@ -327,10 +335,7 @@ __global__ void __launch_bounds__(kThreads, 3) token_logprobs_kernel(const Args 
         }
       }
       const int pass = (base - v0) / (kThreads * kSlots) + 1;
-      if (!careful && ((pass & (pass - 1)) != 0 || (pass & 0x2AAAAAAA) != 0) && base + kThreads * kSlots < v1) {
-        sums = merge(sums, mine, a.scale);
-        continue;
-      }
+      if (!careful && ((pass & (pass - 1)) != 0 || (pass & 0x2AAAAAAA) != 0) && base + kThreads * kSlots < v1) continue;
       __syncthreads();
       const int n = sh.count;
       if (n > kList - kMaxK && !careful && !first) {   // over several passes: once more, ranking after each
@@ -338,7 +343,8 @@ __global__ void __launch_bounds__(kThreads, 3) token_logprobs_kernel(const Args 
         careful = true;
         if (tid < kMaxK) sh.top[tid] = 0;
         if (tid == 0) sh.count = 0;
-        sums = {-INFINITY, 0.f, 0.f};
+        sums = run = {-INFINITY, 0.f, 0.f};
+        at = 0.f;
         base = v0 - kThreads * kSlots;
         load(v0, next);
         continue;
@@ -427,7 +433,13 @@ __global__ void __launch_bounds__(kThreads, 3) token_logprobs_kernel(const Args 
       }
       __syncthreads();
     }
-    sums = merge(sums, mine, a.scale);
+  }
+  if (run.m != -INFINITY) {   // y' was taken from the rounded product: back to the exact one
+    const float off = fmaf(run.m, a.scale, -at), z = off * 0.6931471805599453f;
+    const float f = fabsf(z) < 0.01f ? fmaf(z, fmaf(z, 0.5f, -1.f), 1.f) : exp2f(-off);
+    run.w = fmaf(-off, run.l, run.w) * f;
+    run.l *= f;
+    sums = merge(sums, run, a.scale);
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) sums = merge_lanes(sums, o, a.scale);
