@@ -21,7 +21,8 @@ constexpr float kLog2e = 1.4426950408889634f;
 // ---- write -------------------------------------------------------------------------------------------------------------
 // A lane owns the eight channels of one word, eight lanes a group: minimum and maximum in three shuffles, no shared memory.
 // Bound by HBM and instruction issue (prompts) or by the launch (single tokens): a warp has its next row on the way under the
-// current one, in a rolled loop (eight rows unrolled missed the instruction cache).  blockIdx.x is (sequence, head), so no lane
+// current one, in a rolled loop (eight rows unrolled missed the instruction cache: 21 us for 2 x 4133 rows of 4 heads x 256, 18 now; its
+// HBM floor is 7).  One token: 1.5 us.  blockIdx.x is (sequence, head), so no lane
 // divides.
 struct WriteArgs {
   const void* x[2];
@@ -136,7 +137,7 @@ struct ReadArgs {
   int start, Hk, T, capacity;
 };
 
-// The same split as the write: a lane unpacks one word into 16 bytes of output.
+// The same split as the write: a lane unpacks one word into 16 bytes of output.  65537 rows of 4 heads x 256: 57 us, 6.0 TB/s.
 template <typename T, int D, int kRows>
 __global__ void __launch_bounds__(128) kv4_read_kernel(const ReadArgs a) {
   using TR = MmaTraits<T>;
@@ -204,6 +205,8 @@ __global__ void __launch_bounds__(128) kv4_read_kernel(const ReadArgs a) {
 // down to 2^-28 of the row's largest element.
 // The running maximum moves only when a score exceeds it by 8 octaves (p <= 256 otherwise), so the accumulators are rarely
 // rescaled.  The warps of a block and then the splits of the key range are merged with fp32 partials.
+// Measured (D = 256, bf16): 8 rows, 16 ragged sequences up to 32768: 68 us, 3.0 TB/s, at 75 % of the issue slots; 6 rows over 4097
+// positions: 9.1 us with the combine.
 // Warps of a block.  Two blocks share an SM, so that one starts or merges while the other streams; as many warps as the registers
 // allow (the loop is bound by instruction issue: unpacking, scales and softmax next to the MMAs).
 constexpr int kStages = 3;   // tiles of a warp in shared memory
@@ -838,7 +841,7 @@ bool aligned_rows(const void* p, const long long* s) {
   return !((uintptr_t)p & 15) && s[0] % 8 == 0 && s[1] % 8 == 0 && s[2] % 8 == 0;
 }
 
-// Rows of a warp at once: one while the blocks do not fill the SMs (latency), more for long inputs (loads in flight).
+// Steps of a warp: one while the blocks do not fill the SMs (latency), more for long inputs (the next rows' loads in flight).
 constexpr int kManyRows = 8;
 // Grid of a write or read: (sequence, head) x blocks of rows x sides; true: kManyRows rows a warp.
 bool row_grid(int B, int Hk, int T, int D, int sides, int device, dim3* grid) {

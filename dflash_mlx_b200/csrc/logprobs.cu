@@ -14,9 +14,10 @@
 // ranking after every pass; when one pass alone collects more than the list holds (a row of equal values, sorted logits) the top_k-th largest key is
 // found bit by bit.
 //
-// One row per thread-block cluster: every block keeps its share of the row in registers (16-byte loads, all issued before the
-// first is used), the first block merges the triples and the blocks' lists through distributed shared memory.  Bound by HBM
-// for many rows; one row is bound by the launch, one memory round trip and the merges.
+// One row per thread-block cluster: one block a row when rows alone fill the SMs, up to eight otherwise, whose triples and lists the
+// first block merges through distributed shared memory.  Measured (bf16, 151936 logits): 1999 rows with suppressed tokens and 5
+// alternatives 210 us (2.9 TB/s; bound by instruction issue and the exponentials, HBM floor 93), 16 rows with 20 alternatives 16.7 us
+// (latency: passes, ranking, cluster merge).
 #include <cooperative_groups.h>
 
 #include <mutex>
