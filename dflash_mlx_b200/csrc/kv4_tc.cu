@@ -47,6 +47,7 @@ struct Meta {
   int v_exp[4];
   uint32_t bad[4];
 };
+constexpr int kOdd = 1024;
 constexpr int kMeta = 4;   // scales are looked at no more than three tiles ahead of the softmax
 
 // mbarriers, 8 bytes each.  kBarKEmpty: per slab; V full and empty: per half of the buffer (64 keys); kBarS: per pair of score tiles;
@@ -167,30 +168,83 @@ __device__ __forceinline__ uint32_t splat(float x) {
   const __half2 h = __float2half2_rn(x);
   return *(const uint32_t*)&h;
 }
-// Bit e: byte mask entry of key n0 + e is not 0, for the bits set in `want` (others are not read).
-__device__ __forceinline__ uint32_t mask_bits(const SdpaArgs& a, long long at, int n0, uint32_t want) {
-  const uint8_t* p = (const uint8_t*)a.mask + at + (long long)n0 * a.m_sn;
-  uint32_t bits = 0;
-  if (want == 0xFFFFFFFFu && a.m_sn == 1 && ((uintptr_t)p & 3) == 0) {
+// kWords words of a mask row from byte `from` on, whatever its alignment: aligned 16-byte loads, all in flight at once, then shifted
+// into place (3 instructions a word).  A lane's row is its own, so narrower loads would cost a line of the L1 each.  Words from `end`
+// on are 0.  What an aligned word holds besides bytes of the row (never used) lies in the row's allocation too; a branch for
+// it would make the loads wait for one another.
+template <int kWords>
+__device__ __forceinline__ void mask_words(const uint8_t* row, long long from, long long end, bool want, uint32_t (&w)[kWords + 4]) {
+  const uint8_t* p = row + from;
+  const int s = (int)((uintptr_t)p & 15);
+  const int left = want ? (int)min(end - from + s, (long long)(4 * kWords + 16)) : 0;   // bytes of the row from the first aligned word on
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      uint32_t x = *(const uint32_t*)(p + 4 * i);
-      x = __vcmpne4(x, 0) & 0x08040201u;              // a bit of its own per byte
-      bits |= (((x * 0x01010101u) >> 24) & 15u) << (4 * i);
-    }
-  } else if (want) {
-#pragma unroll 8
-    for (int e = 0; e < 32; ++e)
-      if ((want >> e) & 1) bits |= (uint32_t)(p[e * a.m_sn] != 0) << e;
+  for (int i = 0; i <= kWords; i += 4) {
+    uint4 x = make_uint4(0, 0, 0, 0);
+    if (4 * i < left && (i < kWords || s != 0)) x = *(const uint4*)(p - s + 4 * i);
+    w[i] = x.x; w[i + 1] = x.y; w[i + 2] = x.z; w[i + 3] = x.w;
   }
-  return bits;
+#pragma unroll
+  for (int i = 0; i < kWords + 2; ++i) w[i] = (s & 8) ? w[i + 2] : w[i];
+#pragma unroll
+  for (int i = 0; i < kWords + 1; ++i) w[i] = (s & 4) ? w[i + 1] : w[i];
+#pragma unroll
+  for (int i = 0; i < kWords; ++i) w[i] = __funnelshift_r(w[i], w[i + 1], 8 * (s & 3));
 }
-// Keys n0 .. n0 + 31 that a row sees: up to `lim`, and where a byte mask lets it.
-template <int kMask>
-__device__ __forceinline__ uint32_t seen_bits(const SdpaArgs& a, long long at, int n0, int lim) {
+// Bit e of word q: the byte mask's entry of key n0 + 32 q + e is not 0, for the keys up to `lim` (from `end` on none is read).
+// `shared`: the warp's rows have one mask row, which its lanes read together.
+__device__ __forceinline__ void mask_bits(const SdpaArgs& a, long long mat, bool shared, int n0, int lim, int end, uint32_t (&bits)[2]) {
+  const uint8_t* row = (const uint8_t*)a.mask + mat;
+  bits[0] = bits[1] = 0;
+  if (shared) {
+    const int n = n0 + (threadIdx.x & 31);
+    const uint8_t x0 = n < end ? row[n * a.m_sn] : 0, x1 = n + 32 < end ? row[(n + 32) * a.m_sn] : 0;
+    bits[0] = __ballot_sync(0xffffffffu, x0 != 0);
+    bits[1] = __ballot_sync(0xffffffffu, x1 != 0);
+  } else if (a.m_sn == 1) {
+    uint32_t w[kTile / 4 + 4], zero = 0;
+    mask_words<kTile / 4>(row, n0, a.max_length, lim >= n0, w);
+#pragma unroll
+    for (int i = 0; i < kTile / 4; ++i) zero |= (w[i] - 0x01010101u) & ~w[i];
+    if (__all_sync(0xffffffffu, (zero & 0x80808080u) == 0)) {   // no zero byte anywhere
+      bits[0] = bits[1] = 0xFFFFFFFFu;
+    } else {
+#pragma unroll
+      for (int i = 0; i < kTile / 4; ++i) {
+        const uint32_t x = __vcmpne4(w[i], 0) & 0x08040201u;   // a bit of its own per byte
+        bits[i >> 3] |= (((x * 0x01010101u) >> 24) & 15u) << (4 * (i & 7));
+      }
+    }
+  } else {
+#pragma unroll 8
+    for (int e = 0; e < kTile; ++e)
+      if (n0 + e <= lim && row[(n0 + e) * a.m_sn] != 0) bits[e >> 5] |= 1u << (e & 31);
+  }
+}
+// Entries of keys n0 .. of an additive mask of type E as they lie in memory, as many as fit kWords; behind `lim` anything.
+template <typename E, int kWords>
+__device__ __forceinline__ void mask_entries(const SdpaArgs& a, long long mat, int n0, int lim, uint32_t (&w)[kWords + 4]) {
+  constexpr int kPer = 4 / (int)sizeof(E);
+  const E* row = (const E*)a.mask + mat;
+  if (a.m_sn == 1) {
+    mask_words<kWords>((const uint8_t*)row, (long long)n0 * sizeof(E), (long long)a.max_length * sizeof(E), lim >= n0, w);
+  } else {
+#pragma unroll
+    for (int i = 0; i < kWords; ++i) {
+      w[i] = 0;
+#pragma unroll
+      for (int e = 0; e < kPer; ++e) {
+        const int n = n0 + i * kPer + e;
+        if (n > lim) continue;
+        if (sizeof(E) == 4) w[i] = ((const uint32_t*)row)[n * a.m_sn];
+        else w[i] |= (uint32_t)((const uint16_t*)row)[n * a.m_sn] << (16 * e);
+      }
+    }
+  }
+}
+// Keys n0 .. n0 + 31 that a row sees, without a mask: up to `lim`.
+__device__ __forceinline__ uint32_t seen_bits(int n0, int lim) {
   const int left = lim - n0;   // below 0: none, from 31: all
-  const uint32_t seen = left < 0 ? 0u : left >= 31 ? 0xFFFFFFFFu : (2u << left) - 1u;
-  return kMask == 1 ? mask_bits(a, at, n0, seen) : seen;
+  return left < 0 ? 0u : left >= 31 ? 0xFFFFFFFFu : (2u << left) - 1u;
 }
 // Per half, the larger magnitude of two pairs (the sign bits are to be ignored).
 template <typename T> __device__ __forceinline__ uint32_t abs_max(uint32_t x, uint32_t y);
@@ -365,7 +419,7 @@ __device__ __forceinline__ void unpack_side(const dflash_kv4_cache& c, int b, in
   asm volatile("cp.async.wait_group 0;" ::: "memory");
 }
 
-template <typename T, int D, int kMask>   // 0 = no mask, 1 = bytes, 2 = additive
+template <typename T, int D, int kMask>   // 0 = no mask, 1 = bytes, 2 = additive in T, 3 = additive in fp32
 __global__ void __launch_bounds__(kThreads, 1) kv4_sdpa_tc_kernel(const SdpaArgs a, int* __restrict__ err) {
   using TR = MmaTraits<T>;
   constexpr int G = D / kGroup;
@@ -376,7 +430,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_sdpa_tc_kernel(const SdpaArgs
   uint8_t* sRaw = sV + G * kSlab;                 // codes of the next tile: keys, then values
   uint64_t* bars = (uint64_t*)(sRaw + kKeys * D);
   Meta* meta = (Meta*)(bars + kBars);
-  int* sE = (int*)(meta + kMeta);                 // exponent of each query row
+  int* sE = (int*)(meta + kMeta);                 // exponent of each query row, + kOdd if the row is not finite
   float* sRef = (float*)(sE + kRows);             // [2][128] reference maximum of a row after a tile
   int* sEv = (int*)(sRef + 2 * kRows);            // [2][4] exponent that O carries
   uint32_t* holder = (uint32_t*)(sEv + 8);
@@ -457,14 +511,17 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_sdpa_tc_kernel(const SdpaArgs
       const int eq = min(max((int)(top >> 23) - 127 - 7, -100), 126);
       const float to_q = a.scale < 0.f ? -pow2(-eq) : pow2(-eq);
       uint32_t p[4];
+      float odd = 0.f;   // NaN if an element is not finite
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const float f0 = TR::bits_to_float((uint16_t)(u[e >> 1] >> (16 * (e & 1)))), f1 = TR::bits_to_float((uint16_t)(u[2 + (e >> 1)] >> (16 * (e & 1))));
         const __half2 hh = __floats2half2_rn(f0 * to_q, f1 * to_q);
+        odd = fmaf(f0, 0.f, fmaf(f1, 0.f, odd));
         p[e] = *(const uint32_t*)&hh;
       }
       *place = make_uint4(p[0], p[1], p[2], p[3]);
-      if (j == 0) sE[r] = eq;
+      const bool is_odd = (__ballot_sync(0xffffffffu, odd != 0.f) >> (lane & ~(kLanes - 1)) & (0xFFFFFFFFu >> (32 - kLanes))) != 0;
+      if (j == 0) sE[r] = is_odd ? eq + kOdd : eq;
     }
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     __syncwarp();
@@ -529,12 +586,23 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_sdpa_tc_kernel(const SdpaArgs
     query_rows();
     bool ok = wait_warp(bar0 + 8 * kBarQ, 0);
     if (!ok) atomicCAS(err, 0, 62 | (10 << 8));
-    const float c_row = fabsf(a.scale) * pow2(sE[r]);
+    const int eq = sE[r];
+    const float c_row = fabsf(a.scale) * pow2(eq >= kOdd / 2 ? eq - kOdd : eq);
+    const bool odd = __any_sync(0xffffffffu, eq >= kOdd / 2);
     // last key the row sees; rows behind the last one compute what nobody reads
-    const int lim = row_ok ? min(len - a.T + t, hi - 1) : (kMask ? -1 : 0x7FFFFFFF);
-    const long long mat = kMask && row_ok ? b * a.m_sb + h * a.m_sh + t * a.m_st : 0;
+    const int lim = row_ok ? min(len - a.T + t, hi - 1) : live ? hi - 1 : -1;
+    long long mat = row_ok ? b * a.m_sb + h * a.m_sh + t * a.m_st : 0;   // its mask row, or that of the warp's first row
+    const long long mat0 = __shfl_sync(0xffffffffu, mat, 0);
+    if (!row_ok) mat = mat0;
+    const bool shared = kMask == 1 && __all_sync(0xffffffffu, mat == mat0);
     float m_l = -INFINITY, l = 0.f;   // this half's sum and the reference it is relative to
     for (int i = group; i < tiles && ok; i += 2) {
+      const int n0 = k0 + i * kTile;
+      uint32_t bits[2];                  // the mask, on its way before the scores are waited for (fp32: below)
+      uint32_t words[(kMask == 3 ? 16 : kTile / 2) + 4];
+      if constexpr (kMask == 1) mask_bits(a, mat, shared, n0, lim, hi, bits);
+      if constexpr (kMask == 2) mask_entries<T, kTile / 2>(a, mat, n0, lim, words);
+      if constexpr (kMask == 3) mask_entries<float, 16>(a, mat, n0, lim, words);
       if (!wait_warp(bar0 + 8 * (kBarS + ((i >> 1) & 1)), (i >> 2) & 1)) { atomicCAS(err, 0, 62 | (6 << 8)); ok = false; break; }
       fence_after();
       if (!live) {   // P is whatever is there: lanes of their own
@@ -546,29 +614,43 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_sdpa_tc_kernel(const SdpaArgs
       const uint32_t s_col = tmem + lanes + 64u * (i & 3);
       const Meta& mt = meta[(i >> 1) & (kMeta - 1)];
       const int blk = 2 * (i & 1);   // the tile's 32-key blocks in `mt`: blk and blk + 1
-      const int n0 = k0 + i * kTile;
+      // never 0 (a scale of 0): a hidden score stays -inf under it
+      float c[2] = {fmaxf(c_row * mt.k_factor[blk], 1e-37f), fmaxf(c_row * mt.k_factor[blk + 1], 1e-37f)};
+      if (kMask >= 2) {   // scaled score + mask back into place, 16 at a time: with the entries, all 64 would not fit the registers
+        const bool careful = odd || __any_sync(0xffffffffu, c[0] > 3e38f || c[1] > 3e38f);
+#pragma unroll
+        for (int e0 = 0; e0 < kTile; e0 += 16) {
+          uint32_t x[16];
+          ld16(s_col + e0, x);
+          if constexpr (kMask == 3) if (e0) mask_entries<float, 16>(a, mat, n0 + e0, lim, words);
+          wait_ld();
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            const float y = kMask == 3 ? __uint_as_float(words[e]) : TR::bits_to_float((uint16_t)(words[((e0 + e) >> 1) & 31] >> (16 * (e & 1))));
+            if (careful && y == -INFINITY) x[e] = 0;   // a hidden key stays hidden under a score that is not finite
+            x[e] = __float_as_uint(fmaf(__uint_as_float(x[e]), c[e0 >> 5], y));
+          }
+          st16(s_col + e0, x);
+        }
+        c[0] = c[1] = 1.f;
+        wait_st();
+      }
       uint32_t v[kTile];
       ld32(s_col, v);
       ld32(s_col + 32, v + 32);
-      // never 0 (a scale of 0): a hidden score stays -inf under it
-      float c[2] = {fmaxf(c_row * mt.k_factor[blk], 1e-37f), fmaxf(c_row * mt.k_factor[blk + 1], 1e-37f)};
-      // every key of the tile seen by every row of the warp, and no mask
-      const bool plain = !kMask && __all_sync(0xffffffffu, n0 + kTile - 1 <= lim);
+      // every key of the tile seen by every row of the warp (additive masks aside)
+      const bool plain = __all_sync(0xffffffffu, n0 + kTile - 1 <= lim && (kMask != 1 || (bits[0] & bits[1]) == 0xFFFFFFFFu));
       if (!wait_warp(bar0 + 8 * (kBarVMeta + ((i >> 1) & (kMeta - 1))), (i / (2 * kMeta)) & 1)) { atomicCAS(err, 0, 62 | (13 << 8)); ok = false; }
       wait_ld();
       if (!ok) break;
       if (!plain) {
 #pragma unroll
         for (int q = 0; q < 2; ++q) {
-          const uint32_t seen = seen_bits<kMask>(a, mat, n0 + 32 * q, lim);
+          uint32_t seen = seen_bits(n0 + 32 * q, lim);
+          if (kMask == 1) seen &= bits[q];
 #pragma unroll
-          for (int e = 0; e < 32; ++e) {
-            if (kMask == 2) {
-              if ((seen >> e) & 1) v[32 * q + e] = __float_as_uint(apply_mask<T>(a, __uint_as_float(v[32 * q + e]) * c[q], mat + (n0 + 32 * q + e) * a.m_sn));
-            }
+          for (int e = 0; e < 32; ++e)
             if (!((seen >> e) & 1)) v[32 * q + e] = 0xFF800000u;
-          }
-          if (kMask == 2) c[q] = 1.f;
         }
       }
       if ((mt.bad[blk] | mt.bad[blk + 1]) != 0) {   // a value that is not finite makes the rows NaN that see its key
@@ -642,7 +724,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_sdpa_tc_kernel(const SdpaArgs
 #pragma unroll
           for (int e = 0; e < 16; e += 2) {
             float p0, p1;
-            if (kMask == 2) {   // scores may be the lowest finite value: their difference first
+            if (kMask >= 2) {   // scores may be the lowest finite value: their difference first
               p0 = fmaf(__uint_as_float(v[e0 + e]) - ref, kLog2e, shift);
               p1 = fmaf(__uint_as_float(v[e0 + e + 1]) - ref, kLog2e, shift);
             } else {
@@ -742,10 +824,11 @@ int launch(const SdpaArgs& a, cudaStream_t st, int device) {
   static_assert(kRows * (D * 4 + 16) <= tiles, "the epilogue's rows fit where Q, K and V were");
   constexpr size_t smem = tiles + rest;
   static_assert(smem <= 227 * 1024, "shared memory");
-  const int mask = a.mask_kind == 0 ? 0 : a.mask_kind == 1 ? 1 : 2;
-  auto kern = mask == 0 ? kv4_sdpa_tc_kernel<T, D, 0> : mask == 1 ? kv4_sdpa_tc_kernel<T, D, 1> : kv4_sdpa_tc_kernel<T, D, 2>;
+  const int mask = a.mask_kind;   // 0 .. 3
+  auto kern = mask == 0 ? kv4_sdpa_tc_kernel<T, D, 0> : mask == 1 ? kv4_sdpa_tc_kernel<T, D, 1> :
+              mask == 2 ? kv4_sdpa_tc_kernel<T, D, 2> : kv4_sdpa_tc_kernel<T, D, 3>;
   static std::mutex mu;
-  static bool done[64][3] = {};
+  static bool done[64][4] = {};
   {
     std::lock_guard<std::mutex> lk(mu);
     bool& d = done[device & 63][mask];
