@@ -6,8 +6,8 @@ import torch
 
 pytestmark = pytest.mark.gpu
 
-from dflash_mlx_b200 import _lib, quantized_kv as qkv  # noqa: E402
-from oracle import quantized_kv as ref  # noqa: E402
+from dflash_mlx_b200 import _lib, logprobs, quantized_kv as qkv  # noqa: E402
+from oracle import logprobs as ref_logprobs, quantized_kv as ref  # noqa: E402
 
 DEV = "cuda"
 TYPES = [torch.bfloat16, torch.float16]
@@ -243,6 +243,49 @@ def test_attention_masks(shape, kind, T):
         assert not bool(got[0, 1, 0].any())
 
 
+@pytest.mark.parametrize("T", [5, 40])
+@pytest.mark.parametrize("kind", ["bool", "type", "f32"])
+def test_attention_mask_alignment(kind, T):
+    """A mask's place in memory changes nothing, nor does what lies around it."""
+    B, Hq, Hk, D, n, dtype = 2, 5, 1, 128, 203, torch.bfloat16
+    k, v = make_cache(B, Hk, n, D, dtype)
+    q, scale = states((B, Hq, T, D), dtype, 9), D ** -0.5
+    keep = torch.rand(B, Hq, T, n, generator=gen(3), device=DEV) < 0.7
+    mask, around = keep, True
+    if kind != "bool":
+        mask = torch.where(keep, torch.randn(keep.shape, generator=gen(4), device=DEV), -math.inf).to(dtype if kind == "type" else torch.float32)
+        around = math.nan
+    want = qkv.quantized_kv_sdpa(q, k, v, scale, ints(n, n - 70), mask)
+    check_rows(want, ref.sdpa(q, k, v, scale, [n, n - 70], mask), dtype)
+    for off in [*range(17), 31]:
+        wide = torch.full((B, Hq, T, off + n + off % 3), around, dtype=mask.dtype, device=DEV)
+        wide[..., off:off + n] = mask
+        assert torch.equal(qkv.quantized_kv_sdpa(q, k, v, scale, ints(n, n - 70), wide[..., off:off + n]), want), off
+    for turned in (mask.transpose(-1, -2).contiguous().transpose(-1, -2), mask.repeat_interleave(2, -1)[..., ::2]):
+        assert torch.equal(qkv.quantized_kv_sdpa(q, k, v, scale, ints(n, n - 70), turned), want)
+
+
+@pytest.mark.parametrize("T", [3, 40])
+@pytest.mark.parametrize("kind", ["bool", "type", "f32"])
+@pytest.mark.parametrize("odd", [math.nan, math.inf, -math.inf])
+def test_attention_queries_that_are_not_finite(odd, kind, T):
+    """They make their own row NaN, unless its mask leaves nothing: then it is zero like any other."""
+    B, Hq, Hk, D, n, dtype = 1, 4, 1, 128, 100, torch.bfloat16
+    k, v = make_cache(B, Hk, n, D, dtype)
+    q, scale = states((B, Hq, T, D), dtype, 9), D ** -0.5
+    keep = torch.ones(B, Hq, T, n, dtype=torch.bool, device=DEV)
+    keep[0, 1, 1] = False
+    keep[0, 2, 2, 40:] = False
+    mask = keep if kind == "bool" else torch.where(keep, 0.5, -math.inf).to(dtype if kind == "type" else torch.float32)
+    want = qkv.quantized_kv_sdpa(q, k, v, scale, n, mask)
+    q[0, 1, 1, 5] = q[0, 2, 2, 77] = odd
+    got = qkv.quantized_kv_sdpa(q, k, v, scale, n, mask)
+    assert not bool(want[0, 1, 1].any()) and not bool(got[0, 1, 1].any())
+    assert bool(got[0, 2, 2].isnan().all())
+    got[0, 2, 2] = want[0, 2, 2]
+    assert torch.equal(got, want)
+
+
 @pytest.mark.parametrize("T", [2, 40])
 def test_attention_lowest_finite_mask(T):
     """The type's lowest value is a number: a row that has nothing else is the mean of what it may see."""
@@ -474,6 +517,56 @@ def test_cache_runs_prompt_verify_rollback_and_tokens():
     n = int(at.min())
     assert torch.equal(cache.read(0, n)[0], ref.values(*ref.quantise(dense_k[:, :, :n]), torch.float32).to(dtype))
     assert kept
+
+
+def test_verify_cycle_with_token_probabilities():
+    """What a server runs per cycle, captured once: the block's keys and values enter the cache, its rows attend, a head makes
+    logits, the drafted tokens' log-probabilities decide how many are accepted, and the positions move on, all on the device."""
+    B, Hq, Hk, D, T, V, dtype = 2, 8, 2, 128, 16, 3001, torch.bfloat16
+    head = states((V, Hq * D), dtype, 1, 0.2)
+    cache = qkv.QuantizedKVCache(B, Hk, 400, D, dtype=dtype)
+    prompt = [states((B, h, 300, D), dtype, 2 + i) for i, h in enumerate((Hk, Hk))]
+    cache.update(*prompt)
+    cache.commit(300)
+    q, k, v = states((B, Hq, T, D), dtype, 5), states((B, Hk, T, D), dtype, 6), states((B, Hk, T, D), dtype, 7)
+    drafted = torch.randint(0, V, (B, T), generator=gen(8), device=DEV)
+    threshold = torch.zeros(B, T, device=DEV)
+
+    def cycle():
+        cache.update(k, v)
+        rows = cache.attend(q, D ** -0.5)
+        logits = rows.transpose(1, 2).reshape(B, T, Hq * D) @ head.T
+        lp = logprobs.token_logprobs(logits, drafted, top_k=4)
+        accepted = (lp.logprobs >= threshold).to(torch.int32).cumprod(1).sum(1, dtype=torch.int32)
+        cache.commit(accepted)
+        return rows, logits, lp, accepted
+
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        cycle()                                           # a threshold of probability 1 accepts nothing
+    torch.cuda.current_stream().wait_stream(side)
+    assert cache.offsets.tolist() == [300, 300]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        rows, logits, lp, accepted = cycle()
+    dense = [torch.cat([p, torch.zeros(B, Hk, 100, D, dtype=dtype, device=DEV)], 2) for p in prompt]
+    at = [300, 300]
+    for step, counts in enumerate([(16, 3), (0, 16), (5, 1)]):
+        q.copy_(states(q.shape, dtype, 20 + step)); k.copy_(states(k.shape, dtype, 30 + step)); v.copy_(states(v.shape, dtype, 40 + step))
+        for b in range(B):
+            threshold[b] = -math.inf
+            threshold[b, counts[b]:] = 1.0
+            for d, x in zip(dense, (k, v)):
+                d[b, :, at[b]:at[b] + T] = x[b]
+        graph.replay()
+        check_rows(rows, ref.sdpa(q, ref.quantise(dense[0]), ref.quantise(dense[1]), D ** -0.5, [o + T for o in at]), dtype)
+        want = ref_logprobs.token_logprobs(logits.flatten(0, 1), drafted.flatten().cpu(), 4)
+        # fp32 sums of 3001 terms: 5e-6 of the sum and 2^-23 of values up to some tens
+        assert float((lp.logprobs.flatten().cpu().double() - want[0]).abs().max()) < 2e-5
+        assert torch.equal(lp.top_ids.flatten(0, 1).cpu().long(), want[3])
+        assert accepted.tolist() == list(counts)
+        at = [o + c for o, c in zip(at, counts)]
+        assert cache.offsets.tolist() == at
 
 
 def test_refusals_leave_everything_alone():
