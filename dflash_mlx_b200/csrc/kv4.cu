@@ -631,12 +631,13 @@ __global__ void __launch_bounds__((kWarpsOf<D, NT>) * 32, 2) kv4_sdpa_kernel(con
   }
 }
 
+constexpr int kMaxSplits = 1024;
 // out = sum_s w_s O_s / sum_s w_s l_s, w_s = exp(m_s - max m): one block per row.
 template <typename T, int D>
 __global__ void __launch_bounds__(256) kv4_combine_kernel(const SdpaArgs a) {
   using TR = MmaTraits<T>;
   constexpr int kThreads = 256, kPer = kThreads / (D / 4);   // key ranges read side by side
-  __shared__ float sw[1024];
+  __shared__ float sw[kMaxSplits];
   __shared__ float red[kThreads / 32];
   __shared__ float4 part[kPer][D / 4];
   pdl_wait();
@@ -757,7 +758,7 @@ int choose_splits(long long units, int B, int max_length, int device, int reques
   const int sms = per_sm * sm_count(device);   // blocks at a time
   int best = 1;
   double least = 1e300;
-  for (int s = 1; s <= most && s <= 1024 && units * s <= 4ll * sms; ++s) {
+  for (int s = 1; s <= most && s <= kMaxSplits && units * s <= 4ll * sms; ++s) {
     const double keys = (double)max_length / s + kOverhead;
     double cost = (double)((units * s + sms - 1) / sms) * keys;
     if (B > 1) cost = 0.5 * cost + 0.5 * ((double)(units * s) / sms * (0.6 * max_length / s + kOverhead) + 0.5 * keys);
@@ -832,7 +833,7 @@ int check_sizes(const char* who, int B, int Hk, int T, int D, int capacity, int 
   if (D != 128 && D != 256) return fail(DFLASH_ERR_BAD_SHAPE, "%s: D=%d not in {128,256}", who, D);
   if (capacity < 1) return fail(DFLASH_ERR_BAD_SHAPE, "%s: capacity %d", who, capacity);
   if ((long long)B * Hk > 0x7fffffffll) return fail(DFLASH_ERR_BAD_SHAPE, "%s: B*Hk too large", who);
-  if (T > 0x7fffffff - (1 << 20)) return fail(DFLASH_ERR_BAD_SHAPE, "%s: T=%d too large", who, T);
+  if (T > 0x7fffffff - (1 << 23)) return fail(DFLASH_ERR_BAD_SHAPE, "%s: T=%d too large", who, T);
   if (dtype != DFLASH_BF16 && dtype != DFLASH_F16) return fail(DFLASH_ERR_BAD_ARG, "%s: dtype %d (want bf16 or f16)", who, dtype);
   return DFLASH_OK;
 }
@@ -939,7 +940,7 @@ static int kv4_splits(int B, int Hk, long long rows, int max_length, int device,
 }
 
 extern "C" size_t dflash_kv4_sdpa_workspace_bytes(int B, int Hq, int Hk, int T, int D, int max_length, int num_splits) {
-  if (B < 1 || Hq < 1 || Hk < 1 || T < 1 || D < 1 || max_length < 1 || Hq % Hk != 0 || (long long)(Hq / Hk) * T > 0x7fffffffll) return 0;
+  if (B < 1 || Hq < 1 || Hk < 1 || T < 1 || D < 1 || max_length < 1 || num_splits < 0 || num_splits > kMaxSplits || Hq % Hk != 0 || (long long)(Hq / Hk) * T > 0x7fffffffll) return 0;
   int device = 0;
   cudaGetDevice(&device);
   const long long rows = (long long)(Hq / Hk) * T;
@@ -960,6 +961,9 @@ extern "C" int dflash_kv4_sdpa(const void* q, const long long* q_strides, const 
   if (!q || !q_strides || !out) return fail(DFLASH_ERR_BAD_ARG, "kv4_sdpa: null operand");
   if (mask_kind < 0 || mask_kind > 3 || (mask_kind != 0) != (mask != nullptr) || (mask_kind && !mask_strides))
     return fail(DFLASH_ERR_BAD_ARG, "kv4_sdpa: mask and mask_kind %d do not agree", mask_kind);
+  if (num_splits < 0 || num_splits > kMaxSplits) return fail(DFLASH_ERR_BAD_ARG, "kv4_sdpa: num_splits %d outside 0..%d", num_splits, kMaxSplits);
+  const int entry = mask_kind == 1 ? 1 : mask_kind == 2 ? 2 : 4;
+  if (mask && ((uintptr_t)mask & (entry - 1))) return fail(DFLASH_ERR_MISALIGNED, "kv4_sdpa: a mask must be aligned to its elements");
   if ((rc = check_cache("kv4_sdpa", k_cache, D)) || (rc = check_cache("kv4_sdpa", v_cache, D))) return rc;
   if (!aligned_rows(q, q_strides) || ((uintptr_t)out & 15)) return fail(DFLASH_ERR_MISALIGNED, "kv4_sdpa: q and out need 16-byte aligned rows");
   const long long rows = (long long)(Hq / Hk) * T;

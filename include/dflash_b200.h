@@ -428,7 +428,7 @@ DFLASH_API int dflash_kv4_read(const dflash_kv4_cache* k_cache, const dflash_kv4
  *            2 = additive in dtype, 3 = additive f32.  -inf hides; a finite value, however low, is added.
  *   A row that sees nothing yields zeros.  Keys and values that a row does not see never reach it, NaN and infinities
  *   included; a visible value row with a non-finite scale or bias makes the whole output row NaN.
- *   num_splits: 0 = chosen from the SM count.  workspace: dflash_kv4_sdpa_workspace_bytes() bytes of device memory, 16-byte
+ *   num_splits: key ranges, 0..1024; 0 = chosen from the SM count.  workspace: dflash_kv4_sdpa_workspace_bytes() bytes of device memory, 16-byte
  *   aligned, contents irrelevant, not shared by calls that can overlap. */
 DFLASH_API size_t dflash_kv4_sdpa_workspace_bytes(int B, int Hq, int Hk, int T, int D, int max_length, int num_splits);
 DFLASH_API int dflash_kv4_sdpa(const void* q, const long long* q_strides, const dflash_kv4_cache* k_cache,

@@ -131,3 +131,20 @@ def test_c_entries_refuse_before_any_launch():
     assert lib.dflash_kv4_read(ctypes.byref(ok), None, 0x1000, 0x1000, None, 0, 1, 2, 4, 128, 32, 0, None) == -1
     assert lib.dflash_kv4_read(ctypes.byref(ok), ctypes.byref(ok), None, None, None, 0, 1, 2, 4, 128, 32, 0, None) == -1
     assert lib.dflash_kv4_read(ctypes.byref(ok), ctypes.byref(ok), 0x1000, 0x1000, None, 0, 1, 2, 0, 128, 32, 0, None) == 0
+
+
+def test_c_attention_refuses_splits_and_masks_it_cannot_address():
+    _declare()
+    lib = _lib.lib()
+    ok = _cache_struct()
+    st3, st4 = (ctypes.c_longlong * 3)(256, 128, 128), (ctypes.c_longlong * 4)()
+
+    def sdpa(mask=None, kind=0, splits=0):
+        return lib.dflash_kv4_sdpa(0x1000, st3, ctypes.byref(ok), ctypes.byref(ok), mask, kind, st4, 0x1000, None, 1, 2, 2, 1, 128, 1 << 20, 1 << 20,
+                                   1.0, 0, splits, None, 0, None)
+    assert sdpa(splits=-1) == -1 and sdpa(splits=1025) == -1 and b"num_splits" in lib.dflash_last_error_string()
+    assert sdpa(splits=1024) == -4                         # the workspace is what it lacks
+    for bad in (-1, 1025):
+        assert lib.dflash_kv4_sdpa_workspace_bytes(1, 2, 2, 1, 128, 1 << 20, bad) == 0
+    assert sdpa(mask=0x1001, kind=2) == -3 and sdpa(mask=0x1002, kind=3) == -3
+    assert sdpa(mask=0x1001, kind=1, splits=4) == -4 and sdpa(mask=0x1002, kind=2, splits=4) == -4

@@ -286,6 +286,12 @@ def test_attention_queries_that_are_not_finite(odd, kind, T):
     assert torch.equal(got, want)
 
 
+@pytest.mark.parametrize("T", [1, 17])
+@pytest.mark.parametrize("splits", [9, 600, 1024])
+def test_attention_as_many_splits_as_there_may_be(splits, T):
+    run_sdpa(1, 1, 1, 128, T, [140001], torch.bfloat16, cap=140100, max_length=140001, num_splits=splits)
+
+
 @pytest.mark.parametrize("T", [2, 40])
 def test_attention_lowest_finite_mask(T):
     """The type's lowest value is a number: a row that has nothing else is the mean of what it may see."""
