@@ -7,7 +7,7 @@
 // log2(e) / T), so the result does not depend on timing.
 //
 // A block passes over its share of the row, 32 (16-bit types) or 16 elements a thread at a time, the next ones on their way.
-// Top alternatives: 64 groups of threads give 64 maxima; at least top_k elements are >= the top_k-th largest of them, and only
+// Top alternatives: 64 groups of threads (of those that a short row fills) give 64 maxima; at least top_k elements are >= the top_k-th largest of them, and only
 // those (a few dozen of tens of thousands) are collected and ranked by counting.  Keys are (value, lower index first) and
 // therefore unique.  The first pass sets the bar that way, later passes collect what beats the k-th best so far; the list is ranked
 // after passes 1, 4, 16 ... and the last, between which nothing waits.  If it overflows there, the row starts over with a
@@ -295,10 +295,10 @@ __global__ void __launch_bounds__(kThreads, 3) token_logprobs_kernel(const Args 
       // ---- candidates of this pass ----
       const bool first = base == v0;
       if (first) {   // everything >= the k-th largest group maximum
+        const int wide = v1 - v0 > 2 * kGroups ? 2 : v1 - v0 > kGroups ? 1 : 0;   // 2^wide threads a group: short rows fill few threads
         float g = top;
-#pragma unroll
-        for (int o = 1; o < kThreads / kGroups; o <<= 1) g = fmaxf(g, __shfl_xor_sync(0xffffffffu, g, o));
-        if ((lane & (kThreads / kGroups - 1)) == 0) sh.group_max[tid / (kThreads / kGroups)] = g;
+        for (int o = 1; o < 1 << wide; o <<= 1) g = fmaxf(g, __shfl_xor_sync(0xffffffffu, g, o));
+        if ((lane & ((1 << wide) - 1)) == 0 && tid >> wide < kGroups) sh.group_max[tid >> wide] = g;
         __syncthreads();
         const float g0 = sh.group_max[lane], g1 = sh.group_max[lane + 32];
 #pragma unroll
@@ -313,7 +313,7 @@ __global__ void __launch_bounds__(kThreads, 3) token_logprobs_kernel(const Args 
       }
       const float tau = sh.tau;
       // NaN elements count as the largest; a thread whose own maximum does not reach tau can only hold NaN beyond it
-      const bool has = (first ? top >= tau : !(top <= tau)) || nan;
+      const bool has = ((first ? top >= tau : !(top <= tau)) || nan) && base + tid < v1;
       if (has) {
         uint32_t hits = 0;
 #pragma unroll
@@ -324,6 +324,7 @@ __global__ void __launch_bounds__(kThreads, 3) token_logprobs_kernel(const Args 
             const float f = E::get(raw[s], e);
             hits |= (uint32_t)(first ? !(f < tau) : !(f <= tau)) << (s * kPer + e);
           }
+          if (base + s * kThreads + tid >= v1) hits &= (1u << (s * kPer)) - 1u;   // nothing from here on
         }
         while (hits) {
           const int at_e = __ffs(hits) - 1, s = at_e / kPer, e = at_e % kPer;
