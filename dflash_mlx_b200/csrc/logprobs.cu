@@ -153,6 +153,7 @@ struct Shared {
   unsigned long long top[kMaxK];                  // this block's best, highest first; 0 = none
   unsigned long long gathered[kMaxCluster * kMaxK];         // first block of a cluster: every block's `top`
   int counts[2][kThreads / 32];
+  float given;                                    // the given token's logit; NaN outside the vocabulary
   uint4 stage[4][kThreads];                       // elements of threads that hold candidates, to be picked by number
 };
 
@@ -232,6 +233,11 @@ __global__ void __launch_bounds__(kThreads, 3) token_logprobs_kernel(const Args 
   bool careful = false;
   uint32_t next[kSlots][4];
   if (v0 < v1) load(v0, next);
+  if (me == 0 && tid == kThreads - 1) {   // two dependent reads, under the first vectors'
+    const int token = a.tokens[row];
+    sh.given = token < 0 || token >= a.V ? __int_as_float(0x7FC00000)
+               : a.suppress != nullptr && a.suppress[token] ? -INFINITY : E::load(x + token);
+  }
   for (int base = v0; base < v1; base += kThreads * kSlots) {
     uint32_t raw[kSlots][4];
 #pragma unroll
@@ -253,7 +259,8 @@ __global__ void __launch_bounds__(kThreads, 3) token_logprobs_kernel(const Args 
     if (base + kThreads * kSlots < v1) load(base + kThreads * kSlots, next);   // in flight under this pass
     const float top = E::max_of(raw);   // of this pass's elements; NaN is passed over
     bool nan = false;                   // whether an element was NaN or +inf
-    if (E::can_clamp(top, a.scale) && run.m < 1e30f) {   // hidden elements become a finite value of probability 0, two at a time
+    if (base + warp * 32 >= v1) {   // the warp has nothing of this pass
+    } else if (E::can_clamp(top, a.scale) && run.m < 1e30f) {   // hidden elements become a finite value of probability 0, two at a time
       if (top > run.m) {                // the thread's reference moves: y' = x scale - at, at = rounded(reference scale)
         const float to = top * a.scale, d = run.m == -INFINITY ? 0.f : at - to, f = exp2f(d);
         run.w = fmaf(d, run.l, run.w) * f;
@@ -492,17 +499,9 @@ __global__ void __launch_bounds__(kThreads, 3) token_logprobs_kernel(const Args 
     if (tid <= a.k) {
       // tid 0: the given token and the entropy; tid 1..k: an alternative each.  ln L in double: a peaked row has L = 1 + eps
       const double log_l = log((double)all.l);
-      float value;
-      bool in_range = true;
-      if (tid == 0) {
-        const int token = a.tokens[row];
-        in_range = token >= 0 && token < a.V;
-        value = !in_range || (a.suppress != nullptr && a.suppress[token]) ? -INFINITY : E::load(x + token);
-      } else {
-        value = key_value(sh.list[tid - 1]);
-      }
+      const float value = tid == 0 ? sh.given : key_value(sh.list[tid - 1]);
       float out = empty ? -INFINITY : (float)((double)(value - all.m) * a.inv_t - log_l);
-      if (!in_range) out = __int_as_float(0x7FC00000);
+      if (tid == 0 && value != value) out = value;
       if (tid == 0) {
         a.token_logprob[row] = out;
         if (a.entropy != nullptr)
