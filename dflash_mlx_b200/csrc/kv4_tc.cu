@@ -628,19 +628,25 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_sdpa_tc_kernel(const SdpaArgs
       float c[2] = {fmaxf(c_row * mt.k_factor[blk], 1e-37f), fmaxf(c_row * mt.k_factor[blk + 1], 1e-37f)};
       if (kMask >= 2) {   // scaled score + mask back into place, 16 at a time: with the entries, all 64 would not fit the registers
         const bool careful = odd || __any_sync(0xffffffffu, c[0] > 3e38f || c[1] > 3e38f);
+        uint32_t x[2][16];
+        ld16(s_col, x[0]);
 #pragma unroll
         for (int e0 = 0; e0 < kTile; e0 += 16) {
-          uint32_t x[16];
-          ld16(s_col + e0, x);
+          uint32_t(&y)[16] = x[(e0 >> 4) & 1];
           if constexpr (kMask == 3) if (e0) mask_entries<float, 16>(a, mat, n0 + e0, lim, words);
           wait_ld();
+          if (e0 + 16 < kTile) ld16(s_col + e0 + 16, x[((e0 >> 4) & 1) ^ 1]);
+          auto entry = [&](int e) {
+            return kMask == 3 ? __uint_as_float(words[e]) : TR::bits_to_float((uint16_t)(words[((e0 + e) >> 1) & 31] >> (16 * (e & 1))));
+          };
+          if (careful) {   // a hidden key stays hidden under a score that is not finite
 #pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            const float y = kMask == 3 ? __uint_as_float(words[e]) : TR::bits_to_float((uint16_t)(words[((e0 + e) >> 1) & 31] >> (16 * (e & 1))));
-            if (careful && y == -INFINITY) x[e] = 0;   // a hidden key stays hidden under a score that is not finite
-            x[e] = __float_as_uint(fmaf(__uint_as_float(x[e]), c[e0 >> 5], y));
+            for (int e = 0; e < 16; ++e)
+              if (entry(e) == -INFINITY) y[e] = 0;
           }
-          st16(s_col + e0, x);
+#pragma unroll
+          for (int e = 0; e < 16; ++e) y[e] = __float_as_uint(fmaf(__uint_as_float(y[e]), c[e0 >> 5], entry(e)));
+          st16(s_col + e0, y);
         }
         c[0] = c[1] = 1.f;
         wait_st();
