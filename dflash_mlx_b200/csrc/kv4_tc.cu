@@ -765,8 +765,11 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_sdpa_tc_kernel(const SdpaArgs
     }
     // ---- epilogue: either half of the softmax takes half of the channels; a warp's 32 rows go through shared memory (all of Q, K
     // and V is spent), so that they leave as whole lines ----
-    // the last product; the one four before it is done (the last scores took its columns), so the phase cannot be mistaken
-    if (tiles > 0 && ok && !wait_warp(bar0 + 8 * (kBarO + ((tiles - 1) & 3)), ((tiles - 1) >> 2) & 1)) { atomicCAS(err, 0, 62 | (8 << 8)); ok = false; }
+    // The last product.  First the last scores: with an odd number of tiles the second half has none of that pair and may be early, while
+    // the product four before the last one is still out and the phase could be mistaken; the scores took that one's columns.  Behind both
+    // waits every code has been unpacked, so their buffer is free for sEnd.
+    if (tiles > 0 && ok && !(wait_warp(bar0 + 8 * (kBarS + ((pairs - 1) & 1)), ((pairs - 1) >> 1) & 1) &&
+                             wait_warp(bar0 + 8 * (kBarO + ((tiles - 1) & 3)), ((tiles - 1) >> 2) & 1))) { atomicCAS(err, 0, 62 | (8 << 8)); ok = false; }
     fence_after();
     sEnd[group * kRows + r] = make_float2(m_l, l);
     named_bar_sync(1, 256);

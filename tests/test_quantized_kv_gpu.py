@@ -292,6 +292,19 @@ def test_attention_as_many_splits_as_there_may_be(splits, T):
     run_sdpa(1, 1, 1, 128, T, [140001], torch.bfloat16, cap=140100, max_length=140001, num_splits=splits)
 
 
+@pytest.mark.parametrize("D", [128, 256])
+@pytest.mark.parametrize("n", [2009, 2048 + 64, 2048 + 65, 9001])
+@pytest.mark.parametrize("T", [4, 10, 21])
+def test_attention_few_of_128_rows_over_many_tiles(T, n, D):
+    """Rows that fill only some warps of a block, over ranges that end inside either half of their last 128 keys: nothing may run
+    ahead of the last ones.  The same bits every time, and right."""
+    B, Hq, Hk, dtype = 1, 12, 2, torch.bfloat16
+    _, _, _, _, got = args = run_sdpa(B, Hq, Hk, D, T, [n], dtype, cap=n, max_length=n, num_splits=1)
+    q, k, v, scale = args[:4]
+    for _ in range(30):
+        assert torch.equal(qkv.quantized_kv_sdpa(q, k, v, scale, n, num_splits=1), got)
+
+
 @pytest.mark.parametrize("T", [2, 40])
 def test_attention_lowest_finite_mask(T):
     """The type's lowest value is a number: a row that has nothing else is the mean of what it may see."""
