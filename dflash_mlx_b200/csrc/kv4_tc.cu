@@ -22,7 +22,7 @@
 // to fp16 by a power of two per row, exact down to 2^-22 of the row's largest element.  P is fp16, up to 2^14.
 // The running maximum moves only when a score exceeds it by 8 octaves.  Every wait is bounded (device error code 62).
 //
-// Measured (D = 256, bf16): 128 rows x 131072 keys on 2 KV heads 49 us with the combine (28 clocks a key and SM; the tensor pipe needs 16,
+// Measured (D = 256, bf16): 128 rows x 131072 keys on 2 KV heads 50 us with the combine (28 clocks a key and SM; the tensor pipe needs 16,
 // HBM 12.5); 96 rows x 8192 keys on 4 heads 20 us, of which 4 are start-up and 3 the epilogue.
 #include <mutex>
 
