@@ -43,7 +43,7 @@ constexpr uint32_t kOCol = 256, kCols = 512;   // S / P of tile i at 64 * (i & 3
 // What softmax needs to know about 128 keys: per 32 of them the power of two of K, the exponent of V, and keys whose value is not
 // finite.
 struct Meta {
-  float k_factor[4];
+  float k_factor[4];   // negative: a key is not finite
   int v_exp[4];
   uint32_t bad[4];
 };
@@ -377,8 +377,9 @@ __device__ __forceinline__ void unpack_side(const dflash_kv4_cache& c, int b, in
         m.bad[w] = bads;
         mbar_arrive(bar0 + 8 * (kBarVMeta + (tile & (kMeta - 1))));
       }
-    } else if (lane == 0 && tile < tiles) {
-      m.k_factor[w] = pow2(e);
+    } else {
+      const bool any = __any_sync(0xffffffffu, bad);
+      if (lane == 0 && tile < tiles) m.k_factor[w] = any ? -pow2(e) : pow2(e);
     }
   };
   // the block's queries are converted while the first keys and values are on their way
@@ -625,9 +626,10 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_sdpa_tc_kernel(const SdpaArgs
       const Meta& mt = meta[(i >> 1) & (kMeta - 1)];
       const int blk = 2 * (i & 1);   // the tile's 32-key blocks in `mt`: blk and blk + 1
       // never 0 (a scale of 0): a hidden score stays -inf under it
-      float c[2] = {fmaxf(c_row * mt.k_factor[blk], 1e-37f), fmaxf(c_row * mt.k_factor[blk + 1], 1e-37f)};
+      const float kf0 = mt.k_factor[blk], kf1 = mt.k_factor[blk + 1];
+      float c[2] = {fmaxf(c_row * fabsf(kf0), 1e-37f), fmaxf(c_row * fabsf(kf1), 1e-37f)};
       if (kMask >= 2) {   // scaled score + mask back into place, 16 at a time: with the entries, all 64 would not fit the registers
-        const bool careful = odd || __any_sync(0xffffffffu, c[0] > 3e38f || c[1] > 3e38f);
+        const bool careful = odd || kf0 < 0.f || kf1 < 0.f || __any_sync(0xffffffffu, c[0] > 3e38f || c[1] > 3e38f);
         uint32_t x[2][16];
         ld16(s_col, x[0]);
 #pragma unroll

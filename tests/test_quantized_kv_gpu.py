@@ -538,6 +538,136 @@ def test_cache_runs_prompt_verify_rollback_and_tokens():
     assert kept
 
 
+# ---- many rows over long caches (few rows and short caches take the other kernel) ----------------------------------------
+@pytest.mark.parametrize("D", [128, 256])
+@pytest.mark.parametrize("kind", ["none", "bool", "type", "f32"])
+@pytest.mark.parametrize("shape", ["full", "keys", "heads", "rows"])
+def test_long_attention_masks(shape, kind, D):
+    """Every kind of mask at every alignment of its rows, rows and whole tiles with nothing left among them."""
+    B, Hq, Hk, T, n, dtype = 2, 4, 2, 40, 1311, torch.float16 if shape == "heads" else torch.bfloat16
+    dims = {"full": (B, Hq, T, n), "keys": (B, 1, 1, n), "heads": (1, Hq, 1, n), "rows": (T, n)}[shape]
+    keep = torch.rand(dims, generator=gen(3), device=DEV) < 0.6
+    keep[..., 200:420] = False
+    if shape == "full":
+        keep[0, 1, 0] = False
+        keep[1, 3, :30] = False
+    mask = keep if kind == "bool" else None
+    if kind in ("type", "f32"):
+        mask = torch.where(keep, torch.randn(dims, generator=gen(4), device=DEV), torch.full(dims, -math.inf, device=DEV))
+        mask = mask.to(dtype if kind == "type" else torch.float32)
+    for lengths in ([n, n - 20], [n - 700, n]):
+        _, _, _, _, got = run_sdpa(B, Hq, Hk, D, T, lengths, dtype, mask=mask, cap=n, max_length=n)
+        if shape == "full" and mask is not None:
+            assert not bool(got[0, 1, 0].any()) and not bool(got[1, 3, :30].any())
+
+
+@pytest.mark.parametrize("kind", ["bool", "type", "f32"])
+def test_long_attention_mask_alignment(kind):
+    B, Hq, Hk, D, n, T, dtype = 2, 5, 1, 128, 1203, 40, torch.bfloat16
+    k, v = make_cache(B, Hk, n, D, dtype)
+    q, scale = states((B, Hq, T, D), dtype, 9), D ** -0.5
+    keep = torch.rand(B, Hq, T, n, generator=gen(3), device=DEV) < 0.7
+    mask, around = keep, True
+    if kind != "bool":
+        mask = torch.where(keep, torch.randn(keep.shape, generator=gen(4), device=DEV), -math.inf).to(dtype if kind == "type" else torch.float32)
+        around = math.nan
+    want = qkv.quantized_kv_sdpa(q, k, v, scale, ints(n, n - 70), mask)
+    check_rows(want, ref.sdpa(q, k, v, scale, [n, n - 70], mask), dtype)
+    for off in [*range(17), 31]:
+        wide = torch.full((B, Hq, T, off + n + off % 3), around, dtype=mask.dtype, device=DEV)
+        wide[..., off:off + n] = mask
+        assert torch.equal(qkv.quantized_kv_sdpa(q, k, v, scale, ints(n, n - 70), wide[..., off:off + n]), want), off
+    for turned in (mask.transpose(-1, -2).contiguous().transpose(-1, -2), mask.repeat_interleave(2, -1)[..., ::2]):
+        assert torch.equal(qkv.quantized_kv_sdpa(q, k, v, scale, ints(n, n - 70), turned), want)
+
+
+@pytest.mark.parametrize("kind", ["bool", "type", "f32"])
+@pytest.mark.parametrize("odd", [math.nan, math.inf])
+def test_long_attention_values_that_are_not_finite(odd, kind):
+    """Behind the length, behind the row, under the mask they reach nothing; a query's own row they do."""
+    B, Hq, Hk, D, n, T, dtype = 2, 4, 1, 256, 1290, 40, torch.bfloat16
+    k, v = make_cache(B, Hk, n + 30, D, dtype)
+    q, scale = states((B, Hq, T, D), dtype, 9), D ** -0.5
+    keep = torch.ones(B, Hq, T, n + 30, dtype=torch.bool, device=DEV)
+    keep[:, :, :, [4, 33, 1000]] = False
+    keep[0, 1, 1] = False
+    mask = keep if kind == "bool" else torch.where(keep, 0.5, -math.inf).to(dtype if kind == "type" else torch.float32)
+    want = qkv.quantized_kv_sdpa(q, k, v, scale, ints(n, n - 11), mask)
+    check_rows(want, ref.sdpa(q, k, v, scale, [n, n - 11], mask), dtype)
+    for c in (k, v):
+        for part in (c.scales, c.biases):
+            part[:, :, [4, 33, 1000], 1] = odd
+            part[0, :, n:] = odd
+            part[1, :, n - 11:] = odd
+    assert torch.equal(qkv.quantized_kv_sdpa(q, k, v, scale, ints(n, n - 11), mask), want)
+    q[0, 1, 1, 5] = q[0, 2, 2, 77] = odd
+    got = qkv.quantized_kv_sdpa(q, k, v, scale, ints(n, n - 11), mask)
+    assert not bool(got[0, 1, 1].any()) and bool(got[0, 2, 2].isnan().all())
+    got[0, 2, 2] = want[0, 2, 2]
+    assert torch.equal(got, want)
+    v.biases[0, 0, n - 1, 2] = math.nan                   # seen by the last row alone
+    got = qkv.quantized_kv_sdpa(q, k, v, scale, ints(n, n - 11), mask)
+    assert bool(got[0, :, T - 1].isnan().all()) and torch.equal(got[1], want[1]) and torch.equal(got[0, :, :2].isnan(), torch.zeros_like(got[0, :, :2]).bool())
+
+
+@pytest.mark.parametrize("spread", [1e-6, 1e-3, 300.0, 1e5, 1e30])
+def test_long_attention_value_ranges(spread):
+    B, Hq, Hk, D, n, T, dtype = 1, 8, 1, 128, 1500, 40, torch.bfloat16
+    k, _ = make_cache(B, Hk, n, D, dtype, 1)
+    x = states((B, Hk, n, D), torch.float32, 2) * spread
+    x[:, :, 100:150] *= 1e-4
+    x[:, :, 1200:1300] *= 1e-3
+    v = qkv.QuantizedKV(*ref.quantise(x.to(dtype)))
+    q, scale = states((B, Hq, T, D), dtype, 9), D ** -0.5
+    keep = torch.ones(1, Hq, 1, n, dtype=torch.bool, device=DEV)
+    keep[:, 0, :, :100] = False                           # head 0 sees the small values alone
+    keep[:, 0, :, 150:1200] = False
+    keep[:, 0, :, 1300:] = False
+    got = qkv.quantized_kv_sdpa(q, k, v, scale, n, keep)
+    check_rows(got, ref.sdpa(q, k, v, scale, [n], keep), dtype)
+
+
+@pytest.mark.parametrize("falling", [True, False])
+def test_long_attention_biases_by_distance_and_lowest_values(falling):
+    """Biases that grow or fall along the keys move the running maximum with every tile; the lowest finite value hides nothing."""
+    B, Hq, Hk, D, n, T, dtype = 1, 8, 1, 128, 1400, 40, torch.bfloat16
+    far = torch.arange(n, device=DEV).float()
+    slopes = torch.pow(2.0, -torch.arange(Hq, device=DEV) / 2.0)[None, :, None, None]
+    mask = (slopes * (far - n if falling else -far)).to(dtype).expand(B, Hq, T, n).contiguous()
+    mask[:, 3] = torch.finfo(dtype).min
+    _, _, v, _, got = run_sdpa(B, Hq, Hk, D, T, [n], dtype, mask=mask, cap=n, max_length=n)
+    mean = ref.values(*v)[0, 0, :n - T + 1].mean(0)
+    # P is rounded to fp16 (2^-11), and a mean of 1400 values with both signs is some 30 times smaller than they are
+    assert float((got[0, 3, 0].double() - mean).norm()) < TOL[dtype] * float(mean.norm()) + 2.0 ** -11 * float(ref.values(*v)[0, 0].std())
+
+
+def test_long_attention_negative_scales_and_strides():
+    B, Hq, Hk, D, n, T, dtype = 2, 4, 1, 128, 1300, 40, torch.bfloat16
+    whole = make_cache(3, 4, n + 20, D, dtype, 4)
+    for c in whole:
+        c.biases.copy_((c.biases.float() + 15 * c.scales.float()).to(dtype))
+        c.scales.neg_()
+    k, v = (qkv.QuantizedKV(*[p[1:, 2:3, 8:8 + n] for p in c]) for c in whole)
+    dense = [qkv.QuantizedKV(*[p.contiguous() for p in c]) for c in (k, v)]
+    flat = states((B, T, Hq * D + 8), dtype, 3, 4.0)
+    for start in (0, 3):
+        q = flat[..., start:start + Hq * D].view(B, T, Hq, D).transpose(1, 2)
+        for scale in (0.3, -0.3, 0.0):
+            got = qkv.quantized_kv_sdpa(q, k, v, scale, ints(n, 7))
+            check_rows(got, ref.sdpa(q, *dense, scale, [n, 7]), dtype)
+            assert torch.equal(got, qkv.quantized_kv_sdpa(q.contiguous(), *dense, scale, ints(n, 7)))
+
+
+@pytest.mark.parametrize("D", [128, 256])
+@pytest.mark.parametrize("n", [12009, 12032 + 64, 12032 + 65])
+@pytest.mark.parametrize("T", [4, 10, 21])
+def test_long_attention_of_few_of_128_rows(T, n, D):
+    B, Hq, Hk, dtype = 1, 12, 2, torch.bfloat16
+    _, _, _, _, got = args = run_sdpa(B, Hq, Hk, D, T, [n], dtype, cap=n, max_length=n, num_splits=1)
+    for _ in range(20):
+        assert torch.equal(qkv.quantized_kv_sdpa(*args[:4], n, num_splits=1), got)
+
+
 def test_verify_cycle_with_token_probabilities():
     """What a server runs per cycle, captured once: the block's keys and values enter the cache, its rows attend, a head makes
     logits, the drafted tokens' log-probabilities decide how many are accepted, and the positions move on, all on the device."""
