@@ -809,9 +809,9 @@ int launch_combine(const SdpaArgs& a, cudaStream_t st) {
 }
 
 template <typename T>
-int launch_typed(const SdpaArgs& a, int dtype, int D, cudaStream_t st, int device) {
+int launch_typed(const SdpaArgs& a, bool tc, int dtype, int D, cudaStream_t st, int device) {
   int rc;
-  if (a.rows > kFewRows) rc = launch_partials_tc(a, dtype, D, st, device);
+  if (tc) rc = launch_partials_tc(a, dtype, D, st, device);
   else if (row_tile(a.rows) == 1) rc = D == 128 ? launch_sdpa<T, 128, 1>(a, st, device) : launch_sdpa<T, 256, 1>(a, st, device);
   else rc = D == 128 ? launch_sdpa<T, 128, 2>(a, st, device) : launch_sdpa<T, 256, 2>(a, st, device);
   if (rc || a.splits == 1) return rc;
@@ -933,10 +933,19 @@ extern "C" int dflash_kv4_read(const dflash_kv4_cache* k_cache, const dflash_kv4
   return e == cudaSuccess ? DFLASH_OK : fail(DFLASH_ERR_LAUNCH, "kv4_read launch: %s", cudaGetErrorString(e));
 }
 
+// Whether the rows go to the tcgen05 kernel.  It has the throughput, the other one the shorter way from launch to end: where tiles of 16
+// rows fit the SMs side by side and have little to do in all, they are faster (D = 256, 96 rows a KV head, 4 heads: 128 positions 9.3
+// against 11.7 us, 512 11.2 against 14.4, 2048 16.1 against 16.0; 4 sequences: 128 positions 9.6 against 11.8, 512 16.9 against 15.9).
+static bool takes_tc(int B, int Hk, long long rows, int max_length, int device) {
+  if (rows <= kFewRows) return false;
+  const long long units = (long long)B * Hk * ((rows + 15) / 16), sms = sm_count(device);
+  return units > 2 * sms || units * max_length > 160 * sms;
+}
 static int kv4_splits(int B, int Hk, long long rows, int max_length, int device, int num_splits) {
-  const int tile = rows > kFewRows ? kTcRows : 8 * row_tile((int)rows);
+  const bool tc = takes_tc(B, Hk, rows, max_length, device);
+  const int tile = tc ? kTcRows : 8 * row_tile((int)rows);
   const long long units = (long long)B * Hk * ((rows + tile - 1) / tile);
-  return choose_splits(units, B, max_length, device, num_splits, rows > kFewRows ? 1 : 2);
+  return choose_splits(units, B, max_length, device, num_splits, tc ? 1 : 2);
 }
 
 extern "C" size_t dflash_kv4_sdpa_workspace_bytes(int B, int Hq, int Hk, int T, int D, int max_length, int num_splits) {
@@ -988,5 +997,6 @@ extern "C" int dflash_kv4_sdpa(const void* q, const long long* q_strides, const 
     a.part_l = a.part_m + n;
   }
   cudaStream_t st = (cudaStream_t)stream;
-  return dtype == DFLASH_BF16 ? launch_typed<__nv_bfloat16>(a, dtype, D, st, device) : launch_typed<__half>(a, dtype, D, st, device);
+  const bool tc = takes_tc(B, Hk, rows, max_length, device);
+  return dtype == DFLASH_BF16 ? launch_typed<__nv_bfloat16>(a, tc, dtype, D, st, device) : launch_typed<__half>(a, tc, dtype, D, st, device);
 }

@@ -46,7 +46,7 @@ __device__ __forceinline__ float apply_mask(const SdpaArgs& a, float t, long lon
   return m == -INFINITY ? -INFINITY : t + m;   // a hidden key stays hidden whatever its score (NaN, +inf)
 }
 
-// kv4_tc.cu: the attention's pass over the keys for more than kFewRows rows per KV head (kTcRows rows a block), into the output or,
+// kv4_tc.cu: the attention's pass over the keys for many rows per KV head (always above kFewRows; kTcRows rows a block), into the output or,
 // with several splits, the partials.
 constexpr int kFewRows = 16, kTcRows = 128;
 int launch_partials_tc(const SdpaArgs& a, int dtype, int D, cudaStream_t st, int device);
