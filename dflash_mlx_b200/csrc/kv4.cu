@@ -196,9 +196,13 @@ __global__ void __launch_bounds__(128) kv4_read_kernel(const ReadArgs a) {
 //   S^T [16 keys, 8 rows] += K codes [16, 16 channels] x Q^T : a thread unpacks the two words of its quarter of a group; the
 //       16 channels of an MMA step are any 16 of one group (Q is laid out to match), so a group's sum ends in its own
 //       accumulator and takes its scale there.
-//   O^T [16 channels, 8 rows] += V codes^T [16, 16 keys] x P' : P' = p * sv in fp16 (sv brought into fp16's range by a power of
-//       two per warp that is undone at the end).  Nibble t and 4 + t of a word are rows r and r + 8 of MMA t, so a thread's
-//       words serve four MMAs without crossing lanes.
+//   O^T [16 channels, 8 rows] += V codes^T [16, 16 keys] x P' : P' = p * sv in fp16 (11 bits; fp32's would need four times the
+//       MMAs).  Nibble t and 4 + t of a word are rows r and r + 8 of MMA t, so a thread's words serve four MMAs without crossing
+//       lanes.
+// P' in fp16's range, whatever the scales, and without a row noticing keys that it does not see: a key whose largest |sv| lies in
+// [2^-12, 2^4) is multiplied by 2^3 like all of its kind, so P' <= 2^15 and its bits down to 2^-25; any other key by a power of two of
+// its own, 2^(3 - x), which P' and the row's exponent take back: P' = p sv 2^(3 - ev), ev = 0 until the row sees such a key.  A tile
+// without one, under rows with ev = 0, does not touch any of this.
 // Codes become exact fp16 integers by OR-ing the nibble into 1024 and one packed operation that takes the constant away again
 // (left in, a sum would carry 1024 times sum |q| or sum P', which costs digits); values are centred as code - 8, which halves
 // what the rounding of P' is multiplied with.  q is brought to fp16 by a power of two per row: bf16's 8 bits are exact in it
@@ -211,7 +215,12 @@ __global__ void __launch_bounds__(128) kv4_read_kernel(const ReadArgs a) {
 // allow (the loop is bound by instruction issue: unpacking, scales and softmax next to the MMAs).
 constexpr int kStages = 3;   // tiles of a warp in shared memory
 template <int D, int NT> constexpr int kWarpsOf = NT == 2 ? (D == 256 ? 4 : 6) : (D == 256 ? 6 : 8);
-constexpr float kMaxStep = 5.545177444f;   // 8 ln 2
+constexpr float kLn2 = 0.6931471805599453f, kMaxStep = 8 * kLn2;
+constexpr float kUsual = 8.f;              // the power of two of usual value scales
+__device__ __forceinline__ bool unusual(float big) {   // outside [2^-12, 2^4), and not 0
+  const uint32_t u = __float_as_uint(big);
+  return u - (115u << 23) >= (16u << 23) && u != 0;
+}
 
 template <int D>
 struct Tile {
@@ -266,7 +275,9 @@ __global__ void __launch_bounds__((kWarpsOf<D, NT>) * 32, 2) kv4_sdpa_kernel(con
   uint2* sQ = (uint2*)smem;                                   // [NT][KS][32] fragments of Q^T
   float* sQs = (float*)(smem + NT * KS * 32 * 8);             // [NT][G][8] sums of q over a group
   float* sC = sQs + NT * G * 8;                               // [NT][8] what brings a row's products back to scores
-  uint8_t* ring = smem + NT * KS * 32 * 8 + NT * (G + 1) * 8 * 4 + warp * stages * TL::kBytes;
+  float* sEv = sC + 8 * NT + warp * 8 * NT;                   // [kWarps][8 NT] exponents that the warp's output rows carry
+  constexpr int kFixed = NT * KS * 32 * 8 + NT * (G + 1 + kWarps) * 8 * 4;
+  uint8_t* ring = smem + kFixed + warp * stages * TL::kBytes;
   const uint32_t uring = smem_u32(ring);
   pdl_wait();
   pdl_trigger();
@@ -313,6 +324,7 @@ __global__ void __launch_bounds__((kWarpsOf<D, NT>) * 32, 2) kv4_sdpa_kernel(con
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
   for (int s = 0; s < stages - 1; ++s) fetch(tile + s * kWarps, s);
+  if (lane < 8 * NT) sEv[lane] = 0.f;
 
   // Q^T fragments: a warp per row, a lane per octet j of channels.  In an MMA step lane (r, c) holds row r and the nibble pairs of
   // words 8g + 2c (steps 0 and 1 of group g) and 8g + 2c + 1 (steps 2 and 3).
@@ -373,7 +385,7 @@ __global__ void __launch_bounds__((kWarpsOf<D, NT>) * 32, 2) kv4_sdpa_kernel(con
 #pragma unroll
     for (int i = 0; i < D / 16; ++i) o[i][nt][0] = o[i][nt][1] = o[i][nt][2] = o[i][nt][3] = 0.f;
   }
-  float sv_mul = 0x1p126f;   // power of two that brings this warp's value scales into fp16's range
+  bool shifted = false;   // whether some row's exponent is not 0
 
   int stage = 0;
   for (; tile < tile1; tile += kWarps) {
@@ -389,8 +401,7 @@ __global__ void __launch_bounds__((kWarpsOf<D, NT>) * 32, 2) kv4_sdpa_kernel(con
     const int n0 = tile * 16;
     // scales of keys r and r + 8
     float sk[2][G], bk[2][G], sv[2][G], bv[2][G];
-    float bad[2] = {0.f, 0.f};
-    float big = 0.f;
+    float bad[2] = {0.f, 0.f}, big[2] = {0.f, 0.f};
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
       const uint16_t* sc = (const uint16_t*)(st + 2 * TL::kCodeBytes) + (r + 8 * e) * G;
@@ -406,23 +417,24 @@ __global__ void __launch_bounds__((kWarpsOf<D, NT>) * 32, 2) kv4_sdpa_kernel(con
         bk[e][g] = TR::bits_to_float(h[1][g]);
         sv[e][g] = TR::bits_to_float(h[2][g]);
         const float bb = TR::bits_to_float(h[3][g]);
-        bad[e] = fmaf(sv[e][g], 0.f, fmaf(bb, 0.f, bad[e]));   // NaN when a scale or bias of the value is not finite
         bv[e][g] = fmaf(sv[e][g], 8.f, bb);
-        big = fmaxf(big, fabsf(sv[e][g]));
+        bad[e] = fmaf(bv[e][g], 0.f, bad[e]);   // NaN when a scale or bias of the value, or the middle of its codes, is not finite
+        big[e] = fmaxf(big[e], fabsf(sv[e][g]));
       }
     }
     if (__any_sync(0xffffffffu, !(bad[0] == 0.f) || !(bad[1] == 0.f))) {
       // keep such a value out of the products (0 * NaN would reach rows that do not see it); rows that do see it get NaN
       // through their scores below
-      big = 0.f;
 #pragma unroll
       for (int e = 0; e < 2; ++e)
+        if (!(bad[e] == 0.f)) {
+          big[e] = 0.f;
 #pragma unroll
-        for (int g = 0; g < G; ++g) {
-          if (!(bad[e] == 0.f)) sv[e][g] = bv[e][g] = 0.f;
-          big = fmaxf(big, fabsf(sv[e][g]));
+          for (int g = 0; g < G; ++g) sv[e][g] = bv[e][g] = 0.f;
         }
     }
+    const bool odd = unusual(big[0]) || unusual(big[1]) || shifted;
+    bool careful = false;
     // ---- S^T = K Q^T ----
     uint64_t s2[NT][2];   // key r, then r + 8; rows 2c and 2c + 1 side by side
 #pragma unroll
@@ -462,7 +474,7 @@ __global__ void __launch_bounds__((kWarpsOf<D, NT>) * 32, 2) kv4_sdpa_kernel(con
       unpair(s2[nt][1], s[nt][2], s[nt][3]);
     }
     // ---- visibility, running maximum ----
-    bool grow = big * sv_mul > 64.f;
+    bool grow = odd;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -478,54 +490,85 @@ __global__ void __launch_bounds__((kWarpsOf<D, NT>) * 32, 2) kv4_sdpa_kernel(con
         grow |= t > m[nt][e] + kMaxStep;
       }
     if (__any_sync(0xffffffffu, grow)) {
-      float top = big;
+      // a row's maximum moves for its own scores alone: what other rows see changes no bit of it
+      float xk[2] = {0.f, 0.f};   // the keys' own exponents
+      careful = __any_sync(0xffffffffu, odd);
+      if (careful) {
+        shifted = false;
 #pragma unroll
-      for (int w = 4; w < 32; w <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
-      float ratio = 1.f;
-      if (top * sv_mul > 64.f) {
-        const int ex = max((int)(__float_as_uint(top) >> 23) - 127, -100);
-        const float next = __uint_as_float((uint32_t)(127 + 5 - ex) << 23);   // top * next in [32, 64)
-        ratio = next / sv_mul;
-        sv_mul = next;
+        for (int e = 0; e < 2; ++e) {
+          if (unusual(big[e])) {
+            float all = big[e];
+#pragma unroll
+            for (int g = 0; g < G; ++g) all = fmaxf(all, fabsf(bv[e][g]) * 0.0625f);
+            const int x = max((int)(__float_as_uint(all) >> 23) - 127 - 3, -120);   // 2^(3 - x) |sv| < 2^7
+            const float take = __uint_as_float((uint32_t)(127 - x) << 23);
+            xk[e] = (float)x;
+#pragma unroll
+            for (int g = 0; g < G; ++g) { sv[e][g] *= take; bv[e][g] *= take; }
+          }
+        }
       }
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
         float f[2];
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          float x = fmaxf(m[nt][e], fmaxf(s[nt][e], s[nt][2 + e]));
+          float x = fmaxf(s[nt][e], s[nt][2 + e]);
 #pragma unroll
           for (int w = 4; w < 32; w <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, w));
-          f[e] = x == -INFINITY ? 1.f : ex2((m[nt][e] - x) * kLog2e);   // nothing seen yet: the sums are zero
-          m[nt][e] = x;
+          const float before = m[nt][e], now = x > before + kMaxStep ? x : before;
+          f[e] = now == -INFINITY ? 1.f : ex2((before - now) * kLog2e);   // nothing seen yet: the sums are zero
+          m[nt][e] = now;
           l[nt][e] *= f[e];
+          if (careful) {
+            float y = fmaxf(fmaf(xk[0], kLn2, s[nt][e]), fmaf(xk[1], kLn2, s[nt][2 + e]));
+#pragma unroll
+            for (int w = 4; w < 32; w <<= 1) y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, w));
+            const float ev = sEv[nt * 8 + 2 * c + e], d = (y - now) * kLog2e;   // octaves of the row's largest p 2^x
+            float ev_now = ev;
+            if (now != -INFINITY && (now != before || d > ev + 8.f)) ev_now = fmaxf(ceilf(d), ev + floorf((before - now) * kLog2e));
+            if (now != -INFINITY) f[e] = ex2(fmaf(before - now, kLog2e, ev - ev_now));
+            __syncwarp();
+            if (r == 0) sEv[nt * 8 + 2 * c + e] = ev_now;
+            shifted |= ev_now != 0.f;
+            // p for the sum, P' without its scale for the products: usual keys under ev = 0 have the same bits in both
+            const float ref = now == -INFINITY ? 0.f : now;
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              const float z = s[nt][2 * i + e] - ref;
+              l[nt][e] += ex2(z * kLog2e);
+              s[nt][2 * i + e] = ex2(fmaf(z, kLog2e, xk[i] - ev_now));
+            }
+          }
         }
 #pragma unroll
         for (int g = 0; g < G; ++g) ob[g][nt] = mul2(ob[g][nt], pair(f[0], f[1]));
-        f[0] *= ratio;
-        f[1] *= ratio;
 #pragma unroll
         for (int i = 0; i < D / 16; ++i) {
           o[i][nt][0] *= f[0]; o[i][nt][1] *= f[1];
           o[i][nt][2] *= f[0]; o[i][nt][3] *= f[1];
         }
       }
+      shifted = __any_sync(0xffffffffu, shifted);
     }
     // ---- p, and O^T += V^T P' per group ----
+    if (!careful) {
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
+      for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-      for (int x = 0; x < 4; ++x) {
-        const float ref = m[nt][x & 1] == -INFINITY ? 0.f : m[nt][x & 1];
-        const float p = ex2((s[nt][x] - ref) * kLog2e);
-        s[nt][x] = p;
-        l[nt][x & 1] += p;
-      }
+        for (int x = 0; x < 4; ++x) {
+          const float ref = m[nt][x & 1] == -INFINITY ? 0.f : m[nt][x & 1];
+          const float p = ex2((s[nt][x] - ref) * kLog2e);
+          s[nt][x] = p;
+          l[nt][x & 1] += p;
+        }
+    }
     const uint8_t* sV = st + TL::kCodeBytes;
 #pragma unroll
     for (int g = 0; g < G; ++g) {
       uint32_t pb[NT][2];
-      const float s0 = sv[0][g] * sv_mul, s1 = sv[1][g] * sv_mul;
+      const float s0 = sv[0][g] * kUsual, s1 = sv[1][g] * kUsual;
       const uint64_t bv0 = pair(bv[0][g], bv[0][g]), bv1 = pair(bv[1][g], bv[1][g]);
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
@@ -562,10 +605,10 @@ __global__ void __launch_bounds__((kWarpsOf<D, NT>) * 32, 2) kv4_sdpa_kernel(con
   __syncthreads();   // the rings become the merge buffers
 
   // ---- merge the warps: O [warp][8 NT][D], m and l [warp][8 NT] ----
-  float* mO = (float*)(smem + NT * KS * 32 * 8 + NT * (G + 1) * 8 * 4);
+  float* mO = (float*)(smem + kFixed);
   float* mM = mO + kWarps * 8 * NT * D;
   float* mL = mM + kWarps * 8 * NT;
-  const float undo = 1.f / sv_mul;
+  constexpr float undo = 1.f / kUsual;
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -591,6 +634,11 @@ __global__ void __launch_bounds__((kWarpsOf<D, NT>) * 32, 2) kv4_sdpa_kernel(con
         v0.z = fmaf(o[4 * g + 2][nt][e], undo, y); v0.w = fmaf(o[4 * g + 3][nt][e], undo, y);
         v1.x = fmaf(o[4 * g][nt][2 + e], undo, y); v1.y = fmaf(o[4 * g + 1][nt][2 + e], undo, y);
         v1.z = fmaf(o[4 * g + 2][nt][2 + e], undo, y); v1.w = fmaf(o[4 * g + 3][nt][2 + e], undo, y);
+        if (shifted) {
+          const int ev = (int)sEv[row];
+          v0.x = scalbnf(v0.x, ev); v0.y = scalbnf(v0.y, ev); v0.z = scalbnf(v0.z, ev); v0.w = scalbnf(v0.w, ev);
+          v1.x = scalbnf(v1.x, ev); v1.y = scalbnf(v1.y, ev); v1.z = scalbnf(v1.z, ev); v1.w = scalbnf(v1.w, ev);
+        }
         *(float4*)(po + 64 * g + 8 * r) = v0;
         *(float4*)(po + 64 * g + 8 * r + 4) = v1;
       }
@@ -774,7 +822,7 @@ template <typename T, int D, int NT>
 int launch_sdpa(SdpaArgs a, cudaStream_t st, int device) {
   constexpr int kWarps = (kWarpsOf<D, NT>);
   using TL = Tile<D>;
-  constexpr size_t fixed = (size_t)NT * (D / 16) * 32 * 8 + (size_t)NT * (D / kGroup + 1) * 8 * 4;
+  constexpr size_t fixed = (size_t)NT * (D / 16) * 32 * 8 + (size_t)NT * (D / kGroup + 1 + kWarps) * 8 * 4;
   constexpr size_t merge = (size_t)kWarps * 8 * NT * (D + 2) * 4;
   constexpr size_t ring = (size_t)kWarps * kStages * TL::kBytes;
   constexpr size_t smem = fixed + (ring > merge ? ring : merge);
