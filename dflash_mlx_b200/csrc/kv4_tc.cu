@@ -14,17 +14,22 @@
 //                costs about 100 cycles of it, so each thread waits under the other one's MMAs
 // A slab of keys is refilled as soon as its steps are done, either half of the values while the other one is multiplied.
 //
-// Unpacking costs 9 instructions for 8 codes: a nibble left in place is an fp16 subnormal, code * 2^-24 (or * 2^-20), and one packed
-// fma turns two of them into code * scale + bias with a single rounding to fp16 (2^-11; the cache's scales carry 8 or 11 bits,
-// the codes 4).  For that, every 32 keys share a power of two that brings the scales under 2^-9 and that S (for K) or P (for V)
-// takes back.  Values far below the largest of their 32 keys lose bits at 2^-21 of that largest one: nothing to a score, and values
-// of keys that differ by more than 6 octaves are unpacked in 13 instructions with 11 more bits of range.  q is brought
-// to fp16 by a power of two per row, exact down to 2^-22 of the row's largest element.  P is fp16, up to 2^14.
-// The running maximum moves only when a score exceeds it by 8 octaves.  Every wait is bounded (device error code 62).
+// Unpacking costs 13 instructions for 8 codes: nibbles become whole numbers, and one packed fma makes two of them code * scale + bias
+// with a single rounding to fp16 (at most 2^-11 of a value, 2^-25 of the unit below; the cache's scales carry 8 or 11 bits, the codes 4).
+// A row must not notice keys that it does not see, so nothing is shared between keys: a key or value whose largest element lies in
+// [2^-10, 2^11) is multiplied by 2^4 like all of its kind; any other one by a power of two of its own, which brings that
+// element into [2^14, 2^15).  A column of S takes the power back before its softmax, and P for V: P = p 2^(6 + x - ev), with an
+// exponent ev of the row's output that is 0 until the row sees such a value.  Tiles without them, under rows with ev = 0, do not
+// touch any of this, and the bits of usual keys are the same either way.  (An exponent shared by 32 keys allows 9 instructions for 8
+// codes, 3 % of a long range, but then one large key, seen or not, takes the others' bits.  A cache of unusual keys takes 1.3 times as
+// long, one of unusual values 2.2 times.)  q is brought to fp16 by a power of two per row, exact
+// down to 2^-22 of the row's largest element.  P is fp16, up to 2^15; its sum takes the unrounded p.
+// The running maximum moves only when a score exceeds it by 8 octaves, per row.  Every wait is bounded (device error code 62).
 //
 // Measured (D = 256, bf16): 128 rows x 131072 keys on 2 KV heads 50 us with the combine (28 clocks a key and SM; the tensor pipe needs 16,
 // HBM 12.5); 96 rows x 8192 keys on 4 heads 20 us, of which 4 are start-up and 3 the epilogue.
 #include <mutex>
+#include <type_traits>
 
 #include "kv4.cuh"
 
@@ -32,27 +37,26 @@ namespace dflash {
 namespace kv4 {
 namespace {
 
-constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr int kUnit = -4, kUsualFrom = -10, kUsualTo = 11;   // usual keys and values: in units of 2^kUnit, their largest element's octaves
 constexpr int kRows = 128, kKeys = 128, kTile = 64;   // keys are unpacked by 128, multiplied by 64
 constexpr int kThreads = 18 * 32, kKeyWarp = 8, kValueWarp = 12, kIssuer = 16;   // kIssuer: scores; the next warp: output
-constexpr float kMaxStep = 8 * kLn2;   // natural units
-constexpr float kPShift = 6.f;         // P = p * 2^6 (p <= 2^8): further from fp16's subnormals
+constexpr float kPShift = 6.f;         // P = p * 2^6 (p <= 2^9): further from fp16's subnormals
 constexpr int kSlab = kKeys * 128;     // 128 rows x 64 channels: Q, K or V
 constexpr uint32_t kOCol = 256, kCols = 512;   // S / P of tile i at 64 * (i & 3)
 
-// What softmax needs to know about 128 keys: per 32 of them the power of two of K, the exponent of V, and keys whose value is not
-// finite.
-struct Meta {
-  float k_factor[4];   // negative: a key is not finite
-  int v_exp[4];
-  uint32_t bad[4];
+// What softmax needs to know about 128 keys, a bit of a word per key: keys and values that are unusual or not finite, values that are
+// not finite; and the exponents of blocks of 32 keys or values with an odd one.
+struct __align__(16) Meta {
+  int8_t k_exp[128], v_exp[128];
+  uint32_t k_odd[4], v_odd[4], v_bad[4];
 };
-constexpr int kOdd = 1024;
+constexpr int kOdd = 1024;               // on a query row's exponent: an element is not finite
 constexpr int kMeta = 4;   // scales are looked at no more than three tiles ahead of the softmax
 
 // mbarriers, 8 bytes each.  kBarKEmpty: per slab; V full and empty: per half of the buffer (64 keys); kBarS: per pair of score tiles;
-// P, O: per tile in flight; kBarM: a row reference handed on, per tile parity and 32 rows; kBarVMeta: the values' exponents of 128
-// keys are known
+// P, O: per tile in flight; kBarM: a row reference handed on, per tile parity and 32 rows; kBarVMeta: the values' part of Meta of
+// 128 keys is known
 enum { kBarKFull = 0, kBarQ = 1, kBarVFull = 2, kBarKEmpty = 4, kBarVEmpty = 8, kBarS = 10, kBarP = 12, kBarO = 16, kBarM = 20,
        kBarVMeta = 28, kBars = 32 };
 
@@ -151,12 +155,12 @@ __device__ __forceinline__ void scales_of(const uint32_t (&r)[D / 128], float (&
 #pragma unroll
   for (int g = 0; g < D / kGroup; ++g) s[g] = MmaTraits<T>::bits_to_float((uint16_t)(r[g >> 1] >> (16 * (g & 1))));
 }
-// The largest value a key's scales allow, as bits (15 |scale| + |bias| over its groups): not finite where one of them is not.
+// The largest element a key may hold, as bits: that of codes 0 and 15 over its groups; not finite where one of them is not.
 template <int G>
 __device__ __forceinline__ uint32_t largest_bits(const float (&s)[G], const float (&b)[G]) {
   uint32_t m = 0;
 #pragma unroll
-  for (int g = 0; g < G; ++g) m = max(m, __float_as_uint(fmaf(fabsf(s[g]), 15.f, fabsf(b[g]))) & 0x7FFFFFFFu);
+  for (int g = 0; g < G; ++g) m = max(max(m, __float_as_uint(b[g]) & 0x7FFFFFFFu), __float_as_uint(fmaf(s[g], 15.f, b[g])) & 0x7FFFFFFFu);
   return m;
 }
 __device__ __forceinline__ uint32_t hfma2(uint32_t a, uint32_t b, uint32_t c) {
@@ -258,33 +262,31 @@ template <> __device__ __forceinline__ uint32_t abs_max<__half>(uint32_t x, uint
   const __half2 m = __hmax2(*(const __half2*)&x, *(const __half2*)&y);
   return *(const uint32_t*)&m;
 }
-// 64 codes -> a swizzled 128-byte row; the eight codes of a word land in the order 0 4 1 5 2 6 3 7.  Narrow: the nibbles are
-// fp16 subnormals and one fma makes the value (9 instructions a word); wide: the nibbles become whole numbers first (13).
-template <bool kWide>
-__device__ __forceinline__ void unpack_row(const uint4& c0, const uint4& c1, float scale, float bias, int e, uint32_t row, int key) {
-  const float sx = scale * pow2(kWide ? -e : min(24 - e, 127));   // e >= -100
-  const uint32_t s0 = splat(sx), s1 = splat(sx * 0.0625f), z = splat(bias * pow2(-e));
+// 64 codes -> a swizzled 128-byte row of code * scale + bias (both in the key's unit); the eight codes of a word land in the order
+// 0 4 1 5 2 6 3 7.
+__device__ __forceinline__ void unpack_row(const uint4& c0, const uint4& c1, float scale, float bias, uint32_t row, int key) {
+  const uint32_t s = splat(scale), z = splat(bias);
   const uint32_t w[8] = {c0.x, c0.y, c0.z, c0.w, c1.x, c1.y, c1.z, c1.w};
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     uint32_t v[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const uint32_t x = j < 2 ? w[i] : w[i] >> 8;
-      if (kWide) {
-        const uint32_t u = lop3_and_or(x, (j & 1) ? 0x00F000F0u : 0x000F000Fu, 0x64006400u);
-        // 1024 + c -> c and 1024 + 16 c -> c, exactly
-        const uint32_t c = (j & 1) ? hfma2(u, 0x2C002C00u, 0xD400D400u) : hfma2(u, 0x3C003C00u, 0xE400E400u);
-        v[j] = hfma2(c, s0, z);
-      } else {
-        v[j] = hfma2(x & ((j & 1) ? 0x00F000F0u : 0x000F000Fu), (j & 1) ? s1 : s0, z);
-      }
+      const uint32_t u = lop3_and_or(j < 2 ? w[i] : w[i] >> 8, (j & 1) ? 0x00F000F0u : 0x000F000Fu, 0x64006400u);
+      // 1024 + c -> c and 1024 + 16 c -> c, exactly
+      const uint32_t c = (j & 1) ? hfma2(u, 0x2C002C00u, 0xD400D400u) : hfma2(u, 0x3C003C00u, 0xE400E400u);
+      v[j] = hfma2(c, s, z);
     }
     asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(row + ((uint32_t)(i ^ (key & 7)) << 4)), "r"(v[0]), "r"(v[1]), "r"(v[2]),
                  "r"(v[3])
                  : "memory");
   }
 }
+
+// What takes a key's own power of two back (1 for usual ones), and the exponent of a value's; blocks of 32 without an odd one have
+// stale exponents.
+__device__ __forceinline__ float own_power(const Meta& m, int key) { return m.k_odd[key >> 5] ? pow2(m.k_exp[key]) : 1.f; }
+__device__ __forceinline__ float own_exponent(const Meta& m, int key) { return m.v_odd[key >> 5] ? (float)m.v_exp[key] : 0.f; }
 
 // The order in which a block works through its keys: from the last ones back, 64 at a time, so that under masks that fall with the
 // distance the largest scores come first and O is not rescaled with every tile (64 rows x 4 x 5001 keys of 256 channels: 40.2 -> 34.1
@@ -347,39 +349,41 @@ __device__ __forceinline__ void unpack_side(const dflash_kv4_cache& c, int b, in
     __syncwarp();
     if (lane == 0) mbar_arrive(bar);
   };
-  // Scales of a tile, a tile ahead of its codes: what they say about the tile is published before the codes' buffer is free.
+  // Scales of a tile, a tile ahead of its codes: what the values' say about the tile is published before the codes' buffer is free.
   uint32_t ns[D / 128], nz[D / 128];
-  float s[G], z[G];
-  int e = 0;
-  bool wide = false;
+  float s[G], z[G];   // in the key's unit
   auto prepare = [&](int tile) {
     scales_of<T, D>(ns, s);
     scales_of<T, D>(nz, z);
     const uint32_t largest = largest_bits(s, z);
     const bool bad = largest >= 0x7F800000u;
-    const int hi_e = (int)(__reduce_max_sync(0xffffffffu, bad ? 0u : largest) >> 23) - 127;   // values of the 32 keys are below 2^(hi_e + 1)
-    // |scale| is below 2^(hi_e - 2): times 2^-e it is below 2^-9, where an fp16 scale * 2^24 still fits
-    e = min(max(hi_e + 7, -100), 126);
+    const bool usual = largest - ((uint32_t)(127 + kUsualFrom) << 23) < ((uint32_t)(kUsualTo - kUsualFrom) << 23) || largest == 0;
+    float unit = pow2(-kUnit);
+    const uint32_t odd = __ballot_sync(0xffffffffu, !usual);
     Meta& m = meta[tile & (kMeta - 1)];
-    if (kV) {
-      // keys whose largest value is more than 6 octaves below: the narrow form would lose their bits
-      const int lo_e = (int)(__reduce_min_sync(0xffffffffu, bad || largest == 0 ? 0x7F7FFFFFu : largest) >> 23) - 127;
-      wide = hi_e - lo_e > 6;
-      // values below 2^5: 19 octaves of full precision for them, and only 11 octaves that P has to make up for next to a narrow block
-      if (wide) e = min(max(hi_e - 4, -100), 126);
-      if (bad) {   // out of the products; rows that see it get NaN through its score
+    if (odd != 0) {
+      int x = 0;
+      if (!usual && !bad) {   // 2^(kUnit + x): the largest element to [2^14, 2^15)
+        x = max((int)(largest >> 23) - 127 - 14 - kUnit, -120);
+        unit = pow2(-kUnit - x);
+      }
+      if (kV && bad) {        // out of the products; rows that see it get NaN through its score
 #pragma unroll
         for (int g = 0; g < G; ++g) s[g] = z[g] = 0.f;
       }
+      if (tile < tiles) (kV ? m.v_exp : m.k_exp)[key] = (int8_t)x;
+    }
+#pragma unroll
+    for (int g = 0; g < G; ++g) { s[g] *= unit; z[g] *= unit; }
+    if (kV) {
       const uint32_t bads = __ballot_sync(0xffffffffu, bad);
       if (lane == 0 && tile < tiles) {
-        m.v_exp[w] = e;
-        m.bad[w] = bads;
+        m.v_odd[w] = odd;
+        m.v_bad[w] = bads;
         mbar_arrive(bar0 + 8 * (kBarVMeta + (tile & (kMeta - 1))));
       }
-    } else {
-      const bool any = __any_sync(0xffffffffu, bad);
-      if (lane == 0 && tile < tiles) m.k_factor[w] = any ? -pow2(e) : pow2(e);
+    } else if (lane == 0 && tile < tiles) {
+      m.k_odd[w] = odd;
     }
   };
   // the block's queries are converted while the first keys and values are on their way
@@ -393,8 +397,6 @@ __device__ __forceinline__ void unpack_side(const dflash_kv4_cache& c, int b, in
     float cs[G], cz[G];
 #pragma unroll
     for (int g = 0; g < G; ++g) { cs[g] = s[g]; cz[g] = z[g]; }
-    const int ce = e;
-    const bool cwide = wide;
     if (kV) {
       prepare(t + 1);
       load_scales(t + 2, ns, nz);
@@ -414,13 +416,12 @@ __device__ __forceinline__ void unpack_side(const dflash_kv4_cache& c, int b, in
       for (int i = 1; i < G; ++i)
         if (i == g) { sg = cs[i]; zg = cz[i]; }
       const uint32_t row = smem_u32(buf + g * kSlab + key * 128);
-      if (kV && cwide) unpack_row<true>(c0, c1, sg, zg, ce, row, key);
-      else unpack_row<false>(c0, c1, sg, zg, ce, row, key);
+      unpack_row(c0, c1, sg, zg, row, key);
     }
     if (!ok) break;
     done(bar0 + 8 * (kV ? kBarVFull + (w >> 1) : kBarKFull));
     load(t + 1);
-    if (!kV) {   // a tile's factor is published with its codes: nothing waits for it before
+    if (!kV) {   // a tile's exponents are published with its codes: nothing waits for them before
       prepare(t + 1);
       load_scales(t + 2, ns, nz);
     }
@@ -439,10 +440,11 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_sdpa_tc_kernel(const SdpaArgs
   uint8_t* sRaw = sV + G * kSlab;                 // codes of the next tile: keys, then values
   uint64_t* bars = (uint64_t*)(sRaw + kKeys * D);
   Meta* meta = (Meta*)(bars + kBars);
-  int* sE = (int*)(meta + kMeta);                 // exponent of each query row, + kOdd if the row is not finite
-  float* sRef = (float*)(sE + kRows);             // [2][128] reference maximum of a row after a tile
-  int* sEv = (int*)(sRef + 2 * kRows);            // [2][4] exponent that O carries
-  uint32_t* holder = (uint32_t*)(sEv + 8);
+  float* sRef = (float*)(meta + kMeta);           // reference maximum of a row, handed from tile to tile
+  int16_t* sE = (int16_t*)(sRef + kRows);     // exponent of each query row, + kOdd if the row is not finite
+  int8_t* sEv = (int8_t*)(sE + kRows);            // exponent that a row of O carries
+  int* sOwn = (int*)(sEv + kRows);                // [4] whether some row of 32 carries one that is not 0
+  uint32_t* holder = (uint32_t*)(sOwn + 4);
   float2* sEnd = (float2*)sRaw;                   // [2][128] reference and sum of either half of the softmax, at the end
   const uint32_t bar0 = smem_u32(bars);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -532,7 +534,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_sdpa_tc_kernel(const SdpaArgs
       }
       *place = make_uint4(p[0], p[1], p[2], p[3]);
       const bool is_odd = kMask >= 2 && (__ballot_sync(0xffffffffu, odd != 0.f) >> (lane & ~(kLanes - 1)) & (0xFFFFFFFFu >> (32 - kLanes))) != 0;
-      if (j == 0) sE[r] = is_odd ? eq + kOdd : eq;
+      if (j == 0) sE[r] = (int16_t)(is_odd ? eq + kOdd : eq);
     }
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     __syncwarp();
@@ -597,9 +599,14 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_sdpa_tc_kernel(const SdpaArgs
     query_rows();
     bool ok = wait_warp(bar0 + 8 * kBarQ, 0);
     if (!ok) atomicCAS(err, 0, 62 | (10 << 8));
-    const int eq = sE[r];
-    const float c_row = fabsf(a.scale) * pow2(eq >= kOdd / 2 ? eq - kOdd : eq);
-    const bool odd = __any_sync(0xffffffffu, eq >= kOdd / 2);
+    // scores stay in the products' unit (additive masks: natural units) up to their difference to the reference, so that scores of
+    // any size tell their order; the unit is never 0 (a scale of 0): a hidden score stays -inf under it
+    auto unit_of_scores = [&]() {
+      const int eq = sE[r];
+      return fminf(fmaxf(fabsf(a.scale) * pow2(eq >= kOdd / 2 ? eq - kOdd : eq) * pow2(kUnit), 1e-37f), 2e38f);
+    };
+    const bool odd = kMask >= 2 && __any_sync(0xffffffffu, sE[r] >= kOdd / 2);
+    const float c = kMask >= 2 ? unit_of_scores() : 1.f, cl = (kMask >= 2 ? 1.f : unit_of_scores()) * kLog2e;
     // last key the row sees; rows behind the last one compute what nobody reads
     const int lim = row_ok ? min(len - a.T + t, hi - 1) : live ? hi - 1 : -1;
     long long mat = row_ok ? b * a.m_sb + h * a.m_sh + t * a.m_st : 0;   // its mask row, or that of the warp's first row
@@ -607,29 +614,45 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_sdpa_tc_kernel(const SdpaArgs
     if (!row_ok) mat = mat0;
     const bool shared = kMask == 1 && __all_sync(0xffffffffu, mat == mat0);
     float m_l = -INFINITY, l = 0.f;   // this half's sum and the reference it is relative to
-    for (int i = group; i < tiles && ok; i += 2) {
+    // A tile; false where nothing may follow it.  The usual form gives up, with nothing changed, at the first tile that holds unusual keys
+    // or values or whose rows carry exponents; from there on the general form takes the range, tile after tile.  What those need goes
+    // through tensor memory in rolled loops.  (In one form with branches the usual tiles took 3 to 5 % longer.)
+    bool placed = false;   // the tile's scores have their mask already
+    auto tile = [&](int i, auto general) -> bool {
+      constexpr bool kGeneral = decltype(general)::value;
       const int n0 = order.base(i >> 1) + ((i & 1) * kTile ^ order.flip(i >> 1));
       uint32_t bits[2];                  // the mask, on its way before the scores are waited for (fp32: below)
       uint32_t words[(kMask == 3 ? 16 : kTile / 2) + 4];
       if constexpr (kMask == 1) mask_bits(a, mat, shared, n0, lim, hi, bits);
       if constexpr (kMask == 2) mask_entries<T, kTile / 2>(a, mat, n0, lim, words);
       if constexpr (kMask == 3) mask_entries<float, 16>(a, mat, n0, lim, words);
-      if (!wait_warp(bar0 + 8 * (kBarS + ((i >> 1) & 1)), (i >> 2) & 1)) { atomicCAS(err, 0, 62 | (6 << 8)); ok = false; break; }
+      if (!wait_warp(bar0 + 8 * (kBarS + ((i >> 1) & 1)), (i >> 2) & 1)) { atomicCAS(err, 0, 62 | (6 << 8)); ok = false; return false; }
       fence_after();
       if (!live) {   // P is whatever is there: lanes of their own
         fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(bar0 + 8 * (kBarP + (i & 3)));
-        continue;
+        return true;
       }
       const uint32_t s_col = tmem + lanes + 64u * (i & 3);
       const Meta& mt = meta[(i >> 1) & (kMeta - 1)];
       const int blk = 2 * (i & 1);   // the tile's 32-key blocks in `mt`: blk and blk + 1
-      // never 0 (a scale of 0): a hidden score stays -inf under it
-      const float kf0 = mt.k_factor[blk], kf1 = mt.k_factor[blk + 1];
-      float c[2] = {fmaxf(c_row * fabsf(kf0), 1e-37f), fmaxf(c_row * fabsf(kf1), 1e-37f)};
-      if (kMask >= 2) {   // scaled score + mask back into place, 16 at a time: with the entries, all 64 would not fit the registers
-        const bool careful = odd || kf0 < 0.f || kf1 < 0.f || __any_sync(0xffffffffu, c[0] > 3e38f || c[1] > 3e38f);
+      const bool k_odd = *(const uint64_t*)(mt.k_odd + blk) != 0;
+      if (!kGeneral && k_odd) return false;
+      if (kGeneral && k_odd) {
+#pragma unroll 1
+        for (int e0 = 0; e0 < kTile; e0 += 16) {
+          uint32_t x[16];
+          ld16(s_col + e0, x);
+          wait_ld();
+#pragma unroll
+          for (int e = 0; e < 16; ++e) x[e] = __float_as_uint(__uint_as_float(x[e]) * own_power(mt, 32 * blk + e0 + e));
+          st16(s_col + e0, x);
+        }
+        wait_st();
+      }
+      if (kMask >= 2 && !(kGeneral && placed)) {   // scaled score + mask back into place, 16 at a time: with the entries, all 64 would not fit the registers
+        const bool careful = odd || k_odd || __any_sync(0xffffffffu, c > 1e28f);
         uint32_t x[2][16];
         ld16(s_col, x[0]);
 #pragma unroll
@@ -647,10 +670,9 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_sdpa_tc_kernel(const SdpaArgs
               if (entry(e) == -INFINITY) y[e] = 0;
           }
 #pragma unroll
-          for (int e = 0; e < 16; ++e) y[e] = __float_as_uint(fmaf(__uint_as_float(y[e]), c[e0 >> 5], entry(e)));
+          for (int e = 0; e < 16; ++e) y[e] = __float_as_uint(fmaf(__uint_as_float(y[e]), c, entry(e)));
           st16(s_col + e0, y);
         }
-        c[0] = c[1] = 1.f;
         wait_st();
       }
       uint32_t v[kTile];
@@ -660,7 +682,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_sdpa_tc_kernel(const SdpaArgs
       const bool plain = __all_sync(0xffffffffu, n0 + kTile - 1 <= lim && (kMask != 1 || (bits[0] & bits[1]) == 0xFFFFFFFFu));
       if (!wait_warp(bar0 + 8 * (kBarVMeta + ((i >> 1) & (kMeta - 1))), (i / (2 * kMeta)) & 1)) { atomicCAS(err, 0, 62 | (13 << 8)); ok = false; }
       wait_ld();
-      if (!ok) break;
+      if (!ok) return false;
       if (!plain) {
 #pragma unroll
         for (int q = 0; q < 2; ++q) {
@@ -671,41 +693,58 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_sdpa_tc_kernel(const SdpaArgs
             if (!((seen >> e) & 1)) v[32 * q + e] = 0xFF800000u;
         }
       }
-      if ((mt.bad[blk] | mt.bad[blk + 1]) != 0) {   // a value that is not finite makes the rows NaN that see its key
-#pragma unroll
-        for (int e = 0; e < kTile; ++e)
-          if (((mt.bad[blk + (e >> 5)] >> (e & 31)) & 1) && v[e] != 0xFF800000u) v[e] = 0x7FC00000u;
+      bool own = *(const uint64_t*)(mt.v_odd + blk) != 0;   // the rows' exponents come into play
+      if (!kGeneral && own) {
+        placed = kMask >= 2;
+        return false;
       }
       float top = -INFINITY;
-#pragma unroll
-      for (int q = 0; q < 2; ++q) {
+      {
         float t0 = -INFINITY, t1 = -INFINITY;
 #pragma unroll
-        for (int e = 32 * q; e < 32 * q + 32; e += 4) {
+        for (int e = 0; e < kTile; e += 4) {
           t0 = fmaxf(fmaxf(t0, __uint_as_float(v[e])), __uint_as_float(v[e + 1]));
           t1 = fmaxf(fmaxf(t1, __uint_as_float(v[e + 2])), __uint_as_float(v[e + 3]));
         }
-        t0 = fmaxf(t0, t1);
-        top = fmaxf(top, t0 * c[q]);
+        top = fmaxf(t0, t1);
       }
       // ---- the row's reference: what the tile before left, moved when this tile exceeds it by 8 octaves ----
-      float m = -INFINITY;
-      int ev = -200;
+      float m = -INFINITY, ev = 0.f;
       if (i > 0) {
-        if (!wait_warp(bar0 + 8 * (kBarM + 4 * (group ^ 1) + part), ((i - 1) >> 1) & 1)) { atomicCAS(err, 0, 62 | (12 << 8)); ok = false; break; }
-        m = sRef[(group ^ 1) * kRows + r];
-        ev = sEv[(group ^ 1) * 4 + part];
+        if (!wait_warp(bar0 + 8 * (kBarM + 4 * (group ^ 1) + part), ((i - 1) >> 1) & 1)) { atomicCAS(err, 0, 62 | (12 << 8)); ok = false; return false; }
+        m = sRef[r];
+        if (sOwn[part] != 0) {
+          if (!kGeneral) {
+            placed = kMask >= 2;
+            return false;
+          }
+          own = true;
+          ev = (float)sEv[r];
+        }
       }
-      const int ev0 = mt.v_exp[blk], ev1 = mt.v_exp[blk + 1], ev_tile = max(ev0, ev1);
-      if (__any_sync(0xffffffffu, top > m + kMaxStep) || ev_tile > ev) {
-        const float m_new = fmaxf(m, top);
-        // two octaves of room: the exponents of a sequence's blocks differ by one or two, and each growth rescales O
-        const int ev_new = ev_tile > ev ? ev_tile + 2 : ev;
-        const float f = m_new == -INFINITY ? 1.f : ex2((m - m_new) * kLog2e);
-        const float fo = f * pow2(max(ev - ev_new, -126));
-        m = m_new;
+      bool grow = (top - m) * cl > 8.f;
+      const float now = grow ? top : m;
+      float ev_now = ev;
+      if (kGeneral && own) {
+#pragma unroll
+        for (int e0 = 0; e0 < kTile; e0 += 16) st16(s_col + e0, v + e0);
+        wait_st();
+        float d = -INFINITY;   // octaves of the row's largest p 2^x; NaN counts as none
+#pragma unroll 1
+        for (int e0 = 0; e0 < kTile; e0 += 16) {
+          uint32_t x[16];
+          ld16(s_col + e0, x);
+          wait_ld();
+#pragma unroll
+          for (int e = 0; e < 16; ++e) d = fmaxf(d, fmaf(__uint_as_float(x[e]) - now, cl, own_exponent(mt, 32 * blk + e0 + e)));
+        }
+        grow = grow || d > ev + 9.f;
+        if (grow) ev_now = fminf(fmaxf(fmaxf(ceilf(d), ev + floorf((m - now) * cl)), -126.f), 126.f);
+      }
+      if (__any_sync(0xffffffffu, grow)) {
+        const float fo = grow ? ex2(fmaf(m - now, cl, ev - ev_now)) : 1.f;   // a row that does not grow keeps every bit
         if (i > 0) {
-          if (!wait_warp(bar0 + 8 * (kBarO + ((i - 1) & 3)), ((i - 1) >> 2) & 1)) { atomicCAS(err, 0, 62 | (7 << 8)); ok = false; break; }
+          if (!wait_warp(bar0 + 8 * (kBarO + ((i - 1) & 3)), ((i - 1) >> 2) & 1)) { atomicCAS(err, 0, 62 | (7 << 8)); ok = false; return false; }
           fence_after();
 #pragma unroll 1
           for (int c0 = 0; c0 < D; c0 += 16) {
@@ -718,36 +757,57 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_sdpa_tc_kernel(const SdpaArgs
           }
           wait_st();
         }
-        ev = ev_new;
       }
-      sRef[group * kRows + r] = m;
-      if (lane == 0) sEv[group * 4 + part] = ev;
+      m = now;
+      sRef[r] = m;
+      if (kGeneral && own) sEv[r] = (int8_t)ev_now;
+      if ((kGeneral && own) || i == 0) {
+        const bool any = kGeneral && __any_sync(0xffffffffu, ev_now != 0.f);
+        if (lane == 0) sOwn[part] = any;
+      }
       __syncwarp();
       if (lane == 0) mbar_arrive(bar0 + 8 * (kBarM + 4 * group + part));
       if (m != m_l) {
-        if (m_l != -INFINITY) l *= ex2((m_l - m) * kLog2e);
+        if (m_l != -INFINITY) l *= ex2((m_l - m) * cl);
         m_l = m;
       }
       // ---- P ----
       const float ref = m == -INFINITY ? 0.f : m;
+      const uint64_t cl2 = pair(cl, cl), ref2 = pair(-ref, -ref), shift2 = pair(kPShift, kPShift);
+      uint64_t sum = 0;
+      if (kGeneral && own) {
+        const float off = kPShift - ev_now;
+#pragma unroll 1
+        for (int e0 = 0; e0 < kTile; e0 += 16) {
+          uint32_t x[16], w[8];
+          ld16(s_col + e0, x);
+          wait_ld();
+          const uint32_t bad = mt.v_bad[blk + (e0 >> 5)] >> (e0 & 31);
 #pragma unroll
-      for (int q = 0; q < 2; ++q) {
-        const float shift = kPShift + (float)max((q ? ev1 : ev0) - ev, -100);   // P carries V's power of two
-        const float cl = c[q] * kLog2e, off = shift - ref * kLog2e;
-        const uint64_t cl2 = pair(cl, cl), off2 = pair(off, off);
-        uint64_t sum = 0;
+          for (int e = 0; e < 16; e += 2) {
+            // a value that is not finite makes the rows NaN that see its key
+            const float x0 = ((bad >> e) & 1) && x[e] != 0xFF800000u ? __uint_as_float(0x7FC00000u) : __uint_as_float(x[e]);
+            const float x1 = ((bad >> e) & 2) && x[e + 1] != 0xFF800000u ? __uint_as_float(0x7FC00000u) : __uint_as_float(x[e + 1]);
+            const uint64_t d2 = add2(pair(x0, x1), ref2);
+            float p0, p1;
+            unpair(fma2(d2, cl2, shift2), p0, p1);
+            sum = add2(sum, pair(ex2(p0), ex2(p1)));
+            const int key = 32 * blk + e0 + e;
+            unpair(fma2(d2, cl2, pair(off + own_exponent(mt, key), off + own_exponent(mt, key + 1))), p0, p1);
+            const __half2 p = __floats2half2_rn(ex2(p0), ex2(p1));
+            w[e >> 1] = *(const uint32_t*)&p;
+          }
+          st8(s_col + (e0 >> 1), w);   // over columns that have been read
+        }
+      } else {
 #pragma unroll
-        for (int e0 = 32 * q; e0 < 32 * q + 32; e0 += 16) {
+        for (int e0 = 0; e0 < kTile; e0 += 16) {
           uint32_t w[8];
 #pragma unroll
           for (int e = 0; e < 16; e += 2) {
+            const uint64_t d2 = add2(pair(__uint_as_float(v[e0 + e]), __uint_as_float(v[e0 + e + 1])), ref2);
             float p0, p1;
-            if (kMask >= 2) {   // scores may be the lowest finite value: their difference first
-              p0 = fmaf(__uint_as_float(v[e0 + e]) - ref, kLog2e, shift);
-              p1 = fmaf(__uint_as_float(v[e0 + e + 1]) - ref, kLog2e, shift);
-            } else {
-              unpair(fma2(pair(__uint_as_float(v[e0 + e]), __uint_as_float(v[e0 + e + 1])), cl2, off2), p0, p1);
-            }
+            unpair(fma2(d2, cl2, shift2), p0, p1);
             p0 = ex2(p0);
             p1 = ex2(p1);
             sum = add2(sum, pair(p0, p1));
@@ -756,15 +816,22 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_sdpa_tc_kernel(const SdpaArgs
           }
           st8(s_col + (e0 >> 1), w);   // over columns that are in registers
         }
+      }
+      {
         float sum0, sum1;
         unpair(sum, sum0, sum1);
-        l = fmaf(sum0 + sum1, ex2(-shift), l);
+        l = fmaf(sum0 + sum1, 1.f / 64.f, l);
       }
       wait_st();
       fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(bar0 + 8 * (kBarP + (i & 3)));
-    }
+      placed = false;
+      return true;
+    };
+    int i = group;
+    while (i < tiles && ok && tile(i, std::false_type{})) i += 2;
+    while (i < tiles && ok && tile(i, std::true_type{})) i += 2;
     // ---- epilogue: either half of the softmax takes half of the channels; a warp's 32 rows go through shared memory (all of Q, K
     // and V is spent), so that they leave as whole lines ----
     // The last product.  First the last scores: with an odd number of tiles the second half has none of that pair and may be early, while
@@ -777,15 +844,15 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_sdpa_tc_kernel(const SdpaArgs
     named_bar_sync(1, 256);
     const bool have = tiles > 0 && ok;
     if (live) {
-      const float m = tiles > 0 ? sRef[((tiles - 1) & 1) * kRows + r] : -INFINITY;
-      const int ev = tiles > 0 ? sEv[((tiles - 1) & 1) * 4 + part] : 0;
+      const float m = tiles > 0 ? sRef[r] : -INFINITY;
+      const int ev = tiles > 0 && sOwn[part] != 0 ? sEv[r] : 0;
       l = 0.f;
 #pragma unroll
       for (int g = 0; g < 2; ++g) {
         const float2 x = sEnd[g * kRows + r];
-        l = fmaf(x.y, x.x == -INFINITY ? 1.f : ex2((x.x - m) * kLog2e), l);
+        l = fmaf(x.y, x.x == -INFINITY ? 1.f : ex2((x.x - m) * cl), l);
       }
-      const float undo = pow2(min(max(ev - (int)kPShift, -126), 127));
+      const float undo = pow2(ev);   // after 2^(kUnit - kPShift)
       const bool last = a.splits == 1;
       const float inv = l == 0.f ? 1.f : 1.f / l, nan = l * 0.f;   // a row that sees nothing yields zeros; NaN reaches the whole row
       const size_t at = ((size_t)bhk * a.rows + row) * a.splits + split;
@@ -800,7 +867,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_sdpa_tc_kernel(const SdpaArgs
         }
         float y[32];   // back to the channels' order
 #pragma unroll
-        for (int e = 0; e < 32; ++e) y[(e & ~7) + ((e & 1) << 2) + ((e & 7) >> 1)] = have ? __uint_as_float(o[e]) * undo : 0.f;
+        for (int e = 0; e < 32; ++e) y[(e & ~7) + ((e & 1) << 2) + ((e & 7) >> 1)] = have ? __uint_as_float(o[e]) * pow2(kUnit - (int)kPShift) * undo : 0.f;
         if (last) {
 #pragma unroll
           for (int e = 0; e < 32; e += 8) {
@@ -815,7 +882,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_sdpa_tc_kernel(const SdpaArgs
         }
       }
       if (row_ok && !last && group == 0) {
-        a.part_m[at] = m;
+        a.part_m[at] = kMask >= 2 ? m : m * unit_of_scores();
         a.part_l[at] = l;
       }
       const int bytes = D / 2 * (last ? 2 : 4);   // of half a row: 512, 256 or 128
@@ -841,7 +908,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_sdpa_tc_kernel(const SdpaArgs
 
 template <typename T, int D>
 int launch(const SdpaArgs& a, cudaStream_t st, int device) {
-  constexpr size_t tiles = (size_t)3 * (D / kGroup) * kSlab, rest = (size_t)kKeys * D + kBars * 8 + kMeta * sizeof(Meta) + kRows * 12 + 48;
+  constexpr size_t tiles = (size_t)3 * (D / kGroup) * kSlab, rest = (size_t)kKeys * D + kBars * 8 + kMeta * sizeof(Meta) + kRows * 7 + 32;
   static_assert(kRows * (D * 4 + 16) <= tiles, "the epilogue's rows fit where Q, K and V were");
   constexpr size_t smem = tiles + rest;
   static_assert(smem <= 227 * 1024, "shared memory");

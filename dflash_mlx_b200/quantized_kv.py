@@ -63,9 +63,9 @@ def quantized_kv_sdpa(queries, k_cache, v_cache, scale: float, lengths: Union[in
     the device.  Row ``t`` of sequence ``b`` sees position ``n`` iff ``n <= lengths[b] - T + t`` (and ``n < lengths[b]``).
     ``max_length`` (default: the int, or the capacity) bounds the lengths: positions from it on are not read.  ``mask`` is a bool
     (False hides) or additive (the queries' dtype or float32; -inf hides) tensor that broadcasts to ``[B, Hq, T, max_length]``;
-    it is read in place.  Returns ``[B, Hq, T, D]``; a row that sees nothing is zero.  Hidden keys and values never reach a row,
-    whatever they hold; a visible value with a non-finite scale or bias makes its row NaN.  ``num_splits`` fixes the number of
-    key ranges (0: from the SM count).
+    it is read in place.  Returns ``[B, Hq, T, D]``; a row that sees nothing is zero.  Hidden keys and values change no bit of a
+    row, whatever they hold; a visible value with a scale or bias that is not finite makes its row NaN.  ``num_splits`` fixes the
+    number of key ranges (0: from the SM count).
     """
     return (_lib._native or _lib.native()).kv4_sdpa(queries, *k_cache, *v_cache, scale, lengths, mask, max_length, num_splits)
 

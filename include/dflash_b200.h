@@ -426,8 +426,9 @@ DFLASH_API int dflash_kv4_read(const dflash_kv4_cache* k_cache, const dflash_kv4
  *            captured graph serves every length up to it); positions from max_length on are never read.
  *   mask     element (b,h,t,n) at the four strides (elements; 0 broadcasts); mask_kind 0 = none, 1 = bytes (0 hides),
  *            2 = additive in dtype, 3 = additive f32.  -inf hides; a finite value, however low, is added.
- *   A row that sees nothing yields zeros.  Keys and values that a row does not see never reach it, NaN and infinities
- *   included; a visible value row with a non-finite scale or bias makes the whole output row NaN.
+ *   A row that sees nothing yields zeros.  Keys and values that a row does not see change no bit of it, NaN, infinities and the
+ *   type's largest values included; a visible value with a scale or bias that is not finite, or whose codes reach beyond f32
+ *   (scale * 15 + bias), makes the whole output row NaN.
  *   num_splits: key ranges, 0..1024; 0 = chosen from the SM count.  workspace: dflash_kv4_sdpa_workspace_bytes() bytes of device memory, 16-byte
  *   aligned, contents irrelevant, not shared by calls that can overlap. */
 DFLASH_API size_t dflash_kv4_sdpa_workspace_bytes(int B, int Hq, int Hk, int T, int D, int max_length, int num_splits);

@@ -1,4 +1,4 @@
-"""The 4-bit KV cache's attention where keys and values differ in size as far as their type allows."""
+"""The 4-bit KV cache's attention where keys and values differ in size as far as their type allows, in both kernels."""
 import math
 
 import pytest
@@ -12,8 +12,8 @@ from tests.test_quantized_kv_gpu import TOL, check_rows, gen, ints, make_cache, 
 
 DEV = "cuda"
 BF16, F16 = torch.bfloat16, torch.float16
-# T, keys, capacity: up to 8 and up to 16 rows of 4 heads
-KERNELS = {"eight": (2, 190, 220), "sixteen": (3, 190, 220)}
+# T, keys, capacity: up to 8 and up to 16 rows of 4 heads, and many rows under a bound on the lengths that sends them to the tcgen05 kernel on any SM count up to 160
+KERNELS = {"eight": (2, 190, 220), "sixteen": (3, 190, 220), "many": (40, 1290, 13000)}
 
 
 def part_of(k, v, name):
