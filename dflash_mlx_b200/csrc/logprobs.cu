@@ -92,8 +92,11 @@ template <typename T, uint32_t kInf> struct Elem16 {
       w[i] = (w[i] & ~m) | ((kInf | (kInf << 16)) & m);
     }
   }
-  // whether clamped() keeps a thread's sums right: the clamp (-1e30, fp16: -65504) has probability 0 next to the maximum m
-  __device__ static __forceinline__ bool can_clamp(float m, float scale) { return scale >= 0.01f && scale < 1e6f && m > -40000.f && m < 1e30f; }
+  // whether clamped() keeps a thread's sums right: the clamp (-1e30, fp16: -65504) has probability 0 next to the maximum m, and the
+  // rounding of m * scale, which every y of the thread carries until the end, is no more than 2^-5 octaves
+  __device__ static __forceinline__ bool can_clamp(float m, float scale) {
+    return scale >= 0.01f && scale < 1e6f && m > -40000.f && fabsf(m * scale) < 1048576.f;
+  }
   __device__ static __forceinline__ uint32_t clamped(uint32_t w) {
     const uint32_t low = kInf == 0xFF80u ? 0xF149F149u : 0xFBFFFBFFu;
     const auto m = __hmax2_nan(as_pair(w, T()), as_pair(low, T()));
@@ -260,7 +263,7 @@ __global__ void __launch_bounds__(kThreads, 3) token_logprobs_kernel(const Args 
     const float top = E::max_of(raw);   // of this pass's elements; NaN is passed over
     bool nan = false;                   // whether an element was NaN or +inf
     if (base + warp * 32 >= v1) {   // the warp has nothing of this pass
-    } else if (E::can_clamp(top, a.scale) && run.m < 1e30f) {   // hidden elements become a finite value of probability 0, two at a time
+    } else if (E::can_clamp(top, a.scale)) {   // hidden elements become a finite value of probability 0, two at a time
       if (top > run.m) {                // the thread's reference moves: y' = x scale - at, at = rounded(reference scale)
         const float to = top * a.scale, d = run.m == -INFINITY ? 0.f : at - to, f = exp2f(d);
         run.w = fmaf(d, run.l, run.w) * f;
