@@ -342,7 +342,7 @@ PyObject* py_logprobs(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
   const int64_t k = integer(a[2], "top_k");
   if (V < 1 || k < 0 || k > kMaxTopK || k > V) refuse("top_k=", k, " outside 0..min(", kMaxTopK, ", V=", V, ")");
   const double temperature = number(a[3], "temperature");
-  if (!(temperature >= 1e-30) || !std::isfinite((float)temperature)) refuse("temperature must be finite and at least 1e-30, got ", temperature);
+  if (!(temperature >= 1e-30 && temperature <= 1e38)) refuse("temperature outside 1e-30..1e38, got ", temperature);
   if (suppress && (suppress->scalar_type() != at::kBool || suppress->dim() != 1 || suppress->size(0) != V))
     refuse("suppress must be a bool tensor [V] = [", V, "]");
   const c10::cuda::CUDAGuard guard(d.dev);

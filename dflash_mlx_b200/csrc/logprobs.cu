@@ -542,7 +542,8 @@ extern "C" int dflash_token_logprobs(const void* logits, long long ld, const int
   if (R < 0 || V < 1 || ld < V) return fail(DFLASH_ERR_BAD_SHAPE, "token_logprobs: R=%d V=%d ld=%lld", R, V, ld);
   if (V > 0x7fffffff - 64 * 1024) return fail(DFLASH_ERR_BAD_SHAPE, "token_logprobs: V=%d too large", V);
   if (top_k < 0 || top_k > lp::kMaxK || top_k > V) return fail(DFLASH_ERR_BAD_SHAPE, "token_logprobs: top_k=%d outside 0..min(%d, V)", top_k, lp::kMaxK);
-  if (!(temperature >= 1e-30f) || !(temperature <= 3.0e38f)) return fail(DFLASH_ERR_BAD_ARG, "token_logprobs: temperature must be finite and at least 1e-30");
+  // log2(e) / temperature has to be a normal number: the kernels flush others to 0, and -inf * 0 is NaN
+  if (!(temperature >= 1e-30f) || !(temperature <= 1e38f)) return fail(DFLASH_ERR_BAD_ARG, "token_logprobs: temperature outside 1e-30..1e38");
   if (R == 0) return DFLASH_OK;
   if (!logits || !tokens || !token_logprob || (top_k > 0 && (!top_logprobs || !top_ids))) return fail(DFLASH_ERR_BAD_ARG, "token_logprobs: null operand");
   const int size = dtype == DFLASH_F32 ? 4 : 2;

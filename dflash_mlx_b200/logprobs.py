@@ -23,7 +23,7 @@ class TokenLogprobs(NamedTuple):
 def token_logprobs(logits, tokens, *, top_k: int = 0, temperature: float = 1.0,
                    suppress: Optional[torch.Tensor] = None) -> TokenLogprobs:
     """``logits`` ``[..., V]`` (bf16, fp16 or fp32); ``tokens`` ``[...]`` (int32 or int64); p = softmax(logits / temperature),
-    ``temperature`` finite and at least 1e-30.
+    ``temperature`` from 1e-30 to 1e38.
 
     ``top_k`` (0..min(32, V)) alternatives per row.  ``suppress`` (bool ``[V]``): those tokens have probability 0.  A token
     outside ``[0, V)`` has the log-probability NaN.  A row with nothing but ``-inf`` yields ``-inf`` and the entropy 0; a row

@@ -443,7 +443,7 @@ DFLASH_API int dflash_kv4_sdpa(const void* q, const long long* q_strides, const 
  *   logits    dtype (bf16, f16 or f32) [R,V], rows `ld` elements apart;  x = logits / temperature, p = softmax(x)
  *   tokens    device int[R]; token_logprob[r] = log p[tokens[r]] (NaN for a token outside [0,V))
  *   suppress  uint8[V] of 0 and 1, or NULL: tokens with 1 have probability 0 (log-probability -inf)
- *   temperature finite, at least 1e-30
+ *   1e-30 <= temperature <= 1e38
  *   entropy[r] = -sum p log p in nats (may be NULL)
  *   top_logprobs f32[R,top_k], top_ids int[R,top_k]: the top_k tokens by logit, highest first, ties to the lower index;
  *             0 <= top_k <= min(32, V); both NULL when top_k = 0

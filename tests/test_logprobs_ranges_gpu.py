@@ -1,4 +1,4 @@
-"""Token log-probabilities of logits at the ends of their types' ranges."""
+"""Token log-probabilities of logits and temperatures at the ends of their ranges."""
 import math
 
 import pytest
@@ -7,10 +7,25 @@ import torch
 pytestmark = pytest.mark.gpu
 
 from dflash_mlx_b200 import logprobs  # noqa: E402
-from tests.test_logprobs_gpu import check, ints, logits  # noqa: E402
+from tests.test_logprobs_gpu import TYPES, check, ints, logits  # noqa: E402
 
 DEV = "cuda"
 T16 = [torch.bfloat16, torch.float16]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("V", [100, 9001])
+def test_largest_temperatures(V, dtype):
+    """Up to 1e38 a row is nearly uniform over what is not hidden; beyond, log2(e) / temperature leaves the normal numbers: refused."""
+    x = logits(4, V, dtype, seed=V)
+    x[1, 3] = -math.inf
+    suppress = torch.zeros(V, dtype=torch.bool, device=DEV)
+    suppress[7] = True
+    for temperature in (1e30, 1e38):
+        check(x, ints(0, 3, 7, V - 1), 4, temperature, suppress)
+    for temperature in (1.1e38, 1.3e38, 2.9e38, 3.2e38, 1e39):
+        with pytest.raises(ValueError, match="temperature"):
+            logprobs.token_logprobs(x, ints(0, 1, 2, 3), temperature=temperature)
 
 
 # The products' fp32 sums see differences to the row's maximum only, so the bound of check() holds however large the logits are:
