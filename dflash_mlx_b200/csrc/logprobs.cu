@@ -436,8 +436,7 @@ __global__ void __launch_bounds__(kThreads, 3) token_logprobs_kernel(const Args 
         __syncthreads();
         rank_into(sh.top, sh.list, sh.count, a.k);
       }
-      if (n > 64) __syncthreads();
-      else __syncwarp();
+      __syncthreads();   // every warp has read the count
       // the next pass: only what beats the k-th best (its own index is lower); -inf while there are fewer than k
       if (tid == 0) {
         sh.count = 0;
