@@ -82,7 +82,7 @@ _native = None
 
 
 def native():
-    """The C++ binding (csrc/binding.cpp), bound to this library's functions; built first if absent."""
+    """The C++ binding (csrc/binding.cpp), bound to this library's functions; built first if absent or built for another torch."""
     global _native
     if _native is None:
         handle = lib()
@@ -90,8 +90,8 @@ def native():
             if _native is None:
                 import importlib.util
 
-                from .csrc.build import BINDING, build_binding
-                if not BINDING.exists():
+                from .csrc.build import BINDING, binding_fits, build_binding
+                if not binding_fits():
                     build_binding()
                 spec = importlib.util.spec_from_file_location("dflash_mlx_b200._native", BINDING)
                 module = importlib.util.module_from_spec(spec)
