@@ -139,7 +139,7 @@ struct Rows {
   explicit Rows(const at::Tensor& x) : t(x) {
     bool ok = t.stride(3) == 1 && (uintptr_t)t.data_ptr() % 16 == 0;
     for (int i = 0; i < 3; ++i) ok = ok && (t.size(i) <= 1 || t.stride(i) % 8 == 0);
-    if (!ok) t = t.contiguous();
+    if (!ok) t = t.clone(at::MemoryFormat::Contiguous);   // contiguous() would keep a contiguous tensor where it is
     for (int i = 0; i < 3; ++i) strides[i] = t.size(i) > 1 ? t.stride(i) : 0;
   }
 };

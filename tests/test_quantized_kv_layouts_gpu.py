@@ -1,0 +1,28 @@
+"""The 4-bit KV cache's arguments at unusual places in memory: what is copied, what is refused."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+from dflash_mlx_b200 import quantized_kv as qkv  # noqa: E402
+from oracle import quantized_kv as ref  # noqa: E402
+from tests.test_quantized_kv_gpu import ints, make_cache, no_device_error, states  # noqa: E402, F401
+
+DEV = "cuda"
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("off", [1, 3, 4, 8])
+def test_contiguous_rows_off_their_boundary(off, dtype):
+    """Contiguous tensors that start between two 16-byte boundaries are copied like any others that the kernels cannot read."""
+    B, Hk, T, D, n = 2, 2, 5, 128, 40
+    k_cache, v_cache = make_cache(B, Hk, n, D, dtype)
+    flat = states((off + B * Hk * T * D,), dtype, 1)
+    x = flat[off:].view(B, Hk, T, D)
+    assert x.is_contiguous()
+    qkv.quantized_kv_write(x, x, k_cache, v_cache, ints(3, 7))
+    want = ref.quantise(x)
+    for c in (k_cache, v_cache):
+        for got, part in zip(c, want):
+            assert torch.equal(got[0, :, 3:8], part[0]) and torch.equal(got[1, :, 7:12], part[1])
+    assert torch.equal(qkv.quantized_kv_sdpa(x, k_cache, v_cache, 0.1, n), qkv.quantized_kv_sdpa(x.clone(), k_cache, v_cache, 0.1, n))
