@@ -15,6 +15,7 @@
 #include <cmath>
 #include <sstream>
 #include <string>
+#include <utility>
 
 #include "../../include/dflash_b200.h"
 
@@ -132,6 +133,22 @@ Cache cache(PyObject* const* a, Device* d) {   // six arguments: key codes, scal
   return c;
 }
 
+// A cache that is written: no place of it may belong to two sequences, heads or sides, whose blocks would race for it.
+void check_apart(PyObject* const* a) {
+  for (int i = 0; i < 6; ++i) {
+    const at::Tensor& x = THPVariable_Unpack(a[i]);
+    if (x.numel() == 0) return;
+    const int64_t block = x.size(2) * x.size(3);   // one head's positions, contiguous
+    int64_t n[2] = {x.size(0), x.size(1)}, s[2] = {x.stride(0), x.stride(1)};
+    for (int d = 0; d < 2; ++d) if (n[d] == 1) s[d] = 0;
+    if (s[0] > s[1]) { std::swap(s[0], s[1]); std::swap(n[0], n[1]); }
+    if ((n[0] > 1 && s[0] < block) || (n[1] > 1 && s[1] < (n[0] - 1) * s[0] + block))
+      refuse("a cache that is written must not repeat or overlap its sequences or heads");
+    for (int j = 0; j < i; ++j)
+      if (THPVariable_Unpack(a[j]).data_ptr() == x.data_ptr()) refuse("the arrays of a cache that is written must not be one another");
+  }
+}
+
 // Contiguous rows of D on 16-byte boundaries; anything else is copied.
 struct Rows {
   at::Tensor t;
@@ -183,10 +200,13 @@ PyObject* py_bind(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
   Py_RETURN_NONE;
 }
 
-PyObject* py_check_cache(PyObject*, PyObject* const* a, Py_ssize_t nargs) {   // the six arrays; on any device
+PyObject* py_check_cache(PyObject*, PyObject* const* a, Py_ssize_t nargs) {   // the six arrays, on any device; whether they are written
   BEGIN_CHECKED
+  const bool written = nargs == 7 && PyObject_IsTrue(a[6]) == 1;
+  if (nargs == 7) nargs = 6;
   NEED_ARGS(6)
   cache(a, nullptr);
+  if (written) check_apart(a);
   Py_RETURN_NONE;
   END_CHECKED
 }
@@ -202,10 +222,7 @@ PyObject* py_write(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
   const Cache c = cache(a + 2, &d);
   d.add(&offsets); d.add(counts);
   const Side& k = c.k;
-  for (int i = 2; i < 8; ++i) {
-    const at::Tensor& x = THPVariable_Unpack(a[i]);
-    if ((x.size(0) > 1 && x.stride(0) == 0) || (x.size(1) > 1 && x.stride(1) == 0)) refuse("a cache that is written must not repeat its sequences or heads");
-  }
+  check_apart(a + 2);
   if (keys.dim() != 4 || keys.sizes() != values.sizes() || keys.size(0) != k.B || keys.size(1) != k.Hk || keys.size(3) != k.D)
     refuse("keys and values must be [B, Hk, T, D] = [", k.B, ", ", k.Hk, ", T, ", k.D, "], got ", keys.sizes(), " and ", values.sizes());
   if (keys.scalar_type() != k.type || values.scalar_type() != k.type) refuse("keys and values must have the cache's dtype ", k.type);

@@ -406,7 +406,8 @@ typedef struct dflash_kv4_cache {
  *   scale = dtype(max/15 - min/15), bias = min, code = clamp(round((x - bias) / scale), 0, 15) per 64 channels (ties to
  *   even; scale 0: code 0).  A group that holds a NaN or an infinity is stored as scale = bias = NaN, code 0: it reads back as
  *   NaN.  A row whose position is outside [0, capacity) is NOT stored and sets device error 61 | (t << 8).
- *   D in {128,256}; dtype bf16 or f16.  B = 0 or T = 0 does nothing. */
+ *   No place of the caches may belong to two sequences, heads or sides.  D in {128,256}; dtype bf16 or f16.  B = 0 or T = 0 does
+ *   nothing. */
 DFLASH_API int dflash_kv4_write(const void* keys, const long long* key_strides, const void* values,
                                 const long long* value_strides, const dflash_kv4_cache* k_cache,
                                 const dflash_kv4_cache* v_cache, const int* offsets, const int* counts, int B, int Hk, int T,
