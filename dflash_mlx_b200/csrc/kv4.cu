@@ -1005,6 +1005,19 @@ extern "C" size_t dflash_kv4_sdpa_workspace_bytes(int B, int Hq, int Hk, int T, 
   return splits > 1 ? (size_t)B * Hk * rows * splits * (D + 2) * sizeof(float) : 0;
 }
 
+extern "C" int dflash_kv4_sdpa_plan(int B, int Hq, int Hk, int T, int max_length, int num_splits, int* out, int capacity) {
+  if (B < 1 || Hq < 1 || Hk < 1 || Hq % Hk != 0 || T < 1 || max_length < 1 || num_splits < 0 || num_splits > kMaxSplits ||
+      (long long)(Hq / Hk) * T > 1000000)
+    return fail(DFLASH_ERR_BAD_SHAPE, "kv4_sdpa_plan: bad sizes");
+  if (!out || capacity < 2) return fail(DFLASH_ERR_BAD_ARG, "kv4_sdpa_plan: capacity %d < 2", capacity);
+  int device = 0;
+  cudaGetDevice(&device);
+  const long long rows = (long long)(Hq / Hk) * T;
+  out[0] = takes_tc(B, Hk, rows, max_length, device);
+  out[1] = kv4_splits(B, Hk, rows, max_length, device, num_splits);
+  return 2;
+}
+
 extern "C" int dflash_kv4_sdpa(const void* q, const long long* q_strides, const dflash_kv4_cache* k_cache,
                                const dflash_kv4_cache* v_cache, const void* mask, int mask_kind, const long long* mask_strides,
                                void* out, const int* lengths, int B, int Hq, int Hk, int T, int D, int capacity, int max_length,

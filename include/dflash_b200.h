@@ -433,6 +433,9 @@ DFLASH_API int dflash_kv4_read(const dflash_kv4_cache* k_cache, const dflash_kv4
  *   num_splits: key ranges, 0..1024; 0 = chosen from the SM count.  workspace: dflash_kv4_sdpa_workspace_bytes() bytes of device memory, 16-byte
  *   aligned, contents irrelevant, not shared by calls that can overlap. */
 DFLASH_API size_t dflash_kv4_sdpa_workspace_bytes(int B, int Hq, int Hk, int T, int D, int max_length, int num_splits);
+/* How dflash_kv4_sdpa runs these sizes on the current device: out[0] = 0 (kernel of few rows) or 1 (tcgen05 kernel of many), out[1] =
+ * the key ranges.  Returns the number of entries, 2; a negative status where the sizes or the capacity do not do. */
+DFLASH_API int dflash_kv4_sdpa_plan(int B, int Hq, int Hk, int T, int max_length, int num_splits, int* out, int capacity);
 DFLASH_API int dflash_kv4_sdpa(const void* q, const long long* q_strides, const dflash_kv4_cache* k_cache,
                                const dflash_kv4_cache* v_cache, const void* mask, int mask_kind, const long long* mask_strides,
                                void* out, const int* lengths, int B, int Hq, int Hk, int T, int D, int capacity, int max_length,

@@ -9,11 +9,18 @@ pytestmark = pytest.mark.gpu
 from dflash_mlx_b200 import quantized_kv as qkv  # noqa: E402
 from oracle import quantized_kv as ref  # noqa: E402
 from tests.test_quantized_kv_gpu import TOL, check_rows, gen, ints, make_cache, no_device_error, states  # noqa: E402, F401
+from tests.test_quantized_kv_plan import plan  # noqa: E402
 
 DEV = "cuda"
 BF16, F16 = torch.bfloat16, torch.float16
-# T, keys, capacity: up to 8 and up to 16 rows of 4 heads, and many rows under a bound on the lengths that sends them to the tcgen05 kernel on any SM count up to 160
+# T, keys, capacity: up to 8 and up to 16 rows of 4 heads, and many rows under a bound on the lengths that sends them to the tcgen05
+# kernel
 KERNELS = {"eight": (2, 190, 220), "sixteen": (3, 190, 220), "many": (40, 1290, 13000)}
+
+
+def test_each_kernel_is_reached():
+    for which, (T, _, cap) in KERNELS.items():
+        assert plan(1, 4, 1, T, cap)[0] == plan(2, 4, 1, T, cap)[0] == (which == "many")
 
 
 def part_of(k, v, name):
