@@ -44,7 +44,7 @@ def quantized_kv_write(keys, values, k_cache, v_cache, offsets, *, counts: Optio
     ``offsets`` int32 ``[B]`` on the device (a captured graph replays at any position); ``counts`` int32 ``[B]``: only the first
     ``counts[b]`` rows of sequence ``b`` are stored (a padded batch).  Per 64 channels: scale = max/15 - min/15 and bias = min in
     the cache's type, code = round((x - bias) / scale) in 0..15.  A group that holds a NaN or infinity reads back as NaN.  Rows
-    outside the capacity are not stored and set the device error word (``dflash_device_error``, code 61).  A cache whose
+    outside the capacity are not stored and set the device error word, which ``check_device_error`` raises.  A cache whose
     sequences, heads or sides share memory is refused.
     """
     (_lib._native or _lib.native()).kv4_write(keys, values, *k_cache, *v_cache, offsets, counts)
@@ -71,6 +71,18 @@ def quantized_kv_sdpa(queries, k_cache, v_cache, scale: float, lengths: Union[in
     return (_lib._native or _lib.native()).kv4_sdpa(queries, *k_cache, *v_cache, scale, lengths, mask, max_length, num_splits)
 
 
+def check_device_error(device, where: str) -> None:
+    """Reads (and clears) the status word of ``device`` after a synchronisation and raises ``DFlashError`` where a call was not carried
+    out: rows of a write outside the capacity (code 61), a wait inside the attention that ran out (62)."""
+    index = torch.device(device).index
+    code = _lib.lib().dflash_device_error(torch.cuda.current_device() if index is None else index)
+    if code != 0:
+        what = {61: "rows outside the cache's capacity were not written",
+                62: "an attention kernel abandoned a bounded wait; the results of the last calls are not valid"}
+        raise _lib.DFlashError(f"{where}: device error word {code & 0xFF} (detail {code >> 8}): "
+                               + what.get(code & 0xFF, "a kernel refused its operands or abandoned a bounded wait"))
+
+
 class QuantizedKVCache:
     """One attention layer's cache in 4 bits, with the positions of its sequences on the device.
 
@@ -94,6 +106,11 @@ class QuantizedKVCache:
     def commit(self, accepted: Union[int, torch.Tensor]) -> None:
         """Positions += accepted (an int, or int32 ``[B]`` on the device)."""
         self.offsets += accepted
+
+    def check_device_error(self, where: str) -> None:
+        """Reads (and clears) the device's status word - a row that ``update`` could not place inside the capacity, a kernel that
+        gave up on a bounded wait - and raises.  Synchronises the device: called where the host synchronises anyway."""
+        check_device_error(self.offsets.device, where)
 
     def read(self, start: Union[int, torch.Tensor], length: int):
         return quantized_kv_read(self.keys, self.values, start, length)

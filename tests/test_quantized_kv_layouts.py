@@ -1,4 +1,4 @@
-"""Which caches may be written: no place of them belongs to two sequences, heads or sides."""
+"""Which caches may be written, and how a write that was not carried out is reported."""
 import pytest
 import torch
 
@@ -33,3 +33,17 @@ def test_caches_that_would_be_written_twice():
     for bad in ((*k, *k), (k[0], k[1], k[1], *v), (*k, v[0], k[1], v[2])):
         with pytest.raises(ValueError, match="one another"):
             written(*bad)
+
+
+@pytest.mark.parametrize("code,text", [(61 | (5 << 8), "capacity"), (62 | (3 << 8), "wait"), (31, "refused")])
+def test_a_device_error_is_raised(code, text, monkeypatch):
+    class Library:
+        def dflash_device_error(self, device):
+            assert device == 3
+            return words.pop()
+
+    words = [0, code]
+    monkeypatch.setattr(_lib, "lib", Library)
+    with pytest.raises(_lib.DFlashError, match=f"step 7: device error word {code & 0xFF} .detail {code >> 8}.*{text}"):
+        qkv.check_device_error("cuda:3", "step 7")
+    qkv.check_device_error("cuda:3", "step 8")            # nothing since

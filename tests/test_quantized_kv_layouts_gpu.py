@@ -4,7 +4,7 @@ import torch
 
 pytestmark = pytest.mark.gpu
 
-from dflash_mlx_b200 import quantized_kv as qkv  # noqa: E402
+from dflash_mlx_b200 import _lib, quantized_kv as qkv  # noqa: E402
 from oracle import quantized_kv as ref  # noqa: E402
 from tests.test_quantized_kv_gpu import ints, make_cache, no_device_error, states  # noqa: E402, F401
 
@@ -26,3 +26,18 @@ def test_contiguous_rows_off_their_boundary(off, dtype):
         for got, part in zip(c, want):
             assert torch.equal(got[0, :, 3:8], part[0]) and torch.equal(got[1, :, 7:12], part[1])
     assert torch.equal(qkv.quantized_kv_sdpa(x, k_cache, v_cache, 0.1, n), qkv.quantized_kv_sdpa(x.clone(), k_cache, v_cache, 0.1, n))
+
+
+def test_rows_that_did_not_fit_are_reported():
+    cache = qkv.QuantizedKVCache(2, 1, 20, 128)
+    x = states((2, 1, 8, 128), torch.bfloat16, 1)
+    cache.update(x, x)
+    cache.check_device_error("prompt")
+    cache.commit(ints(8, 15))
+    before = [p.clone() for p in cache.values]
+    cache.update(x, x)
+    with pytest.raises(_lib.DFlashError, match="second block.*61.*capacity"):
+        cache.check_device_error("second block")
+    cache.check_device_error("after")
+    for got, old, part in zip(cache.values, before, ref.quantise(x)):
+        assert torch.equal(got[0, :, 8:16], part[0]) and torch.equal(got[1, :, 15:], part[1, :, :5]) and torch.equal(got[1, :, :15], old[1, :, :15])
