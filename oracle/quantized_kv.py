@@ -17,7 +17,8 @@ def quantise(x: torch.Tensor):
     g = x.float().unflatten(-1, (-1, GROUP))
     fine = torch.isfinite(g).all(-1)
     lo, hi = g.amin(-1), g.amax(-1)
-    scale = torch.where(fine, hi / 15 - lo / 15, torch.nan).to(x.dtype)
+    n15 = torch.full_like(hi, 15)   # a tensor: torch on a GPU multiplies by the rounded reciprocal of a number
+    scale = torch.where(fine, hi / n15 - lo / n15, torch.nan).to(x.dtype)
     bias = torch.where(fine, lo, torch.nan).to(x.dtype)
     s = scale.float()[..., None]
     n = torch.where(s > 0, torch.round((g - bias.float()[..., None]) / s), torch.zeros_like(g)).nan_to_num(0).clamp(0, 15)

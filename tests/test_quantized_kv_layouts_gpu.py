@@ -41,3 +41,20 @@ def test_rows_that_did_not_fit_are_reported():
     cache.check_device_error("after")
     for got, old, part in zip(cache.values, before, ref.quantise(x)):
         assert torch.equal(got[0, :, 8:16], part[0]) and torch.equal(got[1, :, 15:], part[1, :, :5]) and torch.equal(got[1, :, :15], old[1, :, :15])
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_every_value_as_a_group_s_maximum_and_minimum(dtype):
+    """Scales, biases and codes to the last bit, whatever a group's range is."""
+    x = torch.arange(-(1 << 15), 1 << 15, device=DEV, dtype=torch.int32).to(torch.int16).view(dtype)
+    x = x[x.isfinite()]
+    rows = torch.zeros(1, 1, len(x), 128, dtype=dtype, device=DEV)
+    rows[0, 0, :, 7] = x                                  # from zero to x, or from x to zero
+    rows[0, 0, :, 64:] = x.flip(0)[:, None] * torch.linspace(-1, 1, 64, device=DEV).to(dtype)
+    rows[0, 0, :, 64] = x.roll(977)
+    rows = rows.nan_to_num(0, 0, 0)
+    k_cache, v_cache = qkv.allocate(1, 1, len(x), 128, dtype=dtype)
+    qkv.quantized_kv_write(rows, rows, k_cache, v_cache, ints(0))
+    for c in (k_cache, v_cache):
+        for got, want in zip(c, ref.quantise(rows)):
+            assert torch.equal(got, want)
