@@ -493,7 +493,7 @@ __global__ void __launch_bounds__((kWarpsOf<D, NT>) * 32, 2) kv4_sdpa_kernel(con
       // a row's maximum moves for its own scores alone: what other rows see changes no bit of it
       float xk[2] = {0.f, 0.f};   // the keys' own exponents
       careful = __any_sync(0xffffffffu, odd);
-      if (careful) {
+      if (__builtin_expect(careful, 0)) {
         shifted = false;
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
@@ -521,7 +521,7 @@ __global__ void __launch_bounds__((kWarpsOf<D, NT>) * 32, 2) kv4_sdpa_kernel(con
           f[e] = now == -INFINITY ? 1.f : ex2((before - now) * kLog2e);   // nothing seen yet: the sums are zero
           m[nt][e] = now;
           l[nt][e] *= f[e];
-          if (careful) {
+          if (__builtin_expect(careful, 0)) {
             float y = fmaxf(fmaf(xk[0], kLn2, s[nt][e]), fmaf(xk[1], kLn2, s[nt][2 + e]));
 #pragma unroll
             for (int w = 4; w < 32; w <<= 1) y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, w));
@@ -553,7 +553,7 @@ __global__ void __launch_bounds__((kWarpsOf<D, NT>) * 32, 2) kv4_sdpa_kernel(con
       shifted = __any_sync(0xffffffffu, shifted);
     }
     // ---- p, and O^T += V^T P' per group ----
-    if (!careful) {
+    if (__builtin_expect(!careful, 1)) {
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -634,10 +634,11 @@ __global__ void __launch_bounds__((kWarpsOf<D, NT>) * 32, 2) kv4_sdpa_kernel(con
         v0.z = fmaf(o[4 * g + 2][nt][e], undo, y); v0.w = fmaf(o[4 * g + 3][nt][e], undo, y);
         v1.x = fmaf(o[4 * g][nt][2 + e], undo, y); v1.y = fmaf(o[4 * g + 1][nt][2 + e], undo, y);
         v1.z = fmaf(o[4 * g + 2][nt][2 + e], undo, y); v1.w = fmaf(o[4 * g + 3][nt][2 + e], undo, y);
-        if (shifted) {
-          const int ev = (int)sEv[row];
-          v0.x = scalbnf(v0.x, ev); v0.y = scalbnf(v0.y, ev); v0.z = scalbnf(v0.z, ev); v0.w = scalbnf(v0.w, ev);
-          v1.x = scalbnf(v1.x, ev); v1.y = scalbnf(v1.y, ev); v1.z = scalbnf(v1.z, ev); v1.w = scalbnf(v1.w, ev);
+        if (__builtin_expect(shifted, 0)) {   // 2^ev, in two steps where it is no fp32 number
+          const int ev = min(max((int)sEv[row], -200), 200);
+          const float one = __uint_as_float((uint32_t)(127 + ev / 2) << 23), two = __uint_as_float((uint32_t)(127 + ev - ev / 2) << 23);
+          v0.x = v0.x * one * two; v0.y = v0.y * one * two; v0.z = v0.z * one * two; v0.w = v0.w * one * two;
+          v1.x = v1.x * one * two; v1.y = v1.y * one * two; v1.z = v1.z * one * two; v1.w = v1.w * one * two;
         }
         *(float4*)(po + 64 * g + 8 * r) = v0;
         *(float4*)(po + 64 * g + 8 * r + 4) = v1;
