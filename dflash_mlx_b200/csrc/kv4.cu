@@ -497,10 +497,13 @@ __global__ void __launch_bounds__((kWarpsOf<D, NT>) * 32, 2) kv4_sdpa_kernel(con
         shifted = false;
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          if (unusual(big[e])) {
-            float all = big[e];
+          float top = 0.f, all = 0.f;   // once more: kept, they would cost the usual tiles registers
 #pragma unroll
-            for (int g = 0; g < G; ++g) all = fmaxf(all, fabsf(bv[e][g]) * 0.0625f);
+          for (int g = 0; g < G; ++g) {
+            top = fmaxf(top, fabsf(sv[e][g]));
+            all = fmaxf(all, fmaxf(fabsf(sv[e][g]), fabsf(bv[e][g]) * 0.0625f));
+          }
+          if (unusual(top)) {
             const int x = max((int)(__float_as_uint(all) >> 23) - 127 - 3, -120);   // 2^(3 - x) |sv| < 2^7
             const float take = __uint_as_float((uint32_t)(127 - x) << 23);
             xk[e] = (float)x;
@@ -634,12 +637,6 @@ __global__ void __launch_bounds__((kWarpsOf<D, NT>) * 32, 2) kv4_sdpa_kernel(con
         v0.z = fmaf(o[4 * g + 2][nt][e], undo, y); v0.w = fmaf(o[4 * g + 3][nt][e], undo, y);
         v1.x = fmaf(o[4 * g][nt][2 + e], undo, y); v1.y = fmaf(o[4 * g + 1][nt][2 + e], undo, y);
         v1.z = fmaf(o[4 * g + 2][nt][2 + e], undo, y); v1.w = fmaf(o[4 * g + 3][nt][2 + e], undo, y);
-        if (__builtin_expect(shifted, 0)) {   // 2^ev, in two steps where it is no fp32 number
-          const int ev = min(max((int)sEv[row], -200), 200);
-          const float one = __uint_as_float((uint32_t)(127 + ev / 2) << 23), two = __uint_as_float((uint32_t)(127 + ev - ev / 2) << 23);
-          v0.x = v0.x * one * two; v0.y = v0.y * one * two; v0.z = v0.z * one * two; v0.w = v0.w * one * two;
-          v1.x = v1.x * one * two; v1.y = v1.y * one * two; v1.z = v1.z * one * two; v1.w = v1.w * one * two;
-        }
         *(float4*)(po + 64 * g + 8 * r) = v0;
         *(float4*)(po + 64 * g + 8 * r + 4) = v1;
       }
@@ -655,11 +652,12 @@ __global__ void __launch_bounds__((kWarpsOf<D, NT>) * 32, 2) kv4_sdpa_kernel(con
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) {
-      const float f = ex2((mM[w * 8 * NT + row] - ref) * kLog2e);
+      const float f = ex2((mM[w * 8 * NT + row] - ref) * kLog2e), ev = sC[(1 + w) * 8 * NT + row];
+      const float fo = ev == 0.f ? f : ex2(fmaf(mM[w * 8 * NT + row] - ref, kLog2e, ev));   // O carries the row's exponent
       const float4 v = *(const float4*)(mO + ((size_t)w * 8 * NT + row) * D + d);
       den = fmaf(f, mL[w * 8 * NT + row], den);
-      acc.x = fmaf(f, v.x, acc.x); acc.y = fmaf(f, v.y, acc.y);
-      acc.z = fmaf(f, v.z, acc.z); acc.w = fmaf(f, v.w, acc.w);
+      acc.x = fmaf(fo, v.x, acc.x); acc.y = fmaf(fo, v.y, acc.y);
+      acc.z = fmaf(fo, v.z, acc.z); acc.w = fmaf(fo, v.w, acc.w);
     }
     if (a.splits == 1) {
       const float inv = den == 0.f ? 1.f : 1.f / den;   // a row that sees nothing yields zeros; NaN stays
