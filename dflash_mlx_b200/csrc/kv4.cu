@@ -6,8 +6,9 @@
 // Attention over the codes, per KV head with rows = (Hq/Hk) * T query rows r and keys n, group g = 64 channels:
 //   S[r,n] = scale * sum_g ( sk[n,g] * sum_{d in g} q[r,d] ck[n,d]  +  bk[n,g] * sum_{d in g} q[r,d] )
 //   O[r,d] = sum_n p[r,n] sv[n,g] (cv[n,d] - 8)  +  sum_n p[r,n] (bv[n,g] + 8 sv[n,g])          (g the group of d)
-// The codes enter both products as exact small integers; scales and biases are applied in fp32 around them, so the only
-// rounding besides fp32 sums is that of p * sv to fp16 (11 bits; the cache's values themselves are never rounded).
+// In the kernel of few rows below, the codes enter both products as exact small integers; scales and biases are applied in fp32
+// around them, so the only rounding besides fp32 sums is that of p * sv to fp16 (11 bits; q is exact in fp16 but for elements far below
+// its row's largest).  The kernel of many rows (kv4_tc.cu) rounds the cache's values to fp16 as well.
 #include <mutex>
 
 #include "kv4.cuh"
@@ -20,10 +21,10 @@ constexpr float kLog2e = 1.4426950408889634f;
 
 // ---- write -------------------------------------------------------------------------------------------------------------
 // A lane owns the eight channels of one word, eight lanes a group: minimum and maximum in three shuffles, no shared memory.
-// Bound by HBM and instruction issue (prompts) or by the launch (single tokens): a warp has its next row on the way under the
-// current one, in a rolled loop (eight rows unrolled missed the instruction cache: 21 us for 2 x 4133 rows of 4 heads x 256, 18 now; its
-// HBM floor is 7).  One token: 1.5 us.  blockIdx.x is (sequence, head), so no lane
-// divides.
+// Bound by instruction issue (prompts: 76 % of the slots while blocks run, HBM at a quarter of its rate) or by the launch (single
+// tokens): a warp has its next row on the way under the current one, in a rolled loop (eight rows unrolled missed the instruction
+// cache: 21 us for 2 x 4133 rows of 4 heads x 256, 17.9 now; its HBM floor is 7).  One token: 1.6 us.  blockIdx.x is (sequence,
+// head), so no lane divides.
 struct WriteArgs {
   const void* x[2];
   long long sb[2], sh[2], st[2];
@@ -45,8 +46,8 @@ __device__ __forceinline__ float code_of(float v, float bias, float scale, float
   else q = __fdiv_rn(y, scale);
   return fminf(__fsub_rn(__fadd_rn(q, kMagic), kMagic), 15.f);
 }
-// x / 15 to the last bit for every value of the two 16-bit types (verified over all of them): the quotient by the rounded
-// reciprocal and one correction by its residual.
+// x / 15 to the last bit for every value of the two 16-bit types (tested over all of them): the quotient by the rounded reciprocal
+// and one correction by its residual.
 __device__ __forceinline__ float by_15(float x) {
   constexpr float kInv = 1.f / 15.f;
   const float q = __fmul_rn(x, kInv);
@@ -209,8 +210,8 @@ __global__ void __launch_bounds__(128) kv4_read_kernel(const ReadArgs a) {
 // down to 2^-28 of the row's largest element.
 // The running maximum moves only when a score exceeds it by 8 octaves (p <= 256 otherwise), so the accumulators are rarely
 // rescaled.  The warps of a block and then the splits of the key range are merged with fp32 partials.
-// Measured (D = 256, bf16): 8 rows, 16 ragged sequences up to 32768: 68 us, 3.0 TB/s, at 75 % of the issue slots; 6 rows over 4097
-// positions: 9.1 us with the combine.
+// Measured (D = 256, bf16): 8 rows, 16 ragged sequences up to 32768: 70 us, 2.9 TB/s, with 58 % of the issue slots and half of the ALU pipe
+// busy while blocks run and a sixth of the time behind the longest sequence; 6 rows over 4097 positions: 8.9 us with the combine.
 // Warps of a block.  Two blocks share an SM, so that one starts or merges while the other streams; as many warps as the registers
 // allow (the loop is bound by instruction issue: unpacking, scales and softmax next to the MMAs).
 constexpr int kStages = 3;   // tiles of a warp in shared memory
@@ -983,8 +984,8 @@ extern "C" int dflash_kv4_read(const dflash_kv4_cache* k_cache, const dflash_kv4
 }
 
 // Whether the rows go to the tcgen05 kernel.  It has the throughput, the other one the shorter way from launch to end: where tiles of 16
-// rows fit the SMs side by side and have little to do in all, they are faster (D = 256, 96 rows a KV head, 4 heads: 128 positions 9.3
-// against 11.7 us, 512 11.2 against 14.4, 2048 16.1 against 16.0; 4 sequences: 128 positions 9.6 against 11.8, 512 16.9 against 15.9).
+// rows fit the SMs side by side and have little to do in all, they are faster (D = 256, 96 rows a KV head, 4 heads: 128 positions 9.8
+// against 11.9 us, 512 11.7 against 14.6, 2048 16.4 against 16.3; 4 sequences: 128 positions 10.0 against 12.1, 512 17.3 against 16.2).
 static bool takes_tc(int B, int Hk, long long rows, int max_length, int device) {
   if (rows <= kFewRows) return false;
   const long long units = (long long)B * Hk * ((rows + 15) / 16), sms = sm_count(device);

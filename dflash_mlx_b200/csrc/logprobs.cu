@@ -16,8 +16,8 @@
 //
 // One row per thread-block cluster: one block a row when rows alone fill the SMs, up to eight otherwise, whose triples and lists the
 // first block merges through distributed shared memory.  Measured (bf16, 151936 logits): 1999 rows with suppressed tokens and 5
-// alternatives 212 us (2.9 TB/s; bound by instruction issue and the exponentials, HBM floor 93), 16 rows with 20 alternatives 16.7 us
-// (latency: passes, ranking, cluster merge).
+// alternatives 213 us (2.9 TB/s, HBM floor 93: issue slots 69 % busy, exponentials 38 % of their pipe, the rest waits at the rankings'
+// barriers), 16 rows with 20 alternatives 16.5 us (latency: passes, ranking, cluster merge).
 #include <cooperative_groups.h>
 
 #include <mutex>
