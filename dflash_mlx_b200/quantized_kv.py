@@ -43,9 +43,9 @@ def quantized_kv_write(keys, values, k_cache, v_cache, offsets, *, counts: Optio
 
     ``offsets`` int32 ``[B]`` on the device (a captured graph replays at any position); ``counts`` int32 ``[B]``: only the first
     ``counts[b]`` rows of sequence ``b`` are stored (a padded batch).  Per 64 channels: scale = max/15 - min/15 and bias = min in
-    the cache's type, code = round((x - bias) / scale) in 0..15 (the layout of ``mx.quantize``, not its codes).  A group that holds a NaN or infinity reads back as NaN.  Rows
-    outside the capacity are not stored and set the device error word, which ``check_device_error`` raises.  A cache whose
-    sequences, heads or sides share memory is refused.
+    the cache's type, code = round((x - bias) / scale) in 0..15 (the layout of ``mx.quantize``, not its codes).  A group that
+    holds a NaN or infinity reads back as NaN.  Rows outside the capacity are not stored and set the device error word, which
+    ``check_device_error`` raises.  A cache whose sequences, heads or sides share memory is refused.
     """
     (_lib._native or _lib.native()).kv4_write(keys, values, *k_cache, *v_cache, offsets, counts)
 
