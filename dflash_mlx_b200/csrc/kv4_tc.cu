@@ -18,7 +18,7 @@
 // with a single rounding to fp16 (at most 2^-11 of a value, 2^-25 of the unit below; the cache's scales carry 8 or 11 bits, the codes 4).
 // A row must not notice keys that it does not see, so nothing is shared between keys: a key or value whose largest element lies in
 // [2^-10, 2^11) is multiplied by 2^4 like all of its kind; any other one by a power of two of its own, which brings that
-// element into [2^14, 2^15).  A column of S takes the power back before its softmax, and P for V: P = p 2^(6 + x - ev), with an
+// element into [2^14, 2^15), so that its other elements are kept to 2^-39 of it.  A column of S takes the power back before its softmax, and P for V: P = p 2^(6 + x - ev), with an
 // exponent ev of the row's output that is 0 until the row sees such a value.  Tiles without them, under rows with ev = 0, do not
 // touch any of this, and the bits of usual keys are the same either way.  (An exponent shared by 32 keys allows 9 instructions for 8
 // codes, 3 % of a long range, but then one large key, seen or not, takes the others' bits.  A cache of unusual keys takes 1.3 times as

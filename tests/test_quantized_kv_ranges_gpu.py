@@ -111,10 +111,12 @@ def test_sizes_that_differ_within_a_block(octaves, kind, side, which):
 
 
 @pytest.mark.parametrize("which", KERNELS)
-def test_small_values_first_then_large_ones_and_back(which):
+@pytest.mark.parametrize("D", [128, 256])
+@pytest.mark.parametrize("splits", [0, 1])
+def test_small_values_first_then_large_ones_and_back(splits, D, which):
     """A row's values of a size of their own in every stretch of its keys, from the type's smallest to its largest."""
     T, n, cap = KERNELS[which]
-    B, Hq, Hk, D, dtype = 1, 4, 1, 128, BF16
+    B, Hq, Hk, dtype = 1, 4, 1, BF16
     k, _ = make_cache(B, Hk, cap, D, dtype)
     q, scale = states((B, Hq, T, D), dtype, 9), D ** -0.5
     stretch = n // 6
@@ -125,7 +127,7 @@ def test_small_values_first_then_large_ones_and_back(which):
         keep = torch.ones(1, Hq, 1, cap, dtype=torch.bool, device=DEV)
         for h in range(3):                                # a head sees two of the stretches
             keep[:, h] = ((torch.arange(cap, device=DEV) // stretch) % 3 == h)
-        got, want = qkv.quantized_kv_sdpa(q, k, v, scale, ints(n), keep), ref.sdpa(q, k, v, scale, [n], keep)
+        got, want = qkv.quantized_kv_sdpa(q, k, v, scale, ints(n), keep, num_splits=splits), ref.sdpa(q, k, v, scale, [n], keep)
         check_rows(got, want, dtype)
         # however small the row is: half a step of bf16's subnormals in each channel aside
         assert bool(((got.double() - want).norm(dim=-1) <= TOL[dtype] * want.norm(dim=-1) + D ** 0.5 * 2.0 ** -134).all())
@@ -186,3 +188,29 @@ def test_large_scores_under_many_ranges(which):
     for splits in (1, 2, 5, 9):
         got = qkv.quantized_kv_sdpa(q, k, v, 16.0, ints(n), num_splits=splits)
         check_rows(got, ref.sdpa(q, k, v, 16.0, [n]), dtype)
+
+
+@pytest.mark.parametrize("which", KERNELS)
+@pytest.mark.parametrize("kind", ["none", "bool", "type", "f32"])
+@pytest.mark.parametrize("seed", range(8))
+def test_random_sizes(seed, kind, which):
+    """Every key and value at a size of its own, the weights spread over all of them: scores of the same size through the queries' other
+    channels, so that small and large values meet in every row."""
+    T, n, cap = KERNELS[which]
+    B, Hq, Hk, D, dtype = 2, 4, 1, [128, 256][seed % 2], [BF16, F16][seed // 2 % 2]
+    far = 30 if dtype == BF16 else 5
+    k, v = ([states((B, Hk, cap, D), torch.float32, 10 * seed + i) for i in range(2)])
+    size = torch.pow(2.0, (2 * torch.rand(2, B, Hk, cap, 1, generator=gen(seed), device=DEV) - 1) * far)
+    # The queries do not look at these channels.  The tcgen05 kernel keeps a key's elements to 2^-39 of its largest one (2^-25 of a
+    # unit that puts that one at 2^14): next to 2^20 times larger channels, elements of 2^-6 of their own largest to 2^-39 2^26 = 2^-13.
+    # (fp32 products see more only where the queries are 2^-15 times smaller in the large channels, as here.)
+    k[..., 64:] *= torch.pow(size[0], 2 / 3)
+    v = v * torch.where(torch.rand(B, Hk, cap, 1, generator=gen(seed + 50), device=DEV) < 0.3, size[1], torch.ones_like(size[1]))
+    k, v = (qkv.QuantizedKV(*ref.quantise(x.to(dtype))) for x in (k, v))
+    q = states((B, Hq, T, D), dtype, 9)
+    q[..., 64:] = 0
+    keep = torch.rand(B, Hq, 1, cap, generator=gen(seed + 100), device=DEV) < 0.5
+    mask = None if kind == "none" else keep if kind == "bool" else torch.where(keep, 0.5, -math.inf).to(dtype if kind == "type" else torch.float32)
+    lengths = [n, n - 33]
+    got = qkv.quantized_kv_sdpa(q, k, v, 0.125, ints(*lengths), mask, num_splits=[0, 1, 3][seed % 3])
+    check_rows(got, ref.sdpa(q, k, v, 0.125, lengths, mask), dtype)
