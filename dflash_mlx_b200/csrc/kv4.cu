@@ -201,26 +201,26 @@ __global__ void __launch_bounds__(128) kv4_read_kernel(const ReadArgs a) {
 //       MMAs).  Nibble t and 4 + t of a word are rows r and r + 8 of MMA t, so a thread's words serve four MMAs without crossing
 //       lanes.
 // P' in fp16's range, whatever the scales, and without a row noticing keys that it does not see: a key whose largest |sv| lies in
-// [2^-12, 2^4) is multiplied by 2^3 like all of its kind, so P' <= 2^15 and its bits down to 2^-25; any other key by a power of two of
-// its own, 2^(3 - x), which P' and the row's exponent take back: P' = p sv 2^(3 - ev), ev = 0 until the row sees such a key.  A tile
-// without one, under rows with ev = 0, does not touch any of this.
+// [2^-7, 2^3) is multiplied by 2^8 like all of its kind, so P' <= 2^15, and probabilities down to 2^-17 of the largest keep 9 bits under
+// the smallest of these scales; any other key by a power of two of its own, 2^(8 - x), which P' and the row's exponent take back:
+// P' = p sv 2^(8 - ev), ev = 0 until the row sees such a key.  A tile without one, under rows with ev = 0, does not touch any of this.
 // Codes become exact fp16 integers by OR-ing the nibble into 1024 and one packed operation that takes the constant away again
 // (left in, a sum would carry 1024 times sum |q| or sum P', which costs digits); values are centred as code - 8, which halves
 // what the rounding of P' is multiplied with.  q is brought to fp16 by a power of two per row: bf16's 8 bits are exact in it
 // down to 2^-28 of the row's largest element.
-// The running maximum moves only when a score exceeds it by 8 octaves (p <= 256 otherwise), so the accumulators are rarely
+// The running maximum moves only when a score exceeds it by 4 octaves (p <= 16 otherwise), so the accumulators are rarely
 // rescaled.  The warps of a block and then the splits of the key range are merged with fp32 partials.
-// Measured (D = 256, bf16): 8 rows, 16 ragged sequences up to 32768: 70 us, 2.9 TB/s, with 58 % of the issue slots and half of the ALU pipe
-// busy while blocks run and a sixth of the time behind the longest sequence; 6 rows over 4097 positions: 8.9 us with the combine.
+// Measured (D = 256, bf16): 8 rows, 16 ragged sequences up to 32768: 71.5 us, 2.9 TB/s, with 58 % of the issue slots and half of the ALU pipe
+// busy while blocks run and a sixth of the time behind the longest sequence; 6 rows over 4097 positions: 9.1 us with the combine.
 // Warps of a block.  Two blocks share an SM, so that one starts or merges while the other streams; as many warps as the registers
 // allow (the loop is bound by instruction issue: unpacking, scales and softmax next to the MMAs).
 constexpr int kStages = 3;   // tiles of a warp in shared memory
 template <int D, int NT> constexpr int kWarpsOf = NT == 2 ? (D == 256 ? 4 : 6) : (D == 256 ? 6 : 8);
-constexpr float kLn2 = 0.6931471805599453f, kMaxStep = 8 * kLn2;
-constexpr float kUsual = 8.f;              // the power of two of usual value scales
-__device__ __forceinline__ bool unusual(float big) {   // outside [2^-12, 2^4), and not 0
+constexpr float kLn2 = 0.6931471805599453f, kMaxStep = 4 * kLn2;
+constexpr float kUsual = 256.f;            // the power of two of usual value scales
+__device__ __forceinline__ bool unusual(float big) {   // outside [2^-7, 2^3), and not 0
   const uint32_t u = __float_as_uint(big);
-  return u - (115u << 23) >= (16u << 23) && u != 0;
+  return u - (120u << 23) >= (10u << 23) && u != 0;
 }
 
 template <int D>
@@ -492,7 +492,8 @@ __global__ void __launch_bounds__((kWarpsOf<D, NT>) * 32, 2) kv4_sdpa_kernel(con
       }
     if (__any_sync(0xffffffffu, grow)) {
       // a row's maximum moves for its own scores alone: what other rows see changes no bit of it
-      float xk[2] = {0.f, 0.f};   // the keys' own exponents
+      float xk[2] = {0.f, 0.f};   // the keys' own exponents; values of zero ask for none
+      bool own[2] = {false, false};
       careful = __any_sync(0xffffffffu, odd);
       if (__builtin_expect(careful, 0)) {
         shifted = false;
@@ -504,8 +505,10 @@ __global__ void __launch_bounds__((kWarpsOf<D, NT>) * 32, 2) kv4_sdpa_kernel(con
             top = fmaxf(top, fabsf(sv[e][g]));
             all = fmaxf(all, fmaxf(fabsf(sv[e][g]), fabsf(bv[e][g]) * 0.0625f));
           }
-          if (unusual(top)) {
-            const int x = max((int)(__float_as_uint(all) >> 23) - 127 - 3, -120);   // 2^(3 - x) |sv| < 2^7
+          own[e] = unusual(top);
+          if (all == 0.f) xk[e] = -300.f;
+          if (own[e]) {
+            const int x = max((int)(__float_as_uint(all) >> 23) - 127 - 2, -120);   // 2^(8 - x) |sv| < 2^11
             const float take = __uint_as_float((uint32_t)(127 - x) << 23);
             xk[e] = (float)x;
 #pragma unroll
@@ -530,8 +533,11 @@ __global__ void __launch_bounds__((kWarpsOf<D, NT>) * 32, 2) kv4_sdpa_kernel(con
 #pragma unroll
             for (int w = 4; w < 32; w <<= 1) y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, w));
             const float ev = sEv[nt * 8 + 2 * c + e], d = (y - now) * kLog2e;   // octaves of the row's largest p 2^x
+            // a row that sees none of the unusual keys, and saw none, stays as it is
+            const uint32_t sees = __ballot_sync(0xffffffffu, (own[0] && s[nt][e] != -INFINITY) || (own[1] && s[nt][2 + e] != -INFINITY));
+            const bool moves = ((sees >> c) & 0x11111111u) != 0 || ev != 0.f;   // lanes with the same rows
             float ev_now = ev;
-            if (now != -INFINITY && (now != before || d > ev + 8.f)) ev_now = fmaxf(ceilf(d), ev + floorf((before - now) * kLog2e));
+            if (moves && now != -INFINITY && (now != before || d > ev + 4.f)) ev_now = fmaxf(ceilf(d), ev + floorf((before - now) * kLog2e));
             if (now != -INFINITY) f[e] = ex2(fmaf(before - now, kLog2e, ev - ev_now));
             __syncwarp();
             if (r == 0) sEv[nt * 8 + 2 * c + e] = ev_now;

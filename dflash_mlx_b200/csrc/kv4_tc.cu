@@ -364,6 +364,7 @@ __device__ __forceinline__ void unpack_side(const dflash_kv4_cache& c, int b, in
     Meta& m = meta[tile & (kMeta - 1)];
     if (odd != 0) {
       int x = 0;
+      if (kV && largest == 0) x = -128;   // a value of zero asks for no exponent
       if (!usual && !bad) {   // 2^(kUnit + x): the largest element to [2^14, 2^15)
         x = max((int)(largest >> 23) - 127 - 14 - kUnit, -120);
         unit = pow2(-kUnit - x);
@@ -731,6 +732,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_sdpa_tc_kernel(const SdpaArgs
         for (int e0 = 0; e0 < kTile; e0 += 16) st16(s_col + e0, v + e0);
         wait_st();
         float d = -INFINITY;   // octaves of the row's largest p 2^x; NaN counts as none
+        bool moves = ev != 0.f;   // a row that sees none of the unusual values, and saw none, stays as it is
 #pragma unroll 1
         for (int e0 = 0; e0 < kTile; e0 += 16) {
           uint32_t x[16];
@@ -738,9 +740,12 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_sdpa_tc_kernel(const SdpaArgs
           wait_ld();
 #pragma unroll
           for (int e = 0; e < 16; ++e) d = fmaxf(d, fmaf(__uint_as_float(x[e]) - now, cl, own_exponent(mt, 32 * blk + e0 + e)));
+          const uint32_t odd16 = mt.v_odd[blk + (e0 >> 5)] >> (e0 & 31);
+#pragma unroll
+          for (int e = 0; e < 16; ++e) moves = moves || (((odd16 >> e) & 1) && x[e] != 0xFF800000u);
         }
-        grow = grow || d > ev + 9.f;
-        if (grow) ev_now = fminf(fmaxf(fmaxf(ceilf(d), ev + floorf((m - now) * cl)), -126.f), 126.f);
+        grow = grow || (moves && d > ev + 9.f);
+        if (grow && moves) ev_now = fminf(fmaxf(fmaxf(ceilf(d), ev + floorf((m - now) * cl)), -126.f), 126.f);
       }
       if (__any_sync(0xffffffffu, grow)) {
         const float fo = grow ? ex2(fmaf(m - now, cl, ev - ev_now)) : 1.f;   // a row that does not grow keeps every bit

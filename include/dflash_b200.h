@@ -428,7 +428,7 @@ DFLASH_API int dflash_kv4_read(const dflash_kv4_cache* k_cache, const dflash_kv4
  *   mask     element (b,h,t,n) at the four strides (elements; 0 broadcasts); mask_kind 0 = none, 1 = bytes (0 hides),
  *            2 = additive in dtype, 3 = additive f32.  -inf hides; a finite value, however low, is added.
  *   Elements of a key or value are kept to 2^-11 of themselves or, where that is more, 2^-29 of 1 (2^-39 of the key's or value's
- *   largest element where that lies outside [2^-10, 2^11)); the probabilities to 2^-11 of themselves or 2^-31 of the row's largest.
+ *   largest element where that lies outside [2^-10, 2^11)); the probabilities to 2^-11 of themselves or 2^-26 of the row's largest.
  *   A row that sees nothing yields zeros.  Keys and values that a row does not see change no bit of it, NaN, infinities and the
  *   type's largest values included; a visible value with a scale or bias that is not finite, or whose codes reach beyond f32
  *   (scale * 15 + bias), makes the whole output row NaN.

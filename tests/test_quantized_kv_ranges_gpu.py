@@ -214,3 +214,32 @@ def test_random_sizes(seed, kind, which):
     lengths = [n, n - 33]
     got = qkv.quantized_kv_sdpa(q, k, v, 0.125, ints(*lengths), mask, num_splits=[0, 1, 3][seed % 3])
     check_rows(got, ref.sdpa(q, k, v, 0.125, lengths, mask), dtype)
+
+
+@pytest.mark.parametrize("which", KERNELS)
+@pytest.mark.parametrize("octaves", [4, 10, 14, 17, 20])
+@pytest.mark.parametrize("size", [2.0 ** -20, 2.0 ** -8, 2.0 ** -3, 2.0, 2.0 ** 6])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_many_small_weights_behind_a_large_one(dtype, size, octaves, which):
+    """Keys with most of the weight and a value of zero, 63 others behind each 2^-octaves as likely whose values agree: the row is what
+    they say.  A rounding of their weights that goes one way does not average out."""
+    T, _, _ = KERNELS[which]
+    n, D, Hq = 40000, 128, 4
+    # Probabilities p take 2^-25 in fp16 at the least: of p 2^6 in the tcgen05 kernel, in the other one of p times the value's scale,
+    # itself times 2^8 between 2^-7 and 2^3 and brought beyond 2^10 elsewhere.  Cases where that is more than 2^-9 are left out.
+    scaled = 1.3 * size / 15 * 2 ** 8
+    if 2.0 ** -25 > 2.0 ** -9 * 2.0 ** (-octaves - 0.45) * (2 ** 6 if which == "many" else scaled if 2 <= scaled < 2 ** 11 else 2 ** 10):
+        pytest.skip("below what the kernel's probabilities resolve")
+    k, v = qkv.allocate(1, 1, n, D, dtype=dtype)
+    large = torch.arange(n, device=DEV) % 64 == 0
+    v.codes[:, :, ~large] = 0x2E5D4C7B                    # eight different codes, the same for all keys
+    v.scales[:, :, ~large] = size / 15 * 1.3
+    v.biases[:, :, ~large] = -size / 3
+    # not a power of two apart, and the last bit of fp16's eleven differs from key to key
+    far = octaves * math.log(2) + 0.3 + 0.001 * torch.arange(n, device=DEV).remainder(7)
+    mask = torch.where(large, 0.0, -far)[None, None, None]
+    q = states((1, Hq, T, D), dtype, 9)
+    got = qkv.quantized_kv_sdpa(q, k, v, 0.1, ints(n + T), mask, max_length=n).double()
+    want = ref.sdpa(q, k, v, 0.1, [n + T], mask)
+    # TOL has 2^-9 for the probabilities; half a step of fp16's subnormal outputs on top
+    assert bool(((got - want).norm(dim=-1) <= TOL[dtype] * want.norm(dim=-1) + D ** 0.5 * (2.0 ** -25 if dtype == F16 else 0)).all())
