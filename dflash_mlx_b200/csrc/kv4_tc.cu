@@ -21,8 +21,8 @@
 // element into [2^14, 2^15), so that its other elements are kept to 2^-39 of it.  A column of S takes the power back before its softmax, and P for V: P = p 2^(6 + x - ev), with an
 // exponent ev of the row's output that is 0 until the row sees such a value.  Tiles without them, under rows with ev = 0, do not
 // touch any of this, and the bits of usual keys are the same either way.  (An exponent shared by 32 keys allows 9 instructions for 8
-// codes, 3 % of a long range, but then one large key, seen or not, takes the others' bits.  A cache of unusual keys takes 1.3 times as
-// long, one of unusual values 2.2 times.)  q is brought to fp16 by a power of two per row, exact
+// codes, 3 % of a long range, but then one large key, seen or not, takes the others' bits.  A cache of unusual keys takes 1.4 times as
+// long, one of unusual values 1.6 to 1.8 times.)  q is brought to fp16 by a power of two per row, exact
 // down to 2^-22 of the row's largest element.  P is fp16, up to 2^15; its sum takes the unrounded p.
 // The running maximum moves only when a score exceeds it by 8 octaves, per row.  Every wait is bounded (device error code 62).
 //
@@ -284,10 +284,15 @@ __device__ __forceinline__ void unpack_row(const uint4& c0, const uint4& c1, flo
   }
 }
 
-// What takes a key's own power of two back (1 for usual ones), and the exponent of a value's; blocks of 32 without an odd one have
-// stale exponents.
+// What takes a key's own power of two back (1 for usual ones), and the exponents of sixteen values; blocks of 32 without an odd one
+// have stale exponents.
 __device__ __forceinline__ float own_power(const Meta& m, int key) { return m.k_odd[key >> 5] ? pow2(m.k_exp[key]) : 1.f; }
-__device__ __forceinline__ float own_exponent(const Meta& m, int key) { return m.v_odd[key >> 5] ? (float)m.v_exp[key] : 0.f; }
+__device__ __forceinline__ uint4 own_exponents(const Meta& m, int key) {
+  return m.v_odd[key >> 5] ? *(const uint4*)(m.v_exp + key) : make_uint4(0, 0, 0, 0);
+}
+__device__ __forceinline__ float exponent(const uint4& x, int e) {
+  return (float)(int8_t)(((e >> 2) == 0 ? x.x : (e >> 2) == 1 ? x.y : (e >> 2) == 2 ? x.z : x.w) >> (8 * (e & 3)));
+}
 
 // The order in which a block works through its keys: from the last ones back, 64 at a time, so that under masks that fall with the
 // distance the largest scores come first and O is not rescaled with every tile (64 rows x 4 x 5001 keys of 256 channels: 40.2 -> 34.1
@@ -733,16 +738,20 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_sdpa_tc_kernel(const SdpaArgs
         wait_st();
         float d = -INFINITY;   // octaves of the row's largest p 2^x; NaN counts as none
         bool moves = ev != 0.f;   // a row that sees none of the unusual values, and saw none, stays as it is
+        const bool all_move = __all_sync(0xffffffffu, moves);
 #pragma unroll 1
         for (int e0 = 0; e0 < kTile; e0 += 16) {
           uint32_t x[16];
           ld16(s_col + e0, x);
+          const uint4 xs = own_exponents(mt, 32 * blk + e0);
           wait_ld();
 #pragma unroll
-          for (int e = 0; e < 16; ++e) d = fmaxf(d, fmaf(__uint_as_float(x[e]) - now, cl, own_exponent(mt, 32 * blk + e0 + e)));
-          const uint32_t odd16 = mt.v_odd[blk + (e0 >> 5)] >> (e0 & 31);
+          for (int e = 0; e < 16; ++e) d = fmaxf(d, fmaf(__uint_as_float(x[e]) - now, cl, exponent(xs, e)));
+          const uint32_t odd16 = mt.v_odd[blk + (e0 >> 5)] >> (e0 & 31) & 0xFFFFu;
+          if (!all_move && odd16 != 0) {
 #pragma unroll
-          for (int e = 0; e < 16; ++e) moves = moves || (((odd16 >> e) & 1) && x[e] != 0xFF800000u);
+            for (int e = 0; e < 16; ++e) moves = moves || (((odd16 >> e) & 1) && x[e] != 0xFF800000u);
+          }
         }
         grow = grow || (moves && d > ev + 9.f);
         if (grow && moves) ev_now = fminf(fmaxf(fmaxf(ceilf(d), ev + floorf((m - now) * cl)), -126.f), 126.f);
@@ -787,6 +796,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_sdpa_tc_kernel(const SdpaArgs
         for (int e0 = 0; e0 < kTile; e0 += 16) {
           uint32_t x[16], w[8];
           ld16(s_col + e0, x);
+          const uint4 xs = own_exponents(mt, 32 * blk + e0);
           wait_ld();
           const uint32_t bad = mt.v_bad[blk + (e0 >> 5)] >> (e0 & 31);
 #pragma unroll
@@ -798,8 +808,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_sdpa_tc_kernel(const SdpaArgs
             float p0, p1;
             unpair(fma2(d2, cl2, shift2), p0, p1);
             sum = add2(sum, pair(ex2(p0), ex2(p1)));
-            const int key = 32 * blk + e0 + e;
-            unpair(fma2(d2, cl2, pair(off + own_exponent(mt, key), off + own_exponent(mt, key + 1))), p0, p1);
+            unpair(fma2(d2, cl2, pair(off + exponent(xs, e), off + exponent(xs, e + 1))), p0, p1);
             const __half2 p = __floats2half2_rn(ex2(p0), ex2(p1));
             w[e >> 1] = *(const uint32_t*)&p;
           }
