@@ -656,19 +656,24 @@ __global__ void __launch_bounds__((kWarpsOf<D, NT>) * 32, 2) kv4_sdpa_kernel(con
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) mx = fmaxf(mx, mM[w * 8 * NT + row]);
     const float ref = mx == -INFINITY ? 0.f : mx;
+    float f[kWarps];
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      f[w] = ex2((mM[w * 8 * NT + row] - ref) * kLog2e);
+      den = fmaf(f[w], mL[w * 8 * NT + row], den);
+    }
+    const float inv = over_sum(den);   // a row that sees nothing yields zeros; NaN stays
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) {
-      const float f = ex2((mM[w * 8 * NT + row] - ref) * kLog2e), ev = sC[(1 + w) * 8 * NT + row];
-      const float fo = ev == 0.f ? f : ex2(fmaf(mM[w * 8 * NT + row] - ref, kLog2e, ev));   // O carries the row's exponent
+      const float ev = sC[(1 + w) * 8 * NT + row];   // O carries the row's exponent
+      const float fo = (ev == 0.f ? f[w] : ex2(fmaf(mM[w * 8 * NT + row] - ref, kLog2e, ev))) * inv;
       const float4 v = *(const float4*)(mO + ((size_t)w * 8 * NT + row) * D + d);
-      den = fmaf(f, mL[w * 8 * NT + row], den);
       acc.x = fmaf(fo, v.x, acc.x); acc.y = fmaf(fo, v.y, acc.y);
       acc.z = fmaf(fo, v.z, acc.z); acc.w = fmaf(fo, v.w, acc.w);
     }
     if (a.splits == 1) {
-      const float inv = den == 0.f ? 1.f : 1.f / den;   // a row that sees nothing yields zeros; NaN stays
-      const T y[4] = {TR::from_float(acc.x * inv), TR::from_float(acc.y * inv), TR::from_float(acc.z * inv), TR::from_float(acc.w * inv)};
+      const T y[4] = {TR::from_float(acc.x), TR::from_float(acc.y), TR::from_float(acc.z), TR::from_float(acc.w)};
       const float nan = den * 0.f;                       // a NaN sum reaches channels whose own products are finite
       T z[4];
 #pragma unroll
@@ -686,7 +691,7 @@ __global__ void __launch_bounds__((kWarpsOf<D, NT>) * 32, 2) kv4_sdpa_kernel(con
 }
 
 constexpr int kMaxSplits = 1024;
-// out = sum_s w_s O_s / sum_s w_s l_s, w_s = exp(m_s - max m): one block per row.
+// out = sum_s w_s O_s / sum_s w_s, w_s = exp(m_s - max m) l_s: one block per row.
 template <typename T, int D>
 __global__ void __launch_bounds__(256) kv4_combine_kernel(const SdpaArgs a) {
   using TR = MmaTraits<T>;
@@ -720,9 +725,9 @@ __global__ void __launch_bounds__(256) kv4_combine_kernel(const SdpaArgs a) {
   const float ref = mx == -INFINITY ? 0.f : mx;
   float den = 0.f;
   for (int s = tid; s < a.splits; s += kThreads) {
-    const float w = ex2((pm[s] - ref) * kLog2e);
+    const float w = ex2((pm[s] - ref) * kLog2e) * pl[s];
     sw[s] = w;
-    den = fmaf(w, pl[s], den);
+    den += w;
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) den += __shfl_xor_sync(0xffffffffu, den, o);
@@ -731,8 +736,10 @@ __global__ void __launch_bounds__(256) kv4_combine_kernel(const SdpaArgs a) {
   den = red[0];
 #pragma unroll
   for (int i = 1; i < kThreads / 32; ++i) den += red[i];
+  const float inv = over_sum(den), nan = den * 0.f;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
   auto add = [&](float w, const float4& v) {
+    w *= inv;
     acc.x = fmaf(w, v.x, acc.x); acc.y = fmaf(w, v.y, acc.y);
     acc.z = fmaf(w, v.z, acc.z); acc.w = fmaf(w, v.w, acc.w);
   };
@@ -749,8 +756,7 @@ __global__ void __launch_bounds__(256) kv4_combine_kernel(const SdpaArgs a) {
     const float4 v = part[i][d4];
     acc.x += v.x; acc.y += v.y; acc.z += v.z; acc.w += v.w;
   }
-  const float inv = den == 0.f ? 1.f : 1.f / den, nan = den * 0.f;
-  const float v[4] = {acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv};
+  const float v[4] = {acc.x, acc.y, acc.z, acc.w};
   T z[4];
 #pragma unroll
   for (int e = 0; e < 4; ++e) z[e] = TR::from_float(nan == 0.f ? v[e] : nan);
@@ -783,16 +789,20 @@ __global__ void __launch_bounds__(256) kv4_combine_few_kernel(const SdpaArgs a) 
   }
   const float ref = mx == -INFINITY ? 0.f : mx;
   float den = 0.f;
+#pragma unroll
+  for (int s = 0; s < kFewSplits; ++s) {
+    l[s] *= ex2((m[s] - ref) * kLog2e);
+    den += l[s];
+  }
+  const float inv = over_sum(den), nan = den * 0.f;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
   for (int s = 0; s < kFewSplits; ++s) {
-    const float w = ex2((m[s] - ref) * kLog2e);
-    den = fmaf(w, l[s], den);
+    const float w = l[s] * inv;
     acc.x = fmaf(w, v[s].x, acc.x); acc.y = fmaf(w, v[s].y, acc.y);
     acc.z = fmaf(w, v[s].z, acc.z); acc.w = fmaf(w, v[s].w, acc.w);
   }
-  const float inv = den == 0.f ? 1.f : 1.f / den, nan = den * 0.f;
-  const float y[4] = {acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv};
+  const float y[4] = {acc.x, acc.y, acc.z, acc.w};
   T z[4];
 #pragma unroll
   for (int e = 0; e < 4; ++e) z[e] = TR::from_float(nan == 0.f ? y[e] : nan);

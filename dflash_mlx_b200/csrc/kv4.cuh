@@ -16,7 +16,7 @@ struct SdpaArgs {
   int mask_kind;
   long long m_sb, m_sh, m_st, m_sn;
   void* out;
-  float* part_o;   // [B*Hk*rows][splits][D] un-normalised, then part_m / part_l [B*Hk*rows][splits]
+  float* part_o;   // [B*Hk*rows][splits][D], over the range's own sum (a sum of values may be no fp32 number), then part_m / part_l
   float* part_m;
   float* part_l;
   const int* lengths;
@@ -30,6 +30,13 @@ __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+
+// 1 / x to 2^-23, for sums of probabilities (at least about 1, or 0, NaN, +inf); 1 for the sum of nothing.
+__device__ __forceinline__ float over_sum(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return x == 0.f ? 1.f : y;
 }
 
 // Offset of query / output row `r` of (b, hk) in the contiguous output [B,Hq,T,D], in rows.

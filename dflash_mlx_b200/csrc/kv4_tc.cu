@@ -867,9 +867,10 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_sdpa_tc_kernel(const SdpaArgs
         const float2 x = sEnd[g * kRows + r];
         l = fmaf(x.y, x.x == -INFINITY ? 1.f : ex2((x.x - m) * cl), l);
       }
-      const float undo = pow2(ev);   // after 2^(kUnit - kPShift)
       const bool last = a.splits == 1;
-      const float inv = l == 0.f ? 1.f : 1.f / l, nan = l * 0.f;   // a row that sees nothing yields zeros; NaN reaches the whole row
+      const float inv = over_sum(l), nan = l * 0.f;   // a row that sees nothing yields zeros; NaN reaches the whole row
+      // over the range's own sum before the exponent comes back: a sum of large values may be no fp32 number
+      const float over = pow2(kUnit - (int)kPShift) * inv, undo = pow2(ev);
       const size_t at = ((size_t)bhk * a.rows + row) * a.splits + split;
       uint8_t* stage = smem + r * (D * 4 + 16);   // rows 16 bytes apart modulo 128: no bank conflicts
       const int c_first = group * (D / 2);
@@ -882,13 +883,13 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_sdpa_tc_kernel(const SdpaArgs
         }
         float y[32];   // back to the channels' order
 #pragma unroll
-        for (int e = 0; e < 32; ++e) y[(e & ~7) + ((e & 1) << 2) + ((e & 7) >> 1)] = have ? __uint_as_float(o[e]) * pow2(kUnit - (int)kPShift) * undo : 0.f;
+        for (int e = 0; e < 32; ++e) y[(e & ~7) + ((e & 1) << 2) + ((e & 7) >> 1)] = have ? __uint_as_float(o[e]) * over * undo : 0.f;
         if (last) {
 #pragma unroll
           for (int e = 0; e < 32; e += 8) {
             T z[8];
 #pragma unroll
-            for (int x = 0; x < 8; ++x) z[x] = TR::from_float(nan == 0.f ? y[e + x] * inv : nan);
+            for (int x = 0; x < 8; ++x) z[x] = TR::from_float(nan == 0.f ? y[e + x] : nan);
             *(uint4*)(stage + (c0 + e) * 2) = *(const uint4*)z;
           }
         } else {

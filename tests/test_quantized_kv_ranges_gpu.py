@@ -134,17 +134,18 @@ def test_small_values_first_then_large_ones_and_back(splits, D, which):
 
 
 @pytest.mark.parametrize("which", KERNELS)
-@pytest.mark.parametrize("dtype,most", [(BF16, 2.0 ** 104), (F16, 60000.0)])
-def test_values_that_span_their_type(dtype, most, which):
-    """Groups from far below to far above zero, as the write makes them; 60000 (1 + TOL) is still an fp16 number, and the sum of all
-    values of 2^104 an fp32 one."""
+@pytest.mark.parametrize("dtype,most", [(BF16, 2.0 ** 104), (BF16, 2.0 ** 126), (F16, 60000.0)])
+@pytest.mark.parametrize("splits", [0, 1, 12])
+def test_values_that_span_their_type(splits, dtype, most, which):
+    """Groups from far below to far above zero, as the write makes them; 60000 (1 + TOL) is still an fp16 number, and a mean of values of
+    2^126 an fp32 one, although their sum is none."""
     T, n, cap = KERNELS[which]
     k, _ = make_cache(1, 1, cap, 128, dtype)
     x = states((1, 1, cap, 128), dtype, 3)
     x[..., 5], x[..., 6] = most, -most
     v = qkv.QuantizedKV(*ref.quantise(x))
     q, scale = states((1, 4, T, 128), dtype, 9), 128 ** -0.5
-    got = qkv.quantized_kv_sdpa(q, k, v, scale, ints(n))
+    got = qkv.quantized_kv_sdpa(q, k, v, scale, ints(n), num_splits=splits)
     check_rows(got, ref.sdpa(q, k, v, scale, [n]), dtype)
 
 
