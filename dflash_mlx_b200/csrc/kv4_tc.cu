@@ -868,7 +868,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_sdpa_tc_kernel(const SdpaArgs
         l = fmaf(x.y, x.x == -INFINITY ? 1.f : ex2((x.x - m) * cl), l);
       }
       const bool last = a.splits == 1;
-      const float inv = over_sum(l), nan = l * 0.f;   // a row that sees nothing yields zeros; NaN reaches the whole row
+      const float inv = l == 0.f ? 1.f : 1.f / l, nan = l * 0.f;   // a row that sees nothing yields zeros; NaN reaches the whole row
       // over the range's own sum before the exponent comes back: a sum of large values may be no fp32 number
       const float over = pow2(kUnit - (int)kPShift) * inv, undo = pow2(ev);
       const size_t at = ((size_t)bhk * a.rows + row) * a.splits + split;
